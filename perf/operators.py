@@ -270,7 +270,7 @@ def _soft(x, temp):
     """exp of the scaled logits over their row's maximum, and each row's sum.  A pick by a cumulative sum of 10^5
     terms is a discontinuous function of those terms, so sums, probabilities and residuals are held in 64 bits."""
     top = x.amax(-1, keepdim=True)
-    e = torch.exp((x - top) * (1.0 / temp))
+    e = torch.exp((x - top) * (1.0 / torch.tensor(temp, dtype=torch.float32).item()))
     return e, e.sum(-1, dtype=torch.float64)
 
 
