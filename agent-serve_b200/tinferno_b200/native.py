@@ -16,6 +16,7 @@ HEADER = os.path.join(REPO_ROOT, "include", "tinferno_b200.h")
 
 f32p = C.POINTER(C.c_float)
 i32p = C.POINTER(C.c_int)
+u64p = C.POINTER(C.c_ulonglong)
 
 TF_F32, TF_F16, TF_Q4_0, TF_Q4_1, TF_Q8_0, TF_Q6_K = 0, 1, 2, 3, 8, 14
 TF_KV_F32, TF_KV_F16, TF_KV_BF16 = 0, 1, 2
@@ -87,6 +88,15 @@ SIGNATURES = [
     ("tf_op_attn_decode_noalloc", C.c_int, [_V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
     ("tf_op_attn_prefill", C.c_int, [_V, _V, _V, _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
     ("tf_op_argmax", C.c_int, [_V, C.c_int, C.c_int, _V, _V]),
+    ("tf_tree_mask", C.c_int, [i32p, C.c_int, C.c_int, u64p, i32p]),
+    ("tf_op_attn_tree_workspace", C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    ("tf_op_attn_tree", C.c_int, [_V, C.c_int, _V, C.c_int, _V, _V, C.c_int, C.c_longlong, C.c_int, C.c_int, _V, _V, _V,
+                                  _V, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _V, C.c_size_t, _V]),
+    ("tf_op_verify_tree_workspace", C.c_int, [C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    ("tf_op_verify_tree", C.c_int, [_V, _V, _V, _V, C.c_longlong, _V, C.c_longlong, _V, _V, _V, _V, C.c_float, C.c_int,
+                                    C.c_int, C.c_int, _V, C.c_size_t, _V]),
+    ("tf_op_kv_commit", C.c_int, [_V, _V, C.c_int, C.c_int, C.c_longlong, C.c_longlong, C.c_int, C.c_int, _V, _V, _V,
+                                  C.c_int, _V, _V, C.c_int, C.c_int, C.c_int, _V]),
 ]
 
 _lib = None

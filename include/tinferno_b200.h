@@ -251,6 +251,70 @@ TF_API int tf_op_attn_prefill(float* out, const float* q, const float* k, const 
 /* sample_greedy(logits, n)  src/sampler.hpp:9: out[r] = first index of the maximum of row r. */
 TF_API int tf_op_argmax(const float* logits, int n, int rows, int* out, void* stream);
 
+/* ---- speculative decoding with a tree of drafted tokens ---------------------------------
+ * No reference counterpart (the reference decodes one token per weight pass,
+ * src/main.cpp:106-122).  A step checks up to T drafted tokens of a sequence at once: node 0
+ * is the last committed token (its K/V is not in the cache yet), every other node hangs from
+ * an earlier one.  Nodes 0..n_node-1 hold cache rows n_ctx..n_ctx+n_node-1; node t sees the
+ * n_ctx committed rows, its ancestors and itself.  Counts, lengths, slots and paths live on
+ * the device, so a whole step needs no host round trip and can be captured in a CUDA graph.
+ *
+ * Workspaces: the caller allocates `bytes` of device memory (256-byte aligned), zeroes it once
+ * and may use it for any number of calls of at most those sizes, one call in flight at a time.
+ * The calls allocate nothing and do not synchronise.  What a kernel finds wrong on the device
+ * (a slot outside the cache, a context that does not fit, a token outside the vocabulary) goes
+ * to tf_op_device_error. */
+
+/* Host helper: the visibility words of a tree, mask[t][w] bit j = node 64 w + j is node t
+ * itself or an ancestor, W = ceil(T / 64) words per node, and (optional) each node's depth.
+ * parents[0] < 0, 0 <= parents[t] < t; nodes n..T-1 get empty words. */
+TF_API int tf_tree_mask(const int* parents, int n, int T, unsigned long long* mask, int* depth);
+
+/* Attention of B trees of up to T nodes over one layer's cache [n_slots][n_kv_heads][cap]
+ * [head_dim] of kv_type, slots slot_stride elements apart.  q and out: row b * T + t, ld_q and
+ * ld_out floats apart (q may point into fused q | k | v rows).  slots (nullptr: sequence b in
+ * slot b), n_ctx and n_node (nullptr: T) have one entry per sequence.  mask[b][t][W]: the node
+ * rows that node t sees (nullptr: nodes 0..t, a chain); any subset may be given, and a row that
+ * sees nothing, like the rows from n_node on, is zero.  Rows that a node does not see do not
+ * reach its output, whatever they hold.  T <= 256, head_dim a multiple of 8 up to 128, at most
+ * 8 query heads per kv head; B = 1, T = 1 is decode attention.  Scores, softmax and sums are
+ * fp32-equivalent for every kv_type. */
+TF_API int tf_op_attn_tree_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
+TF_API int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, const void* k_cache, const void* v_cache,
+                           int kv_type, long long slot_stride, int cap, int n_slots, const int* slots,
+                           const int* n_ctx, const int* n_node, const unsigned long long* mask, int B, int T,
+                           int n_heads, int n_kv_heads, int head_dim, void* ws, size_t ws_bytes, void* stream);
+
+/* Verification: which drafted nodes the target's distribution keeps, and the token after them.
+ * logits: row b * T + t is the target's logits after node t, `ld` floats apart.  draft
+ * (optional): row b * T + t is the draft's logits from which node t's children were drawn.
+ * p and q are the softmax of those rows at `temperature`.  From the root on, the current node's
+ * children are tried in index order, child t with token x and the uniform number u[b][t]:
+ *   with draft     accepted when u q(x) < r(x), r = p at first; a rejection replaces r by
+ *                  max(r - q, 0), normalised (p itself when that has no mass);
+ *   without        accepted when u < r(x); a rejection takes x out of r and renormalises;
+ *   temperature 0  accepted when x is the first maximum of the logits.
+ * An accepted child becomes the current node.  When none is accepted the next token is the
+ * first i whose cumulative r exceeds u[b][0] times r's total (temperature 0: the argmax).  The
+ * tokens then follow the target's own distribution.  Outputs: path[b][T] the kept nodes from
+ * the root on (-1 behind them), n_path[b] their count (0 when n_node[b] is 0), next[b].
+ * NaN logits weigh nothing; sums are held in 64 bits. */
+TF_API int tf_op_verify_tree_workspace(int B, int T, int V, size_t* bytes);
+TF_API int tf_op_verify_tree(int* path, int* n_path, int* next, const float* logits, long long ld,
+                             const float* draft, long long ld_draft, const int* tokens, const int* parents,
+                             const int* n_node, const float* u, float temperature, int B, int T, int V, void* ws,
+                             size_t ws_bytes, void* stream);
+
+/* Commit: cache row n_ctx[b] + path[b][i] becomes row n_ctx[b] + i for i < n_path[b], in place,
+ * K and V of n_layer layers (layer_stride elements apart) and every kv head; n_new[b]
+ * (optional, not n_ctx itself) = n_ctx[b] + n_path[b].  path[b] (ld_path ints apart) strictly
+ * increasing, slots distinct; a path that is not moves nothing and records
+ * TF_DEV_ERR_POS. */
+TF_API int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_layer, long long layer_stride,
+                           long long slot_stride, int cap, int n_slots, const int* slots, const int* n_ctx,
+                           const int* path, int ld_path, const int* n_path, int* n_new, int B, int n_kv_heads,
+                           int head_dim, void* stream);
+
 /* Pipeline trace of the tensor-core GEMM, no reference counterpart (a finer-grained companion
  * of the reference's --profile timings, src/main.cpp): while `buf` (device memory, 968
  * unsigned 64-bit words, zeroed) is set, every tensor-core GEMM launch of this process has its
