@@ -72,7 +72,7 @@ int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, const void
     if (!kv_ok(kv_type)) return set_error("unknown kv_type");
     if (ld_out < n_heads * head_dim || ld_q < n_heads * head_dim || ld_out % 4 || ld_q % 4)
         return set_error("ld_out and ld_q must be multiples of 4, at least n_heads * head_dim");
-    if (cap < 1 || n_slots < 1 || slot_stride < (long long)n_kv_heads * cap * head_dim || slot_stride % 8)
+    if (cap < 1 || cap > 1 << 30 || n_slots < 1 || slot_stride < (long long)n_kv_heads * cap * head_dim || slot_stride % 8)
         return set_error("bad cache shape (cap, n_slots, slot_stride)");
     if (!aligned(out, 16) || !aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(ws, 256))
         return set_error("out, q and the caches must be 16-byte aligned, the workspace 256-byte aligned");
