@@ -15,7 +15,11 @@
 // exact half; a bf16 row fits one half after the scale (8 bits, and 2^-39 of the tile's maximum
 // where f16 runs out of exponents).  Every tile's P V product starts from zero and joins the
 // running output by an fp32 fma, so its rounding does not grow with the context.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include <atomic>
+#include <cstring>
 
 #include "tree.cuh"
 
@@ -28,6 +32,7 @@ constexpr float kPShift = 15.f;       // p is held as 2^15 exp(s - max): its low
 
 // ---- the split of the tiles over the CTAs ---------------------------------------------------------
 struct TreePlan {
+    int maps;                // wide kernel, f16 cache: the tensor maps are valid
     int grid;                // CTAs of the main kernel
     int rt;                  // rows per row tile
     int pt;                  // positions per tile
@@ -114,6 +119,35 @@ __device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan
     base0 = found_base;
 }
 
+// The next piece of this CTA's range [g0, g1): tiles [t0, t1) of one unit.
+struct TreeSeg {
+    TreeSeq s;
+    int b, kvh, rtile, t0, t1, tiles, last_cta;  // last_cta: the CTA that ends the unit
+};
+__device__ __forceinline__ bool tree_next(const TreeAttnArgs& a, const TreePlan& pl, long long& g0, long long g1,
+                                          long long per, int& b, long long& base, TreeSeg& o) {
+    if (g0 >= g1) return false;
+    o.s = tree_seq(a, b);
+    o.tiles = seq_tiles(o.s, pl.pt);
+    int units = seq_units(a, o.s, pl.rt);
+    while (g0 >= base + (long long)o.tiles * units) {  // next sequence with work
+        base += (long long)o.tiles * units;
+        o.s = tree_seq(a, ++b);
+        o.tiles = seq_tiles(o.s, pl.pt);
+        units = seq_units(a, o.s, pl.rt);
+    }
+    const int unit = (int)((g0 - base) / o.tiles), nrt = units / a.n_kv;
+    const long long u0 = base + (long long)unit * o.tiles;  // the unit's first tile
+    o.b = b;
+    o.kvh = unit / nrt;
+    o.rtile = unit % nrt;
+    o.t0 = (int)(g0 - u0);
+    o.t1 = (int)(g1 - u0 < o.tiles ? g1 - u0 : o.tiles);
+    o.last_cta = (int)((u0 + o.tiles - 1) / per);
+    g0 = u0 + o.t1;
+    return true;
+}
+
 // Rows that no unit covers (nodes from n_node on, bad sequences) are zero.
 template <int NT>
 __device__ __forceinline__ void tree_zero_rows(const TreeAttnArgs& a) {
@@ -171,6 +205,14 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     hi = pack_half2(x, y);
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
     lo = pack_half2(x - f.x, y - f.y);
+}
+// the same by truncation: the high half keeps 10 bits behind the first (exact in f16 from 2^-14
+// on), the low half the rest
+__device__ __forceinline__ void split2t(float2 x, uint32_t& hi, uint32_t& lo) {
+    const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(x.y) & 0xFFFFE000u));
+    const float2 l = __fadd2_rn(x, make_float2(-h.x, -h.y));
+    hi = pack_half2(h.x, h.y);
+    lo = pack_half2(l.x, l.y);
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool in) {  // zeros when !in
     const int n = in ? 16 : 0;
@@ -284,19 +326,10 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
     tree_range<TN_THREADS>(a, pl, g0, g1, per, b, base);
     if (tid == 0) desc[blockIdx.x].b = -1;
 
-    while (g0 < g1) {
-        TreeSeq s = tree_seq(a, b);
-        int tiles = seq_tiles(s, PT), units = seq_units(a, s, RT);
-        while (g0 >= base + (long long)tiles * units) {  // next sequence with work
-            base += (long long)tiles * units;
-            s = tree_seq(a, ++b);
-            tiles = seq_tiles(s, PT);
-            units = seq_units(a, s, RT);
-        }
-        const int unit = (int)((g0 - base) / tiles), nrt = units / a.n_kv;
-        const int kvh = unit / nrt, rtile = unit % nrt;
-        const long long u0 = base + (long long)unit * tiles;  // the unit's first tile
-        const int t0 = (int)(g0 - u0), t1 = (int)(g1 - u0 < tiles ? g1 - u0 : tiles);
+    TreeSeg sg;
+    while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+        const TreeSeq s = sg.s;
+        const int kvh = sg.kvh, rtile = sg.rtile, t0 = sg.t0, t1 = sg.t1;
         const int end = s.n_ctx + s.n_node, rows = s.n_node * rep;
         const size_t off = (size_t)s.slot * a.slot_stride + (size_t)kvh * a.cap * hd;
         const uint8_t* kp = static_cast<const uint8_t*>(a.kc) + off * ESZ;
@@ -324,36 +357,43 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
         load(t0);
         // the rows' queries, TPR threads per row: scaled to [2^14, 2^15), two halves
         {
-            constexpr int TPR = TN_THREADS / RT < HD / 8 ? TN_THREADS / RT : HD / 8, EPT = HD / TPR;
-            const int r = tid / TPR, rr = rtile * RT + r, d0 = (tid % TPR) * EPT;
+            constexpr int TPR = TN_THREADS / RT < HD / 8 ? TN_THREADS / RT : HD / 8, UPT = HD / 8 / TPR;  // 8-dim units per thread
+            const int r = tid / TPR, rr = rtile * RT + r, j0 = tid % TPR;
             if (r < RT) {
-                float x[EPT];
+                float x[UPT][8];
                 uint32_t mb = 0;
                 const int node = div_rep(rr);
                 const float* qp = a.q + ((size_t)b * a.T + node) * a.ld_q + (size_t)(kvh * rep + rr - node * rep) * hd;
 #pragma unroll
-                for (int i = 0; i < EPT; i += 4) {
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (rr < rows && d0 + i < hd) y = *reinterpret_cast<const float4*>(qp + d0 + i);
-                    x[i] = y.x, x[i + 1] = y.y, x[i + 2] = y.z, x[i + 3] = y.w;
+                for (int i = 0; i < UPT; ++i) {
+                    const int d = (j0 + i * TPR) * 8;
+                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f), z = y;
+                    if (rr < rows && d < hd) {
+                        y = *reinterpret_cast<const float4*>(qp + d);
+                        z = *reinterpret_cast<const float4*>(qp + d + 4);
+                    }
+                    x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
+                    x[i][4] = z.x, x[i][5] = z.y, x[i][6] = z.z, x[i][7] = z.w;
                 }
 #pragma unroll
-                for (int i = 0; i < EPT; ++i) mb = max(mb, finite_abs_bits(x[i]));
+                for (int i = 0; i < UPT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mb = max(mb, finite_abs_bits(x[i][j]));
 #pragma unroll
                 for (int o = 1; o < TPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
                 const int e = half_exponent(mb);
                 const float sc = pow2i(-e);
 #pragma unroll
-                for (int i = 0; i < EPT; i += 8) {
+                for (int i = 0; i < UPT; ++i) {
                     uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) split2(x[i + 2 * j] * sc, x[i + 2 * j + 1] * sc, hi[j], lo[j]);
-                    const uint32_t c = (uint32_t)(d0 + i) >> 3;
+                    for (int j = 0; j < 4; ++j) split2(x[i][2 * j] * sc, x[i][2 * j + 1] * sc, hi[j], lo[j]);
+                    const uint32_t c = (uint32_t)(j0 + i * TPR);
                     const uint32_t o = (uint32_t)r * (HD * 2) + ((c ^ (r & 7)) << 4);
                     st_shared16(qh + o, hi);
                     st_shared16(ql + o, lo);
                 }
-                if (d0 == 0) qscale[r] = pow2i(e) * (kLog2e / sqrtf((float)hd));
+                if (j0 == 0) qscale[r] = pow2i(e) * (kLog2e / sqrtf((float)hd));
             }
         }
         if (tid < TREE_MAX_NODES / 32) badrow[tid] = 0;
@@ -568,7 +608,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
             }
         }
         const int anybad = __syncthreads_or(tid < TREE_MAX_NODES / 32 ? badrow[tid] != 0 : 0);
-        const bool whole = t0 == 0 && t1 == tiles;
+        const bool whole = t0 == 0 && t1 == sg.tiles;
         float* part = parts + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * tree_part_floats(RT, hd);
         for (int i = tid; i < RT * (HD / 4); i += TN_THREADS) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, rr = rtile * RT + r;
@@ -618,11 +658,634 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
             }
         }
         if (!whole && t0 == 0 && tid == 0)
-            desc[blockIdx.x] = TreeDesc{b, kvh, rtile, (int)((u0 + tiles - 1) / per)};
-        g0 = u0 + t1;
+            desc[blockIdx.x] = TreeDesc{b, kvh, rtile, sg.last_cta};
         __syncthreads();
     }
     tree_zero_rows<TN_THREADS>(a);
+}
+
+// ---- wide trees: tcgen05, 128 rows per row tile -------------------------------------------------------
+// One CTA per SM and range of tiles, four warpgroups:
+//   0, 1  softmax streams: even and odd tiles of a segment, a thread per row with a running
+//         maximum, sum and output of its own (registers); no shuffles, no exchange until the end;
+//   2     loaders: a tile's K and V rows arrive by one 1-D bulk copy each, are split into f16
+//         halves and written as MMA operands (rows of 64 dims, 128-byte swizzle);
+//   3     MMA issue (one thread).
+// Tensor memory: S_0, S_1 (PT columns each) and D_0, D_1 (HD columns each).  QK: S_w = Q K^T,
+// Q from shared memory, the tile K-major.  The softmax thread overwrites its scores in place,
+// CH columns at a time, with the high halves of p (CH / 2 columns) and the low ones, the A
+// operand of PV: D_w = P V, the same tile layout read MN-major; D_w starts from zero for every
+// tile and joins the registers' output.  QK of tile i + 1 is issued before PV of tile i, so the
+// tensor pipe works while a stream is in its softmax.
+constexpr int TW_THREADS = 512;
+constexpr int TW_RT = 128;
+
+constexpr int TW_LOADERS = 6;  // loader warps: warpgroup 2 and the last two warps of warpgroup 3
+
+template <int HD, int KVT>
+struct WideCfg {
+    static constexpr int ESZ = KVT == KV_F32 ? 4 : 2;
+    static constexpr int PT = KVT == KV_F32 && HD == 128 ? 64 : 128;
+    static constexpr int NLO = KVT == KV_F32 ? 2 : 1;
+    static constexpr int HALF = PT * HD * 2;              // bytes of one half of a K or V tile
+    static constexpr int RAW = PT * HD * ESZ;             // bytes of a raw K or V tile
+    // operand stages, and raw buffers of one K or V tile each
+    static constexpr int OS = KVT == KV_F16 ? (HD == 64 ? 4 : 2) : (KVT == KV_BF16 && HD == 64 ? 2 : 1);
+    static constexpr int RS = HD == 64 ? (KVT == KV_F32 ? 3 : 4) : 2;
+    static constexpr int QH = TW_RT * HD * 2;             // bytes of one half of Q
+    static constexpr int Q_OFF = 0;
+    static constexpr int K_OFF = 2 * QH;
+    static constexpr int V_OFF = K_OFF + OS * NLO * HALF;
+    static constexpr int RAW_OFF = V_OFF + OS * NLO * HALF;
+    static constexpr int SMEM = RAW_OFF + (KVT == KV_F16 ? 0 : RS * RAW) + 1024;
+    // registers per thread of the softmax warpgroups and of the other two (512 in all, four
+    // warpgroups of 128 at launch)
+    static constexpr int REG_S = HD == 64 ? 168 : 184, REG_L = HD == 64 ? 88 : 72;
+    static constexpr int CH = HD == 64 ? 32 : 16;         // score columns a softmax thread holds at a time
+};
+
+__device__ __forceinline__ uint64_t wide_desc(uint32_t saddr, uint32_t lbo) {
+    // start >> 4 [0,14), LBO >> 4 [16,30), SBO >> 4 [32,46) (1024: 8 rows of 128 bytes), version 1
+    // [46,48), 128-byte swizzle [61,64)
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// One MMA / commit, issued by the lane whose `lead` is set (elect_lane) while the whole warp runs
+// the same code: a warp-uniform loop keeps the descriptors in uniform registers and issues 128 x
+// 64 x 16 products every 32 clocks, a loop inside `if (lane == 0)` every 47 to 120.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void wide_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t acc, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(da), "l"(db), "r"(idesc), "r"(acc), "r"(lead));
+}
+__device__ __forceinline__ void wide_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t acc, uint32_t lead) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+        "r"(ta), "l"(db), "r"(idesc), "r"(acc), "r"(lead));
+}
+__device__ __forceinline__ void wide_commit(uint64_t* bar, uint32_t lead) {
+    if (lead)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+    __syncwarp();
+}
+// n columns of a thread's TMEM lane (a load includes its wait)
+__device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(t)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t t, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&r)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(t)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t t, const uint32_t (&r)[32]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+template <int ID, int N>
+__device__ __forceinline__ void named_bar() {
+    asm volatile("bar.sync %0, %1;" ::"n"(ID), "n"(N) : "memory");
+}
+// byte offset of 16-byte chunk c (8 dims) of row r in a tile of `rows` rows (64-dim blocks)
+__device__ __forceinline__ uint32_t wide_off(int rows, int r, int c) {
+    return (uint32_t)(c >> 3) * (uint32_t)(rows * 128) + (uint32_t)r * 128u + (uint32_t)(((c & 7) ^ (r & 7)) << 4);
+}
+
+struct WideShared {
+    uint64_t rawfull[4], rawfree[4];              // raw tiles
+    uint64_t kfull[4], kfree[4], vfull[4], vfree[4];  // operand stages
+    uint64_t sfull[2], pfull[2], dfull[2], qfull, done;
+    uint32_t tmem;
+    int abort;
+    unsigned tmax[4];
+    int ek[4], ev[4];                             // scale exponents of the last four tiles
+    unsigned badrow[8][TREE_MAX_NODES / 32];      // drafted rows with non-finite values, by segment
+    float qscale[TW_RT];
+    float2 ml[2][TW_RT];                          // the streams' row maxima and sums
+};
+
+// Exponent that puts a tile's maximum at 2^8: room for 2^7 more before f16 overflows, and 2^8
+// less before the low halves run out of exponents.
+__device__ __forceinline__ int tile_exponent(uint32_t maxbits) {
+    const int e = (int)(maxbits >> 23) - 127 - 8;
+    return e < -126 ? -126 : (e > 126 ? 126 : e);
+}
+
+template <int HD, int KVT>
+__global__ void __launch_bounds__(TW_THREADS, 1) tf_tree_attn_wide_kernel(const TreeAttnArgs a, const TreePlan pl,
+                                                                           const __grid_constant__ CUtensorMap kmap,
+                                                                           const __grid_constant__ CUtensorMap vmap) {
+    using F = WideCfg<HD, KVT>;
+    constexpr int PT = F::PT, NLO = F::NLO, ESZ = F::ESZ, OS = F::OS, RS = F::RS, CH = F::CH;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(16) WideShared sh;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
+    const int rep = a.n_head / a.n_kv, hd = a.hd;
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sb = smem_u32(smem);
+    volatile int* abort_flag = &sh.abort;
+    const int rep_inv = (65536 + rep - 1) / rep;  // row / rep for rows < 2048 and rep <= 8
+
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+    }
+    if (tid == 32) {
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(&sh.rawfull[i], 1);
+            mbar_init(&sh.rawfree[i], TW_LOADERS);
+            mbar_init(&sh.kfull[i], TW_LOADERS);
+            mbar_init(&sh.vfull[i], TW_LOADERS);
+            mbar_init(&sh.kfree[i], 1);
+            mbar_init(&sh.vfree[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.sfull[i], 1);
+            mbar_init(&sh.pfull[i], 128);
+            mbar_init(&sh.dfull[i], 1);
+        }
+        mbar_init(&sh.qfull, 256);
+        mbar_init(&sh.done, 1);
+        sh.abort = 0;
+        for (int i = 0; i < 4; ++i) sh.tmax[i] = 0;
+        mbar_fence_init();
+    }
+    pdl_trigger();
+    pdl_wait();
+    TreeDesc* desc = static_cast<TreeDesc*>(a.ws);
+    float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + 65536);
+    if (tid == 0) desc[blockIdx.x].b = -1;
+    long long g0, g1, per, base;
+    int b;
+    tc_fence_before();
+    tree_range<TW_THREADS>(a, pl, g0, g1, per, b, base);  // (block barriers inside)
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    TreeSeg sg;
+
+    // Every role walks the same segments and tiles; after an abort the waits return at once and
+    // the roles run on without effect, so that all of them meet at every barrier.
+    // A tile that needs no work on its values (f16, all of it committed context) goes straight
+    // to its operand stage through the tensor maps.
+    auto direct = [&](const TreeSeg& g, int t) { return KVT == KV_F16 && pl.maps && (t + 1) * PT <= g.s.n_ctx; };
+    if (wg >= 2) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REG_L));
+    if (wg == 2 || warp >= 14) {
+        constexpr int LT = TW_LOADERS * 32;
+        const int lt = wg == 2 ? tid - 256 : tid - 320;
+        int n = 0, nr = 0, seg = 0;  // running tile, raw buffer and segment
+        int e2k = 0, e2v = 0;        // current exponents of K and V
+        while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+            const TreeSeq s = sg.s;
+            const int end = s.n_ctx + s.n_node;
+            if (lt < TREE_MAX_NODES / 32) sh.badrow[seg & 7][lt] = 0;  // read by others long ago
+            named_bar<2, LT>();
+            for (int t = sg.t0; t < sg.t1; ++t, ++n) {
+                const int os = n % OS, rows = min(PT, end - t * PT);
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    uint64_t* full = which ? &sh.vfull[os] : &sh.kfull[os];
+                    uint64_t* free = which ? &sh.vfree[os] : &sh.kfree[os];
+                    const uint32_t off = (which ? F::V_OFF : F::K_OFF) + os * NLO * F::HALF;
+                    // the operand stage is free once the MMAs of OS tiles ago are done
+                    if (direct(sg, t)) {
+                        if (lane == 0) {
+                            if (n >= OS) mbar_wait(free, (n / OS - 1) & 1, a.err, ERR_WAIT_EMPTY, abort_flag);
+                            if (lt == 0 && !*abort_flag) {
+                                mbar_expect_tx(full, F::HALF);
+                                const int row = (int)(((size_t)s.slot * a.slot_stride) / hd + (size_t)sg.kvh * a.cap) + t * PT;
+#pragma unroll
+                                for (int c = 0; c < HD / 64; ++c)
+                                    asm volatile(
+                                        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
+                                        "[%1, {%2, %3}], [%4];" ::"r"(sb + off + c * PT * 128),
+                                        "l"(reinterpret_cast<uint64_t>(which ? &vmap : &kmap)), "r"(64 * c), "r"(row), "r"(smem_u32(full))
+                                        : "memory");
+                            } else {
+                                mbar_arrive(full);
+                            }
+                        }
+                        continue;
+                    }
+                    const int rs = nr % RS;
+                    uint8_t* raw = smem + F::RAW_OFF + rs * F::RAW;
+                    if (KVT != KV_F16) mbar_wait(&sh.rawfull[rs], (nr / RS) & 1, a.err, ERR_WAIT_FULL, abort_flag);
+                    if (n >= OS) mbar_wait(free, (n / OS - 1) & 1, a.err, ERR_WAIT_EMPTY, abort_flag);
+                    __syncwarp();
+                    ++nr;
+                    constexpr int UNITS = PT * HD / 8, UPR = HD / 8;  // 8-element units, per row
+                    if (KVT != KV_F16 && which && (t + 1) * PT > s.n_ctx)  // non-finite drafted values leave the operand (see the narrow kernel)
+                        for (int v = lt; v < UNITS; v += LT) {
+                            const int r = v / UPR, c = (v % UPR) * 8, p = t * PT + r;
+                            if (r >= rows || c >= hd || p < s.n_ctx) continue;
+                            uint4* x = reinterpret_cast<uint4*>(raw + ((size_t)r * hd + c) * ESZ);
+                            for (int k = 0; k < ESZ / 2; ++k) {
+                                uint4 y = x[k];
+                                if (zero_nonfinite<KVT>(y)) {
+                                    x[k] = y;
+                                    atomicOr(&sh.badrow[seg & 7][(p - s.n_ctx) >> 5], 1u << ((p - s.n_ctx) & 31));
+                                }
+                            }
+                        }
+                    const uint32_t dst = sb + off, rawa = smem_u32(raw);
+                    // converted with the last tile's exponent; when the tile's maximum turns out not
+                    // to fit it (seldom), once more with its own
+                    for (;;) {
+                        const int ec = which ? e2v : e2k;
+                        const float f = pow2i(-ec);
+                        float mf = 0.f;       // largest |x| of fp32 values
+                        uint32_t mw = 0;      // largest |x| of bf16 values, two lanes
+#pragma unroll 4
+                        for (int v = lt; v < UNITS; v += LT) {
+                            const int r = v / UPR, c = v % UPR;
+                            uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+                            if (r < rows && c * 8 < hd) {
+                                const uint32_t x = rawa + (uint32_t)((r * hd + c * 8) * ESZ);
+                                if (KVT == KV_F16) {  // the few such tiles come straight from the cache
+                                    const int p = t * PT + r;
+                                    const size_t at = (size_t)s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + p) * hd + c * 8;
+                                    x0 = *reinterpret_cast<const uint4*>(static_cast<const __half*>(which ? a.vc : a.kc) + at);
+                                    if (which && p >= s.n_ctx && zero_nonfinite<KVT>(x0))
+                                        atomicOr(&sh.badrow[seg & 7][(p - s.n_ctx) >> 5], 1u << ((p - s.n_ctx) & 31));
+                                } else {
+                                    x0 = ld_shared16(x);
+                                    if (KVT == KV_F32) x1 = ld_shared16(x + 16);
+                                }
+                            }
+                            const uint32_t o = dst + wide_off(PT, r, c);
+                            if (KVT == KV_F32) {
+                                uint32_t hi[4], lo[4];
+                                const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    const float2 y = make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
+                                    mf = fmaxf(mf, fmaxf(fabsf(y.x), fabsf(y.y)));
+                                    split2t(__fmul2_rn(y, make_float2(f, f)), hi[j], lo[j]);
+                                }
+                                st_shared16(o, hi);
+                                st_shared16(o + F::HALF, lo);
+                            } else {
+                                uint32_t w[4] = {x0.x, x0.y, x0.z, x0.w};
+                                if (KVT == KV_BF16) {
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) {
+                                        mw = __vmaxu2(mw, w[j] & 0x7FFF7FFFu);
+                                        w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
+                                    }
+                                }
+                                st_shared16(o, w);
+                            }
+                        }
+                        uint32_t mb = KVT == KV_F32 ? __float_as_uint(mf) : max(mw << 16, mw & 0xFFFF0000u);
+                        if (KVT != KV_F16 && __any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
+                            mb = 0;
+                            for (int v = lt; v < UNITS; v += LT) {
+                                const int r = v / UPR, c = v % UPR;
+                                if (r >= rows || c * 8 >= hd) continue;
+                                const uint32_t x = rawa + (uint32_t)((r * hd + c * 8) * ESZ);
+                                mb = max(mb, max_bits<KVT>(ld_shared16(x)));
+                                if (KVT == KV_F32) mb = max(mb, max_bits<KVT>(ld_shared16(x + 16)));
+                            }
+                            __syncwarp();
+                        }
+                        if (KVT == KV_F16) break;
+                        mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+                        unsigned* tm = &sh.tmax[2 * (n & 1) + which];
+                        if (lane == 0) atomicMax(tm, mb);
+                        named_bar<2, LT>();
+                        const uint32_t all = *tm;
+                        // fits: the maximum is within [2^0, 2^15) after the scale
+                        const int e = tile_exponent(all), d = e - ec;
+                        if (all == 0 || d == 0 || (d > -8 && d < 7)) break;
+                        named_bar<2, LT>();  // every thread has read the exponent's base
+                        if (which) e2v = e;
+                        else e2k = e;
+                    }
+                    if (lt == 0) {
+                        sh.tmax[2 * (~n & 1) + which] = 0;  // the next tile's, read last a tile ago
+                        (which ? sh.ev : sh.ek)[n & 3] = which ? e2v : e2k;
+                    }
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(full);
+                        if (KVT != KV_F16) mbar_arrive(&sh.rawfree[rs]);
+                    }
+                }
+            }
+            ++seg;
+        }
+        // after an abort: copies of the last stages may still be on their way
+        if (lt == 0 && *abort_flag)
+            for (int i = max(0, n - OS); i < n; ++i) {
+                mbar_wait(&sh.kfull[i % OS], (i / OS) & 1, a.err, ERR_WAIT_FULL, nullptr);
+                mbar_wait(&sh.vfull[i % OS], (i / OS) & 1, a.err, ERR_WAIT_FULL, nullptr);
+            }
+    } else if (warp == 13) {
+        // raw copies, RS buffers ahead
+        if (KVT != KV_F16 && lane == 0) {
+            int nr = 0, last[RS];  // last copy into each buffer
+#pragma unroll
+            for (int i = 0; i < RS; ++i) last[i] = -1;
+            while (tree_next(a, pl, g0, g1, per, b, base, sg))
+                for (int t = sg.t0; t < sg.t1; ++t) {
+                    const int rows = min(PT, sg.s.n_ctx + sg.s.n_node - t * PT);
+                    const uint32_t bytes = (uint32_t)(rows * hd * ESZ);
+                    const size_t off = ((size_t)sg.s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + (size_t)t * PT) * hd) * ESZ;
+                    for (int which = 0; which < 2; ++which, ++nr) {
+                        const int rs = nr % RS;
+                        if (nr >= RS) mbar_wait(&sh.rawfree[rs], (nr / RS - 1) & 1, a.err, ERR_WAIT_EMPTY, abort_flag);
+                        if (*abort_flag) continue;
+                        mbar_expect_tx(&sh.rawfull[rs], bytes);
+                        bulk_g2s(smem + F::RAW_OFF + rs * F::RAW, static_cast<const uint8_t*>(which ? a.vc : a.kc) + off, bytes, &sh.rawfull[rs]);
+                        last[rs] = nr / RS;
+                    }
+                }
+            if (*abort_flag)  // copies that may still be on their way
+                for (int i = 0; i < RS; ++i)
+                    if (last[i] >= 0) mbar_wait(&sh.rawfull[i], last[i] & 1, a.err, ERR_WAIT_FULL, nullptr);
+        }
+        __syncwarp();
+    } else if (warp == 12) {
+        // D f32, A / B f16, M = 128: QK with N = PT, both K-major; PV with N = HD, B MN-major
+        constexpr uint32_t iqk = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(TW_RT >> 4) << 24);
+        constexpr uint32_t ipv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TW_RT >> 4) << 24);
+        const uint32_t lead = elect_lane(), tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+        int n = 0, seg = 0;
+        int cnt0 = 0, cnt1 = 0;  // PVs issued per stream
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, int parity) {
+            ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(bar, parity & 1, a.err, ERR_WAIT_FULL, abort_flag));
+        };
+        auto pv = [&](int m, int w) {  // tile m of the run, stream w
+            const int os = m % OS;
+            wait(&sh.pfull[w], w ? cnt1 : cnt0);
+            wait(&sh.vfull[os], m / OS);
+            if (w) ++cnt1;
+            else ++cnt0;
+            if (!ok) return;
+            tc_fence_after();
+            const uint32_t d = tm + 256 + w * HD, p = tm + w * 128;
+            const uint64_t vh = wide_desc(sb + F::V_OFF + os * NLO * F::HALF, PT * 128);
+            const uint64_t vl = wide_desc(sb + F::V_OFF + os * NLO * F::HALF + (NLO - 1) * F::HALF, PT * 128);
+#pragma unroll
+            for (int j = 0; j < PT / 16; ++j) {  // 16 positions: 2048 bytes of rows; p's halves in blocks of CH columns
+                const uint32_t ph = CH == 32 ? p + 32 * (j / 2) + 8 * (j % 2) : p + 16 * j;
+                wide_mma_ts(d, ph, vh + 128u * j, ipv, j > 0, lead);
+                wide_mma_ts(d, ph + CH / 2, vh + 128u * j, ipv, 1, lead);
+                if (NLO == 2) wide_mma_ts(d, ph, vl + 128u * j, ipv, 1, lead);
+            }
+            wide_commit(&sh.vfree[os], lead);
+            wide_commit(&sh.dfull[w], lead);
+        };
+        while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+            wait(&sh.qfull, seg);
+            for (int t = sg.t0; t < sg.t1; ++t, ++n) {
+                const int w = (t - sg.t0) & 1, os = n % OS;
+                wait(&sh.kfull[os], n / OS);
+                if (ok) {
+                    tc_fence_after();
+                    const uint32_t d = tm + w * 128;
+                    const uint64_t kb = wide_desc(sb + F::K_OFF + os * NLO * F::HALF, 16), qb = wide_desc(sb + F::Q_OFF, 16);
+#pragma unroll
+                    for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes along the rows of a 64-dim block
+                        const uint64_t q = qb + ((j / 4) * (TW_RT * 128) + (j % 4) * 32) / 16;
+                        const uint64_t k = kb + ((j / 4) * (PT * 128) + (j % 4) * 32) / 16;
+                        wide_mma_ss(d, q, k, iqk, j > 0, lead);
+                        wide_mma_ss(d, q + F::QH / 16, k, iqk, 1, lead);
+                        if (NLO == 2) wide_mma_ss(d, q, k + F::HALF / 16, iqk, 1, lead);
+                    }
+                    wide_commit(&sh.kfree[os], lead);
+                    wide_commit(&sh.sfull[w], lead);
+                }
+                if (t > sg.t0) pv(n - 1, w ^ 1);
+            }
+            pv(n - 1, (sg.t1 - 1 - sg.t0) & 1);
+            ++seg;
+        }
+        wide_commit(&sh.done, lead);  // arrives once every MMA issued above has completed
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REG_S));
+        const int row = tid & 127;                                  // TMEM lane
+        const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
+        const uint32_t ts = tl + wg * 128, td = tl + 256 + wg * HD;
+        int n = 0, seg = 0, cnt = 0;
+        while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+            const TreeSeq s = sg.s;
+            const int rows = s.n_node * rep;
+            {   // queries, HD / 8 lanes per row: scaled to [2^14, 2^15), two halves
+                constexpr int LPR = HD / 8, RPW = 32 / LPR, STEPS = TW_RT / (8 * RPW);
+                float4 x[STEPS][2];
+                const int c = lane % LPR;
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const int r = (i * 8 + warp) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
+                    const float* qp = a.q + ((size_t)sg.b * a.T + nd) * a.ld_q + (size_t)(sg.kvh * rep + q - nd * rep) * hd + c * 8;
+                    x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (q < rows && c * 8 < hd) {
+                        x[i][0] = reinterpret_cast<const float4*>(qp)[0];
+                        x[i][1] = reinterpret_cast<const float4*>(qp)[1];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) {
+                    const int r = (i * 8 + warp) * RPW + lane / LPR;
+                    const float y[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
+                    uint32_t mb = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) mb = max(mb, finite_abs_bits(y[j]));
+#pragma unroll
+                    for (int o = 1; o < LPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
+                    const int e = half_exponent(mb);
+                    const float sc = pow2i(-e);
+                    uint32_t hi[4], lo[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) split2(y[2 * j] * sc, y[2 * j + 1] * sc, hi[j], lo[j]);
+                    const uint32_t o = sb + F::Q_OFF + wide_off(TW_RT, r, c);
+                    st_shared16(o, hi);
+                    st_shared16(o + F::QH, lo);
+                    if (c == 0) sh.qscale[r] = pow2i(e) * (kLog2e / sqrtf((float)hd));
+                }
+                fence_async();
+                mbar_arrive(&sh.qfull);
+                named_bar<1, 256>();
+            }
+            const float qs = sh.qscale[row];
+            const int rr = sg.rtile * TW_RT + row, node = (rr * rep_inv) >> 16;
+            float O[HD], m = -INFINITY, l = 0.f;
+#pragma unroll
+            for (int i = 0; i < HD; ++i) O[i] = 0.f;
+            const int n0 = n;
+            for (int t = sg.t0 + wg; t < sg.t1; t += 2, ++cnt) {
+                const int nt = n0 + t - sg.t0;
+                mbar_wait(&sh.sfull[wg], cnt & 1, a.err, ERR_WAIT_FULL, abort_flag);
+                __syncwarp();
+                tc_fence_after();
+                const float f = KVT == KV_F16 ? qs : qs * pow2i(sh.ek[nt & 3]);
+                const bool tail = (t + 1) * PT > s.n_ctx;
+                // (the loops over 32-column chunks stay loops: unrolled, the code outgrows the
+                // instruction cache and the one warp per scheduler waits for its fetches)
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < PT / CH; ++c) {
+                    uint32_t x[CH];
+                    tmem_ld(ts + CH * c, x);
+                    if (tail) {
+                        const uint32_t vis = tree_window(a, s, sg.b, node, t * PT + CH * c - s.n_ctx);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < CH; ++i) x[i] = (vis >> i) & 1 ? x[i] : 0xFF800000u;
+                        tmem_st(ts + CH * c, x);  // masked scores are -infinity from here on
+                    }
+                    float m0 = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+#pragma unroll
+                    for (int i = 2; i < CH; i += 2) m0 = fmaxf(m0, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                    mx = fmaxf(mx, m0);
+                }
+                if (tail) tmem_wait_st();
+                mx = fmaxf(m, mx * f);
+                const float ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(m - ref), shift = kPShift - ref;
+                m = mx;
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < PT / CH; ++c) {
+                    uint32_t x[CH], y[CH];
+                    tmem_ld(ts + CH * c, x);
+#pragma unroll
+                    for (int i = 0; i < CH; i += 2) {
+                        const float p0 = exp2_fast(fmaf(__uint_as_float(x[i]), f, shift));
+                        const float p1 = exp2_fast(fmaf(__uint_as_float(x[i + 1]), f, shift));
+                        sum0 += p0;
+                        sum1 += p1;
+                        // high halves by truncation (exact in f16 down to 2^-14), low halves what is left
+                        const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
+                        const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
+                        y[i / 2] = pack_half2(h0, h1);
+                        y[CH / 2 + i / 2] = pack_half2(p0 - h0, p1 - h1);
+                    }
+                    tmem_st(ts + CH * c, y);
+                }
+                l = fmaf(l, alpha, sum0 + sum1);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sh.pfull[wg]);
+                mbar_wait(&sh.dfull[wg], cnt & 1, a.err, ERR_WAIT_FULL, abort_flag);
+                __syncwarp();
+                tc_fence_after();
+                const float fv = KVT == KV_F16 ? 1.f : pow2i(sh.ev[nt & 3]);
+#pragma unroll
+                for (int c = 0; c < HD / CH; ++c) {
+                    uint32_t x[CH];
+                    tmem_ld(td + CH * c, x);
+#pragma unroll
+                    for (int i = 0; i < CH; ++i) O[CH * c + i] = fmaf(__uint_as_float(x[i]), fv, O[CH * c + i] * alpha);
+                }
+                tc_fence_before();
+            }
+            n += sg.t1 - sg.t0;
+            // The streams meet in Q's shared memory (every QK of the segment is done): maxima and
+            // sums first, then stream 1's weighted output, stream 0 adds its own, and the rows
+            // leave coalesced.  fp32 rows of HD, 16-byte chunk c of row r at c ^ (r & 7).
+            sh.ml[wg][row] = make_float2(m, l);
+            named_bar<1, 256>();
+            const float2 other = sh.ml[wg ^ 1][row];
+            const float M = fmaxf(m, other.x), mref = M == -INFINITY ? 0.f : M, wgt = exp2_fast(m - mref);
+            const float L = fmaf(l, wgt, other.y * exp2_fast(other.x - mref));
+            const uint32_t srow = sb + F::Q_OFF + (uint32_t)row * (HD * 4);
+            if (wg == 1) {
+#pragma unroll
+                for (int c = 0; c < HD / 4; ++c)
+                    st_shared16(srow + ((uint32_t)(c ^ (row & 7)) << 4),
+                                {__float_as_uint(O[4 * c] * wgt), __float_as_uint(O[4 * c + 1] * wgt),
+                                 __float_as_uint(O[4 * c + 2] * wgt), __float_as_uint(O[4 * c + 3] * wgt)});
+            }
+            named_bar<1, 256>();
+            const bool whole = sg.t0 == 0 && sg.t1 == sg.tiles;
+            float* part = parts + ((size_t)blockIdx.x * 2 + (sg.t0 == 0 ? 1 : 0)) * tree_part_floats(TW_RT, hd);
+            if (wg == 0) {
+                const float inv = !whole ? 1.f : (L == 0.f ? 0.f : 1.f / L);
+                const bool none = whole && L == 0.f;
+#pragma unroll
+                for (int c = 0; c < HD / 4; ++c) {
+                    const uint32_t at = srow + ((uint32_t)(c ^ (row & 7)) << 4);
+                    const uint4 x = ld_shared16(at);
+                    const float y[4] = {fmaf(O[4 * c], wgt, __uint_as_float(x.x)), fmaf(O[4 * c + 1], wgt, __uint_as_float(x.y)),
+                                        fmaf(O[4 * c + 2], wgt, __uint_as_float(x.z)), fmaf(O[4 * c + 3], wgt, __uint_as_float(x.w))};
+                    uint32_t z[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) z[j] = none ? 0u : __float_as_uint(y[j] * inv);
+                    st_shared16(at, z);
+                }
+                if (rr < rows) {
+                    const size_t off = (size_t)s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + s.n_ctx) * hd;
+#pragma unroll 1
+                    for (int w = 0; w < TREE_MAX_NODES / 32; ++w)  // non-finite drafted values that the row sees
+#pragma unroll 1
+                        for (unsigned bits = sh.badrow[seg & 7][w] & tree_window(a, s, sg.b, node, 32 * w); bits; bits &= bits - 1) {
+                            const size_t at = off + (size_t)(w * 32 + __ffs(bits) - 1) * hd;
+#pragma unroll 1
+                            for (int i = 0; i < hd; ++i) {
+                                const float v = kv_load(a.vc, (long long)(at + i), KVT);
+                                float* o = reinterpret_cast<float*>(smem + F::Q_OFF + (size_t)row * (HD * 4) + (((i >> 2) ^ (row & 7)) << 4)) + (i & 3);
+                                if (!(fabsf(v) < INFINITY)) *o += v;
+                            }
+                        }
+                    if (!whole && !*abort_flag) {
+                        part[(size_t)TW_RT * hd + row] = M;
+                        part[(size_t)TW_RT * hd + TW_RT + row] = L;
+                    }
+                }
+                if (!whole && sg.t0 == 0 && row == 0) desc[blockIdx.x] = TreeDesc{sg.b, sg.kvh, sg.rtile, sg.last_cta};
+            }
+            named_bar<1, 256>();
+            {
+                constexpr int LPR = HD / 4, RPW = 32 / LPR;  // lanes per row, rows per warp and step
+                const int c = lane % LPR;
+#pragma unroll 4
+                for (int i = warp; i < TW_RT / RPW; i += 8) {
+                    const int r = i * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
+                    if (q >= rows || c * 4 >= hd || *abort_flag) continue;
+                    const uint4 x = ld_shared16(sb + F::Q_OFF + (uint32_t)r * (HD * 4) + ((uint32_t)(c ^ (r & 7)) << 4));
+                    float* dst = whole ? a.out + ((size_t)sg.b * a.T + nd) * a.ld_out + (size_t)(sg.kvh * rep + q - nd * rep) * hd
+                                       : part + (size_t)r * hd;
+                    *reinterpret_cast<uint4*>(dst + c * 4) = x;
+                }
+            }
+            named_bar<1, 256>();  // Q's shared memory takes the next segment's queries
+            __syncwarp();
+            ++seg;
+        }
+    }
+    // TMEM stays allocated until every issued MMA has completed
+    __syncwarp();
+    if (warp == 0) mbar_wait(&sh.done, 0, a.err, ERR_WAIT_FULL, nullptr);
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    tree_zero_rows<TW_THREADS>(a);
 }
 
 // ---- joins the partial results of units that were split over CTAs ------------------------------------
@@ -689,7 +1352,7 @@ static int tree_sms() {
 size_t tree_attn_ws_bytes(int B, int T, int n_head, int n_kv, int hd) {
     (void)B;
     const int rows = T * (n_head / n_kv), rt = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
-    return 65536 + (size_t)2 * tree_sms() * 2 * tree_part_floats(rt, hd) * sizeof(float);
+    return 65536 + (size_t)2 * tree_sms() * 2 * tree_part_floats(rt, hd) * sizeof(float);  // wide: half the CTAs, twice the rows
 }
 
 static cudaError_t tree_launch(const void* fn, dim3 grid, int threads, size_t smem, void** args, cudaStream_t st, bool pdl) {
@@ -725,6 +1388,7 @@ static cudaError_t narrow_launch(const TreeAttnArgs& a, cudaStream_t st, bool pd
     pl.grid = 2 * tree_sms();
     pl.rt = F::RT;
     pl.pt = F::PT;
+    pl.maps = 0;
     pl.min_tiles = 2;
     TreeAttnArgs aa = a;
     void* args[] = {&aa, &pl};
@@ -733,11 +1397,66 @@ static cudaError_t narrow_launch(const TreeAttnArgs& a, cudaStream_t st, bool pd
     return tree_launch((const void*)tf_tree_combine_kernel, dim3(pl.grid, F::RT / (TC_THREADS / 32)), TC_THREADS, 0, args, st, true);
 }
 
+// The f16 cache as a 2-D tensor map: rows of hd halves, boxes of `pt` rows x 64 halves with the
+// 128-byte swizzle (one 64-dim block of an operand tile).
+static bool tree_map(CUtensorMap* m, const TreeAttnArgs& a, const void* base, int pt) {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> enc{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 f = enc.load();
+    if (!f) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return false;
+        f = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+        enc.store(f);
+    }
+    if (a.slot_stride % a.hd || a.hd % 64) return false;
+    const long long rows = a.slot_stride / a.hd * a.n_slots;
+    if (rows > 0x7FFFFFFFll) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.hd, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.hd * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)pt};
+    const cuuint32_t es[2] = {1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void*>(base), dims, strides, box, es,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int HD, int KVT>
+static cudaError_t wide_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
+    using F = WideCfg<HD, KVT>;
+    const void* fn = (const void*)tf_tree_attn_wide_kernel<HD, KVT>;
+    static std::atomic<bool> ready[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (!ready[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
+        if (e != cudaSuccess) return e;
+        ready[dev].store(true);
+    }
+    TreePlan pl;
+    pl.grid = tree_sms();
+    pl.rt = TW_RT;
+    pl.pt = F::PT;
+    pl.min_tiles = 2;
+    alignas(64) CUtensorMap maps[2];
+    memset(maps, 0, sizeof(maps));
+    pl.maps = KVT == KV_F16 && a.hd == HD && tree_map(&maps[0], a, a.kc, F::PT) && tree_map(&maps[1], a, a.vc, F::PT);
+    TreeAttnArgs aa = a;
+    void* args[] = {&aa, &pl, &maps[0], &maps[1]};
+    cudaError_t e = tree_launch(fn, dim3(pl.grid), TW_THREADS, F::SMEM, args, st, pdl);
+    if (e != cudaSuccess) return e;
+    return tree_launch((const void*)tf_tree_combine_kernel, dim3(pl.grid, TW_RT / (TC_THREADS / 32)), TC_THREADS, 0, args, st, true);
+}
+
 template <int HD, int KVT>
 static cudaError_t narrow_rows(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
     const int rows = a.T * (a.n_head / a.n_kv);
     if (rows <= 16) return narrow_launch<HD, 1, KVT>(a, st, pdl);
     if (rows <= 32) return narrow_launch<HD, 2, KVT>(a, st, pdl);
+    if (rows > 64) return wide_launch<HD, KVT>(a, st, pdl);
     return narrow_launch<HD, 4, KVT>(a, st, pdl);
 }
 template <int HD>
