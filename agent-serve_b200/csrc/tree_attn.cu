@@ -32,10 +32,12 @@ constexpr float kPShift = 15.f;       // p is held as 2^15 exp(s - max): its low
 
 // ---- the split of the tiles over the CTAs ---------------------------------------------------------
 struct TreePlan {
-    int maps;                // wide kernel, f16 cache: the tensor maps are valid
+    int maps;                // wide kernel, 16-bit cache: the tensor maps are valid
+    int slot_rows;           // rows of the tensor maps per slot
     int grid;                // CTAs of the main kernel
     int rt;                  // rows per row tile
-    int pt;                  // positions per tile
+    int rep;                 // query heads per kv head
+    int rep_inv;             // (x * rep_inv) >> 16 = x / rep for x < 2048 and rep <= 8
     int min_tiles;           // tiles per CTA at least
 };
 struct TreeDesc {            // a unit split over CTAs c0..c1, found at slot c0
@@ -58,33 +60,43 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeAttnArgs& a, int b) {
     return s;
 }
 // tiles of one unit of the sequence, and its units
-__device__ __forceinline__ int seq_tiles(const TreeSeq& s, int pt) {
-    return s.n_node ? (s.n_ctx + s.n_node + pt - 1) / pt : 0;
+template <int PT>
+__device__ __forceinline__ int seq_tiles(const TreeSeq& s) {
+    return s.n_node ? (unsigned)(s.n_ctx + s.n_node + PT - 1) / PT : 0;
 }
-__device__ __forceinline__ int seq_units(const TreeAttnArgs& a, const TreeSeq& s, int rt) {
-    return a.n_kv * ((s.n_node * (a.n_head / a.n_kv) + rt - 1) / rt);
+template <int RT>
+__device__ __forceinline__ int seq_units(int n_kv, int rep, const TreeSeq& s) {
+    return n_kv * ((unsigned)(s.n_node * rep + RT - 1) / RT);
 }
 
-// This CTA's range of tiles [g0, g1): the sequence it starts in, and the global index of that
-// sequence's first tile.  Block-wide; NT threads.
-template <int NT>
-__device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan& pl, long long& g0, long long& g1,
-                                           long long& per, int& b0, long long& base0) {
-    __shared__ long long wsum[NT / 32];
-    __shared__ long long found_base;
-    __shared__ int found_b;
+// A CTA's place in its range of tiles [g0, g1): the sequence it is in and the global index of
+// that sequence's first tile.  (32 bits: a call has fewer than 2^31 tiles, tree_attn_launch.)
+struct TreeIter {
+    int g0, g1, per, base, b;
+};
+// The next piece of the range: tiles [t0, t1) of one unit.
+struct TreeSeg {
+    TreeSeq s;
+    int b, kvh, rtile, t0, t1, tiles, last_cta;  // last_cta: the CTA that ends the unit
+};
+
+// Finds this CTA's range.  Block-wide; NT threads.
+template <int NT, int PT, int RT>
+__device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan& pl, TreeIter& it) {
+    __shared__ int wsum[NT / 32], found_base, found_b;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int chunk = (a.B + NT - 1) / NT, lo = min(a.B, tid * chunk), hi = min(a.B, lo + chunk);
-    long long mine = 0;
+    int mine = 0;
+#pragma unroll 1
     for (int b = lo; b < hi; ++b) {
         const TreeSeq s = tree_seq(a, b);
-        mine += (long long)seq_tiles(s, pl.pt) * seq_units(a, s, pl.rt);
+        mine += seq_tiles<PT>(s) * seq_units<RT>(a.n_kv, pl.rep, s);
         if (s.bad && blockIdx.x == 0) atomicCAS(a.err, 0, ERR_POS);
     }
-    long long inc = mine;
-#pragma unroll
+    int inc = mine;
+#pragma unroll 1
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+        const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
         if (lane >= o) inc += v;
     }
     if (lane == 31) wsum[warp] = inc;
@@ -93,20 +105,22 @@ __device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan
         found_base = 0;
     }
     __syncthreads();
-    long long before = inc - mine, total = 0;
+    int before = inc - mine, total = 0;
+#pragma unroll 1
     for (int w = 0; w < NT / 32; ++w) {
         if (w < warp) before += wsum[w];
         total += wsum[w];
     }
-    per = (total + pl.grid - 1) / pl.grid;
-    if (per < pl.min_tiles) per = pl.min_tiles;
-    g0 = per * blockIdx.x;
-    g1 = g0 + per < total ? g0 + per : total;
-    if (g0 >= before && g0 < before + mine) {
+    it.per = (unsigned)(total + pl.grid - 1) / (unsigned)pl.grid;
+    if (it.per < pl.min_tiles) it.per = pl.min_tiles;
+    it.g0 = (int)min((long long)it.per * blockIdx.x, (long long)total);
+    it.g1 = min(it.g0 + it.per, total);
+    if (it.g0 >= before && it.g0 < before + mine) {
+#pragma unroll 1
         for (int b = lo; b < hi; ++b) {
             const TreeSeq s = tree_seq(a, b);
-            const long long t = (long long)seq_tiles(s, pl.pt) * seq_units(a, s, pl.rt);
-            if (g0 < before + t) {
+            const int t = seq_tiles<PT>(s) * seq_units<RT>(a.n_kv, pl.rep, s);
+            if (it.g0 < before + t) {
                 found_b = b;
                 found_base = before;
                 break;
@@ -115,36 +129,32 @@ __device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan
         }
     }
     __syncthreads();
-    b0 = found_b;
-    base0 = found_base;
+    it.b = found_b;
+    it.base = found_base;
 }
 
-// The next piece of this CTA's range [g0, g1): tiles [t0, t1) of one unit.
-struct TreeSeg {
-    TreeSeq s;
-    int b, kvh, rtile, t0, t1, tiles, last_cta;  // last_cta: the CTA that ends the unit
-};
-__device__ __forceinline__ bool tree_next(const TreeAttnArgs& a, const TreePlan& pl, long long& g0, long long g1,
-                                          long long per, int& b, long long& base, TreeSeg& o) {
-    if (g0 >= g1) return false;
-    o.s = tree_seq(a, b);
-    o.tiles = seq_tiles(o.s, pl.pt);
-    int units = seq_units(a, o.s, pl.rt);
-    while (g0 >= base + (long long)o.tiles * units) {  // next sequence with work
-        base += (long long)o.tiles * units;
-        o.s = tree_seq(a, ++b);
-        o.tiles = seq_tiles(o.s, pl.pt);
-        units = seq_units(a, o.s, pl.rt);
+template <int PT, int RT>
+__device__ __forceinline__ bool tree_next(const TreeAttnArgs& a, int rep, TreeIter& it, TreeSeg& o) {
+    if (it.g0 >= it.g1) return false;
+    o.s = tree_seq(a, it.b);
+    o.tiles = seq_tiles<PT>(o.s);
+    int units = seq_units<RT>(a.n_kv, rep, o.s);
+#pragma unroll 1
+    while (it.g0 >= it.base + o.tiles * units) {  // next sequence with work
+        it.base += o.tiles * units;
+        o.s = tree_seq(a, ++it.b);
+        o.tiles = seq_tiles<PT>(o.s);
+        units = seq_units<RT>(a.n_kv, rep, o.s);
     }
-    const int unit = (int)((g0 - base) / o.tiles), nrt = units / a.n_kv;
-    const long long u0 = base + (long long)unit * o.tiles;  // the unit's first tile
-    o.b = b;
-    o.kvh = unit / nrt;
-    o.rtile = unit % nrt;
-    o.t0 = (int)(g0 - u0);
-    o.t1 = (int)(g1 - u0 < o.tiles ? g1 - u0 : o.tiles);
-    o.last_cta = (int)((u0 + o.tiles - 1) / per);
-    g0 = u0 + o.t1;
+    const int unit = (unsigned)(it.g0 - it.base) / (unsigned)o.tiles, nrt = (unsigned)(o.s.n_node * rep + RT - 1) / RT;
+    const int u0 = it.base + unit * o.tiles;  // the unit's first tile
+    o.b = it.b;
+    o.kvh = (unsigned)unit / (unsigned)nrt;
+    o.rtile = unit - o.kvh * nrt;
+    o.t0 = it.g0 - u0;
+    o.t1 = min(it.g1 - u0, o.tiles);
+    o.last_cta = (unsigned)(u0 + o.tiles - 1) / (unsigned)it.per;
+    it.g0 = u0 + o.t1;
     return true;
 }
 
@@ -152,30 +162,84 @@ __device__ __forceinline__ bool tree_next(const TreeAttnArgs& a, const TreePlan&
 template <int NT>
 __device__ __forceinline__ void tree_zero_rows(const TreeAttnArgs& a) {
     const int n4 = a.n_head * a.hd / 4, per = NT / 32;
+#pragma unroll 1
     for (long long r = (long long)blockIdx.x * per + (threadIdx.x >> 5); r < (long long)a.B * a.T; r += (long long)gridDim.x * per) {
         const TreeSeq s = tree_seq(a, (int)(r / a.T));
         if ((int)(r % a.T) < s.n_node) continue;
         float4* o = reinterpret_cast<float4*>(a.out + r * a.ld_out);
+#pragma unroll 1
         for (int i = threadIdx.x & 31; i < n4; i += 32) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     }
 }
 
-// Visibility to `node` of the 32 positions from drafted index x0 on (negative: committed
-// context, always seen); nothing from n_node on.
-__device__ __forceinline__ uint32_t tree_window(const TreeAttnArgs& a, const TreeSeq& s, int b, int node, int x0) {
-    auto word = [&](int w) -> unsigned long long {  // nodes 64 w .. 64 w + 63
-        if (w < 0) return ~0ull;
-        if (64 * w >= s.n_node || node >= s.n_node) return 0ull;
-        unsigned long long v;
-        if (a.mask) v = a.mask[((size_t)b * a.T + node) * ((a.T + 63) / 64) + w];
-        else v = 64 * w > node ? 0ull : (node - 64 * w >= 63 ? ~0ull : (2ull << (node - 64 * w)) - 1);
-        const int left = s.n_node - 64 * w;
-        return left >= 64 ? v : v & ((1ull << left) - 1);
-    };
+// What a row sees of the drafted nodes, as 32-bit words in shared memory: words 1 .. 8 hold nodes
+// 0 .. 255 (none from n_node on), word 0 all ones for the committed positions before them, word 9
+// zero for what lies behind.
+constexpr int VIS_WORDS = TREE_MAX_NODES / 32 + 2;
+__device__ __forceinline__ void vis_fill(uint32_t* vis, const TreeAttnArgs& a, const TreeSeq& s, int b, int node) {
+    vis[0] = 0xFFFFFFFFu;
+    vis[VIS_WORDS - 1] = 0;
+    const uint32_t* mw = a.mask ? reinterpret_cast<const uint32_t*>(a.mask + ((size_t)b * a.T + node) * ((a.T + 63) / 64)) : nullptr;
+#pragma unroll 1
+    for (int w = 0; w < TREE_MAX_NODES / 32; ++w) {
+        uint32_t v = 0;
+        const int left = s.n_node - 32 * w;
+        if (left > 0 && node < s.n_node) {
+            if (mw) v = mw[w];
+            else v = node < 32 * w ? 0u : (node - 32 * w >= 31 ? 0xFFFFFFFFu : (2u << (node - 32 * w)) - 1);
+            if (left < 32) v &= (1u << left) - 1;
+        }
+        vis[w + 1] = v;
+    }
+}
+// the 32 positions from drafted index x0 on (negative: committed)
+__device__ __forceinline__ uint32_t vis_window(const uint32_t* vis, int x0) {
     if (x0 <= -32) return 0xFFFFFFFFu;
-    const int w = x0 >> 6, sh = x0 & 63;
-    const unsigned long long lo = word(w) >> sh;
-    return (uint32_t)(sh > 32 ? lo | (word(w + 1) << (64 - sh)) : lo);
+    const int w = min((x0 >> 5) + 1, VIS_WORDS - 2);
+    return x0 >= TREE_MAX_NODES ? 0u : __funnelshift_r(vis[w], vis[w + 1], x0 & 31);
+}
+
+// Bounded wait on an mbarrier phase with the hardware's own suspension (up to 20 us a try, 2^16
+// tries); false after a timeout, or when another thread of the block gave up.
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, int parity, int* err, int code, volatile int* abort) {
+#pragma unroll 1
+    for (int i = 0; i < 65536; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 20000;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity & 1)
+            : "memory");
+        if (ok) return true;
+        if (abort && *abort) return false;
+    }
+    atomicCAS(err, 0, code);
+    if (abort) *abort = 1;
+    return false;
+}
+
+// Takes the non-finite values of drafted rows, which the operands hold as zeros, up in the rows
+// that see them: adds them to what has been written of the segment's rows (after a barrier).
+template <int KVT>
+__device__ __forceinline__ void tree_fix_rows(const TreeAttnArgs& a, const TreeSeg& sg, int rt, int rep, const unsigned* badrow,
+                                           const uint32_t* vis, float* part, bool whole, int tid, int threads) {
+    const int hd = a.hd, rows = sg.s.n_node * rep;
+#pragma unroll 1
+    for (int i = tid; i < rt * hd; i += threads) {
+        const int r = i / hd, d = i - r * hd, rr = sg.rtile * rt + r, node = rr / rep;
+        if (rr >= rows) return;
+        float* dst = whole ? a.out + ((size_t)sg.b * a.T + node) * a.ld_out + (size_t)(sg.kvh * rep + rr - node * rep) * hd + d : part + i;
+#pragma unroll 1
+        for (int w = 0; w < TREE_MAX_NODES / 32; ++w)
+#pragma unroll 1
+            for (unsigned bits = badrow[w] & vis[r * VIS_WORDS + w + 1]; bits; bits &= bits - 1) {
+                const float v = kv_load(a.vc, (long long)sg.s.slot * a.slot_stride +
+                                                  ((long long)sg.kvh * a.cap + sg.s.n_ctx + 32 * w + __ffs(bits) - 1) * hd + d, KVT);
+                if (!(fabsf(v) < INFINITY)) *dst += v;
+            }
+    }
 }
 
 // ---- small pieces ---------------------------------------------------------------------------------
@@ -200,14 +264,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-// two values into their high halves (packed) and what the halves leave
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    hi = pack_half2(x, y);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    lo = pack_half2(x - f.x, y - f.y);
-}
-// the same by truncation: the high half keeps 10 bits behind the first (exact in f16 from 2^-14
-// on), the low half the rest
+// Two values in halves: the high one by truncation, 10 bits behind the first (exact in f16 from
+// 2^-14 on), the low one the rest.
 __device__ __forceinline__ void split2t(float2 x, uint32_t& hi, uint32_t& lo) {
     const float2 h = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(x.y) & 0xFFFFE000u));
     const float2 l = __fadd2_rn(x, make_float2(-h.x, -h.y));
@@ -255,6 +313,28 @@ __device__ __forceinline__ uint32_t max_bits(const uint4& x) {
     }
     return m;
 }
+// |x| of a vector's largest value, as fp32 bits (fp32 or bf16; 0x7F800000 and more: not all finite)
+template <int KVT>
+__device__ __forceinline__ uint32_t abs_bits(const uint4& x) {
+    if (KVT == KV_F32) {
+        const uint32_t m = 0x7FFFFFFFu;
+        return max(max(x.x & m, x.y & m), max(x.z & m, x.w & m));
+    }
+    const uint32_t m = 0x7FFF7FFFu;
+    const uint32_t v = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
+    return max(v << 16, v & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t finite_max4(const float4& x) {
+    return max(max(finite_abs_bits(x.x), finite_abs_bits(x.y)), max(finite_abs_bits(x.z), finite_abs_bits(x.w)));
+}
+// eight values times f in two halves
+__device__ __forceinline__ void split8(const float4& x, const float4& y, float f, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+    const float2 g = make_float2(f, f);
+    split2t(__fmul2_rn(make_float2(x.x, x.y), g), hi[0], lo[0]);
+    split2t(__fmul2_rn(make_float2(x.z, x.w), g), hi[1], lo[1]);
+    split2t(__fmul2_rn(make_float2(y.x, y.y), g), hi[2], lo[2]);
+    split2t(__fmul2_rn(make_float2(y.z, y.w), g), hi[3], lo[3]);
+}
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -299,19 +379,22 @@ struct NarrowCfg {
 };
 
 template <int HD, int MT, int KVT>
-__global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(const TreeAttnArgs a, const TreePlan pl) {
+__global__ void __launch_bounds__(TN_THREADS, 2)
+    tf_tree_attn_narrow_kernel(const __grid_constant__ TreeAttnArgs a, const __grid_constant__ TreePlan pl) {
     using F = NarrowCfg<HD, MT, KVT>;
     constexpr int PT = F::PT, RT = F::RT, NG = F::NG, PB = F::PB, NLO = F::NLO, ESZ = F::ESZ;
     constexpr int VEC = 16 / ESZ, VPR = HD / VEC, NV = TN_TILE_BYTES / 2 / 16 / TN_THREADS;  // vectors: elements, per row, per thread
+    constexpr uint32_t HALF_TILE = TN_TILE_BYTES / 2;
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ float qscale[RT];
-    __shared__ unsigned tmax[4];        // maxima of K, V (bits) of this tile and the next
+    __shared__ uint32_t vis[RT][VIS_WORDS];
+    __shared__ unsigned tmax[4];                      // maxima of K, V (bits) of this tile and the next
     __shared__ unsigned badrow[TREE_MAX_NODES / 32];  // drafted rows of the unit with non-finite values
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int rep = a.n_head / a.n_kv, hd = a.hd;
+    const int rep = pl.rep, hd = a.hd;
     const uint32_t sb = smem_u32(smem);
     const uint32_t qh = sb + 2 * TN_TILE_BYTES, ql = qh + F::Q_BYTES;
-    const int rep_inv = (65536 + rep - 1) / rep;  // row / rep for rows < 2048 and rep <= 8
+    const int rep_inv = pl.rep_inv;
     auto div_rep = [&](int x) { return (x * rep_inv) >> 16; };
     const int wm = warp % MT, wg = warp / MT;  // row block, position group
     const bool active = wg < NG;
@@ -321,15 +404,14 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
     pdl_wait();
     TreeDesc* desc = static_cast<TreeDesc*>(a.ws);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + 65536);
-    long long g0, g1, per, base;
-    int b;
-    tree_range<TN_THREADS>(a, pl, g0, g1, per, b, base);
+    TreeIter it;
+    tree_range<TN_THREADS, PT, RT>(a, pl, it);
     if (tid == 0) desc[blockIdx.x].b = -1;
 
     TreeSeg sg;
-    while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+    while (tree_next<PT, RT>(a, rep, it, sg)) {
         const TreeSeq s = sg.s;
-        const int kvh = sg.kvh, rtile = sg.rtile, t0 = sg.t0, t1 = sg.t1;
+        const int b = sg.b, kvh = sg.kvh, rtile = sg.rtile, t0 = sg.t0, t1 = sg.t1;
         const int end = s.n_ctx + s.n_node, rows = s.n_node * rep;
         const size_t off = (size_t)s.slot * a.slot_stride + (size_t)kvh * a.cap * hd;
         const uint8_t* kp = static_cast<const uint8_t*>(a.kc) + off * ESZ;
@@ -337,48 +419,44 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
 
         // tile t into its buffer: vector v = tid + i * threads of the PT x HD tile, K then V
         // (f16: at its operand place, the buffers alternating; else in the order of the threads)
-        auto place = [&](int t, int i) -> uint32_t {
-            const int v = tid + i * TN_THREADS, r = v / VPR, c = v % VPR;
-            if (KVT != KV_F16) return sb + 16u * v;
-            return sb + (uint32_t)(t & 1) * TN_TILE_BYTES + (uint32_t)r * (HD * 2) + (((uint32_t)c ^ (r & 7)) << 4);
-        };
+        const int r0 = tid / VPR, c0 = tid % VPR;
+        constexpr int RSTEP = TN_THREADS / VPR;  // a multiple of 8: chunk c0 stays at c0 ^ (r0 & 7)
+        const uint32_t own = KVT == KV_F16 ? sb + (uint32_t)r0 * (HD * 2) + (uint32_t)((c0 ^ (r0 & 7)) << 4) : sb + 16u * tid;
+        constexpr uint32_t OSTEP = KVT == KV_F16 ? RSTEP * HD * 2 : 16 * TN_THREADS;
         auto load = [&](int t) {
+            const uint32_t o = own + (KVT == KV_F16 ? (uint32_t)(t & 1) * TN_TILE_BYTES : 0u);
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int v = tid + i * TN_THREADS, p = t * PT + v / VPR, c = (v % VPR) * VEC;
-                const bool in = p < end && c < hd;
-                const size_t e = in ? ((size_t)p * hd + c) * ESZ : 0;
-                const uint32_t o = place(t, i);
-                cp_async16(o, kp + e, in);
-                cp_async16(o + TN_TILE_BYTES / 2, vp + e, in);
+                const int p = t * PT + r0 + i * RSTEP;
+                const bool in = p < end && c0 * VEC < hd;
+                const size_t e = in ? ((size_t)p * hd + c0 * VEC) * ESZ : 0;
+                cp_async16(o + i * OSTEP, kp + e, in);
+                cp_async16(o + i * OSTEP + HALF_TILE, vp + e, in);
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         load(t0);
-        // the rows' queries, TPR threads per row: scaled to [2^14, 2^15), two halves
+        // the rows' queries, TPR threads per row: scaled to [2^14, 2^15), two halves; what they see
         {
             constexpr int TPR = TN_THREADS / RT < HD / 8 ? TN_THREADS / RT : HD / 8, UPT = HD / 8 / TPR;  // 8-dim units per thread
             const int r = tid / TPR, rr = rtile * RT + r, j0 = tid % TPR;
             if (r < RT) {
-                float x[UPT][8];
+                float4 x[UPT][2];
                 uint32_t mb = 0;
                 const int node = div_rep(rr);
                 const float* qp = a.q + ((size_t)b * a.T + node) * a.ld_q + (size_t)(kvh * rep + rr - node * rep) * hd;
 #pragma unroll
                 for (int i = 0; i < UPT; ++i) {
                     const int d = (j0 + i * TPR) * 8;
-                    float4 y = make_float4(0.f, 0.f, 0.f, 0.f), z = y;
+                    x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (rr < rows && d < hd) {
-                        y = *reinterpret_cast<const float4*>(qp + d);
-                        z = *reinterpret_cast<const float4*>(qp + d + 4);
+                        x[i][0] = *reinterpret_cast<const float4*>(qp + d);
+                        x[i][1] = *reinterpret_cast<const float4*>(qp + d + 4);
                     }
-                    x[i][0] = y.x, x[i][1] = y.y, x[i][2] = y.z, x[i][3] = y.w;
-                    x[i][4] = z.x, x[i][5] = z.y, x[i][6] = z.z, x[i][7] = z.w;
                 }
+                if (j0 == 0) vis_fill(vis[r], a, s, b, node);
 #pragma unroll
-                for (int i = 0; i < UPT; ++i)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) mb = max(mb, finite_abs_bits(x[i][j]));
+                for (int i = 0; i < UPT; ++i) mb = max(mb, max(finite_max4(x[i][0]), finite_max4(x[i][1])));
 #pragma unroll
                 for (int o = 1; o < TPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
                 const int e = half_exponent(mb);
@@ -386,8 +464,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
 #pragma unroll
                 for (int i = 0; i < UPT; ++i) {
                     uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) split2(x[i][2 * j] * sc, x[i][2 * j + 1] * sc, hi[j], lo[j]);
+                    split8(x[i][0], x[i][1], sc, hi, lo);
                     const uint32_t c = (uint32_t)(j0 + i * TPR);
                     const uint32_t o = (uint32_t)r * (HD * 2) + ((c ^ (r & 7)) << 4);
                     st_shared16(qh + o, hi);
@@ -404,55 +481,58 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
 #pragma unroll
         for (int i = 0; i < HD / 8; ++i) O[i][0] = O[i][1] = O[i][2] = O[i][3] = 0.f;
 
+#pragma unroll 1
         for (int t = t0; t < t1; ++t) {
             int ek = 0, ev = 0;
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            // non-finite values of drafted rows leave the V tile (another row's zero weight
-            // must not meet them); rows that see them take them up at the end
             const bool tail = (t + 1) * PT > s.n_ctx;
-            uint32_t kh = sb + (KVT == KV_F16 ? (uint32_t)(t & 1) * TN_TILE_BYTES : TN_TILE_BYTES), vh = kh + TN_TILE_BYTES / 2;
-            uint32_t mk = 0, mv = 0;
-            if (KVT != KV_F16 || tail) {
-#pragma unroll
+            const uint32_t kh = sb + (KVT == KV_F16 ? (uint32_t)(t & 1) * TN_TILE_BYTES : TN_TILE_BYTES), vh = kh + HALF_TILE;
+            const uint32_t mine = KVT == KV_F16 ? own + (uint32_t)(t & 1) * TN_TILE_BYTES : own;
+            if (tail) {
+                // non-finite values of drafted rows leave the V tile (another row's zero weight
+                // must not meet them); rows that see them take them up at the end
+#pragma unroll 1
                 for (int i = 0; i < NV; ++i) {
-                    const uint32_t o = place(t, i) + TN_TILE_BYTES / 2;
-                    uint4 x = ld_shared16(o);
-                    const int p = t * PT + (tid + i * TN_THREADS) / VPR;
-                    if (tail && p >= s.n_ctx && zero_nonfinite<KVT>(x)) {
-                        atomicOr(&badrow[(p - s.n_ctx) >> 5], 1u << ((p - s.n_ctx) & 31));
-                        st_shared16(o, {x.x, x.y, x.z, x.w});
-                    }
-                    if (KVT != KV_F16) {
-                        mv = max(mv, max_bits<KVT>(x));
-                        mk = max(mk, max_bits<KVT>(ld_shared16(o - TN_TILE_BYTES / 2)));
+                    const uint32_t o = mine + i * OSTEP + HALF_TILE;
+                    const int x = t * PT + r0 + i * RSTEP - s.n_ctx;
+                    uint4 v = ld_shared16(o);
+                    if (x >= 0 && zero_nonfinite<KVT>(v)) {
+                        atomicOr(&badrow[x >> 5], 1u << (x & 31));
+                        st_shared16(o, {v.x, v.y, v.z, v.w});
                     }
                 }
             }
             if (KVT != KV_F16) {
-                mk = __reduce_max_sync(0xFFFFFFFFu, mk);
-                mv = __reduce_max_sync(0xFFFFFFFFu, mv);
-                if (lane == 0) {
-                    atomicMax(&tmax[2 * (t & 1)], mk);
-                    atomicMax(&tmax[2 * (t & 1) + 1], mv);
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    uint32_t mb = 0;
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) mb = max(mb, abs_bits<KVT>(ld_shared16(mine + i * OSTEP + which * HALF_TILE)));
+                    if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
+                        mb = 0;
+#pragma unroll 1
+                        for (int i = 0; i < NV; ++i) mb = max(mb, max_bits<KVT>(ld_shared16(mine + i * OSTEP + which * HALF_TILE)));
+                    }
+                    mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+                    if (lane == 0) atomicMax(&tmax[2 * (t & 1) + which], mb);
                 }
                 __syncthreads();  // the maxima; the last tile's operands are free
                 ek = half_exponent(tmax[2 * (t & 1)]);
                 ev = half_exponent(tmax[2 * (t & 1) + 1]);
                 if (tid < 2) tmax[2 * (~t & 1) + tid] = 0;  // the next tile's, last read a barrier ago
-                const float sk = pow2i(-ek), sv = pow2i(-ev);
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+                    const float f = pow2i(which ? -ev : -ek);
+                    const uint32_t dst = which ? vh : kh;
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int v = tid + i * TN_THREADS, r = v / VPR, c = v % VPR;
-#pragma unroll
-                    for (int which = 0; which < 2; ++which) {
-                        const uint4 x = ld_shared16(place(t, i) + which * (TN_TILE_BYTES / 2));
-                        const float f = which ? sv : sk;
-                        const uint32_t dst = which ? vh : kh;
+                    for (int i = 0; i < NV; ++i) {
+                        const int r = r0 + i * RSTEP;
+                        const uint4 x = ld_shared16(mine + i * OSTEP + which * HALF_TILE);
                         if (KVT == KV_F32) {
                             uint32_t h0, l0, h1, l1;
-                            split2(__uint_as_float(x.x) * f, __uint_as_float(x.y) * f, h0, l0);
-                            split2(__uint_as_float(x.z) * f, __uint_as_float(x.w) * f, h1, l1);
-                            const uint32_t o = dst + (uint32_t)r * (HD * 2) + ((((uint32_t)c >> 1) ^ (r & 7)) << 4) + (c & 1) * 8;
+                            split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), make_float2(f, f)), h0, l0);
+                            split2t(__fmul2_rn(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), make_float2(f, f)), h1, l1);
+                            const uint32_t o = dst + (uint32_t)r * (HD * 2) + ((((uint32_t)c0 >> 1) ^ (r & 7)) << 4) + (c0 & 1) * 8;
                             asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
                             asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::TILE_H), "r"(l0), "r"(l1) : "memory");
                         } else {
@@ -460,7 +540,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
                                 w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
-                            st_shared16(dst + (uint32_t)r * (HD * 2) + (((uint32_t)c ^ (r & 7)) << 4), w);
+                            st_shared16(dst + (uint32_t)r * (HD * 2) + (((uint32_t)c0 ^ (r & 7)) << 4), w);
                         }
                     }
                 }
@@ -478,64 +558,48 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
                 for (int i = 0; i < PB / 8; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) S[i][j] = S1[i][j] = 0.f;
-#pragma unroll
+                const int ra = wm * 16 + (lane & 15), ca = lane >> 4, rb = pl0 + (lane & 7) + ((lane >> 4) << 3), cb = (lane >> 3) & 1;
+                const uint32_t qrow = (uint32_t)ra * (HD * 2), krow = kh + (uint32_t)rb * (HD * 2);
+#pragma unroll 2
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     uint32_t ah[4], al[4];
-                    {
-                        const int r = wm * 16 + (lane & 15), c = 2 * kk + (lane >> 4);
-                        const uint32_t o = (uint32_t)r * (HD * 2) + (((uint32_t)c ^ (r & 7)) << 4);
-                        ldsm4(ah, qh + o);
-                        ldsm4(al, ql + o);
-                    }
+                    const uint32_t oa = qrow + (uint32_t)(((2 * kk + ca) ^ (ra & 7)) << 4);
+                    const uint32_t ob = krow + (uint32_t)(((2 * kk + cb) ^ (rb & 7)) << 4);
+                    ldsm4(ah, qh + oa);
+                    ldsm4(al, ql + oa);
 #pragma unroll
                     for (int nb = 0; nb < PB / 16; ++nb) {
-                        const int r = pl0 + nb * 16 + (lane & 7) + ((lane >> 4) << 3), c = 2 * kk + ((lane >> 3) & 1);
-                        const uint32_t o = kh + (uint32_t)r * (HD * 2) + (((uint32_t)c ^ (r & 7)) << 4);
                         uint32_t bh[4];
-                        ldsm4(bh, o);
+                        ldsm4(bh, ob + nb * 16 * HD * 2);
                         mma16816(S[2 * nb], ah, bh[0], bh[1]);
                         mma16816(S[2 * nb + 1], ah, bh[2], bh[3]);
                         mma16816(S1[2 * nb], al, bh[0], bh[1]);
                         mma16816(S1[2 * nb + 1], al, bh[2], bh[3]);
                         if (NLO == 2) {
                             uint32_t bl[4];
-                            ldsm4(bl, o + F::TILE_H);
+                            ldsm4(bl, ob + nb * 16 * HD * 2 + F::TILE_H);
                             mma16816(S1[2 * nb], ah, bl[0], bl[1]);
                             mma16816(S1[2 * nb + 1], ah, bl[2], bl[3]);
                         }
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < PB / 8; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) S[i][j] += S1[i][j];
                 // base-2 scores, masks, running maximum and sum of this thread's two rows
                 float alpha[2];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int r = wm * 16 + g8 + 8 * half;
                     const float f = qscale[r] * fk;
+                    // bit i: position i of the step is seen
+                    const uint32_t seen = (tail ? vis_window(vis[r], t * PT + pl0 - s.n_ctx) : 0xFFFFFFFFu) >> (2 * q4);
                     float mx = m[half];
-                    if (!tail) {
 #pragma unroll
-                        for (int i = 0; i < PB / 8; ++i)
+                    for (int i = 0; i < PB / 8; ++i)
 #pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                S[i][2 * half + j] *= f;
-                                mx = fmaxf(mx, S[i][2 * half + j]);
-                            }
-                    } else {
-                        // bit i of vis: position i of the step is seen
-                        const int node = div_rep(rtile * RT + r), x0 = t * PT + pl0 - s.n_ctx;
-                        const uint32_t vis = tree_window(a, s, b, node, x0);
-#pragma unroll
-                        for (int i = 0; i < PB / 8; ++i)
-#pragma unroll
-                            for (int j = 0; j < 2; ++j) {
-                                S[i][2 * half + j] = (vis >> (i * 8 + 2 * q4 + j)) & 1 ? S[i][2 * half + j] * f : -INFINITY;
-                                mx = fmaxf(mx, S[i][2 * half + j]);
-                            }
-                    }
+                        for (int j = 0; j < 2; ++j) {
+                            const float x = (S[i][2 * half + j] + S1[i][2 * half + j]) * f;
+                            S[i][2 * half + j] = (seen >> (i * 8 + j)) & 1 ? x : -INFINITY;
+                            mx = fmaxf(mx, S[i][2 * half + j]);
+                        }
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
                     const float ref = mx == -INFINITY ? 0.f : mx;
@@ -555,28 +619,27 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
                 // P in two halves (A operand), P V from zero, joined to the running output
                 uint32_t ph[PB / 16][4], pq[PB / 16][4];
 #pragma unroll
-                for (int i = 0; i < PB / 16; ++i) {
-                    split2(S[2 * i][0], S[2 * i][1], ph[i][0], pq[i][0]);
-                    split2(S[2 * i][2], S[2 * i][3], ph[i][1], pq[i][1]);
-                    split2(S[2 * i + 1][0], S[2 * i + 1][1], ph[i][2], pq[i][2]);
-                    split2(S[2 * i + 1][2], S[2 * i + 1][3], ph[i][3], pq[i][3]);
-                }
+                for (int i = 0; i < PB / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        split2t(make_float2(S[2 * i + (j >> 1)][2 * (j & 1)], S[2 * i + (j >> 1)][2 * (j & 1) + 1]), ph[i][j], pq[i][j]);
+                const int rv = pl0 + (lane & 15);
+                const uint32_t vrow = vh + (uint32_t)rv * (HD * 2);
 #pragma unroll
                 for (int db = 0; db < HD / 16; ++db) {
                     float d0[4] = {0.f, 0.f, 0.f, 0.f}, d1[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint32_t o = vrow + (uint32_t)(((2 * db + (lane >> 4)) ^ (rv & 7)) << 4);
 #pragma unroll
                     for (int i = 0; i < PB / 16; ++i) {
-                        const int r = pl0 + i * 16 + (lane & 15), c = 2 * db + (lane >> 4);
-                        const uint32_t o = vh + (uint32_t)r * (HD * 2) + (((uint32_t)c ^ (r & 7)) << 4);
                         uint32_t bh[4];
-                        ldsm4t(bh, o);
+                        ldsm4t(bh, o + i * 16 * HD * 2);
                         mma16816(d0, ph[i], bh[0], bh[1]);
                         mma16816(d1, ph[i], bh[2], bh[3]);
                         mma16816(d0, pq[i], bh[0], bh[1]);
                         mma16816(d1, pq[i], bh[2], bh[3]);
                         if (NLO == 2) {
                             uint32_t bl[4];
-                            ldsm4t(bl, o + F::TILE_H);
+                            ldsm4t(bl, o + i * 16 * HD * 2 + F::TILE_H);
                             mma16816(d0, ph[i], bl[0], bl[1]);
                             mma16816(d1, ph[i], bl[2], bl[3]);
                         }
@@ -610,45 +673,34 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
         const int anybad = __syncthreads_or(tid < TREE_MAX_NODES / 32 ? badrow[tid] != 0 : 0);
         const bool whole = t0 == 0 && t1 == sg.tiles;
         float* part = parts + ((size_t)blockIdx.x * 2 + (t0 == 0 ? 1 : 0)) * tree_part_floats(RT, hd);
+#pragma unroll 1
         for (int i = tid; i < RT * (HD / 4); i += TN_THREADS) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4, rr = rtile * RT + r;
             if (rr >= rows || d >= hd) continue;
+            const float* fr = fin + (size_t)r * (HD + 4);
             float M = -INFINITY;
 #pragma unroll
-            for (int g = 0; g < NG; ++g) M = fmaxf(M, fin[((size_t)g * RT + r) * (HD + 4) + HD]);
+            for (int g = 0; g < NG; ++g) M = fmaxf(M, fr[(size_t)g * RT * (HD + 4) + HD]);
             const float ref = M == -INFINITY ? 0.f : M;
             float L = 0.f;
             float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const float* fr = fin + ((size_t)g * RT + r) * (HD + 4);
-                const float w = exp2_fast(fr[HD] - ref);
-                const float4 x = *reinterpret_cast<const float4*>(fr + d);
-                L = fmaf(fr[HD + 1], w, L);
+                const float* fg = fr + (size_t)g * RT * (HD + 4);
+                const float w = exp2_fast(fg[HD] - ref);
+                const float4 x = *reinterpret_cast<const float4*>(fg + d);
+                L = fmaf(fg[HD + 1], w, L);
                 o.x = fmaf(x.x, w, o.x);
                 o.y = fmaf(x.y, w, o.y);
                 o.z = fmaf(x.z, w, o.z);
                 o.w = fmaf(x.w, w, o.w);
             }
             const int node = div_rep(rr);
-            for (int w = 0; w < TREE_MAX_NODES / 32 && anybad; ++w)  // non-finite drafted values that the row sees
-                for (unsigned bits = badrow[w]; bits; bits &= bits - 1) {
-                    const int x = w * 32 + __ffs(bits) - 1;
-                    const bool vis = a.mask ? (a.mask[((size_t)b * a.T + node) * ((a.T + 63) / 64) + (x >> 6)] >> (x & 63)) & 1 : x <= node;
-                    if (!vis) continue;
-                    float* oo = &o.x;
-                    for (int j = 0; j < 4; ++j) {
-                        const float v = kv_load(a.vc, (long long)off + (long long)(s.n_ctx + x) * hd + d + j, KVT);
-                        if (!(fabsf(v) < INFINITY)) oo[j] += v;
-                    }
-                }
             if (whole) {
                 const float inv = L == 0.f ? 0.f : 1.f / L;
-                o.x = L == 0.f ? 0.f : o.x * inv;
-                o.y = L == 0.f ? 0.f : o.y * inv;
-                o.z = L == 0.f ? 0.f : o.z * inv;
-                o.w = L == 0.f ? 0.f : o.w * inv;
-                *reinterpret_cast<float4*>(a.out + ((size_t)b * a.T + node) * a.ld_out + (size_t)(kvh * rep + rr - node * rep) * hd + d) = o;
+                float4 y = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+                if (L == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                *reinterpret_cast<float4*>(a.out + ((size_t)b * a.T + node) * a.ld_out + (size_t)(kvh * rep + rr - node * rep) * hd + d) = y;
             } else {
                 *reinterpret_cast<float4*>(part + (size_t)r * hd + d) = o;
                 if (d == 0) {
@@ -660,6 +712,10 @@ __global__ void __launch_bounds__(TN_THREADS, 2) tf_tree_attn_narrow_kernel(cons
         if (!whole && t0 == 0 && tid == 0)
             desc[blockIdx.x] = TreeDesc{b, kvh, rtile, sg.last_cta};
         __syncthreads();
+        if (anybad) {
+            tree_fix_rows<KVT>(a, sg, RT, rep, badrow, &vis[0][0], part, whole, tid, TN_THREADS);
+            __syncthreads();
+        }
     }
     tree_zero_rows<TN_THREADS>(a);
 }
@@ -688,19 +744,20 @@ struct WideCfg {
     static constexpr int PT = KVT == KV_F32 && HD == 128 ? 64 : 128;
     static constexpr int NLO = KVT == KV_F32 ? 2 : 1;
     static constexpr int HALF = PT * HD * 2;              // bytes of one half of a K or V tile
-    static constexpr int RAW = PT * HD * ESZ;             // bytes of a raw K or V tile
-    // operand stages, and raw buffers of one K or V tile each
-    static constexpr int OS = KVT == KV_F16 ? (HD == 64 ? 4 : 2) : (KVT == KV_BF16 && HD == 64 ? 2 : 1);
-    static constexpr int RS = HD == 64 ? (KVT == KV_F32 ? 3 : 4) : 2;
+    static constexpr int RAW = PT * HD * ESZ;             // bytes of a raw fp32 K or V tile
+    // operand stages of K and V, raw buffers (fp32)
+    static constexpr int KS = KVT == KV_F16 ? (HD == 64 ? 4 : 2) : (KVT == KV_BF16 ? (HD == 64 ? 4 : 2) : 1);
+    static constexpr int VS = KVT == KV_F32 ? (HD == 64 ? 2 : 1) : KS;
+    static constexpr int RS = 2;
     static constexpr int QH = TW_RT * HD * 2;             // bytes of one half of Q
     static constexpr int Q_OFF = 0;
     static constexpr int K_OFF = 2 * QH;
-    static constexpr int V_OFF = K_OFF + OS * NLO * HALF;
-    static constexpr int RAW_OFF = V_OFF + OS * NLO * HALF;
-    static constexpr int SMEM = RAW_OFF + (KVT == KV_F16 ? 0 : RS * RAW) + 1024;
+    static constexpr int V_OFF = K_OFF + KS * NLO * HALF;
+    static constexpr int RAW_OFF = V_OFF + VS * NLO * HALF;
+    static constexpr int SMEM = RAW_OFF + (KVT == KV_F32 ? RS * RAW : 0) + 1024;
     // registers per thread of the softmax warpgroups and of the other two (512 in all, four
     // warpgroups of 128 at launch)
-    static constexpr int REG_S = HD == 64 ? 168 : 184, REG_L = HD == 64 ? 88 : 72;
+    static constexpr int REG_S = HD == 64 ? 144 : 192, REG_L = HD == 64 ? 112 : 64;
     static constexpr int CH = HD == 64 ? 32 : 16;         // score columns a softmax thread holds at a time
 };
 
@@ -772,258 +829,285 @@ __device__ __forceinline__ uint32_t wide_off(int rows, int r, int c) {
 }
 
 struct WideShared {
-    uint64_t rawfull[4], rawfree[4];              // raw tiles
-    uint64_t kfull[4], kfree[4], vfull[4], vfree[4];  // operand stages
-    uint64_t sfull[2], pfull[2], dfull[2], qfull, done;
+    // mbarriers, initialised in order by count()
+    uint64_t rawfull[8];                          // raw fp32 tiles, bf16 tiles in their operand stages
+    uint64_t kfree[4], vfree[4];                  // operand stages: their MMAs are done
+    uint64_t sfull[2], dfull[2], done;
+    uint64_t kfull[4], vfull[4], rawfree[2];      // one arrival per loader warp
+    uint64_t pfull[2], qfull;
+    static constexpr int N_BARS = 34;
+    __device__ static uint32_t count(int i) { return i < 21 ? 1 : (i < 31 ? TW_LOADERS : (i < 33 ? 128 : 256)); }
     uint32_t tmem;
     int abort;
     unsigned tmax[4];
-    int ek[4], ev[4];                             // scale exponents of the last four tiles
+    int ek[8], ev[8];                             // scale exponents of the last eight tiles
     unsigned badrow[8][TREE_MAX_NODES / 32];      // drafted rows with non-finite values, by segment
     float qscale[TW_RT];
     float2 ml[2][TW_RT];                          // the streams' row maxima and sums
+    uint32_t vis[256][VIS_WORDS];                 // what each softmax thread's row sees
 };
 
-// Exponent that puts a tile's maximum at 2^8: room for 2^7 more before f16 overflows, and 2^8
-// less before the low halves run out of exponents.
-__device__ __forceinline__ int tile_exponent(uint32_t maxbits) {
-    const int e = (int)(maxbits >> 23) - 127 - 8;
-    return e < -126 ? -126 : (e > 126 ? 126 : e);
+// Half h of a segment's rows from the two streams' staged halves: added, scaled by the row's
+// factor, written coalesced.
+template <int HD>
+__device__ __forceinline__ void wide_rows_out(const TreeAttnArgs& a, const TreeSeg& sg, uint32_t stage, const float2* scale,
+                                              bool whole, float* part, int h, int rep, int rep_inv, const volatile int* abort_flag) {
+    constexpr int LPR = HD / 8, RPW = 32 / LPR;  // lanes per half row, rows per warp and step
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % LPR, d = h * (HD / 2) + c * 4;
+    const int rows = sg.s.n_node * rep, hd = a.hd;
+#pragma unroll 2
+    for (int i = warp; i < TW_RT / RPW; i += 8) {
+        const int r = i * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
+        if (q >= rows || d >= hd || *abort_flag) continue;
+        const uint32_t at = stage + (uint32_t)r * (HD * 2) + ((uint32_t)(c ^ (r & 7)) << 4);
+        const uint4 x = ld_shared16(at), y = ld_shared16(at + TW_RT * HD * 2);
+        const float f = scale[r].x;
+        float4 o = make_float4(__uint_as_float(x.x) + __uint_as_float(y.x), __uint_as_float(x.y) + __uint_as_float(y.y),
+                               __uint_as_float(x.z) + __uint_as_float(y.z), __uint_as_float(x.w) + __uint_as_float(y.w));
+        // (a row that saw nothing has the factor 0 and zeros; its sum cannot be anything else)
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        float* dst = whole ? a.out + ((size_t)sg.b * a.T + nd) * a.ld_out + (size_t)(sg.kvh * rep + q - nd * rep) * hd
+                           : part + (size_t)r * hd;
+        *reinterpret_cast<float4*>(dst + d) = o;
+    }
+}
+__device__ __forceinline__ bool badrow_any(const unsigned* badrow) {
+    unsigned v = 0;
+#pragma unroll
+    for (int w = 0; w < TREE_MAX_NODES / 32; ++w) v |= badrow[w];
+    return v != 0;
 }
 
 template <int HD, int KVT>
-__global__ void __launch_bounds__(TW_THREADS, 1) tf_tree_attn_wide_kernel(const TreeAttnArgs a, const TreePlan pl,
-                                                                           const __grid_constant__ CUtensorMap kmap,
-                                                                           const __grid_constant__ CUtensorMap vmap) {
+__global__ void __launch_bounds__(TW_THREADS, 1)
+    tf_tree_attn_wide_kernel(const __grid_constant__ TreeAttnArgs a, const __grid_constant__ TreePlan pl,
+                             const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using F = WideCfg<HD, KVT>;
-    constexpr int PT = F::PT, NLO = F::NLO, ESZ = F::ESZ, OS = F::OS, RS = F::RS, CH = F::CH;
+    constexpr int PT = F::PT, NLO = F::NLO, ESZ = F::ESZ, KS = F::KS, VS = F::VS, RS = F::RS, CH = F::CH;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) WideShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
-    const int rep = a.n_head / a.n_kv, hd = a.hd;
+    const int rep = pl.rep, hd = a.hd;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sb = smem_u32(smem);
     volatile int* abort_flag = &sh.abort;
-    const int rep_inv = (65536 + rep - 1) / rep;  // row / rep for rows < 2048 and rep <= 8
+    const int rep_inv = pl.rep_inv;
 
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "r"(512u));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
     }
     if (tid == 32) {
-        for (int i = 0; i < 4; ++i) {
-            mbar_init(&sh.rawfull[i], 1);
-            mbar_init(&sh.rawfree[i], TW_LOADERS);
-            mbar_init(&sh.kfull[i], TW_LOADERS);
-            mbar_init(&sh.vfull[i], TW_LOADERS);
-            mbar_init(&sh.kfree[i], 1);
-            mbar_init(&sh.vfree[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.sfull[i], 1);
-            mbar_init(&sh.pfull[i], 128);
-            mbar_init(&sh.dfull[i], 1);
-        }
-        mbar_init(&sh.qfull, 256);
-        mbar_init(&sh.done, 1);
+#pragma unroll 1
+        for (int i = 0; i < WideShared::N_BARS; ++i) mbar_init(&sh.rawfull[i], WideShared::count(i));
         sh.abort = 0;
-        for (int i = 0; i < 4; ++i) sh.tmax[i] = 0;
         mbar_fence_init();
     }
+    if (tid < 4) sh.tmax[tid] = 0;
     pdl_trigger();
     pdl_wait();
     TreeDesc* desc = static_cast<TreeDesc*>(a.ws);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + 65536);
     if (tid == 0) desc[blockIdx.x].b = -1;
-    long long g0, g1, per, base;
-    int b;
+    TreeIter it;
     tc_fence_before();
-    tree_range<TW_THREADS>(a, pl, g0, g1, per, b, base);  // (block barriers inside)
+    tree_range<TW_THREADS, PT, TW_RT>(a, pl, it);  // (block barriers inside)
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     TreeSeg sg;
 
     // Every role walks the same segments and tiles; after an abort the waits return at once and
     // the roles run on without effect, so that all of them meet at every barrier.
-    // A tile that needs no work on its values (f16, all of it committed context) goes straight
-    // to its operand stage through the tensor maps.
-    auto direct = [&](const TreeSeg& g, int t) { return KVT == KV_F16 && pl.maps && (t + 1) * PT <= g.s.n_ctx; };
+    // A 16-bit tile of committed context comes straight to its operand stage through the tensor
+    // maps: f16 is done then, bf16 is converted in place.  The last tiles of a sequence (drafted
+    // rows, the end of the cache) are fetched by the loaders' own loads.
+    auto direct = [&](const TreeSeg& g, int t) { return KVT != KV_F32 && pl.maps && (t + 1) * PT <= g.s.n_ctx; };
+    auto tma_tile = [&](const TreeSeg& g, int t, int which, uint32_t off, uint64_t* bar) {
+        mbar_expect_tx(bar, F::HALF);
+        const int row = g.s.slot * pl.slot_rows + g.kvh * a.cap + t * PT;
+#pragma unroll
+        for (int c = 0; c < HD / 64; ++c)
+            asm volatile(
+                "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+                    sb + off + c * PT * 128),
+                "l"(reinterpret_cast<uint64_t>(which ? &vmap : &kmap)), "r"(64 * c), "r"(row), "r"(smem_u32(bar))
+                : "memory");
+    };
     if (wg >= 2) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F::REG_L));
     if (wg == 2 || warp >= 14) {
         constexpr int LT = TW_LOADERS * 32;
         const int lt = wg == 2 ? tid - 256 : tid - 320;
-        int n = 0, nr = 0, seg = 0;  // running tile, raw buffer and segment
-        int e2k = 0, e2v = 0;        // current exponents of K and V
-        while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+        int n = 0, nr = 0, nd = 0, seg = 0;  // running tile, raw buffer, direct tile, segment
+        constexpr int VPR = HD * ESZ / 16, RSTEP = LT / VPR;  // 16-byte vectors per row, rows per step of all loaders
+        constexpr int UNR = KVT == KV_F32 ? 4 : 2;
+        const int r0 = lt / VPR, c0 = lt % VPR;
+        while (tree_next<PT, TW_RT>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
-            const int end = s.n_ctx + s.n_node;
             if (lt < TREE_MAX_NODES / 32) sh.badrow[seg & 7][lt] = 0;  // read by others long ago
             named_bar<2, LT>();
+#pragma unroll 1
             for (int t = sg.t0; t < sg.t1; ++t, ++n) {
-                const int os = n % OS, rows = min(PT, end - t * PT);
+                const int rows = min(PT, s.n_ctx + s.n_node - t * PT);
+                const bool dir = direct(sg, t), tail = (t + 1) * PT > s.n_ctx;
 #pragma unroll 1
                 for (int which = 0; which < 2; ++which) {
+                    const int st = which ? VS : KS, os = n % st;
                     uint64_t* full = which ? &sh.vfull[os] : &sh.kfull[os];
                     uint64_t* free = which ? &sh.vfree[os] : &sh.kfree[os];
-                    const uint32_t off = (which ? F::V_OFF : F::K_OFF) + os * NLO * F::HALF;
-                    // the operand stage is free once the MMAs of OS tiles ago are done
-                    if (direct(sg, t)) {
+                    const uint32_t off = which ? F::V_OFF + os * NLO * F::HALF : F::K_OFF + os * NLO * F::HALF;
+                    const uint32_t dst = sb + off;
+                    // the operand stage is free once the MMAs of its last tile are done (every loader
+                    // waits for every tile: a wait tells a phase from its neighbours only)
+                    if (n >= st) tree_wait(free, n / st - 1, a.err, ERR_WAIT_EMPTY, abort_flag);
+                    __syncwarp();
+                    if (KVT == KV_F16 && dir) {
                         if (lane == 0) {
-                            if (n >= OS) mbar_wait(free, (n / OS - 1) & 1, a.err, ERR_WAIT_EMPTY, abort_flag);
-                            if (lt == 0 && !*abort_flag) {
-                                mbar_expect_tx(full, F::HALF);
-                                const int row = (int)(((size_t)s.slot * a.slot_stride) / hd + (size_t)sg.kvh * a.cap) + t * PT;
-#pragma unroll
-                                for (int c = 0; c < HD / 64; ++c)
-                                    asm volatile(
-                                        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], "
-                                        "[%1, {%2, %3}], [%4];" ::"r"(sb + off + c * PT * 128),
-                                        "l"(reinterpret_cast<uint64_t>(which ? &vmap : &kmap)), "r"(64 * c), "r"(row), "r"(smem_u32(full))
-                                        : "memory");
-                            } else {
-                                mbar_arrive(full);
-                            }
+                            if (lt == 0 && !*abort_flag) tma_tile(sg, t, which, off, full);
+                            else mbar_arrive(full);
                         }
+                        __syncwarp();
                         continue;
                     }
-                    const int rs = nr % RS;
-                    uint8_t* raw = smem + F::RAW_OFF + rs * F::RAW;
-                    if (KVT != KV_F16) mbar_wait(&sh.rawfull[rs], (nr / RS) & 1, a.err, ERR_WAIT_FULL, abort_flag);
-                    if (n >= OS) mbar_wait(free, (n / OS - 1) & 1, a.err, ERR_WAIT_EMPTY, abort_flag);
-                    __syncwarp();
-                    ++nr;
-                    constexpr int UNITS = PT * HD / 8, UPR = HD / 8;  // 8-element units, per row
-                    if (KVT != KV_F16 && which && (t + 1) * PT > s.n_ctx)  // non-finite drafted values leave the operand (see the narrow kernel)
-                        for (int v = lt; v < UNITS; v += LT) {
-                            const int r = v / UPR, c = (v % UPR) * 8, p = t * PT + r;
-                            if (r >= rows || c >= hd || p < s.n_ctx) continue;
-                            uint4* x = reinterpret_cast<uint4*>(raw + ((size_t)r * hd + c) * ESZ);
-                            for (int k = 0; k < ESZ / 2; ++k) {
-                                uint4 y = x[k];
-                                if (zero_nonfinite<KVT>(y)) {
-                                    x[k] = y;
-                                    atomicOr(&sh.badrow[seg & 7][(p - s.n_ctx) >> 5], 1u << ((p - s.n_ctx) & 31));
-                                }
-                            }
-                        }
-                    const uint32_t dst = sb + off, rawa = smem_u32(raw);
-                    // converted with the last tile's exponent; when the tile's maximum turns out not
-                    // to fit it (seldom), once more with its own
-                    for (;;) {
-                        const int ec = which ? e2v : e2k;
-                        const float f = pow2i(-ec);
-                        float mf = 0.f;       // largest |x| of fp32 values
-                        uint32_t mw = 0;      // largest |x| of bf16 values, two lanes
+                    uint32_t src = 0;  // this thread's first vector in shared memory, rows sstep bytes apart
+                    if (KVT == KV_F32) {
+                        const int rs = nr % RS;
+                        src = sb + F::RAW_OFF + rs * F::RAW + (uint32_t)(r0 * hd * 4 + c0 * 16);
+                        tree_wait(&sh.rawfull[rs], nr / RS, a.err, ERR_WAIT_FULL, abort_flag);
+                    } else if (dir) {
+                        tree_wait(&sh.rawfull[(nd & 3) * 2 + which], nd >> 2, a.err, ERR_WAIT_FULL, abort_flag);
+                    } else {  // from the cache to the operand's place
+                        const uint8_t* g = static_cast<const uint8_t*>(which ? a.vc : a.kc) +
+                                           ((size_t)s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + (size_t)t * PT) * hd + c0 * 8) * 2;
 #pragma unroll 4
-                        for (int v = lt; v < UNITS; v += LT) {
-                            const int r = v / UPR, c = v % UPR;
-                            uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-                            if (r < rows && c * 8 < hd) {
-                                const uint32_t x = rawa + (uint32_t)((r * hd + c * 8) * ESZ);
-                                if (KVT == KV_F16) {  // the few such tiles come straight from the cache
-                                    const int p = t * PT + r;
-                                    const size_t at = (size_t)s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + p) * hd + c * 8;
-                                    x0 = *reinterpret_cast<const uint4*>(static_cast<const __half*>(which ? a.vc : a.kc) + at);
-                                    if (which && p >= s.n_ctx && zero_nonfinite<KVT>(x0))
-                                        atomicOr(&sh.badrow[seg & 7][(p - s.n_ctx) >> 5], 1u << ((p - s.n_ctx) & 31));
-                                } else {
-                                    x0 = ld_shared16(x);
-                                    if (KVT == KV_F32) x1 = ld_shared16(x + 16);
-                                }
-                            }
-                            const uint32_t o = dst + wide_off(PT, r, c);
-                            if (KVT == KV_F32) {
-                                uint32_t hi[4], lo[4];
-                                const uint32_t w[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-#pragma unroll
-                                for (int j = 0; j < 4; ++j) {
-                                    const float2 y = make_float2(__uint_as_float(w[2 * j]), __uint_as_float(w[2 * j + 1]));
-                                    mf = fmaxf(mf, fmaxf(fabsf(y.x), fabsf(y.y)));
-                                    split2t(__fmul2_rn(y, make_float2(f, f)), hi[j], lo[j]);
-                                }
-                                st_shared16(o, hi);
-                                st_shared16(o + F::HALF, lo);
-                            } else {
-                                uint32_t w[4] = {x0.x, x0.y, x0.z, x0.w};
-                                if (KVT == KV_BF16) {
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) {
-                                        mw = __vmaxu2(mw, w[j] & 0x7FFF7FFFu);
-                                        w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
-                                    }
-                                }
-                                st_shared16(o, w);
+                        for (int r = r0; r < PT; r += RSTEP) {
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (r < rows && c0 * 8 < hd) x = *reinterpret_cast<const uint4*>(g + (size_t)r * hd * 2);
+                            st_shared16(dst + wide_off(PT, r, c0), {x.x, x.y, x.z, x.w});
+                        }
+                    }
+                    __syncwarp();
+                    const bool col = KVT != KV_F32 || c0 * 4 < hd;
+                    auto at = [&](int r) { return KVT == KV_F32 ? src + (uint32_t)((r - r0) * hd * 4) : dst + wide_off(PT, r, c0); };
+                    if (which && tail && col) {  // non-finite drafted values leave the operand (see the narrow kernel)
+#pragma unroll 1
+                        for (int r = r0; r < rows; r += RSTEP) {
+                            const int p = t * PT + r - s.n_ctx;
+                            if (p < 0) continue;
+                            uint4 x = ld_shared16(at(r));
+                            if (zero_nonfinite<KVT>(x)) {
+                                atomicOr(&sh.badrow[seg & 7][p >> 5], 1u << (p & 31));
+                                st_shared16(at(r), {x.x, x.y, x.z, x.w});
                             }
                         }
-                        uint32_t mb = KVT == KV_F32 ? __float_as_uint(mf) : max(mw << 16, mw & 0xFFFF0000u);
-                        if (KVT != KV_F16 && __any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
+                    }
+                    if (KVT != KV_F16) {
+                        // the tile's largest finite |x|
+                        uint32_t mb = 0;
+                        if (col) {
+#pragma unroll 4
+                            for (int r = r0; r < rows; r += RSTEP) mb = max(mb, abs_bits<KVT>(ld_shared16(at(r))));
+                        }
+                        if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: once more without them
                             mb = 0;
-                            for (int v = lt; v < UNITS; v += LT) {
-                                const int r = v / UPR, c = v % UPR;
-                                if (r >= rows || c * 8 >= hd) continue;
-                                const uint32_t x = rawa + (uint32_t)((r * hd + c * 8) * ESZ);
-                                mb = max(mb, max_bits<KVT>(ld_shared16(x)));
-                                if (KVT == KV_F32) mb = max(mb, max_bits<KVT>(ld_shared16(x + 16)));
-                            }
+                            if (col)
+#pragma unroll 1
+                                for (int r = r0; r < rows; r += RSTEP) mb = max(mb, max_bits<KVT>(ld_shared16(at(r))));
                             __syncwarp();
                         }
-                        if (KVT == KV_F16) break;
                         mb = __reduce_max_sync(0xFFFFFFFFu, mb);
                         unsigned* tm = &sh.tmax[2 * (n & 1) + which];
                         if (lane == 0) atomicMax(tm, mb);
                         named_bar<2, LT>();
-                        const uint32_t all = *tm;
-                        // fits: the maximum is within [2^0, 2^15) after the scale
-                        const int e = tile_exponent(all), d = e - ec;
-                        if (all == 0 || d == 0 || (d > -8 && d < 7)) break;
-                        named_bar<2, LT>();  // every thread has read the exponent's base
-                        if (which) e2v = e;
-                        else e2k = e;
-                    }
-                    if (lt == 0) {
-                        sh.tmax[2 * (~n & 1) + which] = 0;  // the next tile's, read last a tile ago
-                        (which ? sh.ev : sh.ek)[n & 3] = which ? e2v : e2k;
+                        const int e = half_exponent(*tm);
+                        const float f = pow2i(-e);
+                        if (lt == 0) {
+                            sh.tmax[2 * (~n & 1) + which] = 0;  // the next tile's, read last a tile ago
+                            (which ? sh.ev : sh.ek)[n & 7] = e;
+                        }
+#pragma unroll UNR
+                        for (int r = r0; r < PT; r += RSTEP) {
+                            uint4 x = make_uint4(0, 0, 0, 0);
+                            if (KVT != KV_F32 || (r < rows && col)) x = ld_shared16(at(r));
+                            if (KVT == KV_F32) {
+                                uint32_t h0, l0, h1, l1;
+                                split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), make_float2(f, f)), h0, l0);
+                                split2t(__fmul2_rn(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), make_float2(f, f)), h1, l1);
+                                const uint32_t o = dst + wide_off(PT, r, c0 >> 1) + (c0 & 1) * 8;
+                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
+                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::HALF), "r"(l0), "r"(l1) : "memory");
+                            } else {
+                                uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
+                                st_shared16(at(r), w);
+                            }
+                        }
                     }
                     fence_async();
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive(full);
-                        if (KVT != KV_F16) mbar_arrive(&sh.rawfree[rs]);
+                        if (KVT == KV_F32) mbar_arrive(&sh.rawfree[nr % RS]);
                     }
+                    ++nr;
                 }
+                if (KVT == KV_BF16 && dir) ++nd;
             }
             ++seg;
         }
         // after an abort: copies of the last stages may still be on their way
-        if (lt == 0 && *abort_flag)
-            for (int i = max(0, n - OS); i < n; ++i) {
-                mbar_wait(&sh.kfull[i % OS], (i / OS) & 1, a.err, ERR_WAIT_FULL, nullptr);
-                mbar_wait(&sh.vfull[i % OS], (i / OS) & 1, a.err, ERR_WAIT_FULL, nullptr);
+        if (KVT == KV_F16 && lt == 0 && *abort_flag)
+#pragma unroll 1
+            for (int i = max(0, n - KS); i < n; ++i) {
+                tree_wait(&sh.kfull[i % KS], i / KS, a.err, ERR_WAIT_FULL, nullptr);
+                tree_wait(&sh.vfull[i % KS], i / KS, a.err, ERR_WAIT_FULL, nullptr);
             }
     } else if (warp == 13) {
-        // raw copies, RS buffers ahead
+        // copies ahead of the loaders: raw fp32 tiles, bf16 tiles into their operand stages
         if (KVT != KV_F16 && lane == 0) {
-            int nr = 0, last[RS];  // last copy into each buffer
-#pragma unroll
-            for (int i = 0; i < RS; ++i) last[i] = -1;
-            while (tree_next(a, pl, g0, g1, per, b, base, sg))
-                for (int t = sg.t0; t < sg.t1; ++t) {
-                    const int rows = min(PT, sg.s.n_ctx + sg.s.n_node - t * PT);
-                    const uint32_t bytes = (uint32_t)(rows * hd * ESZ);
-                    const size_t off = ((size_t)sg.s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + (size_t)t * PT) * hd) * ESZ;
-                    for (int which = 0; which < 2; ++which, ++nr) {
-                        const int rs = nr % RS;
-                        if (nr >= RS) mbar_wait(&sh.rawfree[rs], (nr / RS - 1) & 1, a.err, ERR_WAIT_EMPTY, abort_flag);
-                        if (*abort_flag) continue;
-                        mbar_expect_tx(&sh.rawfull[rs], bytes);
-                        bulk_g2s(smem + F::RAW_OFF + rs * F::RAW, static_cast<const uint8_t*>(which ? a.vc : a.kc) + off, bytes, &sh.rawfull[rs]);
-                        last[rs] = nr / RS;
+            int n = 0, nr = 0, nd = 0;
+            unsigned issued = 0, par = 0;  // per barrier: a copy was issued, parity of the last one
+            while (tree_next<PT, TW_RT>(a, rep, it, sg))
+#pragma unroll 1
+                for (int t = sg.t0; t < sg.t1; ++t, ++n)
+#pragma unroll 1
+                    for (int which = 0; which < 2; ++which) {
+                        const bool dir = direct(sg, t);
+                        int bar, phase;
+                        if (KVT == KV_F32) {
+                            const int rs = nr % RS;
+                            if (nr >= RS) tree_wait(&sh.rawfree[rs], nr / RS - 1, a.err, ERR_WAIT_EMPTY, abort_flag);
+                            bar = rs;
+                            phase = nr / RS;
+                        } else {
+                            // every tile's stage is waited for, the loaders' own tiles among them
+                            const int os = n % KS;
+                            if (n >= KS) tree_wait(which ? &sh.vfree[os] : &sh.kfree[os], n / KS - 1, a.err, ERR_WAIT_EMPTY, abort_flag);
+                            bar = (nd & 3) * 2 + which;
+                            phase = nd >> 2;
+                        }
+                        ++nr;
+                        if (!*abort_flag && (KVT == KV_F32 || dir)) {
+                            if (KVT == KV_F32) {
+                                const uint32_t bytes = (uint32_t)(min(PT, sg.s.n_ctx + sg.s.n_node - t * PT) * hd * ESZ);
+                                const size_t off = ((size_t)sg.s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + (size_t)t * PT) * hd) * ESZ;
+                                mbar_expect_tx(&sh.rawfull[bar], bytes);
+                                bulk_g2s(smem + F::RAW_OFF + bar * F::RAW, static_cast<const uint8_t*>(which ? a.vc : a.kc) + off, bytes,
+                                         &sh.rawfull[bar]);
+                            } else {
+                                tma_tile(sg, t, which, (which ? F::V_OFF : F::K_OFF) + (n % KS) * F::HALF, &sh.rawfull[bar]);
+                            }
+                            issued |= 1u << bar;
+                            par = (par & ~(1u << bar)) | ((unsigned)(phase & 1) << bar);
+                        }
+                        if (which && dir) ++nd;
                     }
-                }
             if (*abort_flag)  // copies that may still be on their way
-                for (int i = 0; i < RS; ++i)
-                    if (last[i] >= 0) mbar_wait(&sh.rawfull[i], last[i] & 1, a.err, ERR_WAIT_FULL, nullptr);
+#pragma unroll 1
+                for (int i = 0; i < 8; ++i)
+                    if (issued >> i & 1) tree_wait(&sh.rawfull[i], par >> i & 1, a.err, ERR_WAIT_FULL, nullptr);
         }
         __syncwarp();
     } else if (warp == 12) {
@@ -1031,56 +1115,59 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tf_tree_attn_wide_kernel(const 
         constexpr uint32_t iqk = (1u << 4) | ((uint32_t)(PT >> 3) << 17) | ((uint32_t)(TW_RT >> 4) << 24);
         constexpr uint32_t ipv = (1u << 4) | (1u << 16) | ((uint32_t)(HD >> 3) << 17) | ((uint32_t)(TW_RT >> 4) << 24);
         const uint32_t lead = elect_lane(), tm = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-        int n = 0, seg = 0;
-        int cnt0 = 0, cnt1 = 0;  // PVs issued per stream
+        int n = 0, seg = 0, cnt[2] = {0, 0};  // running tile, segment, PVs issued per stream
         bool ok = true;
         auto wait = [&](uint64_t* bar, int parity) {
-            ok = __all_sync(0xFFFFFFFFu, ok && mbar_wait(bar, parity & 1, a.err, ERR_WAIT_FULL, abort_flag));
+            ok = __all_sync(0xFFFFFFFFu, ok && tree_wait(bar, parity, a.err, ERR_WAIT_FULL, abort_flag));
         };
-        auto pv = [&](int m, int w) {  // tile m of the run, stream w
-            const int os = m % OS;
-            wait(&sh.pfull[w], w ? cnt1 : cnt0);
-            wait(&sh.vfull[os], m / OS);
-            if (w) ++cnt1;
-            else ++cnt0;
-            if (!ok) return;
-            tc_fence_after();
-            const uint32_t d = tm + 256 + w * HD, p = tm + w * 128;
-            const uint64_t vh = wide_desc(sb + F::V_OFF + os * NLO * F::HALF, PT * 128);
-            const uint64_t vl = wide_desc(sb + F::V_OFF + os * NLO * F::HALF + (NLO - 1) * F::HALF, PT * 128);
-#pragma unroll
-            for (int j = 0; j < PT / 16; ++j) {  // 16 positions: 2048 bytes of rows; p's halves in blocks of CH columns
-                const uint32_t ph = CH == 32 ? p + 32 * (j / 2) + 8 * (j % 2) : p + 16 * j;
-                wide_mma_ts(d, ph, vh + 128u * j, ipv, j > 0, lead);
-                wide_mma_ts(d, ph + CH / 2, vh + 128u * j, ipv, 1, lead);
-                if (NLO == 2) wide_mma_ts(d, ph, vl + 128u * j, ipv, 1, lead);
-            }
-            wide_commit(&sh.vfree[os], lead);
-            wide_commit(&sh.dfull[w], lead);
-        };
-        while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+        while (tree_next<PT, TW_RT>(a, rep, it, sg)) {
             wait(&sh.qfull, seg);
-            for (int t = sg.t0; t < sg.t1; ++t, ++n) {
-                const int w = (t - sg.t0) & 1, os = n % OS;
-                wait(&sh.kfull[os], n / OS);
-                if (ok) {
-                    tc_fence_after();
-                    const uint32_t d = tm + w * 128;
-                    const uint64_t kb = wide_desc(sb + F::K_OFF + os * NLO * F::HALF, 16), qb = wide_desc(sb + F::Q_OFF, 16);
+            // QK of tile t, then PV of tile t - 1 (one step more than there are tiles)
+#pragma unroll 1
+            for (int t = sg.t0; t <= sg.t1; ++t) {
+                const int w = (t - sg.t0) & 1;
+                if (t < sg.t1) {
+                    const int os = n % KS;
+                    wait(&sh.kfull[os], n / KS);
+                    if (ok) {
+                        tc_fence_after();
+                        const uint32_t d = tm + w * 128;
+                        const uint64_t kb = wide_desc(sb + F::K_OFF + os * NLO * F::HALF, 16), qb = wide_desc(sb + F::Q_OFF, 16);
 #pragma unroll
-                    for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes along the rows of a 64-dim block
-                        const uint64_t q = qb + ((j / 4) * (TW_RT * 128) + (j % 4) * 32) / 16;
-                        const uint64_t k = kb + ((j / 4) * (PT * 128) + (j % 4) * 32) / 16;
-                        wide_mma_ss(d, q, k, iqk, j > 0, lead);
-                        wide_mma_ss(d, q + F::QH / 16, k, iqk, 1, lead);
-                        if (NLO == 2) wide_mma_ss(d, q, k + F::HALF / 16, iqk, 1, lead);
+                        for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes along the rows of a 64-dim block
+                            const uint64_t q = qb + ((j / 4) * (TW_RT * 128) + (j % 4) * 32) / 16;
+                            const uint64_t k = kb + ((j / 4) * (PT * 128) + (j % 4) * 32) / 16;
+                            wide_mma_ss(d, q, k, iqk, j > 0, lead);
+                            wide_mma_ss(d, q + F::QH / 16, k, iqk, 1, lead);
+                            if (NLO == 2) wide_mma_ss(d, q, k + F::HALF / 16, iqk, 1, lead);
+                        }
+                        wide_commit(&sh.kfree[os], lead);
+                        wide_commit(&sh.sfull[w], lead);
                     }
-                    wide_commit(&sh.kfree[os], lead);
-                    wide_commit(&sh.sfull[w], lead);
+                    ++n;
                 }
-                if (t > sg.t0) pv(n - 1, w ^ 1);
+                if (t > sg.t0) {
+                    const int mt = t < sg.t1 ? n - 2 : n - 1, v = w ^ 1, os = mt % VS;  // tile, stream, stage
+                    wait(&sh.pfull[v], v ? cnt[1] : cnt[0]);
+                    wait(&sh.vfull[os], mt / VS);
+                    if (v) ++cnt[1];
+                    else ++cnt[0];
+                    if (ok) {
+                        tc_fence_after();
+                        const uint32_t d = tm + 256 + v * HD, p = tm + v * 128;
+                        const uint64_t vh = wide_desc(sb + F::V_OFF + os * NLO * F::HALF, PT * 128);
+#pragma unroll
+                        for (int j = 0; j < PT / 16; ++j) {  // 16 positions: 2048 bytes of rows; p's halves in blocks of CH columns
+                            const uint32_t ph = CH == 32 ? p + 32 * (j / 2) + 8 * (j % 2) : p + 16 * j;
+                            wide_mma_ts(d, ph, vh + 128u * j, ipv, j > 0, lead);
+                            wide_mma_ts(d, ph + CH / 2, vh + 128u * j, ipv, 1, lead);
+                            if (NLO == 2) wide_mma_ts(d, ph, vh + F::HALF / 16 + 128u * j, ipv, 1, lead);
+                        }
+                        wide_commit(&sh.vfree[os], lead);
+                        wide_commit(&sh.dfull[v], lead);
+                    }
+                }
             }
-            pv(n - 1, (sg.t1 - 1 - sg.t0) & 1);
             ++seg;
         }
         wide_commit(&sh.done, lead);  // arrives once every MMA issued above has completed
@@ -1091,41 +1178,39 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tf_tree_attn_wide_kernel(const 
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t ts = tl + wg * 128, td = tl + 256 + wg * HD;
         int n = 0, seg = 0, cnt = 0;
-        while (tree_next(a, pl, g0, g1, per, b, base, sg)) {
+        while (tree_next<PT, TW_RT>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
             const int rows = s.n_node * rep;
             {   // queries, HD / 8 lanes per row: scaled to [2^14, 2^15), two halves
-                constexpr int LPR = HD / 8, RPW = 32 / LPR, STEPS = TW_RT / (8 * RPW);
-                float4 x[STEPS][2];
+                constexpr int LPR = HD / 8, RPW = 32 / LPR, STEPS = TW_RT / (8 * RPW), U = 4;
                 const int c = lane % LPR;
+#pragma unroll 1
+                for (int i0 = 0; i0 < STEPS; i0 += U) {
+                    float4 x[U][2];
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
-                    const int r = (i * 8 + warp) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
-                    const float* qp = a.q + ((size_t)sg.b * a.T + nd) * a.ld_q + (size_t)(sg.kvh * rep + q - nd * rep) * hd + c * 8;
-                    x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (q < rows && c * 8 < hd) {
-                        x[i][0] = reinterpret_cast<const float4*>(qp)[0];
-                        x[i][1] = reinterpret_cast<const float4*>(qp)[1];
+                    for (int i = 0; i < U; ++i) {
+                        const int r = ((i0 + i) * 8 + warp) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
+                        const float* qp = a.q + ((size_t)sg.b * a.T + nd) * a.ld_q + (size_t)(sg.kvh * rep + q - nd * rep) * hd + c * 8;
+                        x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (q < rows && c * 8 < hd) {
+                            x[i][0] = reinterpret_cast<const float4*>(qp)[0];
+                            x[i][1] = reinterpret_cast<const float4*>(qp)[1];
+                        }
                     }
-                }
 #pragma unroll
-                for (int i = 0; i < STEPS; ++i) {
-                    const int r = (i * 8 + warp) * RPW + lane / LPR;
-                    const float y[8] = {x[i][0].x, x[i][0].y, x[i][0].z, x[i][0].w, x[i][1].x, x[i][1].y, x[i][1].z, x[i][1].w};
-                    uint32_t mb = 0;
+                    for (int i = 0; i < U; ++i) {
+                        const int r = ((i0 + i) * 8 + warp) * RPW + lane / LPR;
+                        uint32_t mb = max(finite_max4(x[i][0]), finite_max4(x[i][1]));
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) mb = max(mb, finite_abs_bits(y[j]));
-#pragma unroll
-                    for (int o = 1; o < LPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
-                    const int e = half_exponent(mb);
-                    const float sc = pow2i(-e);
-                    uint32_t hi[4], lo[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) split2(y[2 * j] * sc, y[2 * j + 1] * sc, hi[j], lo[j]);
-                    const uint32_t o = sb + F::Q_OFF + wide_off(TW_RT, r, c);
-                    st_shared16(o, hi);
-                    st_shared16(o + F::QH, lo);
-                    if (c == 0) sh.qscale[r] = pow2i(e) * (kLog2e / sqrtf((float)hd));
+                        for (int o = 1; o < LPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
+                        const int e = half_exponent(mb);
+                        uint32_t hi[4], lo[4];
+                        split8(x[i][0], x[i][1], pow2i(-e), hi, lo);
+                        const uint32_t o = sb + F::Q_OFF + wide_off(TW_RT, r, c);
+                        st_shared16(o, hi);
+                        st_shared16(o + F::QH, lo);
+                        if (c == 0) sh.qscale[r] = pow2i(e) * (kLog2e / sqrtf((float)hd));
+                    }
                 }
                 fence_async();
                 mbar_arrive(&sh.qfull);
@@ -1133,30 +1218,32 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tf_tree_attn_wide_kernel(const 
             }
             const float qs = sh.qscale[row];
             const int rr = sg.rtile * TW_RT + row, node = (rr * rep_inv) >> 16;
+            uint32_t* vis = sh.vis[tid];
+            vis_fill(vis, a, s, sg.b, node);
             float O[HD], m = -INFINITY, l = 0.f;
 #pragma unroll
             for (int i = 0; i < HD; ++i) O[i] = 0.f;
-            const int n0 = n;
+            const int n0 = n - sg.t0;
+#pragma unroll 1
             for (int t = sg.t0 + wg; t < sg.t1; t += 2, ++cnt) {
-                const int nt = n0 + t - sg.t0;
-                mbar_wait(&sh.sfull[wg], cnt & 1, a.err, ERR_WAIT_FULL, abort_flag);
+                tree_wait(&sh.sfull[wg], cnt, a.err, ERR_WAIT_FULL, abort_flag);
                 __syncwarp();
                 tc_fence_after();
-                const float f = KVT == KV_F16 ? qs : qs * pow2i(sh.ek[nt & 3]);
+                const float f = KVT == KV_F16 ? qs : qs * pow2i(sh.ek[(n0 + t) & 7]);
                 const bool tail = (t + 1) * PT > s.n_ctx;
-                // (the loops over 32-column chunks stay loops: unrolled, the code outgrows the
+                // (the loops over CH-column chunks stay loops: unrolled, the code outgrows the
                 // instruction cache and the one warp per scheduler waits for its fetches)
                 float mx = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < PT / CH; ++c) {
+                for (int c = 0; c < PT; c += CH) {
                     uint32_t x[CH];
-                    tmem_ld(ts + CH * c, x);
+                    tmem_ld(ts + c, x);
                     if (tail) {
-                        const uint32_t vis = tree_window(a, s, sg.b, node, t * PT + CH * c - s.n_ctx);
-                        __syncwarp();
+                        const uint32_t seen = vis_window(vis, t * PT + c - s.n_ctx);
 #pragma unroll
-                        for (int i = 0; i < CH; ++i) x[i] = (vis >> i) & 1 ? x[i] : 0xFF800000u;
-                        tmem_st(ts + CH * c, x);  // masked scores are -infinity from here on
+                        for (int i = 0; i < CH; ++i) x[i] = (seen >> i) & 1 ? x[i] : 0xFF800000u;
+                        __syncwarp();
+                        tmem_st(ts + c, x);  // masked scores are -infinity from here on
                     }
                     float m0 = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 #pragma unroll
@@ -1169,117 +1256,93 @@ __global__ void __launch_bounds__(TW_THREADS, 1) tf_tree_attn_wide_kernel(const 
                 m = mx;
                 float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll 1
-                for (int c = 0; c < PT / CH; ++c) {
+                for (int c = 0; c < PT; c += CH) {
                     uint32_t x[CH], y[CH];
-                    tmem_ld(ts + CH * c, x);
+                    tmem_ld(ts + c, x);
 #pragma unroll
                     for (int i = 0; i < CH; i += 2) {
                         const float p0 = exp2_fast(fmaf(__uint_as_float(x[i]), f, shift));
                         const float p1 = exp2_fast(fmaf(__uint_as_float(x[i + 1]), f, shift));
                         sum0 += p0;
                         sum1 += p1;
-                        // high halves by truncation (exact in f16 down to 2^-14), low halves what is left
-                        const float h0 = __uint_as_float(__float_as_uint(p0) & 0xFFFFE000u);
-                        const float h1 = __uint_as_float(__float_as_uint(p1) & 0xFFFFE000u);
-                        y[i / 2] = pack_half2(h0, h1);
-                        y[CH / 2 + i / 2] = pack_half2(p0 - h0, p1 - h1);
+                        split2t(make_float2(p0, p1), y[i / 2], y[CH / 2 + i / 2]);
                     }
-                    tmem_st(ts + CH * c, y);
+                    tmem_st(ts + c, y);
                 }
                 l = fmaf(l, alpha, sum0 + sum1);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&sh.pfull[wg]);
-                mbar_wait(&sh.dfull[wg], cnt & 1, a.err, ERR_WAIT_FULL, abort_flag);
+                tree_wait(&sh.dfull[wg], cnt, a.err, ERR_WAIT_FULL, abort_flag);
                 __syncwarp();
                 tc_fence_after();
-                const float fv = KVT == KV_F16 ? 1.f : pow2i(sh.ev[nt & 3]);
+                const float fv = KVT == KV_F16 ? 1.f : pow2i(sh.ev[(n0 + t) & 7]);
 #pragma unroll
                 for (int c = 0; c < HD / CH; ++c) {
                     uint32_t x[CH];
                     tmem_ld(td + CH * c, x);
 #pragma unroll
-                    for (int i = 0; i < CH; ++i) O[CH * c + i] = fmaf(__uint_as_float(x[i]), fv, O[CH * c + i] * alpha);
+                    for (int i = 0; i < CH; i += 2) {
+                        const float2 o = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(fv, fv),
+                                                    __fmul2_rn(make_float2(O[CH * c + i], O[CH * c + i + 1]), make_float2(alpha, alpha)));
+                        O[CH * c + i] = o.x;
+                        O[CH * c + i + 1] = o.y;
+                    }
                 }
                 tc_fence_before();
             }
             n += sg.t1 - sg.t0;
-            // The streams meet in Q's shared memory (every QK of the segment is done): maxima and
-            // sums first, then stream 1's weighted output, stream 0 adds its own, and the rows
-            // leave coalesced.  fp32 rows of HD, 16-byte chunk c of row r at c ^ (r & 7).
+            // The streams meet in Q's shared memory (every QK of the segment is done), half of the
+            // columns at a time: both leave their rows weighted, then all threads add the two,
+            // divide, and write coalesced.  fp32 rows of HD / 2 per stream, 16-byte chunk c of row
+            // r at c ^ (r & 7).
             sh.ml[wg][row] = make_float2(m, l);
-            named_bar<1, 256>();
-            const float2 other = sh.ml[wg ^ 1][row];
-            const float M = fmaxf(m, other.x), mref = M == -INFINITY ? 0.f : M, wgt = exp2_fast(m - mref);
-            const float L = fmaf(l, wgt, other.y * exp2_fast(other.x - mref));
-            const uint32_t srow = sb + F::Q_OFF + (uint32_t)row * (HD * 4);
-            if (wg == 1) {
-#pragma unroll
-                for (int c = 0; c < HD / 4; ++c)
-                    st_shared16(srow + ((uint32_t)(c ^ (row & 7)) << 4),
-                                {__float_as_uint(O[4 * c] * wgt), __float_as_uint(O[4 * c + 1] * wgt),
-                                 __float_as_uint(O[4 * c + 2] * wgt), __float_as_uint(O[4 * c + 3] * wgt)});
-            }
             named_bar<1, 256>();
             const bool whole = sg.t0 == 0 && sg.t1 == sg.tiles;
             float* part = parts + ((size_t)blockIdx.x * 2 + (sg.t0 == 0 ? 1 : 0)) * tree_part_floats(TW_RT, hd);
-            if (wg == 0) {
-                const float inv = !whole ? 1.f : (L == 0.f ? 0.f : 1.f / L);
-                const bool none = whole && L == 0.f;
-#pragma unroll
-                for (int c = 0; c < HD / 4; ++c) {
-                    const uint32_t at = srow + ((uint32_t)(c ^ (row & 7)) << 4);
-                    const uint4 x = ld_shared16(at);
-                    const float y[4] = {fmaf(O[4 * c], wgt, __uint_as_float(x.x)), fmaf(O[4 * c + 1], wgt, __uint_as_float(x.y)),
-                                        fmaf(O[4 * c + 2], wgt, __uint_as_float(x.z)), fmaf(O[4 * c + 3], wgt, __uint_as_float(x.w))};
-                    uint32_t z[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) z[j] = none ? 0u : __float_as_uint(y[j] * inv);
-                    st_shared16(at, z);
-                }
-                if (rr < rows) {
-                    const size_t off = (size_t)s.slot * a.slot_stride + ((size_t)sg.kvh * a.cap + s.n_ctx) * hd;
-#pragma unroll 1
-                    for (int w = 0; w < TREE_MAX_NODES / 32; ++w)  // non-finite drafted values that the row sees
-#pragma unroll 1
-                        for (unsigned bits = sh.badrow[seg & 7][w] & tree_window(a, s, sg.b, node, 32 * w); bits; bits &= bits - 1) {
-                            const size_t at = off + (size_t)(w * 32 + __ffs(bits) - 1) * hd;
-#pragma unroll 1
-                            for (int i = 0; i < hd; ++i) {
-                                const float v = kv_load(a.vc, (long long)(at + i), KVT);
-                                float* o = reinterpret_cast<float*>(smem + F::Q_OFF + (size_t)row * (HD * 4) + (((i >> 2) ^ (row & 7)) << 4)) + (i & 3);
-                                if (!(fabsf(v) < INFINITY)) *o += v;
-                            }
-                        }
-                    if (!whole && !*abort_flag) {
+            float wgt;
+            {
+                const float2 other = sh.ml[wg ^ 1][row];
+                const float M = fmaxf(m, other.x), mref = M == -INFINITY ? 0.f : M;
+                wgt = exp2_fast(m - mref);
+                const float L = fmaf(l, wgt, other.y * exp2_fast(other.x - mref));
+                named_bar<1, 256>();
+                if (wg == 0) {
+                    sh.ml[0][row].x = !whole ? 1.f : (L == 0.f ? 0.f : 1.f / L);
+                    if (!whole && rr < rows && !*abort_flag) {
                         part[(size_t)TW_RT * hd + row] = M;
                         part[(size_t)TW_RT * hd + TW_RT + row] = L;
                     }
                 }
-                if (!whole && sg.t0 == 0 && row == 0) desc[blockIdx.x] = TreeDesc{sg.b, sg.kvh, sg.rtile, sg.last_cta};
             }
-            named_bar<1, 256>();
-            {
-                constexpr int LPR = HD / 4, RPW = 32 / LPR;  // lanes per row, rows per warp and step
-                const int c = lane % LPR;
-#pragma unroll 4
-                for (int i = warp; i < TW_RT / RPW; i += 8) {
-                    const int r = i * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
-                    if (q >= rows || c * 4 >= hd || *abort_flag) continue;
-                    const uint4 x = ld_shared16(sb + F::Q_OFF + (uint32_t)r * (HD * 4) + ((uint32_t)(c ^ (r & 7)) << 4));
-                    float* dst = whole ? a.out + ((size_t)sg.b * a.T + nd) * a.ld_out + (size_t)(sg.kvh * rep + q - nd * rep) * hd
-                                       : part + (size_t)r * hd;
-                    *reinterpret_cast<uint4*>(dst + c * 4) = x;
+            constexpr int HC = HD / 8;  // 16-byte chunks of half a row
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t srow = sb + F::Q_OFF + (uint32_t)wg * (TW_RT * HD * 2) + (uint32_t)row * (HD * 2);
+#pragma unroll
+                for (int c = 0; c < HC; ++c) {
+                    const int i = h * (HD / 2) + 4 * c;
+                    st_shared16(srow + ((uint32_t)(c ^ (row & 7)) << 4),
+                                {__float_as_uint(O[i] * wgt), __float_as_uint(O[i + 1] * wgt), __float_as_uint(O[i + 2] * wgt),
+                                 __float_as_uint(O[i + 3] * wgt)});
                 }
+                named_bar<1, 256>();
+                wide_rows_out<HD>(a, sg, sb + F::Q_OFF, sh.ml[0], whole, part, h, rep, rep_inv, abort_flag);
+                named_bar<1, 256>();  // the shared memory takes the next half, or the next segment's queries
             }
-            named_bar<1, 256>();  // Q's shared memory takes the next segment's queries
+            if (!whole && sg.t0 == 0 && tid == 0) desc[blockIdx.x] = TreeDesc{sg.b, sg.kvh, sg.rtile, sg.last_cta};
+            if (badrow_any(sh.badrow[seg & 7])) {
+                if (!*abort_flag)
+                    tree_fix_rows<KVT>(a, sg, TW_RT, rep, sh.badrow[seg & 7], &sh.vis[0][0], part, whole, tid, 256);
+                named_bar<1, 256>();  // (its reads of vis end before the next segment's)
+            }
             __syncwarp();
             ++seg;
         }
     }
     // TMEM stays allocated until every issued MMA has completed
     __syncwarp();
-    if (warp == 0) mbar_wait(&sh.done, 0, a.err, ERR_WAIT_FULL, nullptr);
+    if (warp == 0) tree_wait(&sh.done, 0, a.err, ERR_WAIT_FULL, nullptr);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -1305,12 +1368,14 @@ __global__ void __launch_bounds__(TC_THREADS) tf_tree_combine_kernel(const TreeA
     if (r >= rt || rr >= n_node * rep) return;
     auto part = [&](int i) { return parts + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * pf; };
     float M = -INFINITY;
+#pragma unroll 1
     for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[(size_t)rt * hd + r]);
     M = warp_max(M);
     const float ref = M == -INFINITY ? 0.f : M;
     float L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     const int d = lane * 4;
+#pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 32) {
         float w = 0.f, lw = 0.f;
         if (i0 + lane < n) {
@@ -1387,8 +1452,10 @@ static cudaError_t narrow_launch(const TreeAttnArgs& a, cudaStream_t st, bool pd
     TreePlan pl;
     pl.grid = 2 * tree_sms();
     pl.rt = F::RT;
-    pl.pt = F::PT;
+    pl.rep = a.n_head / a.n_kv;
+    pl.rep_inv = (65536 + pl.rep - 1) / pl.rep;
     pl.maps = 0;
+    pl.slot_rows = 0;
     pl.min_tiles = 2;
     TreeAttnArgs aa = a;
     void* args[] = {&aa, &pl};
@@ -1397,7 +1464,7 @@ static cudaError_t narrow_launch(const TreeAttnArgs& a, cudaStream_t st, bool pd
     return tree_launch((const void*)tf_tree_combine_kernel, dim3(pl.grid, F::RT / (TC_THREADS / 32)), TC_THREADS, 0, args, st, true);
 }
 
-// The f16 cache as a 2-D tensor map: rows of hd halves, boxes of `pt` rows x 64 halves with the
+// A 16-bit cache as a 2-D tensor map: rows of hd elements, boxes of `pt` rows x 64 elements with the
 // 128-byte swizzle (one 64-dim block of an operand tile).
 static bool tree_map(CUtensorMap* m, const TreeAttnArgs& a, const void* base, int pt) {
     static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> enc{nullptr};
@@ -1439,11 +1506,13 @@ static cudaError_t wide_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl)
     TreePlan pl;
     pl.grid = tree_sms();
     pl.rt = TW_RT;
-    pl.pt = F::PT;
+    pl.rep = a.n_head / a.n_kv;
+    pl.rep_inv = (65536 + pl.rep - 1) / pl.rep;
     pl.min_tiles = 2;
     alignas(64) CUtensorMap maps[2];
     memset(maps, 0, sizeof(maps));
-    pl.maps = KVT == KV_F16 && a.hd == HD && tree_map(&maps[0], a, a.kc, F::PT) && tree_map(&maps[1], a, a.vc, F::PT);
+    pl.slot_rows = (int)(a.slot_stride / a.hd);
+    pl.maps = KVT != KV_F32 && a.hd == HD && tree_map(&maps[0], a, a.kc, F::PT) && tree_map(&maps[1], a, a.vc, F::PT);
     TreeAttnArgs aa = a;
     void* args[] = {&aa, &pl, &maps[0], &maps[1]};
     cudaError_t e = tree_launch(fn, dim3(pl.grid), TW_THREADS, F::SMEM, args, st, pdl);
@@ -1467,6 +1536,8 @@ static cudaError_t narrow_type(const TreeAttnArgs& a, cudaStream_t st, bool pdl)
 }
 
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
+    const long long rows = (long long)a.T * (a.n_head / a.n_kv);
+    if ((long long)a.B * a.n_kv * ((rows + 15) / 16) * ((long long)a.cap / 32 + 1) > 0x7FFFFFFFll - 4096) return cudaErrorInvalidValue;
     return a.hd <= 64 ? narrow_type<64>(a, st, pdl) : narrow_type<128>(a, st, pdl);
 }
 
