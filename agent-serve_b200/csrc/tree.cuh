@@ -52,6 +52,7 @@ struct TreeVerifyArgs {
     int* err;
 };
 size_t tree_verify_ws_bytes(int B, int T, int V);
+int tree_verify_max_vocab(bool draft);  // a row's slices fit the shared memory of a cluster
 cudaError_t tree_verify_launch(const TreeVerifyArgs& a, cudaStream_t st);
 
 struct KvCommitArgs {

@@ -122,6 +122,7 @@ int tf_op_verify_tree(int* path, int* n_path, int* next, const float* logits, lo
     if (!(inv < INFINITY) || (temperature > 0.0f && inv == 0.0f)) return set_error("temperature out of range");
     if (ld < V || (draft && ld_draft < V)) return set_error("ld must be at least V");
     if (!aligned(ws, 256)) return set_error("the workspace must be 256-byte aligned");
+    if (V > tree_verify_max_vocab(draft && temperature > 0.0f)) return set_error("V is above the limit (409600 with draft, 655360 without)");
     if (ws_bytes < tree_verify_ws_bytes(B, T, V)) return set_error("workspace too small");
     TreeVerifyArgs a = {};
     if (op_err_word(&a.err)) return -1;

@@ -17,11 +17,14 @@
 // 64 bits.
 //
 // One thread-block cluster per sequence reads only the rows that its walk visits; each CTA has a
-// contiguous slice of the vocabulary, each warp a contiguous piece of the slice.  A visited row
-// takes two passes (maximum, sums; the second one from L2) with one exchange of C values through
-// distributed shared memory after each; a rejection with a draft distribution and the final pick
-// take one more pass each.  Every CTA holds the same sums in the same order and so takes the same
-// decisions.
+// contiguous slice of the vocabulary, each warp a contiguous piece of the slice, which it brings
+// into shared memory by a bulk copy of its own.  A visited row takes two passes (maximum, then
+// weights, in place, and sums), a rejection with a draft distribution and the final pick one more
+// each over the weights.  After a pass every warp writes its value into every CTA's shared memory,
+// one cluster barrier, and every warp adds the C x 16 values in the same order: all CTAs hold the
+// same sums and take the same decisions.  A walk is a chain of such rows, so its latency bounds
+// it: when all rows of all trees fit on the GPU at once, one cluster per row finds every row's
+// maximum and sum first (ROWS), and the walk behind it takes passes for rejections and picks only.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -35,46 +38,105 @@ namespace tfb {
 constexpr int TV_THREADS = 512;
 constexpr int TV_WARPS = TV_THREADS / 32;
 constexpr int TV_MAX_CLUSTER = 16;
+constexpr int TV_SLOTS = TV_MAX_CLUSTER * TV_WARPS;  // one value per warp of the cluster
 
-// exp(l / temp - max): 1 at the maximum itself (also an infinite one); a NaN logit weighs nothing
-__device__ __forceinline__ float tv_weight(float l, float mx, float inv_temp) {
-    const float e = expf(__fmul_rn(__fsub_rn(l, mx), inv_temp));
-    return l == mx ? 1.f : (l != l ? 0.f : e);
-}
+struct TvStats {                       // of a node's rows: maxima, and 1 / sum of the weights relative to them
+    double ip, iq;
+    float mp, mq;
+    int best, pad;                     // temperature 0: the argmax
+};
+constexpr int TV_MAX_STATS = 18;       // rows whose clusters fit the GPU at once (16 CTAs each, two per SM)
 
 struct TvShared {
-    double ex[2][TV_MAX_CLUSTER][2];   // exchanged values of the cluster's CTAs, two exchanges
-    double red[TV_WARPS][2];
-    unsigned long long key[TV_WARPS];
+    double2 ex[2][TV_SLOTS];           // exchanged values, [rank][warp], of the last two exchanges
+    uint64_t landed[TV_WARPS];
     int par[TREE_MAX_NODES], tok[TREE_MAX_NODES];
     float u[TREE_MAX_NODES];
-    float2 child[TREE_MAX_NODES];      // logits of the current node's children: target, draft
+    float2 child[TREE_MAX_NODES];      // each node's logits in its parent's rows: target, draft
+    TvStats st[TV_MAX_STATS];
     unsigned kids[TREE_MAX_NODES / 32];
     int gone[TREE_MAX_NODES];          // tokens taken out of p at this node
-    int pick;
 };
 
-// N elements of a row from element i on, aligned when VEC (N = 4)
-template <int N>
-__device__ __forceinline__ void tv_load(float (&x)[N], const float* p) {
-    if (N == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(p);
-        x[0] = v.x, x[1 % N] = v.y, x[2 % N] = v.z, x[3 % N] = v.w;
-    } else {
-        x[0] = *p;
+struct TvPlan {
+    int slice, piece;                  // elements of a CTA, of a warp (multiples of 4)
+    int prefetch;                      // few sequences: bring the first child's rows into L2 ahead
+    int stats;                         // walk: the rows' statistics are in the workspace
+};
+
+// A row's softmax weights relative to its maximum: exp((l - max) / temp), 1 at an infinite
+// maximum, 0 for a NaN logit.
+struct TvRow {
+    float mx, inv_temp;
+    bool inf;
+    __device__ __forceinline__ float weight(float l) const {
+        const float e = fmaxf(expf(__fmul_rn(__fsub_rn(l, mx), inv_temp)), 0.f);
+        return inf ? (l == mx ? 1.f : 0.f) : e;
     }
+};
+__device__ __forceinline__ TvRow tv_row(float mx, float inv_temp) { return TvRow{mx, inv_temp, !(fabsf(mx) < INFINITY)}; }
+
+// A warp's piece of logits into weights, in place, and their sums; elements behind its end become
+// weights of zero.  (One copy of the code: it is fetched anew by each CTA.)
+template <bool DRAFT>
+__device__ __noinline__ double2 tv_weights(float* rp, float* rq, int wn, TvRow P, TvRow Q) {
+    double2 s = make_double2(0.0, 0.0);
+#pragma unroll 2
+    for (int i = (threadIdx.x & 31) * 4; i < wn; i += 128) {
+        const int k = wn - i;  // elements left
+        float4 x = *reinterpret_cast<const float4*>(rp + i), y = x;
+        if (DRAFT) y = *reinterpret_cast<const float4*>(rq + i);
+        x = make_float4(P.weight(x.x), k > 1 ? P.weight(x.y) : 0.f, k > 2 ? P.weight(x.z) : 0.f, k > 3 ? P.weight(x.w) : 0.f);
+        *reinterpret_cast<float4*>(rp + i) = x;
+        s.x += ((double)x.x + (double)x.y) + ((double)x.z + (double)x.w);
+        if (DRAFT) {
+            y = make_float4(Q.weight(y.x), k > 1 ? Q.weight(y.y) : 0.f, k > 2 ? Q.weight(y.z) : 0.f, k > 3 ? Q.weight(y.w) : 0.f);
+            *reinterpret_cast<float4*>(rq + i) = y;
+            s.y += ((double)y.x + (double)y.y) + ((double)y.z + (double)y.w);
+        }
+    }
+    __syncwarp();
+    return make_double2(warp_sum_d(s.x), DRAFT ? warp_sum_d(s.y) : 0.0);
 }
 
-template <int N, bool DRAFT>
-__global__ void __launch_bounds__(TV_THREADS, 2) tf_tree_verify_kernel(const __grid_constant__ TreeVerifyArgs a, int slice, int piece) {
-    extern __shared__ uint32_t out_bits[];  // without a draft distribution: the slice's tokens that are out of p
-    __shared__ TvShared sh;
+// the residual p - c q of weights x and y (ip = 1 / sum x, cq = c / sum y)
+template <bool DRAFT>
+__device__ __forceinline__ double tv_left(float x, float y, double ip, double cq) {
+    const double r = (double)x * ip;
+    return DRAFT ? fmax(r - (double)y * cq, 0.0) : r;
+}
+// its sum over a warp's piece
+template <bool DRAFT>
+__device__ __noinline__ double tv_rest(const float* rp, const float* rq, int wn, double ip, double cq) {
+    double s = 0.0;
+#pragma unroll 2
+    for (int i = (threadIdx.x & 31) * 4; i < wn; i += 128) {
+        const float4 x = *reinterpret_cast<const float4*>(rp + i);
+        const float4 y = DRAFT ? *reinterpret_cast<const float4*>(rq + i) : x;
+        s += (tv_left<DRAFT>(x.x, y.x, ip, cq) + tv_left<DRAFT>(x.y, y.y, ip, cq)) +
+             (tv_left<DRAFT>(x.z, y.z, ip, cq) + tv_left<DRAFT>(x.w, y.w, ip, cq));
+    }
+    return warp_sum_d(s);
+}
+
+// VEC: rows are 16-byte aligned and V % 4 == 0 (bulk copies); ROWS: statistics of every node's rows,
+// one cluster each, else the walk, one cluster per sequence
+template <bool VEC, bool DRAFT, bool ROWS>
+__global__ void __launch_bounds__(TV_THREADS, 2)
+    tf_tree_verify_kernel(const __grid_constant__ TreeVerifyArgs a, const __grid_constant__ TvPlan pl) {
+    extern __shared__ __align__(16) float rows[];  // the slice of the target's row, of the draft's
+    __shared__ __align__(16) TvShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-    const int b = blockIdx.x / C, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.V;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.V;
+    const int b = ROWS ? blockIdx.x / C / a.T : blockIdx.x / C;
+    pdl_trigger();
+    pdl_wait();
     const int n = a.n_node ? min(max(a.n_node[b], 0), a.T) : a.T;
+    int cur = ROWS ? blockIdx.x / C % a.T : 0;
+    if (ROWS && cur >= n) return;
     int* path = a.path + (size_t)b * a.T;
-    if (n == 0) {
+    if (!ROWS && n == 0) {
         if (rank == 0) {
             for (int i = tid; i < a.T; i += TV_THREADS) path[i] = -1;
             if (tid == 0) {
@@ -85,215 +147,248 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tf_tree_verify_kernel(const __g
         return;
     }
     const bool greedy = a.inv_temp == 0.f;
-    if (tid < n) {
-        sh.par[tid] = a.parents[(size_t)b * a.T + tid];
-        sh.tok[tid] = a.tokens[(size_t)b * a.T + tid];
-        sh.u[tid] = greedy ? 0.f : a.u[(size_t)b * a.T + tid];
+    TvStats* stats = static_cast<TvStats*>(a.ws);
+    if (!ROWS) {
+        if (tid < n) {
+            sh.par[tid] = a.parents[(size_t)b * a.T + tid];
+            sh.tok[tid] = a.tokens[(size_t)b * a.T + tid];
+            sh.u[tid] = greedy ? 0.f : a.u[(size_t)b * a.T + tid];
+            const int x = sh.tok[tid], p = sh.par[tid];
+            if (!greedy && x >= 0 && x < V && p >= 0 && p < tid) {
+                const size_t r = (size_t)b * a.T + p;
+                sh.child[tid] = make_float2(a.logits[r * a.ld + x], DRAFT ? a.draft[r * a.ld_draft + x] : 0.f);
+            }
+            if (pl.stats) sh.st[tid] = stats[(size_t)b * a.T + tid];
+        }
+        if (rank == 0 && tid < a.T) path[tid] = tid == 0 ? 0 : -1;
     }
-    if (!DRAFT)
-        for (int i = tid; i < (slice + 31) / 32; i += TV_THREADS) out_bits[i] = 0;
-    __syncthreads();
+    if (tid < TV_WARPS) mbar_init(&sh.landed[tid], 1);
+    if (tid == 0) mbar_fence_init();
+    cluster.sync();  // (a CTA's shared memory is written by others only once it runs)
 
-    // this warp's elements: [w0, w1) of the row
-    const int s0 = min(V, rank * slice), s1 = min(V, s0 + slice);
-    const int w0 = min(s1, s0 + warp * piece), w1 = min(s1, w0 + piece);
-    int parity = 0;
-    // the cluster's values of `mine` (two per CTA), by rank, after one barrier
+    // this warp's elements [w0, w1) of the row, at rp and rq
+    const int s0 = min(V, rank * pl.slice), s1 = min(V, s0 + pl.slice);
+    const int w0 = min(s1, s0 + warp * pl.piece), w1 = min(s1, w0 + pl.piece), wn = w1 - w0;
+    float* const rp = rows + warp * pl.piece;
+    float* const rq = rp + pl.slice;
+    int parity = 0, loads = 0;
+    const float *lp = nullptr, *lq = nullptr;
+    auto load_begin = [&]() {
+        if (VEC) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && wn) {
+                mbar_expect_tx(&sh.landed[warp], (uint32_t)wn * (DRAFT ? 8u : 4u));
+                bulk_g2s(rp, lp + w0, (uint32_t)wn * 4u, &sh.landed[warp]);
+                if (DRAFT) bulk_g2s(rq, lq + w0, (uint32_t)wn * 4u, &sh.landed[warp]);
+            }
+        }
+    };
+    auto load_end = [&]() {
+        if (VEC) {
+            if (wn) mbar_wait(&sh.landed[warp], loads & 1, a.err, ERR_WAIT_FULL, nullptr);
+            ++loads;
+        } else {
+#pragma unroll 4
+            for (int i = lane; i < wn; i += 32) {
+                rp[i] = lp[w0 + i];
+                if (DRAFT) rq[i] = lq[w0 + i];
+            }
+        }
+        __syncwarp();
+    };
+    // f(p, q, index) on the lane's vectors of the piece (its last one may reach behind the end)
+    auto each = [&](auto f) {
+#pragma unroll 2
+        for (int i = lane * 4; i < wn; i += 128) {
+            float4 x = *reinterpret_cast<const float4*>(rp + i), y = x;
+            if (DRAFT) y = *reinterpret_cast<const float4*>(rq + i);
+            f(x, y, i);
+        }
+        __syncwarp();
+    };
+    // one value pair per warp to every CTA of the cluster
     auto exchange = [&](double x, double y) {
         parity ^= 1;
-        if (tid < C) {
-            double* o = cluster.map_shared_rank(&sh.ex[parity][rank][0], tid);
-            o[0] = x;
-            o[1] = y;
-        }
+        if (lane < C) *cluster.map_shared_rank(&sh.ex[parity][rank * TV_WARPS + warp], lane) = make_double2(x, y);
         cluster.sync();
     };
-    // block sums of two doubles (every thread gets them)
-    auto block_sum = [&](double& x, double& y) {
+    // the sums of what was exchanged (in the same order in every warp)
+    auto collect = [&](double& x, double& y) {
+        x = y = 0.0;
+#pragma unroll 2
+        for (int i = lane; i < C * TV_WARPS; i += 32) {
+            const double2 v = sh.ex[parity][i];
+            x += v.x;
+            y += v.y;
+        }
         x = warp_sum_d(x);
         if (DRAFT) y = warp_sum_d(y);
-        __syncthreads();
-        if (lane == 0) {
-            sh.red[warp][0] = x;
-            sh.red[warp][1] = y;
-        }
-        __syncthreads();
-        x = y = 0.0;
-#pragma unroll 4
-        for (int w = 0; w < TV_WARPS; ++w) {
-            x += sh.red[w][0];
-            y += sh.red[w][1];
-        }
-    };
-    // f(index, p logit, q logit) over the warp's elements, several loads in flight
-    const float *lp = nullptr, *lq = nullptr;
-    auto each = [&](auto f) {
-#pragma unroll 1
-        for (int i0 = w0 + lane * N; i0 < w1; i0 += 32 * N * 4) {
-            float x[4][N], y[4][N];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = i0 + 32 * N * k;
-                if (i < w1) {
-                    tv_load<N>(x[k], lp + i);
-                    if (DRAFT) tv_load<N>(y[k], lq + i);
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int i = i0 + 32 * N * k;
-#pragma unroll
-                for (int j = 0; j < N; ++j)
-                    if (i + j < w1) f(i + j, x[k][j], DRAFT ? y[k][j] : 0.f);
-            }
-        }
     };
 
-    int cur = 0, count = 1;
-    if (rank == 0)
-        for (int i = tid; i < a.T; i += TV_THREADS) path[i] = i == 0 ? 0 : -1;
+    int count = 1;
     for (;;) {
         lp = a.logits + ((size_t)b * a.T + cur) * a.ld;
         if (DRAFT) lq = a.draft + ((size_t)b * a.T + cur) * a.ld_draft;
-        // the node's children and their logits
-        if (tid < TREE_MAX_NODES) {
+        if (ROWS || !pl.stats) load_begin();
+        // the node's children (read after the next barrier)
+        if (!ROWS && tid < TREE_MAX_NODES) {
             const bool kid = tid > cur && tid < n && sh.par[tid] == cur;
             const unsigned m = __ballot_sync(0xFFFFFFFFu, kid);
             if (lane == 0) sh.kids[warp] = m;
-            if (kid && !greedy) {
-                const int x = sh.tok[tid];
-                if (x >= 0 && x < V) sh.child[tid] = make_float2(lp[x], DRAFT ? lq[x] : 0.f);
+            if (pl.prefetch && !pl.stats && m) {
+                const size_t t = (size_t)b * a.T + 32 * warp + __ffs(m) - 1;
+#pragma unroll 1
+                for (int i = s0 + 32 * lane; i < s1; i += 32 * 32) {
+                    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.logits + t * a.ld + i));
+                    if (DRAFT) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.draft + t * a.ld_draft + i));
+                }
             }
         }
-        // pass 1: the maximum (temperature 0: with its first place)
         int best = 0;
-        float mp = -INFINITY, mq = -INFINITY;
-        if (greedy) {
-            unsigned long long key = 0;
-            each([&](int i, float x, float) {
-                const unsigned long long k = argmax_key(x, (uint32_t)i);
-                key = k > key ? k : key;
-            });
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, key, o);
-                key = k > key ? k : key;
-            }
+        TvRow P, Q;
+        double ip = 0.0, iq = 0.0;
+        bool weights = false;  // the slice holds weights
+        if (!ROWS && pl.stats) {
+            best = sh.st[cur].best;
+            P = tv_row(sh.st[cur].mp, a.inv_temp);
+            Q = tv_row(sh.st[cur].mq, a.inv_temp);
+            ip = sh.st[cur].ip;
+            iq = sh.st[cur].iq;
             __syncthreads();
-            if (lane == 0) sh.key[warp] = key;
-            __syncthreads();
-            for (int w = 0; w < TV_WARPS; ++w) key = sh.key[w] > key ? sh.key[w] : key;
-            exchange(__longlong_as_double((long long)key), 0.0);
-            for (int r = 0; r < C; ++r) {
-                const unsigned long long k = (unsigned long long)__double_as_longlong(sh.ex[parity][r][0]);
-                key = k > key ? k : key;
-            }
-            best = (int)key_index(key);
         } else {
-            each([&](int, float x, float y) {
-                mp = fmaxf(mp, x);
-                if (DRAFT) mq = fmaxf(mq, y);
-            });
-            mp = warp_max(mp);
-            if (DRAFT) mq = warp_max(mq);
-            __syncthreads();
-            if (lane == 0) {
-                sh.red[warp][0] = (double)mp;
-                sh.red[warp][1] = (double)mq;
-            }
-            __syncthreads();
-            for (int w = 0; w < TV_WARPS; ++w) {
-                mp = fmaxf(mp, (float)sh.red[w][0]);
-                mq = fmaxf(mq, (float)sh.red[w][1]);
-            }
-            exchange((double)mp, (double)mq);
-            for (int r = 0; r < C; ++r) {
-                mp = fmaxf(mp, (float)sh.ex[parity][r][0]);
-                mq = fmaxf(mq, (float)sh.ex[parity][r][1]);
+            load_end();
+            if (greedy) {  // the maximum with its first place
+                unsigned long long key = 0;
+                each([&](float4 x, float4, int i) {
+                    const float v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const unsigned long long k = i + e < wn ? argmax_key(v[e], (uint32_t)(w0 + i + e)) : 0ull;
+                        key = k > key ? k : key;
+                    }
+                });
+                auto key_max = [&]() {
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, key, o);
+                        key = k > key ? k : key;
+                    }
+                };
+                key_max();
+                exchange(__longlong_as_double((long long)key), 0.0);
+#pragma unroll 1
+                for (int i = lane; i < C * TV_WARPS; i += 32) {
+                    const unsigned long long k = (unsigned long long)__double_as_longlong(sh.ex[parity][i].x);
+                    key = k > key ? k : key;
+                }
+                key_max();
+                best = (int)key_index(key);
+            } else {
+                float mp = -INFINITY, mq = -INFINITY;
+                each([&](float4 x, float4 y, int i) {
+                    const int k = wn - i;
+                    mp = fmaxf(mp, x.x);
+                    if (k > 1) mp = fmaxf(mp, x.y);
+                    if (k > 2) mp = fmaxf(mp, x.z);
+                    if (k > 3) mp = fmaxf(mp, x.w);
+                    if (DRAFT) {
+                        mq = fmaxf(mq, y.x);
+                        if (k > 1) mq = fmaxf(mq, y.y);
+                        if (k > 2) mq = fmaxf(mq, y.z);
+                        if (k > 3) mq = fmaxf(mq, y.w);
+                    }
+                });
+                mp = warp_max(mp);
+                if (DRAFT) mq = warp_max(mq);
+                exchange((double)mp, (double)mq);
+#pragma unroll 1
+                for (int i = lane; i < C * TV_WARPS; i += 32) {
+                    const double2 v = sh.ex[parity][i];
+                    mp = fmaxf(mp, (float)v.x);
+                    mq = fmaxf(mq, (float)v.y);
+                }
+                P = tv_row(warp_max(mp), a.inv_temp);
+                Q = DRAFT ? tv_row(warp_max(mq), a.inv_temp) : P;
+                const double2 ws = tv_weights<DRAFT>(rp, rq, wn, P, Q);
+                weights = true;
+                exchange(ws.x, ws.y);
+                double Sp, Sq;
+                collect(Sp, Sq);
+                ip = 1.0 / Sp;
+                if (DRAFT) iq = 1.0 / Sq;
             }
         }
-        // pass 2: the sums
-        double Sp = 0.0, Sq = 0.0;
-        if (!greedy) {
-            each([&](int, float x, float y) {
-                Sp += (double)tv_weight(x, mp, a.inv_temp);
-                if (DRAFT) Sq += (double)tv_weight(y, mq, a.inv_temp);
-            });
-            block_sum(Sp, Sq);
-            exchange(Sp, Sq);
-            Sp = Sq = 0.0;
-            for (int r = 0; r < C; ++r) {
-                Sp += sh.ex[parity][r][0];
-                Sq += sh.ex[parity][r][1];
-            }
+        if (ROWS) {
+            if (rank == 0 && tid == 0)
+                stats[(size_t)b * a.T + cur] = greedy ? TvStats{0.0, 0.0, 0.f, 0.f, best, 0} : TvStats{ip, iq, P.mx, DRAFT ? Q.mx : 0.f, 0, 0};
+            return;
         }
-        const double ip = 1.0 / Sp;
-        // the weight of a token in the residual p - c q, and the residual's sum over the cluster
-        auto left = [&](float x, float y, double cq) {
-            const double r = (double)tv_weight(x, mp, a.inv_temp) * ip;
-            return DRAFT ? fmax(r - (double)tv_weight(y, mq, a.inv_temp) * cq, 0.0) : r;
+        auto need_weights = [&]() {
+            if (weights) return;
+            load_begin();
+            load_end();
+            tv_weights<DRAFT>(rp, rq, wn, P, Q);
+            weights = true;
         };
         double c = 0.0, W = 1.0;
         int n_gone = 0, taken = -1;
 #pragma unroll 1
-        for (int w = 0; w < (n + 31) / 32 && taken < 0; ++w)
-#pragma unroll 1
-            for (unsigned m = sh.kids[w]; m && taken < 0; m &= m - 1) {
-                const int t = 32 * w + __ffs(m) - 1, x = sh.tok[t];
-                if (x < 0 || x >= V) {
-                    if (tid == 0 && rank == 0) atomicCAS(a.err, 0, ERR_BAD_TOKEN);
-                    continue;
-                }
-                if (greedy) {
-                    if (x == best) taken = t;
-                    continue;
-                }
-                const float2 l = sh.child[t];
-                const double ut = (double)sh.u[t];
-                if (DRAFT) {
-                    const double qx = (double)tv_weight(l.y, mq, a.inv_temp) / Sq;
-                    if (ut * W * qx < left(l.x, l.y, c / Sq)) {
-                        taken = t;
-                    } else {
-                        c += W;
-                        const double cq = c / Sq;
-                        double s = 0.0, z = 0.0;
-                        each([&](int, float p, float q) { s += left(p, q, cq); });
-                        block_sum(s, z);
-                        exchange(s, 0.0);
-                        W = 0.0;
-                        for (int r = 0; r < C; ++r) W += sh.ex[parity][r][0];
-                        if (!(W > 0.0)) {
-                            c = 0.0;
-                            W = 1.0;
-                        }
-                    }
+        for (int t = cur + 1; t < n && taken < 0; ++t) {
+            // the next child from t on
+            const unsigned m = sh.kids[t >> 5] >> (t & 31);
+            if (!m) {
+                t |= 31;
+                continue;
+            }
+            t += __ffs(m) - 1;
+            const int x = sh.tok[t];
+            if (x < 0 || x >= V) {
+                if (tid == 0 && rank == 0) atomicCAS(a.err, 0, ERR_BAD_TOKEN);
+                continue;
+            }
+            if (greedy) {
+                if (x == best) taken = t;
+                continue;
+            }
+            const float2 l = sh.child[t];
+            const float xw = P.weight(l.x);
+            const double ut = (double)sh.u[t];
+            if (DRAFT) {
+                const float yw = Q.weight(l.y);
+                if (ut * W * ((double)yw * iq) < tv_left<DRAFT>(xw, yw, ip, c * iq)) {
+                    taken = t;
                 } else {
-                    const bool out = __syncthreads_or(tid < n_gone && sh.gone[tid] == x);
-                    const double r = out ? 0.0 : left(l.x, 0.f, 0.0);
-                    if (ut * W < r) {
-                        taken = t;
-                    } else if (!out) {
-                        W -= r;
-                        if (tid == 0) {
-                            sh.gone[n_gone] = x;
-                            if (x >= s0 && x < s1) out_bits[(x - s0) >> 5] |= 1u << ((x - s0) & 31);
-                        }
-                        ++n_gone;
-                        __syncthreads();
+                    need_weights();
+                    c += W;
+                    double z;
+                    exchange(tv_rest<DRAFT>(rp, rq, wn, ip, c * iq), 0.0);
+                    collect(W, z);
+                    if (!(W > 0.0)) {
+                        c = 0.0;
+                        W = 1.0;
                     }
                 }
+            } else {
+                const bool out = __syncthreads_or(tid < n_gone && sh.gone[tid] == x);
+                const double r = out ? 0.0 : tv_left<DRAFT>(xw, 0.f, ip, 0.0);
+                if (ut * W < r) {
+                    taken = t;
+                } else if (!out) {
+                    W -= r;
+                    if (tid == 0) {
+                        sh.gone[n_gone] = x;
+                    }
+                    ++n_gone;
+                    __syncthreads();
+                }
             }
+        }
         if (taken >= 0) {
-            if (tid == 0) {
-                if (rank == 0) path[count] = taken;
-                if (!DRAFT)
-                    for (int g = 0; g < n_gone; ++g)
-                        if (sh.gone[g] >= s0 && sh.gone[g] < s1) out_bits[(sh.gone[g] - s0) >> 5] = 0;
-            }
+            if (rank == 0 && tid == 0) path[count] = taken;
             ++count;
             cur = taken;
-            __syncthreads();
+            __syncthreads();  // the children's table is read
             continue;
         }
         // no child: the next token
@@ -302,120 +397,150 @@ __global__ void __launch_bounds__(TV_THREADS, 2) tf_tree_verify_kernel(const __g
             if (rank == 0 && tid == 0) a.next[b] = best;
             return;
         }
-        const double cq = DRAFT ? c / Sq : 0.0;
-        auto rest = [&](int i, float p, float q) -> double {
-            if (!DRAFT && n_gone && (out_bits[(i - s0) >> 5] >> ((i - s0) & 31) & 1)) return 0.0;
-            return left(p, q, cq);
-        };
-        double mine = 0.0;
-        each([&](int i, float p, float q) { mine += rest(i, p, q); });
-        mine = warp_sum_d(mine);
-        __syncthreads();
-        if (lane == 0) sh.red[warp][0] = mine;
-        __syncthreads();
-        double sum = 0.0;
-        for (int w = 0; w < TV_WARPS; ++w) sum += sh.red[w][0];
-        exchange(sum, 0.0);
-        double total = 0.0;
-        for (int r = 0; r < C; ++r) total += sh.ex[parity][r][0];
-        const double lim = (double)sh.u[0] * total;
-        // the CTA, then the warp, whose part holds the limit (the last one with mass if rounding leaves none)
-        double before = 0.0, at = 0.0;
-        int cta = -1;
-        for (int r = 0; r < C; ++r) {
-            const double v = sh.ex[parity][r][0];
-            if (v > 0.0) {
-                cta = r;
-                at = before;
-                if (before + v > lim) break;
+        need_weights();
+        const double cq = c * iq;
+        if (!DRAFT && n_gone) {  // tokens out of p weigh nothing
+            for (int g = lane; g < n_gone; g += 32) {
+                const int x = sh.gone[g];
+                if (x >= w0 && x < w1) rp[x - w0] = 0.f;
             }
-            before += v;
+            __syncwarp();
         }
-        if (cta < 0) {  // a row without mass
+        exchange(tv_rest<DRAFT>(rp, rq, wn, ip, cq), 0.0);
+        // the warp whose piece holds the limit: lane i has the 8 pieces from 8 i on (pieces of rank
+        // r's warp w are number r * 16 + w); the last piece with mass if rounding leaves none
+        double v[8], inc = 0.0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            v[k] = 8 * lane + k < C * TV_WARPS ? sh.ex[parity][8 * lane + k].x : 0.0;
+            inc += v[k];
+        }
+        const double own = inc;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double z = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+            if (lane >= o) inc += z;
+        }
+        const double lim = (double)sh.u[0] * __shfl_sync(0xFFFFFFFFu, inc, 31);
+        double at = inc - own, hit_at = 0.0;
+        int hit = -1;   // the lane's piece: the first that passes the limit, else its last with mass
+        bool over = false;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (v[k] > 0.0 && !over) {
+                hit = 8 * lane + k;
+                hit_at = at;
+                over = at + v[k] > lim;
+            }
+            at += v[k];
+        }
+        const unsigned any = __ballot_sync(0xFFFFFFFFu, over), some = __ballot_sync(0xFFFFFFFFu, hit >= 0);
+        if (!some) {  // a row without mass
             if (rank == 0 && tid == 0) a.next[b] = 0;
             return;
         }
-        if (cta != rank) return;
-        before = at;
-        int hit = -1;
-        for (int w = 0; w < TV_WARPS; ++w) {
-            const double v = sh.red[w][0];
-            if (v > 0.0) {
-                hit = w;
-                at = before;
-                if (before + v > lim) break;
-            }
-            before += v;
-        }
-        if (warp != hit) return;
-        // 32 elements at a time: their prefix sums, the first that exceeds the limit
+        const int src = any ? __ffs(any) - 1 : 31 - __clz(some);
+        hit = __shfl_sync(0xFFFFFFFFu, hit, src);
+        at = __shfl_sync(0xFFFFFFFFu, hit_at, src);
+        if (hit != rank * TV_WARPS + warp) return;
+        // 128 elements at a time, four per lane: prefix sums, the first that passes the limit
         int last = -1;
-        for (int i0 = w0; i0 < w1; i0 += 32) {
-            const int i = i0 + lane;
-            const double r = i < w1 ? rest(i, lp[i], DRAFT ? lq[i] : 0.f) : 0.0;
-            double inc = r;
+#pragma unroll 1
+        for (int i0 = 0; i0 < wn; i0 += 128) {
+            const int i = i0 + 4 * lane;
+            double r[4] = {0.0, 0.0, 0.0, 0.0}, sum = 0.0;
+            if (i < wn) {
+                const float4 x = *reinterpret_cast<const float4*>(rp + i), y = DRAFT ? *reinterpret_cast<const float4*>(rq + i) : x;
+                r[0] = tv_left<DRAFT>(x.x, y.x, ip, cq), r[1] = tv_left<DRAFT>(x.y, y.y, ip, cq);
+                r[2] = tv_left<DRAFT>(x.z, y.z, ip, cq), r[3] = tv_left<DRAFT>(x.w, y.w, ip, cq);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum += r[k];
+            double s = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const double v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-                if (lane >= o) inc += v;
+                const double z = __shfl_up_sync(0xFFFFFFFFu, s, o);
+                if (lane >= o) s += z;
             }
-            const unsigned over = __ballot_sync(0xFFFFFFFFu, r > 0.0 && at + inc > lim), some = __ballot_sync(0xFFFFFFFFu, r > 0.0);
-            if (over) {
-                if (lane == 0) a.next[b] = i0 + __ffs(over) - 1;
+            double run = at + (s - sum);
+            int first = -1, pos = -1;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                run += r[k];
+                if (r[k] > 0.0) {
+                    pos = i + k;
+                    if (first < 0 && run > lim) first = i + k;
+                }
+            }
+            const unsigned m = __ballot_sync(0xFFFFFFFFu, first >= 0), w = __ballot_sync(0xFFFFFFFFu, pos >= 0);
+            if (m) {
+                if (lane == __ffs(m) - 1) a.next[b] = w0 + first;
                 return;
             }
-            if (some) last = i0 + 31 - __clz(some);
-            at += __shfl_sync(0xFFFFFFFFu, inc, 31);
+            if (w) last = w0 + __shfl_sync(0xFFFFFFFFu, pos, 31 - __clz(w));
+            at += __shfl_sync(0xFFFFFFFFu, s, 31);
         }
         if (lane == 0) a.next[b] = last;
         return;
     }
 }
 
-size_t tree_verify_ws_bytes(int, int, int) { return 256; }
+size_t tree_verify_ws_bytes(int B, int T, int) { return 256 + (size_t)B * T * sizeof(TvStats); }
 
-template <int N, bool DRAFT>
-static cudaError_t verify_launch(const TreeVerifyArgs& a, int C, cudaStream_t st) {
-    auto fn = tf_tree_verify_kernel<N, DRAFT>;
-    // slices of whole warps' pieces, pieces of whole vectors of 32 lanes
-    const int unit = 32 * N, piece = ((a.V + C * TV_WARPS - 1) / (C * TV_WARPS) + unit - 1) / unit * unit, slice = piece * TV_WARPS;
-    const size_t smem = DRAFT ? 0 : (size_t)(slice + 31) / 32 * 4;
+int tree_verify_max_vocab(bool draft) { return (TV_MAX_CLUSTER * (200 * 1024 / (draft ? 8 : 4))) / 1024 * 1024; }
+
+template <bool VEC, bool DRAFT, bool ROWS>
+static cudaError_t verify_launch(const TreeVerifyArgs& a, int C, TvPlan pl, cudaStream_t st, bool pdl) {
+    auto fn = tf_tree_verify_kernel<VEC, DRAFT, ROWS>;
+    pl.piece = ((a.V + C * TV_WARPS - 1) / (C * TV_WARPS) + 3) / 4 * 4;
+    pl.slice = pl.piece * TV_WARPS;
+    const size_t smem = (size_t)pl.slice * (DRAFT ? 8 : 4);
     static std::atomic<bool> ready[64] = {};  // set once per device; twice is harmless
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64) dev = 0;
     if (!ready[dev]) {
         cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         if (e != cudaSuccess) return e;
         ready[dev].store(true);
     }
-    if (smem > 100 * 1024) return cudaErrorInvalidValue;
-    if (smem > 40 * 1024) {
-        cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-    }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(a.B * C));
+    cfg.gridDim = dim3((unsigned)((ROWS ? a.B * a.T : a.B) * C));
     cfg.blockDim = dim3(TV_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = (unsigned)C;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, fn, a, slice, piece);
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, fn, a, pl);
+}
+
+template <bool VEC, bool DRAFT>
+static cudaError_t verify_run(const TreeVerifyArgs& a, cudaStream_t st) {
+    TvPlan pl = {};
+    const int C = TV_MAX_CLUSTER;
+    pl.prefetch = a.B <= 8;
+    pl.stats = a.T > 1 && a.B * a.T <= TV_MAX_STATS;
+    if (pl.stats) {
+        const cudaError_t e = verify_launch<VEC, DRAFT, true>(a, C, pl, st, false);
+        if (e != cudaSuccess) return e;
+    }
+    return verify_launch<VEC, DRAFT, false>(a, C, pl, st, pl.stats);
 }
 
 cudaError_t tree_verify_launch(const TreeVerifyArgs& a, cudaStream_t st) {
-    // CTAs per sequence: up to 16 while the batch leaves SMs free, so that two CTAs per SM hold it
-    int C = TV_MAX_CLUSTER;
-    while (C > 1 && (long long)a.B * C > 296) C /= 2;
     const bool vec = a.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 &&
                      (!a.draft || (a.ld_draft % 4 == 0 && (reinterpret_cast<uintptr_t>(a.draft) & 15) == 0)) && a.V % 4 == 0;
-    if (a.draft) return vec ? verify_launch<4, true>(a, C, st) : verify_launch<1, true>(a, C, st);
-    return vec ? verify_launch<4, false>(a, C, st) : verify_launch<1, false>(a, C, st);
+    if (a.draft) return vec ? verify_run<true, true>(a, st) : verify_run<false, true>(a, st);
+    return vec ? verify_run<true, false>(a, st) : verify_run<false, false>(a, st);
 }
 
 }  // namespace tfb
