@@ -26,6 +26,8 @@
 namespace tfb {
 
 constexpr int TN_THREADS = 256;
+constexpr int TN_UNIT_COST = 2;       // tiles that a unit's start and end take the time of: narrow, wide kernel
+constexpr int TW_UNIT_COST = 5;
 constexpr int TN_TILE_BYTES = 32768;  // K and V bytes of a tile in the cache's type: 32 registers per thread
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPShift = 15.f;       // p is held as 2^15 exp(s - max): its low half keeps 2^-24 / 2^15 of it
@@ -80,82 +82,70 @@ struct TreeSeg {
     int b, kvh, rtile, t0, t1, tiles, last_cta;  // last_cta: the CTA that ends the unit
 };
 
-// Finds this CTA's range.  Block-wide; NT threads.
-template <int NT, int PT, int RT>
+// Each unit counts for its tiles and UC more, the time (in tiles) that starting and ending a unit
+// takes.  Finds this CTA's range; every warp by itself, lanes over the sequences.
+template <int PT, int RT, int UC>
 __device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan& pl, TreeIter& it) {
-    __shared__ int wsum[NT / 32], found_base, found_b;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int chunk = (a.B + NT - 1) / NT, lo = min(a.B, tid * chunk), hi = min(a.B, lo + chunk);
+    const int lane = threadIdx.x & 31;
+    const int chunk = (a.B + 31) >> 5, lo = min(a.B, lane * chunk), hi = min(a.B, lo + chunk);
     int mine = 0;
 #pragma unroll 1
     for (int b = lo; b < hi; ++b) {
         const TreeSeq s = tree_seq(a, b);
-        mine += seq_tiles<PT>(s) * seq_units<RT>(a.n_kv, pl.rep, s);
-        if (s.bad && blockIdx.x == 0) atomicCAS(a.err, 0, ERR_POS);
+        if (s.n_node) mine += (seq_tiles<PT>(s) + UC) * seq_units<RT>(a.n_kv, pl.rep, s);
+        if (s.bad && blockIdx.x == 0 && threadIdx.x < 32) atomicCAS(a.err, 0, ERR_POS);
     }
     int inc = mine;
-#pragma unroll 1
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
         if (lane >= o) inc += v;
     }
-    if (lane == 31) wsum[warp] = inc;
-    if (tid == 0) {
-        found_b = a.B;
-        found_base = 0;
-    }
-    __syncthreads();
-    int before = inc - mine, total = 0;
-#pragma unroll 1
-    for (int w = 0; w < NT / 32; ++w) {
-        if (w < warp) before += wsum[w];
-        total += wsum[w];
-    }
-    it.per = (unsigned)(total + pl.grid - 1) / (unsigned)pl.grid;
-    if (it.per < pl.min_tiles) it.per = pl.min_tiles;
+    const int total = __shfl_sync(0xFFFFFFFFu, inc, 31);
+    it.per = max((int)((unsigned)(total + pl.grid - 1) / (unsigned)pl.grid), pl.min_tiles);
     it.g0 = (int)min((long long)it.per * blockIdx.x, (long long)total);
     it.g1 = min(it.g0 + it.per, total);
-    if (it.g0 >= before && it.g0 < before + mine) {
+    // the lane whose sequences hold g0, then the sequence
+    const unsigned in = __ballot_sync(0xFFFFFFFFu, it.g0 < inc);
+    const int src = in ? __ffs(in) - 1 : 31;
+    int base = inc - mine, b = lo;
+    if (lane == src)
 #pragma unroll 1
-        for (int b = lo; b < hi; ++b) {
+        for (; b + 1 < hi; ++b) {
             const TreeSeq s = tree_seq(a, b);
-            const int t = seq_tiles<PT>(s) * seq_units<RT>(a.n_kv, pl.rep, s);
-            if (it.g0 < before + t) {
-                found_b = b;
-                found_base = before;
-                break;
-            }
-            before += t;
+            const int t = s.n_node ? (seq_tiles<PT>(s) + UC) * seq_units<RT>(a.n_kv, pl.rep, s) : 0;
+            if (it.g0 < base + t) break;
+            base += t;
         }
-    }
-    __syncthreads();
-    it.b = found_b;
-    it.base = found_base;
+    it.b = __shfl_sync(0xFFFFFFFFu, b, src);
+    it.base = __shfl_sync(0xFFFFFFFFu, base, src);
 }
 
-template <int PT, int RT>
+template <int PT, int RT, int UC>
 __device__ __forceinline__ bool tree_next(const TreeAttnArgs& a, int rep, TreeIter& it, TreeSeg& o) {
-    if (it.g0 >= it.g1) return false;
-    o.s = tree_seq(a, it.b);
-    o.tiles = seq_tiles<PT>(o.s);
-    int units = seq_units<RT>(a.n_kv, rep, o.s);
 #pragma unroll 1
-    while (it.g0 >= it.base + o.tiles * units) {  // next sequence with work
-        it.base += o.tiles * units;
-        o.s = tree_seq(a, ++it.b);
+    while (it.g0 < it.g1) {
+        o.s = tree_seq(a, it.b);
         o.tiles = seq_tiles<PT>(o.s);
-        units = seq_units<RT>(a.n_kv, rep, o.s);
+        const int nrt = (unsigned)(o.s.n_node * rep + RT - 1) / RT, cost = o.tiles + UC;
+        if (!o.s.n_node || it.g0 >= it.base + cost * a.n_kv * nrt) {  // next sequence
+            if (o.s.n_node) it.base += cost * a.n_kv * nrt;
+            ++it.b;
+            continue;
+        }
+        const int unit = (unsigned)(it.g0 - it.base) / (unsigned)cost;
+        const int u0 = it.base + unit * cost;  // the unit's start
+        o.t0 = max(0, it.g0 - u0 - UC);
+        o.t1 = min(it.g1 - u0, cost) - UC;
+        it.g0 = min(it.g1, u0 + cost);
+        if (o.t1 <= o.t0) continue;
+        o.b = it.b;
+        o.kvh = (unsigned)unit / (unsigned)nrt;
+        o.rtile = unit - o.kvh * nrt;
+        o.last_cta = (unsigned)(u0 + cost - 1) / (unsigned)it.per;
+        return true;
     }
-    const int unit = (unsigned)(it.g0 - it.base) / (unsigned)o.tiles, nrt = (unsigned)(o.s.n_node * rep + RT - 1) / RT;
-    const int u0 = it.base + unit * o.tiles;  // the unit's first tile
-    o.b = it.b;
-    o.kvh = (unsigned)unit / (unsigned)nrt;
-    o.rtile = unit - o.kvh * nrt;
-    o.t0 = it.g0 - u0;
-    o.t1 = min(it.g1 - u0, o.tiles);
-    o.last_cta = (unsigned)(u0 + o.tiles - 1) / (unsigned)it.per;
-    it.g0 = u0 + o.t1;
-    return true;
+    return false;
 }
 
 // Rows that no unit covers (nodes from n_node on, bad sequences) are zero.
@@ -250,6 +240,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+// Whether a tile whose largest |x| is maxbits may be split after the scale 2^-e: its maximum within
+// [2^-4, 2^15), so that nothing overflows and the low halves keep 21 bits below it; and an exponent
+// that puts it in the middle.
+__device__ __forceinline__ bool tile_fits(uint32_t maxbits, int e) {
+    const int x = (int)(maxbits >> 23) - 127 - e;
+    return maxbits == 0 || (x >= -4 && x < 15);
+}
+__device__ __forceinline__ int tile_exponent(uint32_t maxbits) {
+    const int e = (int)(maxbits >> 23) - 127 - 6;
+    return e < -126 ? -126 : (e > 126 ? 126 : e);
+}
 // exponent e such that |x| 2^-e lies in [2^14, 2^15) for the largest finite |x| (its bits
 // without sign), kept where 2^e and 2^-e are normal numbers
 __device__ __forceinline__ int half_exponent(uint32_t maxbits) {
@@ -405,11 +406,12 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
     TreeDesc* desc = static_cast<TreeDesc*>(a.ws);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + 65536);
     TreeIter it;
-    tree_range<TN_THREADS, PT, RT>(a, pl, it);
+    tree_range<PT, RT, TN_UNIT_COST>(a, pl, it);
     if (tid == 0) desc[blockIdx.x].b = -1;
 
     TreeSeg sg;
-    while (tree_next<PT, RT>(a, rep, it, sg)) {
+    int ek = 0, ev = 0;  // scale exponents of K and V, kept from tile to tile
+    while (tree_next<PT, RT, TN_UNIT_COST>(a, rep, it, sg)) {
         const TreeSeq s = sg.s;
         const int b = sg.b, kvh = sg.kvh, rtile = sg.rtile, t0 = sg.t0, t1 = sg.t1;
         const int end = s.n_ctx + s.n_node, rows = s.n_node * rep;
@@ -483,7 +485,6 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
 
 #pragma unroll 1
         for (int t = t0; t < t1; ++t) {
-            int ek = 0, ev = 0;
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             const bool tail = (t + 1) * PT > s.n_ctx;
             const uint32_t kh = sb + (KVT == KV_F16 ? (uint32_t)(t & 1) * TN_TILE_BYTES : TN_TILE_BYTES), vh = kh + HALF_TILE;
@@ -503,49 +504,54 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
                 }
             }
             if (KVT != KV_F16) {
+                if (t > t0) __syncthreads();  // the last tile's operands are free
+                // split after the last tile's scale; when the maximum turns out not to fit it
+                // (seldom), once more after its own
+                for (;;) {
 #pragma unroll 1
-                for (int which = 0; which < 2; ++which) {
-                    uint32_t mb = 0;
+                    for (int which = 0; which < 2; ++which) {
+                        const float f = pow2i(which ? -ev : -ek);
+                        const uint32_t dst = which ? vh : kh;
+                        uint32_t mb = 0;
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) mb = max(mb, abs_bits<KVT>(ld_shared16(mine + i * OSTEP + which * HALF_TILE)));
-                    if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
-                        mb = 0;
-#pragma unroll 1
-                        for (int i = 0; i < NV; ++i) mb = max(mb, max_bits<KVT>(ld_shared16(mine + i * OSTEP + which * HALF_TILE)));
-                    }
-                    mb = __reduce_max_sync(0xFFFFFFFFu, mb);
-                    if (lane == 0) atomicMax(&tmax[2 * (t & 1) + which], mb);
-                }
-                __syncthreads();  // the maxima; the last tile's operands are free
-                ek = half_exponent(tmax[2 * (t & 1)]);
-                ev = half_exponent(tmax[2 * (t & 1) + 1]);
-                if (tid < 2) tmax[2 * (~t & 1) + tid] = 0;  // the next tile's, last read a barrier ago
-#pragma unroll 1
-                for (int which = 0; which < 2; ++which) {
-                    const float f = pow2i(which ? -ev : -ek);
-                    const uint32_t dst = which ? vh : kh;
+                        for (int i = 0; i < NV; ++i) {
+                            const int r = r0 + i * RSTEP;
+                            const uint4 x = ld_shared16(mine + i * OSTEP + which * HALF_TILE);
+                            mb = max(mb, abs_bits<KVT>(x));
+                            if (KVT == KV_F32) {
+                                uint32_t h0, l0, h1, l1;
+                                split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), make_float2(f, f)), h0, l0);
+                                split2t(__fmul2_rn(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), make_float2(f, f)), h1, l1);
+                                const uint32_t o = dst + (uint32_t)r * (HD * 2) + ((((uint32_t)c0 >> 1) ^ (r & 7)) << 4) + (c0 & 1) * 8;
+                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
+                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::TILE_H), "r"(l0), "r"(l1) : "memory");
+                            } else {
+                                uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) {
-                        const int r = r0 + i * RSTEP;
-                        const uint4 x = ld_shared16(mine + i * OSTEP + which * HALF_TILE);
-                        if (KVT == KV_F32) {
-                            uint32_t h0, l0, h1, l1;
-                            split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), make_float2(f, f)), h0, l0);
-                            split2t(__fmul2_rn(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), make_float2(f, f)), h1, l1);
-                            const uint32_t o = dst + (uint32_t)r * (HD * 2) + ((((uint32_t)c0 >> 1) ^ (r & 7)) << 4) + (c0 & 1) * 8;
-                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
-                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::TILE_H), "r"(l0), "r"(l1) : "memory");
-                        } else {
-                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
-                            st_shared16(dst + (uint32_t)r * (HD * 2) + (((uint32_t)c0 ^ (r & 7)) << 4), w);
+                                for (int j = 0; j < 4; ++j)
+                                    w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
+                                st_shared16(dst + (uint32_t)r * (HD * 2) + (((uint32_t)c0 ^ (r & 7)) << 4), w);
+                            }
                         }
+                        if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
+                            mb = 0;
+#pragma unroll 1
+                            for (int i = 0; i < NV; ++i) mb = max(mb, max_bits<KVT>(ld_shared16(mine + i * OSTEP + which * HALF_TILE)));
+                        }
+                        mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+                        if (lane == 0) atomicMax(&tmax[2 * (t & 1) + which], mb);
                     }
+                    __syncthreads();
+                    const uint32_t mk = tmax[2 * (t & 1)], mv = tmax[2 * (t & 1) + 1];
+                    const bool fk = tile_fits(mk, ek), fv = tile_fits(mv, ev);
+                    if (fk && fv) break;
+                    if (!fk) ek = tile_exponent(mk);
+                    if (!fv) ev = tile_exponent(mv);
                 }
+                if (tid < 2) tmax[2 * (~t & 1) + tid] = 0;  // the next tile's, last read two barriers ago
+            } else {
+                __syncthreads();
             }
-            __syncthreads();
             if (t + 1 < t1) load(t + 1);
             if (!active) continue;
             const float fk = pow2i(ek), fv = pow2i(ev);
@@ -560,7 +566,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
                     for (int j = 0; j < 4; ++j) S[i][j] = S1[i][j] = 0.f;
                 const int ra = wm * 16 + (lane & 15), ca = lane >> 4, rb = pl0 + (lane & 7) + ((lane >> 4) << 3), cb = (lane >> 3) & 1;
                 const uint32_t qrow = (uint32_t)ra * (HD * 2), krow = kh + (uint32_t)rb * (HD * 2);
-#pragma unroll 2
+#pragma unroll 4
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     uint32_t ah[4], al[4];
                     const uint32_t oa = qrow + (uint32_t)(((2 * kk + ca) ^ (ra & 7)) << 4);
@@ -910,8 +916,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + 65536);
     if (tid == 0) desc[blockIdx.x].b = -1;
     TreeIter it;
+    tree_range<PT, TW_RT, TW_UNIT_COST>(a, pl, it);
     tc_fence_before();
-    tree_range<TW_THREADS, PT, TW_RT>(a, pl, it);  // (block barriers inside)
+    __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
     TreeSeg sg;
@@ -942,7 +949,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         constexpr int VPR = HD * ESZ / 16, RSTEP = LT / VPR;  // 16-byte vectors per row, rows per step of all loaders
         constexpr int UNR = KVT == KV_F32 ? 4 : 2;
         const int r0 = lt / VPR, c0 = lt % VPR;
-        while (tree_next<PT, TW_RT>(a, rep, it, sg)) {
+        while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
             if (lt < TREE_MAX_NODES / 32) sh.badrow[seg & 7][lt] = 0;  // read by others long ago
             named_bar<2, LT>();
@@ -1069,7 +1076,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         if (KVT != KV_F16 && lane == 0) {
             int n = 0, nr = 0, nd = 0;
             unsigned issued = 0, par = 0;  // per barrier: a copy was issued, parity of the last one
-            while (tree_next<PT, TW_RT>(a, rep, it, sg))
+            while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg))
 #pragma unroll 1
                 for (int t = sg.t0; t < sg.t1; ++t, ++n)
 #pragma unroll 1
@@ -1120,7 +1127,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         auto wait = [&](uint64_t* bar, int parity) {
             ok = __all_sync(0xFFFFFFFFu, ok && tree_wait(bar, parity, a.err, ERR_WAIT_FULL, abort_flag));
         };
-        while (tree_next<PT, TW_RT>(a, rep, it, sg)) {
+        while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             wait(&sh.qfull, seg);
             // QK of tile t, then PV of tile t - 1 (one step more than there are tiles)
 #pragma unroll 1
@@ -1178,7 +1185,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
         const uint32_t ts = tl + wg * 128, td = tl + 256 + wg * HD;
         int n = 0, seg = 0, cnt = 0;
-        while (tree_next<PT, TW_RT>(a, rep, it, sg)) {
+        while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
             const int rows = s.n_node * rep;
             {   // queries, HD / 8 lanes per row: scaled to [2^14, 2^15), two halves
