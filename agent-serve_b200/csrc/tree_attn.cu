@@ -325,8 +325,10 @@ __device__ __forceinline__ uint32_t abs_bits(const uint4& x) {
     const uint32_t v = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
     return max(v << 16, v & 0xFFFF0000u);
 }
-__device__ __forceinline__ uint32_t finite_max4(const float4& x) {
-    return max(max(finite_abs_bits(x.x), finite_abs_bits(x.y)), max(finite_abs_bits(x.z), finite_abs_bits(x.w)));
+// largest |x| of eight values (NaN aside), as fp32 bits
+__device__ __forceinline__ uint32_t max8(const float4& x, const float4& y) {
+    return __float_as_uint(fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
+                                 fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
 }
 // eight values times f in two halves
 __device__ __forceinline__ void split8(const float4& x, const float4& y, float f, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
@@ -349,7 +351,7 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
                  : "memory");
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -458,7 +460,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
                 }
                 if (j0 == 0) vis_fill(vis[r], a, s, b, node);
 #pragma unroll
-                for (int i = 0; i < UPT; ++i) mb = max(mb, max(finite_max4(x[i][0]), finite_max4(x[i][1])));
+                for (int i = 0; i < UPT; ++i) mb = max(mb, max8(x[i][0], x[i][1]));
 #pragma unroll
                 for (int o = 1; o < TPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
                 const int e = half_exponent(mb);
@@ -513,10 +515,13 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
                         const float f = pow2i(which ? -ev : -ek);
                         const uint32_t dst = which ? vh : kh;
                         uint32_t mb = 0;
+                        uint4 xs[NV];  // (all loads before the first store: the compiler keeps their order)
+#pragma unroll
+                        for (int i = 0; i < NV; ++i) xs[i] = ld_shared16(mine + i * OSTEP + which * HALF_TILE);
 #pragma unroll
                         for (int i = 0; i < NV; ++i) {
                             const int r = r0 + i * RSTEP;
-                            const uint4 x = ld_shared16(mine + i * OSTEP + which * HALF_TILE);
+                            const uint4 x = xs[i];
                             mb = max(mb, abs_bits<KVT>(x));
                             if (KVT == KV_F32) {
                                 uint32_t h0, l0, h1, l1;
@@ -861,20 +866,26 @@ __device__ __forceinline__ void wide_rows_out(const TreeAttnArgs& a, const TreeS
     constexpr int LPR = HD / 8, RPW = 32 / LPR;  // lanes per half row, rows per warp and step
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % LPR, d = h * (HD / 2) + c * 4;
     const int rows = sg.s.n_node * rep, hd = a.hd;
-#pragma unroll 2
-    for (int i = warp; i < TW_RT / RPW; i += 8) {
-        const int r = i * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
-        if (q >= rows || d >= hd || *abort_flag) continue;
+    if (*abort_flag) return;
+    constexpr int U = TW_RT / RPW / 8;
+    uint4 x[U], y[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const int r = (warp + 8 * k) * RPW + lane / LPR;
         const uint32_t at = stage + (uint32_t)r * (HD * 2) + ((uint32_t)(c ^ (r & 7)) << 4);
-        const uint4 x = ld_shared16(at), y = ld_shared16(at + TW_RT * HD * 2);
+        x[k] = ld_shared16(at);
+        y[k] = ld_shared16(at + TW_RT * HD * 2);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+        const int r = (warp + 8 * k) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
         const float f = scale[r].x;
-        float4 o = make_float4(__uint_as_float(x.x) + __uint_as_float(y.x), __uint_as_float(x.y) + __uint_as_float(y.y),
-                               __uint_as_float(x.z) + __uint_as_float(y.z), __uint_as_float(x.w) + __uint_as_float(y.w));
         // (a row that saw nothing has the factor 0 and zeros; its sum cannot be anything else)
-        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+        const float4 o = make_float4((__uint_as_float(x[k].x) + __uint_as_float(y[k].x)) * f, (__uint_as_float(x[k].y) + __uint_as_float(y[k].y)) * f,
+                                     (__uint_as_float(x[k].z) + __uint_as_float(y[k].z)) * f, (__uint_as_float(x[k].w) + __uint_as_float(y[k].w)) * f);
         float* dst = whole ? a.out + ((size_t)sg.b * a.T + nd) * a.ld_out + (size_t)(sg.kvh * rep + q - nd * rep) * hd
                            : part + (size_t)r * hd;
-        *reinterpret_cast<float4*>(dst + d) = o;
+        if (q < rows && d < hd) *reinterpret_cast<float4*>(dst + d) = o;
     }
 }
 __device__ __forceinline__ bool badrow_any(const unsigned* badrow) {
@@ -947,7 +958,8 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         const int lt = wg == 2 ? tid - 256 : tid - 320;
         int n = 0, nr = 0, nd = 0, seg = 0;  // running tile, raw buffer, direct tile, segment
         constexpr int VPR = HD * ESZ / 16, RSTEP = LT / VPR;  // 16-byte vectors per row, rows per step of all loaders
-        constexpr int UNR = KVT == KV_F32 ? 4 : 2;
+        constexpr int UNR = 6;               // vectors in flight per thread
+        int ek = 0, ev = 0;                  // scale exponents of K and V, kept from tile to tile
         const int r0 = lt / VPR, c0 = lt % VPR;
         while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
@@ -1009,46 +1021,75 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         }
                     }
                     if (KVT != KV_F16) {
-                        // the tile's largest finite |x|
-                        uint32_t mb = 0;
-                        if (col) {
-#pragma unroll 4
-                            for (int r = r0; r < rows; r += RSTEP) mb = max(mb, abs_bits<KVT>(ld_shared16(at(r))));
-                        }
-                        if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: once more without them
-                            mb = 0;
-                            if (col)
-#pragma unroll 1
-                                for (int r = r0; r < rows; r += RSTEP) mb = max(mb, max_bits<KVT>(ld_shared16(at(r))));
-                            __syncwarp();
-                        }
-                        mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+                        // split after the last tile's scale; when the maximum turns out not to fit it
+                        // (seldom), once more after its own.  bf16 tiles are converted in place, so
+                        // their maximum is found first.
                         unsigned* tm = &sh.tmax[2 * (n & 1) + which];
-                        if (lane == 0) atomicMax(tm, mb);
-                        named_bar<2, LT>();
-                        const int e = half_exponent(*tm);
-                        const float f = pow2i(-e);
+                        for (;;) {
+                            const int e = which ? ev : ek;
+                            const float f = pow2i(-e);
+                            uint32_t mb = 0;
+                            // (batches: all loads before the first store, the compiler keeps their order)
+#pragma unroll 1
+                            for (int rb = r0; rb < PT; rb += UNR * RSTEP) {
+                                uint4 x[UNR];
+#pragma unroll
+                                for (int k = 0; k < UNR; ++k) {
+                                    const int r = rb + k * RSTEP;
+                                    x[k] = make_uint4(0, 0, 0, 0);
+                                    if (r < rows && col) x[k] = ld_shared16(at(r));
+                                }
+#pragma unroll
+                                for (int k = 0; k < UNR; ++k) {
+                                    mb = max(mb, abs_bits<KVT>(x[k]));
+                                    const int r = rb + k * RSTEP;
+                                    if (KVT == KV_F32 && r < PT) {
+                                        uint32_t h0, l0, h1, l1;
+                                        split2t(__fmul2_rn(make_float2(__uint_as_float(x[k].x), __uint_as_float(x[k].y)), make_float2(f, f)), h0, l0);
+                                        split2t(__fmul2_rn(make_float2(__uint_as_float(x[k].z), __uint_as_float(x[k].w)), make_float2(f, f)), h1, l1);
+                                        const uint32_t o = dst + wide_off(PT, r, c0 >> 1) + (c0 & 1) * 8;
+                                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
+                                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::HALF), "r"(l0), "r"(l1) : "memory");
+                                    }
+                                }
+                            }
+                            if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
+                                mb = 0;
+                                if (col)
+#pragma unroll 1
+                                    for (int r = r0; r < rows; r += RSTEP) mb = max(mb, max_bits<KVT>(ld_shared16(at(r))));
+                                __syncwarp();
+                            }
+                            mb = __reduce_max_sync(0xFFFFFFFFu, mb);
+                            if (lane == 0) atomicMax(tm, mb);
+                            named_bar<2, LT>();
+                            const uint32_t all = *tm;
+                            if (tile_fits(all, e)) break;
+                            (which ? ev : ek) = tile_exponent(all);
+                            named_bar<2, LT>();  // (the maximum is read by all before it is raised again)
+                        }
                         if (lt == 0) {
                             sh.tmax[2 * (~n & 1) + which] = 0;  // the next tile's, read last a tile ago
-                            (which ? sh.ev : sh.ek)[n & 7] = e;
+                            (which ? sh.ev : sh.ek)[n & 7] = which ? ev : ek;
                         }
-#pragma unroll UNR
-                        for (int r = r0; r < PT; r += RSTEP) {
-                            uint4 x = make_uint4(0, 0, 0, 0);
-                            if (KVT != KV_F32 || (r < rows && col)) x = ld_shared16(at(r));
-                            if (KVT == KV_F32) {
-                                uint32_t h0, l0, h1, l1;
-                                split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), make_float2(f, f)), h0, l0);
-                                split2t(__fmul2_rn(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), make_float2(f, f)), h1, l1);
-                                const uint32_t o = dst + wide_off(PT, r, c0 >> 1) + (c0 & 1) * 8;
-                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
-                                asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::HALF), "r"(l0), "r"(l1) : "memory");
-                            } else {
-                                uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                        if (KVT == KV_BF16) {
+                            const float f = pow2i(which ? -ev : -ek);
+#pragma unroll 1
+                            for (int rb = r0; rb < PT; rb += UNR * RSTEP) {
+                                uint4 x[UNR];
 #pragma unroll
-                                for (int j = 0; j < 4; ++j)
-                                    w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
-                                st_shared16(at(r), w);
+                                for (int k = 0; k < UNR; ++k) {
+                                    x[k] = make_uint4(0, 0, 0, 0);
+                                    if (rb + k * RSTEP < PT) x[k] = ld_shared16(at(rb + k * RSTEP));
+                                }
+#pragma unroll
+                                for (int k = 0; k < UNR; ++k) {
+                                    uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j)
+                                        w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
+                                    if (rb + k * RSTEP < PT) st_shared16(at(rb + k * RSTEP), w);
+                                }
                             }
                         }
                     }
@@ -1189,7 +1230,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
             const TreeSeq s = sg.s;
             const int rows = s.n_node * rep;
             {   // queries, HD / 8 lanes per row: scaled to [2^14, 2^15), two halves
-                constexpr int LPR = HD / 8, RPW = 32 / LPR, STEPS = TW_RT / (8 * RPW), U = 4;
+                constexpr int LPR = HD / 8, RPW = 32 / LPR, STEPS = TW_RT / (8 * RPW), U = STEPS;
                 const int c = lane % LPR;
 #pragma unroll 1
                 for (int i0 = 0; i0 < STEPS; i0 += U) {
@@ -1207,7 +1248,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
                         const int r = ((i0 + i) * 8 + warp) * RPW + lane / LPR;
-                        uint32_t mb = max(finite_max4(x[i][0]), finite_max4(x[i][1]));
+                        uint32_t mb = max8(x[i][0], x[i][1]);
 #pragma unroll
                         for (int o = 1; o < LPR; o <<= 1) mb = max(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
                         const int e = half_exponent(mb);
