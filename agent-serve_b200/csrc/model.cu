@@ -1362,6 +1362,9 @@ int tf_cuda_prefill(tf_model* m, int seq, const int* tokens, int n, float* logit
         }
         CK(cudaMemcpyAsync(m->d_wstart + seq, m->hi + 3, sizeof(int), cudaMemcpyHostToDevice, m->stream));
         m->hpos[seq] += n;
+        // the prompt's logits are row 0 of the last step, as after a short prompt (tf_cuda_sample)
+        CK(cudaMemcpyAsync(m->logits, m->logits + (size_t)(rows - 1) * m->V, sizeof(float) * m->V, cudaMemcpyDeviceToDevice,
+                           m->stream));
         return read_outputs_row(m, rows - 1, logits, argmax_out);
     }
     if (set_slot_row(m, 0, seq, tokens[0])) return -1;
