@@ -28,6 +28,7 @@
 #include "dots.cuh"
 #include "gemm.cuh"
 #include "sample.cuh"
+#include "tree.cuh"
 #include "persist.cuh"
 #include "upload.cuh"
 #include "engine.cuh"
@@ -163,6 +164,17 @@ struct tf_model {
     // of the last step enqueued
     unsigned long long* d_gvtrace = nullptr;
     std::vector<int> gvt_meta;
+    // speculative steps: drafted trees of up to tree_rows nodes (device words; pinned staging)
+    int tree_rows = 0, tree_tile = 1;
+    int tree_n = 0, tree_seq = -1;  // the tree of the last tree step, until it is accepted
+    int *d_ttok = nullptr, *d_tpar = nullptr, *d_tdepth = nullptr;  // tokens, parents, depths
+    unsigned long long* d_tmask = nullptr;
+    float* d_tu = nullptr;
+    int* d_tout = nullptr;          // [tree_rows] path | n_path | next | new position
+    int* d_tpos = nullptr;          // positions the step's finish kernel may advance (not used)
+    uint8_t* d_tws = nullptr;       // workspaces: attention, then verification
+    size_t tws_attn = 0, tws_verify = 0;
+    int* h_tree = nullptr;
     std::string err;
 };
 
@@ -318,7 +330,10 @@ int fuse_attn_ok(const tf_model* m, int end_pos) {
 // `tile` rows with the same prologue and epilogue.  A prefill chunk (`chunk`) computes the
 // lm_head for its last row only: Model::prefill returns that row's logits alone
 // (src/model.cpp:183-195).
-int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk) {
+// A speculative step (`tree`): the M rows are the nodes of one sequence's drafted tree (M >= 1); K and
+// V go to the rows behind the context, attention follows the tree's mask, every node's logits are
+// computed and no position moves.
+int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk, bool tree = false) {
     const int D = m->D, H = m->H, KV = m->KV, FF = m->FF, V = m->V;
     const int ldq = H + 2 * KV;
     int launches = 0;
@@ -391,8 +406,9 @@ int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk) 
             launches += 2;
             return 0;
         }
-        for (int b = 0; b < rows; b += m->tile) {
-            const int mc = std::min(m->tile, rows - b), r = r0 + b;
+        const int tile = tree ? m->tree_tile : m->tile;
+        for (int b = 0; b < rows; b += tile) {
+            const int mc = std::min(tile, rows - b), r = r0 + b;
             GemvArgs a = gemv_base(m, w, q.n_items, q.P, mc);
             a.pro = q.embed ? PRO_EMBED_RMSNORM : q.norm_w ? PRO_RMSNORM : PRO_COPY;
             a.x = q.x + (size_t)r * q.ldx;
@@ -426,13 +442,40 @@ int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk) 
             return -1;
         {
             AttnArgs a = attn_args(m, li);
-            if (chunk) {  // one sequence's prompt rows: store every row's K/V, then attend
+            if (tree) {
+                CK(tree_rope_store_launch(a, m->d_tdepth, M, m->stream));
+                TreeAttnArgs t = {};
+                t.out = m->attn;
+                t.ld_out = H;
+                t.q = m->qkv;
+                t.ld_q = ldq;
+                t.kc = a.kc;
+                t.vc = a.vc;
+                t.kv_type = a.kv_type;
+                t.slot_stride = m->slot_elems;
+                t.cap = m->opt.max_seq;
+                t.n_slots = m->opt.max_batch;
+                t.slots = m->d_slots;
+                t.n_ctx = m->d_tpos + m->opt.max_batch;
+                t.mask = m->d_tmask;
+                t.B = 1;
+                t.T = M;
+                t.n_head = a.n_head;
+                t.n_kv = a.n_kv;
+                t.hd = a.hd;
+                t.ws = m->d_tws;
+                t.err = m->d_err;
+                CK(tree_attn_launch(t, m->stream, true));
+                launches += 3;
+            } else if (chunk) {  // one sequence's prompt rows: store every row's K/V, then attend
                 CK(rope_store_launch(a, M, m->stream));
                 a.fresh = 2;
                 ++launches;
             }
-            CK(attn_decode_launch(a, M, m->stream, true));
-            ++launches;
+            if (!tree) {
+                CK(attn_decode_launch(a, M, m->stream, true));
+                ++launches;
+            }
         }
         if (matmul({&Ld.wo, D, 1, EPI_RESID, m->attn, H, nullptr, false, nullptr, 0, nullptr, m->x, nullptr}, 0, M))
             return -1;
@@ -453,9 +496,9 @@ int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk) 
     f.M = M;
     f.keys = m->keys;
     f.tok_next = m->d_tokens;
-    f.pos = m->d_pos;
+    f.pos = tree ? m->d_tpos : m->d_pos;
     f.slots = m->d_slots;
-    f.hist = m->d_hist;
+    f.hist = tree ? nullptr : m->d_hist;
     f.ctl = m->ctl;
     f.argmax = head ? 1 : 0;
     CK(finish_launch(f, m->stream));
@@ -466,7 +509,8 @@ int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk) 
 
 // fused: CTAs per query head of the attention fused into the QKV kernel (0: separate kernel)
 int enqueue_step(tf_model* m, int M, bool head, bool pdl, int* n_launch, int fused, bool chunk = false,
-                 bool from_key = false) {
+                 bool from_key = false, bool tree = false) {
+    if (tree) return enqueue_step_gemm(m, M, head, n_launch, false, true);
     if (chunk) return enqueue_step_gemm(m, M, head, n_launch, true);
     if (M >= GM_MIN_M && m->gtile >= M) return enqueue_step_gemm(m, M, head, n_launch, false);
     const int D = m->D, H = m->H, KV = m->KV, FF = m->FF, V = m->V;
@@ -627,17 +671,17 @@ int enqueue_step(tf_model* m, int M, bool head, bool pdl, int* n_launch, int fus
 }
 
 // Run one step for M rows (tokens in d_tokens[0..M), slots in d_slots[0..M)).
-int run_step(tf_model* m, int M, bool head, int fused, bool chunk = false, bool from_key = false) {
-    if (!m->opt.use_graph) return enqueue_step(m, M, head, true, nullptr, fused, chunk, from_key);
+int run_step(tf_model* m, int M, bool head, int fused, bool chunk = false, bool from_key = false, bool tree = false) {
+    if (!m->opt.use_graph) return enqueue_step(m, M, head, true, nullptr, fused, chunk, from_key, tree);
     // graphs are keyed by everything that changes the launch sequence or its arguments
     const bool split = head && m->split_step && M == 1;
     const long long key = ((long long)fused << 40) + ((long long)(split ? 1 + m->vs_row0 : 0) << 20) +
-                          (long long)M * 32 + (head ? 1 : 0) + (chunk ? 4 : 0) + (from_key ? 8 : 0);
+                          (long long)M * 32 + (head ? 1 : 0) + (chunk ? 4 : 0) + (from_key ? 8 : 0) + (tree ? 16 : 0);
     auto it = m->graphs.find(key);
     if (it == m->graphs.end()) {
         cudaGraph_t g = nullptr;
         CK(cudaStreamBeginCapture(m->stream, cudaStreamCaptureModeThreadLocal));
-        int rc = enqueue_step(m, M, head, true, nullptr, fused, chunk, from_key);
+        int rc = enqueue_step(m, M, head, true, nullptr, fused, chunk, from_key, tree);
         cudaError_t e = cudaStreamEndCapture(m->stream, &g);
         if (rc) {
             if (g) cudaGraphDestroy(g);
@@ -813,7 +857,7 @@ int finish_call(tf_model* m) {
     if (m->hi[60] != 0) {
         const int c = m->hi[60];
         cudaMemsetAsync(m->d_err, 0, sizeof(int), m->stream);
-        const int T = std::max(m->tile, m->gtile);
+        const int T = std::max(std::max(m->tile, m->tree_rows), std::max(m->gtile, m->ptile));
         cudaMemsetAsync(m->counters, 0, sizeof(unsigned) * (size_t)T * m->hp.n_kv_head, m->stream);
         cudaMemsetAsync(m->ctl, 0, sizeof(unsigned), m->stream);
         cudaMemsetAsync(m->keys, 0, sizeof(unsigned long long) * T, m->stream);
@@ -911,6 +955,10 @@ int tf_cuda_destroy(tf_model* m) {
                    m->xplanes, m->d_gvtrace};
     for (void* p : dev)
         if (p) cudaFree(p);
+    void* tree[] = {m->d_ttok, m->d_tpar, m->d_tdepth, m->d_tmask, m->d_tu, m->d_tout, m->d_tpos, m->d_tws};
+    for (void* p : tree)
+        if (p) cudaFree(p);
+    if (m->h_tree) cudaFreeHost(m->h_tree);
     sample_scratch_destroy(m->smp);
     if (m->hi) cudaFreeHost(m->hi);
     if (m->hb) cudaFreeHost(m->hb);
@@ -1214,7 +1262,10 @@ int tf_cuda_create(const tf_tensor_desc* t, int nt, const tf_hparams* hp_in, con
     m->ptile = m->gemm_ok ? std::min(GM_BM, o.max_seq) : 0;
     if (m->ptile < GM_MIN_M) m->ptile = 0;
     m->n_split = attn_pick_split(o.max_seq);
-    const int T = std::max(m->tile, std::max(m->gtile, m->ptile));
+    // speculative steps: trees of up to 64 nodes, more where prefill chunks are larger
+    m->tree_tile = std::max(1, tile);
+    m->tree_rows = std::min(o.max_seq, std::max(64, m->ptile));
+    const int T = std::max(std::max(m->tile, m->tree_rows), std::max(m->gtile, m->ptile));
     if (m->gtile || m->ptile) {
         const int Kmax = std::max(m->D, std::max(m->H, m->FF));
         const size_t rows = (size_t)(std::max(m->gtile, m->ptile) + GM_ROW_PAD - 1) / GM_ROW_PAD * GM_ROW_PAD;
@@ -1596,7 +1647,7 @@ int tf_cuda_prefill_batch(tf_model* m, const int* seq_ids, const int* tokens, in
 int tf_cuda_sample(tf_model* m, int row, float temperature, float top_p, float r, int* out_id) {
     if (!m) return set_error("null model");
     if (!out_id) return fail(m, "out_id is null");
-    const int T = std::max(m->tile, std::max(m->gtile, m->ptile));
+    const int T = std::max(std::max(m->tile, m->tree_rows), std::max(m->gtile, m->ptile));
     if (row < 0 || row >= T) return fail(m, "row out of range");
     CK(cudaSetDevice(m->device));
     const float* lg = m->logits + (size_t)row * m->V;
@@ -1611,6 +1662,123 @@ int tf_cuda_sample(tf_model* m, int row, float temperature, float top_p, float r
     if (rc) return rc;
     *out_id = m->hb[0];
     return 0;
+}
+
+int tf_cuda_tree_capacity(tf_model* m) { return m ? m->tree_rows : -1; }
+
+void* tf_cuda_logits(tf_model* m) { return m ? static_cast<void*>(m->logits) : nullptr; }
+
+}  // extern "C"
+
+namespace {
+// Buffers of the speculative steps, at the first one.
+int tree_init(tf_model* m) {
+    if (m->h_tree) return 0;
+    const size_t R = (size_t)m->tree_rows;
+    auto round = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    m->tws_attn = round(tree_attn_ws_bytes(1, m->tree_rows, m->hp.n_head, m->hp.n_kv_head, m->hd));
+    m->tws_verify = round(tree_verify_ws_bytes(1, m->tree_rows, m->V));
+    if (!m->d_ttok) CK(cudaMalloc(&m->d_ttok, sizeof(int) * R));
+    if (!m->d_tpar) CK(cudaMalloc(&m->d_tpar, sizeof(int) * R));
+    if (!m->d_tdepth) CK(cudaMalloc(&m->d_tdepth, sizeof(int) * R));
+    if (!m->d_tmask) CK(cudaMalloc(&m->d_tmask, sizeof(unsigned long long) * R * ((R + 63) / 64)));
+    if (!m->d_tu) CK(cudaMalloc(&m->d_tu, sizeof(float) * R));
+    if (!m->d_tout) CK(cudaMalloc(&m->d_tout, sizeof(int) * (R + 3)));
+    if (!m->d_tpos) CK(cudaMalloc(&m->d_tpos, sizeof(int) * (m->opt.max_batch + 1)));
+    if (!m->d_tws) CK(cudaMalloc(&m->d_tws, m->tws_attn + m->tws_verify));
+    CK(cudaMemsetAsync(m->d_tpos, 0, sizeof(int) * (m->opt.max_batch + 1), m->stream));
+    CK(cudaMemsetAsync(m->d_tws, 0, m->tws_attn + m->tws_verify, m->stream));
+    CK(cudaMallocHost(&m->h_tree, sizeof(int) * 5 * R + sizeof(unsigned long long) * R * ((R + 63) / 64) + 64));
+    return 0;
+}
+}  // namespace
+
+extern "C" {
+
+int tf_cuda_tree_step(tf_model* m, int seq, const int* tokens, const int* parents, int n, float* logits, int* argmax_out) {
+    if (!m) return set_error("null model");
+    CK(cudaSetDevice(m->device));
+    if (check_seq(m, seq)) return -1;
+    if (!tokens || !parents) return fail(m, "null tokens or parents");
+    if (n < 1 || n > m->tree_rows) return fail(m, "tree size out of range (tf_cuda_tree_capacity)");
+    if (m->hpos[seq] + n > m->opt.max_seq) return fail(m, "tree step exceeds max_seq");
+    for (int i = 0; i < n; ++i)
+        if (tokens[i] < 0 || tokens[i] >= m->V) return fail(m, "token id out of range");
+    if (tree_init(m)) return -1;
+    // staging: masks | tokens, parents, depths, slots, position
+    unsigned long long* mask = reinterpret_cast<unsigned long long*>(m->h_tree);
+    const size_t words = (size_t)n * ((n + 63) / 64);
+    int* st = reinterpret_cast<int*>(mask + words);
+    CK(cudaStreamSynchronize(m->stream));  // the staging of an earlier call
+    if (tf_tree_mask(parents, n, n, mask, st + 2 * n)) return fail(m, last_error_tls());
+    m->tree_n = 0;
+    memcpy(st, tokens, sizeof(int) * n);
+    memcpy(st + n, parents, sizeof(int) * n);
+    for (int i = 0; i < n; ++i) st[3 * n + i] = seq;
+    st[4 * n] = m->hpos[seq];
+    CK(cudaMemcpyAsync(m->d_tmask, mask, sizeof(unsigned long long) * words, cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_ttok, st, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_tokens, st, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_tpar, st + n, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_tdepth, st + 2 * n, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_slots, st + 3 * n, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_tpos + m->opt.max_batch, st + 4 * n, sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    if (run_step(m, n, true, 0, false, false, true)) return -1;
+    const int rc = read_outputs(m, n, logits, argmax_out);
+    if (rc) return rc;
+    m->tree_n = n;
+    m->tree_seq = seq;
+    return 0;
+}
+
+int tf_cuda_tree_accept(tf_model* m, int seq, const float* draft, float temperature, const float* u, int* nodes, int* n_nodes,
+                        int* next) {
+    if (!m) return set_error("null model");
+    CK(cudaSetDevice(m->device));
+    if (check_seq(m, seq)) return -1;
+    if (!nodes || !n_nodes || !next) return fail(m, "null outputs");
+    if (m->tree_n < 1 || m->tree_seq != seq) return fail(m, "no tree step of this sequence to accept");
+    const int n = m->tree_n;
+    if (temperature > 0.0f) {
+        if (!u) return fail(m, "u must not be null at a positive temperature");
+        memcpy(m->h_tree, u, sizeof(float) * n);
+        CK(cudaMemcpyAsync(m->d_tu, m->h_tree, sizeof(float) * n, cudaMemcpyHostToDevice, m->stream));
+    }
+    int *path = m->d_tout, *n_path = path + m->tree_rows, *nx = n_path + 1, *pos = nx + 1;
+    if (tf_op_verify_tree(path, n_path, nx, m->logits, m->V, draft, m->V, m->d_ttok, m->d_tpar, nullptr, m->d_tu, temperature, 1,
+                          n, m->V, m->d_tws + m->tws_attn, m->tws_verify, m->stream))
+        return fail(m, last_error_tls());
+    const int* n_ctx = m->d_tpos + m->opt.max_batch;
+    if (tf_op_kv_commit(m->kc, m->vc, m->opt.kv_type, m->hp.n_layer, m->layer_elems, m->slot_elems, m->opt.max_seq,
+                        m->opt.max_batch, m->d_slots, n_ctx, path, n, n_path, pos, 1, m->hp.n_kv_head, m->hd, m->stream))
+        return fail(m, last_error_tls());
+    CK(cudaMemcpyAsync(m->d_pos + seq, pos, sizeof(int), cudaMemcpyDeviceToDevice, m->stream));
+    int* back = m->h_tree + m->tree_rows;
+    CK(cudaMemcpyAsync(back, m->d_tout, sizeof(int) * (m->tree_rows + 3), cudaMemcpyDeviceToHost, m->stream));
+    m->tree_n = 0;
+    const int rc = finish_call(m);
+    if (rc) return rc;
+    int code = 0;
+    if (tf_op_device_error(m->stream, &code)) return fail(m, last_error_tls());
+    if (code) return fail(m, err_code_text(code));
+    const int k = back[m->tree_rows];
+    memcpy(nodes, back, sizeof(int) * k);
+    *n_nodes = k;
+    *next = back[m->tree_rows + 1];
+    m->hpos[seq] = back[m->tree_rows + 2];
+    return 0;
+}
+
+int tf_cuda_rewind(tf_model* m, int seq, int n_pos) {
+    if (!m) return set_error("null model");
+    CK(cudaSetDevice(m->device));
+    if (check_seq(m, seq)) return -1;
+    if (n_pos < 0 || n_pos > m->hpos[seq]) return fail(m, "a sequence can be rewound to an earlier position only");
+    m->hi[2] = n_pos;
+    CK(cudaMemcpyAsync(m->d_pos + seq, m->hi + 2, sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    m->hpos[seq] = n_pos;
+    if (m->tree_seq == seq) m->tree_n = 0;
+    return finish_call(m);
 }
 
 int tf_cuda_n_pos(tf_model* m, int seq) {

@@ -72,5 +72,7 @@ struct KvCommitArgs {
     int* err;
 };
 cudaError_t kv_commit_launch(const KvCommitArgs& a, cudaStream_t st);
+// RoPE at each node's depth and K / V store of a tree step's M nodes (AttnArgs of the step)
+cudaError_t tree_rope_store_launch(const AttnArgs& a, const int* depth, int M, cudaStream_t st);
 
 }  // namespace tfb

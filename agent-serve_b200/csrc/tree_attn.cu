@@ -40,7 +40,6 @@ struct TreePlan {
     int rt;                  // rows per row tile
     int rep;                 // query heads per kv head
     int rep_inv;             // (x * rep_inv) >> 16 = x / rep for x < 2048 and rep <= 8
-    int min_tiles;           // tiles per CTA at least
 };
 struct TreeDesc {            // a unit split over CTAs c0..c1, found at slot c0
     int b, kvh, rtile, c1;   // b < 0: none
@@ -88,11 +87,15 @@ template <int PT, int RT, int UC>
 __device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan& pl, TreeIter& it) {
     const int lane = threadIdx.x & 31;
     const int chunk = (a.B + 31) >> 5, lo = min(a.B, lane * chunk), hi = min(a.B, lo + chunk);
-    int mine = 0;
+    int mine = 0, units = 0;
 #pragma unroll 1
     for (int b = lo; b < hi; ++b) {
         const TreeSeq s = tree_seq(a, b);
-        if (s.n_node) mine += (seq_tiles<PT>(s) + UC) * seq_units<RT>(a.n_kv, pl.rep, s);
+        if (s.n_node) {
+            const int u = seq_units<RT>(a.n_kv, pl.rep, s);
+            mine += (seq_tiles<PT>(s) + UC) * u;
+            units += u;
+        }
         if (s.bad && blockIdx.x == 0 && threadIdx.x < 32) atomicCAS(a.err, 0, ERR_POS);
     }
     int inc = mine;
@@ -102,7 +105,10 @@ __device__ __forceinline__ void tree_range(const TreeAttnArgs& a, const TreePlan
         if (lane >= o) inc += v;
     }
     const int total = __shfl_sync(0xFFFFFFFFu, inc, 31);
-    it.per = max((int)((unsigned)(total + pl.grid - 1) / (unsigned)pl.grid), pl.min_tiles);
+    // (units of two tiles and less stay whole: a split unit costs the second kernel's work)
+    units = __reduce_add_sync(0xFFFFFFFFu, units);
+    const int least = total - units * UC <= 2 * units ? 2 + UC : 2;
+    it.per = max((int)((unsigned)(total + pl.grid - 1) / (unsigned)pl.grid), least);
     it.g0 = (int)min((long long)it.per * blockIdx.x, (long long)total);
     it.g1 = min(it.g0 + it.per, total);
     // the lane whose sequences hold g0, then the sequence
@@ -1504,7 +1510,6 @@ static cudaError_t narrow_launch(const TreeAttnArgs& a, cudaStream_t st, bool pd
     pl.rep_inv = (65536 + pl.rep - 1) / pl.rep;
     pl.maps = 0;
     pl.slot_rows = 0;
-    pl.min_tiles = 2;
     TreeAttnArgs aa = a;
     void* args[] = {&aa, &pl};
     cudaError_t e = tree_launch(fn, dim3(pl.grid), TN_THREADS, F::SMEM, args, st, pdl);
@@ -1556,7 +1561,6 @@ static cudaError_t wide_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl)
     pl.rt = TW_RT;
     pl.rep = a.n_head / a.n_kv;
     pl.rep_inv = (65536 + pl.rep - 1) / pl.rep;
-    pl.min_tiles = 2;
     alignas(64) CUtensorMap maps[2];
     memset(maps, 0, sizeof(maps));
     pl.slot_rows = (int)(a.slot_stride / a.hd);

@@ -63,6 +63,56 @@ __global__ void __launch_bounds__(KC_THREADS) tf_kv_commit_kernel(const KvCommit
     }
 }
 
+// ---- the drafted nodes' rows: RoPE of q (in place) and k at the node's depth, K / V store -------------
+// Node m of the sequence in slots[m] stands at position pos[slot] + depth[m] and takes cache row
+// pos[slot] + m (siblings share a position).  One CTA per (node, head), a thread per rotation pair,
+// as the prefill chunk's kernel.
+__global__ void tf_tree_rope_store_kernel(const AttnArgs a, const int* depth) {
+    pdl_trigger();
+    pdl_wait();
+    const int m = blockIdx.x, h = blockIdx.y, j = threadIdx.x;
+    const int hd = a.hd, d2 = hd / 2;
+    const int slot = a.slots[m], row_pos = a.pos[slot] + m, pos = a.pos[slot] + depth[m];
+    if (a.pos[slot] < 0 || row_pos >= a.cap || depth[m] < 0 || depth[m] > m) {
+        if (j == 0) atomicCAS(a.err, 0, ERR_POS);
+        return;
+    }
+    float* row = const_cast<float*>(a.qkv) + (size_t)m * a.ld_qkv;
+    const float c = a.cosb[(size_t)pos * d2 + j], sn = a.sinb[(size_t)pos * d2 + j];
+    if (h < a.n_head) {
+        float* q = row + (size_t)h * hd;
+        float x0 = q[j], x1 = q[j + d2];
+        rope_pair(x0, x1, c, sn);
+        q[j] = x0;
+        q[j + d2] = x1;
+    } else {
+        const int kvh = h - a.n_head;
+        const float* k = row + (size_t)a.n_head * hd + (size_t)kvh * hd;
+        const float* v = row + (size_t)(a.n_head + a.n_kv) * hd + (size_t)kvh * hd;
+        float x0 = k[j], x1 = k[j + d2];
+        rope_pair(x0, x1, c, sn);
+        const size_t off = (size_t)slot * a.slot_stride + (size_t)kvh * a.cap * hd + (size_t)row_pos * hd;
+        kv_store(a.kc, (long long)(off + j), a.kv_type, x0);
+        kv_store(a.kc, (long long)(off + j + d2), a.kv_type, x1);
+        kv_store(a.vc, (long long)(off + j), a.kv_type, v[j]);
+        kv_store(a.vc, (long long)(off + j + d2), a.kv_type, v[j + d2]);
+    }
+}
+
+cudaError_t tree_rope_store_launch(const AttnArgs& a, const int* depth, int M, cudaStream_t st) {
+    if (a.hd > AT_MAX_HD || a.hd % 2) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(M, a.n_head + a.n_kv);
+    cfg.blockDim = dim3(a.hd / 2);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, tf_tree_rope_store_kernel, a, depth);
+}
+
 cudaError_t kv_commit_launch(const KvCommitArgs& a, cudaStream_t st) {
     const long long warps = (long long)a.n_layer * a.B * a.n_kv * 2, per = KC_THREADS / 32;
     if ((warps + per - 1) / per > 0x7FFFFFFFll) return cudaErrorInvalidValue;

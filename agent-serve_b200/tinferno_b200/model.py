@@ -126,6 +126,36 @@ def tensor_descs(g: GGUFReader):
     return arr, keep
 
 
+def lookup_tree(text: Sequence[int], width: int, depth: int, room: int):
+    """(tokens, parents) of a drafted tree under the text's last token: the continuations of up to
+    `width` latest earlier occurrences of the last two tokens (else of the last one), `depth` tokens
+    each, common beginnings shared, at most `room` nodes."""
+    tokens, parents, kids = [int(text[-1])], [-1], {}
+    for g in (2, 1):
+        if len(text) <= g:
+            continue
+        key, found = list(text[-g:]), 0
+        for i in range(len(text) - g - 1, -1, -1):
+            if list(text[i:i + g]) != key:
+                continue
+            cur = 0
+            for x in text[i + g:i + g + depth]:
+                nxt = kids.get((cur, x))
+                if nxt is None:
+                    if len(tokens) >= room:
+                        break
+                    nxt = kids[(cur, x)] = len(tokens)
+                    tokens.append(int(x))
+                    parents.append(cur)
+                cur = nxt
+            found += 1
+            if found >= width or len(tokens) >= room:
+                break
+        if found:
+            break
+    return tokens, parents
+
+
 class Model:
     def __init__(self, path: str, cfg: Optional[RunConfig] = None):
         self.cfg = cfg or RunConfig()
@@ -233,6 +263,78 @@ class Model:
             out.append(t)
             self.decode(t)
         return out
+
+    # ---- speculative decoding (include/tinferno_b200.h, tf_cuda_tree_step / tf_cuda_tree_accept) ----
+    @property
+    def tree_capacity(self) -> int:
+        """Drafted tokens per tree, the root included."""
+        return int(self.L.tf_cuda_tree_capacity(self.h))
+
+    @property
+    def logits_ptr(self) -> int:
+        """Device address of the last step's logits [rows][n_vocab]."""
+        return int(self.L.tf_cuda_logits(self.h) or 0)
+
+    def tree_step(self, tokens: Sequence[int], parents: Sequence[int], seq: int = 0, want_logits: bool = False):
+        """One forward pass over a tree of drafted tokens: tokens[0] is the token decode() would take
+        next, parents[0] = -1, every other node's parent precedes it.  Returns the greedy id after
+        each node (and the logits).  The position stays; tree_accept keeps what is right."""
+        t = np.ascontiguousarray(tokens, dtype=np.int32)
+        p = np.ascontiguousarray(parents, dtype=np.int32)
+        if t.ndim != 1 or t.shape != p.shape:
+            raise ValueError("tokens and parents must be lists of the same length")
+        am = np.zeros(max(1, len(t)), np.int32)
+        lg = np.empty((len(t), self.n_vocab), np.float32) if want_logits else None
+        native.check(self.L.tf_cuda_tree_step(self.h, seq, t.ctypes.data_as(native.i32p), p.ctypes.data_as(native.i32p),
+                                              len(t), lg.ctypes.data_as(native.f32p) if want_logits else None,
+                                              am.ctypes.data_as(native.i32p)), self.h)
+        self._tree = t
+        return (am, lg) if want_logits else am
+
+    def tree_accept(self, temperature: float = 0.0, u: Optional[Sequence[float]] = None, draft_ptr: int = 0, seq: int = 0):
+        """Verifies the last tree_step's tree against the model's distribution at `temperature`
+        (draft_ptr: device address of the [nodes][n_vocab] logits that each node's children were drawn
+        from, 0 for drafts without a distribution; u: one uniform number per node).  Returns
+        (accepted tokens, next token); the accepted path stays in the cache, next is the next root."""
+        n = len(self._tree)
+        nodes, k, nxt = np.zeros(n, np.int32), C.c_int(0), C.c_int(0)
+        uu = np.zeros(n, np.float32) if u is None else np.ascontiguousarray(u, dtype=np.float32)
+        if len(uu) < n:
+            raise ValueError("u needs one number per node")
+        native.check(self.L.tf_cuda_tree_accept(self.h, seq, C.c_void_p(draft_ptr) if draft_ptr else None, float(temperature),
+                                                uu.ctypes.data_as(native.f32p), nodes.ctypes.data_as(native.i32p),
+                                                C.byref(k), C.byref(nxt)), self.h)
+        return [int(self._tree[i]) for i in nodes[1:k.value]], nxt.value
+
+    def rewind(self, n_pos: int, seq: int = 0):
+        """Back to an earlier position of the sequence (the cache rows behind it are overwritten later)."""
+        native.check(self.L.tf_cuda_rewind(self.h, seq, int(n_pos)), self.h)
+
+    def generate_lookup(self, prompt: Sequence[int], n: int, temperature: float = 0.0, seed: int = 42, eos: int = -1,
+                        width: int = 3, depth: int = 6, seq: int = 0) -> list:
+        """generate() with drafts looked up in the text so far: each step drafts the tokens that
+        followed the latest occurrences of the last two tokens (else of the last one), as a tree of up
+        to `width` branches of `depth` tokens, and keeps what the model's own distribution keeps.  The
+        tokens follow the same distribution as generate() at top_p = 1; at temperature 0 they are the
+        greedy ones."""
+        rng = Mt19937Uniform(seed)
+        text = [int(t) for t in prompt]
+        self.prefill(text, seq=seq)
+        root = self.sample(temperature, 1.0, rng.next() if temperature > 0 else 0.0)
+        out = [root]
+        while len(out) < n and not (root == eos and len(out) > 1):
+            text.append(root)
+            room = min(self.tree_capacity, self.cfg.max_seq - self.n_pos(seq), n - len(out))
+            tokens, parents = lookup_tree(text, width, depth, room)
+            self.tree_step(tokens, parents, seq=seq)
+            u = [rng.next() for _ in tokens] if temperature > 0 else None
+            kept, root = self.tree_accept(temperature, u, seq=seq)
+            text += kept
+            out += kept + [root]
+            if eos >= 0 and eos in out[1:]:
+                out = out[:out.index(eos, 1)]
+                break
+        return out[:n]
 
     # ---- vocab-split lm_head (include/tinferno_b200.h, tf_cuda_set_vocab_shard) ----
     def set_vocab_shard(self, rank: int, world: int):

@@ -64,6 +64,11 @@ SIGNATURES = [
     ("tf_cuda_trace_read", C.c_int, [_V, C.POINTER(C.c_ulonglong), C.c_int, i32p]),
     ("tf_cuda_launch_trace", C.c_int, [_V, C.POINTER(C.c_ulonglong), C.c_int, i32p, i32p]),
     ("tf_cuda_reset", C.c_int, [_V, C.c_int]),
+    ("tf_cuda_tree_step", C.c_int, [_V, C.c_int, i32p, i32p, C.c_int, f32p, i32p]),
+    ("tf_cuda_tree_accept", C.c_int, [_V, C.c_int, _V, C.c_float, f32p, i32p, i32p, i32p]),
+    ("tf_cuda_rewind", C.c_int, [_V, C.c_int, C.c_int]),
+    ("tf_cuda_tree_capacity", C.c_int, [_V]),
+    ("tf_cuda_logits", C.c_void_p, [_V]),
     ("tf_cuda_n_pos", C.c_int, [_V, C.c_int]),
     ("tf_cuda_n_vocab", C.c_int, [_V]),
     ("tf_cuda_weight_bytes", C.c_ulonglong, [_V]),

@@ -165,6 +165,29 @@ TF_API int tf_cuda_launch_trace(tf_model* m, unsigned long long* out, int max_la
 /* Model::reset()  src/model.cpp:80-83 (one slot; seq < 0 resets every slot). */
 TF_API int tf_cuda_reset(tf_model* m, int seq);
 
+/* Speculative decoding of one sequence, no reference counterpart (one token per weight pass,
+ * src/main.cpp:106-122); the operators below on the engine's own buffers:
+ *   tf_cuda_tree_step    one forward pass over a tree of n drafted tokens (the root, the token that
+ *                        decode would take next, first; parents[0] < 0, parents[i] < i).  Logits of
+ *                        every node (host, n * n_vocab, optional) and greedy ids (host, n, optional)
+ *                        come back; the position does not move;
+ *   tf_cuda_tree_accept  verifies that tree (tf_op_verify_tree: `draft`, device memory [n][n_vocab]
+ *                        or nullptr; u, host, n uniform numbers, for temperature > 0), moves the
+ *                        kept path's K/V rows up in every layer and advances the position by the
+ *                        path's length.  nodes (host, n ints) receives the kept nodes, the root
+ *                        first, *n_nodes their count, *next the token after them: the next root;
+ *   tf_cuda_rewind       takes a sequence back to an earlier position (a draft model's cache after
+ *                        a refused draft);
+ *   tf_cuda_tree_capacity  nodes per tree (64, or the prefill chunk's rows);
+ *   tf_cuda_logits       device address of the last step's logits [rows][n_vocab]. */
+TF_API int tf_cuda_tree_step(tf_model* m, int seq, const int* tokens, const int* parents, int n, float* logits,
+                             int* argmax_out);
+TF_API int tf_cuda_tree_accept(tf_model* m, int seq, const float* draft, float temperature, const float* u, int* nodes,
+                               int* n_nodes, int* next);
+TF_API int tf_cuda_rewind(tf_model* m, int seq, int n_pos);
+TF_API int tf_cuda_tree_capacity(tf_model* m);
+TF_API void* tf_cuda_logits(tf_model* m);
+
 /* Accessors: Model::n_pos / n_vocab / weight_bytes  src/model.hpp:35-43. */
 TF_API int tf_cuda_n_pos(tf_model* m, int seq);
 TF_API int tf_cuda_n_vocab(tf_model* m);
