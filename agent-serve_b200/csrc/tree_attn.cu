@@ -332,6 +332,21 @@ __device__ __forceinline__ uint32_t abs_bits(const uint4& x) {
     return max(v << 16, v & 0xFFFF0000u);
 }
 // largest |x| of eight values (NaN aside), as fp32 bits
+// running maximum of |x| over vectors, cheaper: fp32 as a float, bf16 as two packed values whose
+// signs are not meaningful; NaN aside
+template <int KVT>
+__device__ __forceinline__ void abs_max(uint32_t& m, const uint4& x) {
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (KVT == KV_F32) m = __float_as_uint(fmaxf(__uint_as_float(m), fabsf(__uint_as_float(w[j]))));
+        else asm("max.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(m) : "r"(m), "r"(w[j]));
+    }
+}
+template <int KVT>
+__device__ __forceinline__ uint32_t abs_max_bits(uint32_t m) {
+    return KVT == KV_F32 ? m : max((m << 16) & 0x7FFF0000u, m & 0x7FFF0000u);
+}
 __device__ __forceinline__ uint32_t max8(const float4& x, const float4& y) {
     return __float_as_uint(fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
                                  fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
@@ -967,6 +982,16 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         constexpr int UNR = 6;               // vectors in flight per thread
         int ek = 0, ev = 0;                  // scale exponents of K and V, kept from tile to tile
         const int r0 = lt / VPR, c0 = lt % VPR;
+        // where this thread's vectors of a whole tile go: row r0 + k * RSTEP at rel[k % NB] + k * RSTEP * 128
+        // (the swizzle depends on the row modulo 8)
+        constexpr int NVT = (PT + RSTEP - 1) / RSTEP, NB = RSTEP % 8 == 0 ? 1 : (RSTEP % 4 == 0 ? 2 : 4);
+        uint32_t rel[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int c = KVT == KV_F32 ? c0 >> 1 : c0;
+            rel[j] = wide_off(PT, r0, c) - (uint32_t)(((c & 7) ^ (r0 & 7)) << 4) + (uint32_t)(((c & 7) ^ ((r0 + j * RSTEP) & 7)) << 4) +
+                     (KVT == KV_F32 ? (c0 & 1) * 8 : 0);
+        }
         while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
             if (lt < TREE_MAX_NODES / 32) sh.badrow[seg & 7][lt] = 0;  // read by others long ago
@@ -1031,32 +1056,57 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         // (seldom), once more after its own.  bf16 tiles are converted in place, so
                         // their maximum is found first.
                         unsigned* tm = &sh.tmax[2 * (n & 1) + which];
+                        // a whole tile's vectors lie at compile-time distances; this thread's last one
+                        // may not exist
+                        const bool whole_tile = rows == PT && hd == HD, has_last = r0 + (NVT - 1) * RSTEP < PT;
+                        uint32_t place[NB];
+#pragma unroll
+                        for (int j = 0; j < NB; ++j) place[j] = dst + rel[j];
+                        auto from = [&](int k) { return KVT == KV_F32 ? src + (uint32_t)(k * RSTEP * HD * 4) : place[k % NB] + (uint32_t)(k * RSTEP * 128); };
+                        auto split_store = [&](const uint4& x, float2 f, uint32_t o) {  // fp32 halves
+                            uint32_t h0, l0, h1, l1;
+                            split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), f), h0, l0);
+                            split2t(__fmul2_rn(make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), f), h1, l1);
+                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
+                            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::HALF), "r"(l0), "r"(l1) : "memory");
+                        };
+                        auto half_store = [&](const uint4& x, float2 f, uint32_t o) {  // bf16 in one half
+                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const float2 y = __fmul2_rn(make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u)), f);
+                                w[j] = pack_half2(y.x, y.y);
+                            }
+                            st_shared16(o, w);
+                        };
                         for (;;) {
                             const int e = which ? ev : ek;
-                            const float f = pow2i(-e);
+                            const float2 f = make_float2(pow2i(-e), pow2i(-e));
                             uint32_t mb = 0;
-                            // (batches: all loads before the first store, the compiler keeps their order)
-#pragma unroll 1
-                            for (int rb = r0; rb < PT; rb += UNR * RSTEP) {
-                                uint4 x[UNR];
+                            if (whole_tile) {
 #pragma unroll
-                                for (int k = 0; k < UNR; ++k) {
-                                    const int r = rb + k * RSTEP;
-                                    x[k] = make_uint4(0, 0, 0, 0);
-                                    if (r < rows && col) x[k] = ld_shared16(at(r));
-                                }
+                                for (int k0 = 0; k0 < NVT; k0 += UNR) {  // (all loads before the first store: the compiler keeps their order)
+                                    uint4 x[UNR];
 #pragma unroll
-                                for (int k = 0; k < UNR; ++k) {
-                                    mb = max(mb, abs_bits<KVT>(x[k]));
-                                    const int r = rb + k * RSTEP;
-                                    if (KVT == KV_F32 && r < PT) {
-                                        uint32_t h0, l0, h1, l1;
-                                        split2t(__fmul2_rn(make_float2(__uint_as_float(x[k].x), __uint_as_float(x[k].y)), make_float2(f, f)), h0, l0);
-                                        split2t(__fmul2_rn(make_float2(__uint_as_float(x[k].z), __uint_as_float(x[k].w)), make_float2(f, f)), h1, l1);
-                                        const uint32_t o = dst + wide_off(PT, r, c0 >> 1) + (c0 & 1) * 8;
-                                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o), "r"(h0), "r"(h1) : "memory");
-                                        asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(o + F::HALF), "r"(l0), "r"(l1) : "memory");
+                                    for (int k = k0; k < k0 + UNR && k < NVT; ++k) {
+                                        x[k - k0] = make_uint4(0, 0, 0, 0);
+                                        if (k < NVT - 1 || has_last) x[k - k0] = ld_shared16(from(k));
                                     }
+#pragma unroll
+                                    for (int k = k0; k < k0 + UNR && k < NVT; ++k) {
+                                        abs_max<KVT>(mb, x[k - k0]);
+                                        if (KVT == KV_F32 && (k < NVT - 1 || has_last))
+                                            split_store(x[k - k0], f, place[k % NB] + (uint32_t)(k * RSTEP * 128));
+                                    }
+                                }
+                                mb = abs_max_bits<KVT>(mb);
+                            } else {
+#pragma unroll 1
+                                for (int r = r0; r < PT; r += RSTEP) {
+                                    uint4 x = make_uint4(0, 0, 0, 0);
+                                    if (r < rows && col) x = ld_shared16(at(r));
+                                    mb = max(mb, abs_bits<KVT>(x));
+                                    if (KVT == KV_F32) split_store(x, f, dst + wide_off(PT, r, c0 >> 1) + (c0 & 1) * 8);
                                 }
                             }
                             if (__any_sync(0xFFFFFFFFu, mb >= 0x7F800000u)) {  // infinities or NaN: the finite maximum
@@ -1079,23 +1129,23 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                             (which ? sh.ev : sh.ek)[n & 7] = which ? ev : ek;
                         }
                         if (KVT == KV_BF16) {
-                            const float f = pow2i(which ? -ev : -ek);
+                            const float2 f = make_float2(pow2i(which ? -ev : -ek), pow2i(which ? -ev : -ek));
+                            if (whole_tile) {
+#pragma unroll
+                                for (int k0 = 0; k0 < NVT; k0 += UNR) {
+                                    uint4 x[UNR];
+#pragma unroll
+                                    for (int k = k0; k < k0 + UNR && k < NVT; ++k) {
+                                        x[k - k0] = make_uint4(0, 0, 0, 0);
+                                        if (k < NVT - 1 || has_last) x[k - k0] = ld_shared16(from(k));
+                                    }
+#pragma unroll
+                                    for (int k = k0; k < k0 + UNR && k < NVT; ++k)
+                                        if (k < NVT - 1 || has_last) half_store(x[k - k0], f, from(k));
+                                }
+                            } else {
 #pragma unroll 1
-                            for (int rb = r0; rb < PT; rb += UNR * RSTEP) {
-                                uint4 x[UNR];
-#pragma unroll
-                                for (int k = 0; k < UNR; ++k) {
-                                    x[k] = make_uint4(0, 0, 0, 0);
-                                    if (rb + k * RSTEP < PT) x[k] = ld_shared16(at(rb + k * RSTEP));
-                                }
-#pragma unroll
-                                for (int k = 0; k < UNR; ++k) {
-                                    uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j)
-                                        w[j] = pack_half2(__uint_as_float(w[j] << 16) * f, __uint_as_float(w[j] & 0xFFFF0000u) * f);
-                                    if (rb + k * RSTEP < PT) st_shared16(at(rb + k * RSTEP), w);
-                                }
+                                for (int r = r0; r < PT; r += RSTEP) half_store(ld_shared16(at(r)), f, at(r));
                             }
                         }
                     }
