@@ -876,37 +876,37 @@ struct WideShared {
     unsigned badrow[8][TREE_MAX_NODES / 32];      // drafted rows with non-finite values, by segment
     float qscale[TW_RT];
     float2 ml[2][TW_RT];                          // the streams' row maxima and sums
+    float* dst[TW_RT];                            // where a segment's rows go
     uint32_t vis[256][VIS_WORDS];                 // what each softmax thread's row sees
 };
 
 // Half h of a segment's rows from the two streams' staged halves: added, scaled by the row's
-// factor, written coalesced.
+// factor (scale[r].x), written coalesced to where dst[r] points (nullptr: not a row).
 template <int HD>
-__device__ __forceinline__ void wide_rows_out(const TreeAttnArgs& a, const TreeSeg& sg, uint32_t stage, const float2* scale,
-                                              bool whole, float* part, int h, int rep, int rep_inv, const volatile int* abort_flag) {
-    constexpr int LPR = HD / 8, RPW = 32 / LPR;  // lanes per half row, rows per warp and step
+__device__ __forceinline__ void wide_rows_out(uint32_t stage, const float2* scale, float* const* dst, int h, int hd) {
+    constexpr int LPR = HD / 8, RPW = 32 / LPR, N = TW_RT / RPW / 8, U = 4;  // lanes per half row, rows per warp and step, steps
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane % LPR, d = h * (HD / 2) + c * 4;
-    const int rows = sg.s.n_node * rep, hd = a.hd;
-    if (*abort_flag) return;
-    constexpr int U = TW_RT / RPW / 8;
-    uint4 x[U], y[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const int r = (warp + 8 * k) * RPW + lane / LPR;
-        const uint32_t at = stage + (uint32_t)r * (HD * 2) + ((uint32_t)(c ^ (r & 7)) << 4);
-        x[k] = ld_shared16(at);
-        y[k] = ld_shared16(at + TW_RT * HD * 2);
-    }
+    for (int k0 = 0; k0 < N; k0 += U) {
+        uint4 x[U], y[U];
+        float f[U];
+        float* to[U];
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-        const int r = (warp + 8 * k) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
-        const float f = scale[r].x;
-        // (a row that saw nothing has the factor 0 and zeros; its sum cannot be anything else)
-        const float4 o = make_float4((__uint_as_float(x[k].x) + __uint_as_float(y[k].x)) * f, (__uint_as_float(x[k].y) + __uint_as_float(y[k].y)) * f,
-                                     (__uint_as_float(x[k].z) + __uint_as_float(y[k].z)) * f, (__uint_as_float(x[k].w) + __uint_as_float(y[k].w)) * f);
-        float* dst = whole ? a.out + ((size_t)sg.b * a.T + nd) * a.ld_out + (size_t)(sg.kvh * rep + q - nd * rep) * hd
-                           : part + (size_t)r * hd;
-        if (q < rows && d < hd) *reinterpret_cast<float4*>(dst + d) = o;
+        for (int k = 0; k < U; ++k) {
+            const int r = (warp + 8 * (k0 + k)) * RPW + lane / LPR;
+            const uint32_t at = stage + (uint32_t)r * (HD * 2) + ((uint32_t)(c ^ (r & 7)) << 4);
+            x[k] = ld_shared16(at);
+            y[k] = ld_shared16(at + TW_RT * HD * 2);
+            f[k] = scale[r].x;
+            to[k] = dst[r];
+        }
+#pragma unroll
+        for (int k = 0; k < U; ++k)
+            // (a row that saw nothing has the factor 0 and zeros; its sum cannot be anything else)
+            if (to[k] && d < hd)
+                *reinterpret_cast<float4*>(to[k] + d) =
+                    make_float4((__uint_as_float(x[k].x) + __uint_as_float(y[k].x)) * f[k], (__uint_as_float(x[k].y) + __uint_as_float(y[k].y)) * f[k],
+                                (__uint_as_float(x[k].z) + __uint_as_float(y[k].z)) * f[k], (__uint_as_float(x[k].w) + __uint_as_float(y[k].w)) * f[k]);
     }
 }
 __device__ __forceinline__ bool badrow_any(const unsigned* badrow) {
@@ -1037,6 +1037,10 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         }
                     }
                     __syncwarp();
+                    if (KVT == KV_F32 && rows < PT)  // rows behind the end are zeros
+#pragma unroll 1
+                        for (int r = r0; r < PT; r += RSTEP)
+                            if (r >= rows) st_shared16(src + (uint32_t)((r - r0) * hd * 4), {0u, 0u, 0u, 0u});
                     const bool col = KVT != KV_F32 || c0 * 4 < hd;
                     auto at = [&](int r) { return KVT == KV_F32 ? src + (uint32_t)((r - r0) * hd * 4) : dst + wide_off(PT, r, c0); };
                     if (which && tail && col) {  // non-finite drafted values leave the operand (see the narrow kernel)
@@ -1058,7 +1062,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         unsigned* tm = &sh.tmax[2 * (n & 1) + which];
                         // a whole tile's vectors lie at compile-time distances; this thread's last one
                         // may not exist
-                        const bool whole_tile = rows == PT && hd == HD, has_last = r0 + (NVT - 1) * RSTEP < PT;
+                        const bool whole_tile = hd == HD, has_last = r0 + (NVT - 1) * RSTEP < PT;
                         uint32_t place[NB];
 #pragma unroll
                         for (int j = 0; j < NB; ++j) place[j] = dst + rel[j];
@@ -1288,13 +1292,15 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
             {   // queries, HD / 8 lanes per row: scaled to [2^14, 2^15), two halves
                 constexpr int LPR = HD / 8, RPW = 32 / LPR, STEPS = TW_RT / (8 * RPW), U = STEPS;
                 const int c = lane % LPR;
+                const float* qb = a.q + (size_t)sg.b * a.T * a.ld_q + (size_t)sg.kvh * rep * hd + c * 8;
+                const float qk = kLog2e / sqrtf((float)hd);
 #pragma unroll 1
                 for (int i0 = 0; i0 < STEPS; i0 += U) {
                     float4 x[U][2];
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
                         const int r = ((i0 + i) * 8 + warp) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
-                        const float* qp = a.q + ((size_t)sg.b * a.T + nd) * a.ld_q + (size_t)(sg.kvh * rep + q - nd * rep) * hd + c * 8;
+                        const float* qp = qb + (nd * a.ld_q + (q - nd * rep) * hd);
                         x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (q < rows && c * 8 < hd) {
                             x[i][0] = reinterpret_cast<const float4*>(qp)[0];
@@ -1313,7 +1319,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         const uint32_t o = sb + F::Q_OFF + wide_off(TW_RT, r, c);
                         st_shared16(o, hi);
                         st_shared16(o + F::QH, lo);
-                        if (c == 0) sh.qscale[r] = pow2i(e) * (kLog2e / sqrtf((float)hd));
+                        if (c == 0) sh.qscale[r] = pow2i(e) * qk;
                     }
                 }
                 fence_async();
@@ -1412,6 +1418,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                 const float L = fmaf(l, wgt, other.y * exp2_fast(other.x - mref));
                 named_bar<1, 256>();
                 if (wg == 0) {
+                    float* to = whole ? a.out + ((size_t)sg.b * a.T + node) * a.ld_out + (size_t)(sg.kvh * rep + rr - node * rep) * hd
+                                      : part + (size_t)row * hd;
+                    sh.dst[row] = rr < rows && !*abort_flag ? to : nullptr;
                     sh.ml[0][row].x = !whole ? 1.f : (L == 0.f ? 0.f : 1.f / L);
                     if (!whole && rr < rows && !*abort_flag) {
                         part[(size_t)TW_RT * hd + row] = M;
@@ -1431,7 +1440,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                                  __float_as_uint(O[i + 3] * wgt)});
                 }
                 named_bar<1, 256>();
-                wide_rows_out<HD>(a, sg, sb + F::Q_OFF, sh.ml[0], whole, part, h, rep, rep_inv, abort_flag);
+                wide_rows_out<HD>(sb + F::Q_OFF, sh.ml[0], sh.dst, h, hd);
                 named_bar<1, 256>();  // the shared memory takes the next half, or the next segment's queries
             }
             if (!whole && sg.t0 == 0 && tid == 0) desc[blockIdx.x] = TreeDesc{sg.b, sg.kvh, sg.rtile, sg.last_cta};
