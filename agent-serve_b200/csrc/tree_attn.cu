@@ -759,13 +759,12 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
 //   2     loaders: a tile's K and V rows arrive by one 1-D bulk copy each, are split into f16
 //         halves and written as MMA operands (rows of 64 dims, 128-byte swizzle);
 //   3     MMA issue (one thread).
-// Tensor memory: two or three S (PT columns each), taken in turn by the tiles, and D_0, D_1 (HD
-// columns each, a stream's).  QK: S = Q K^T,
+// Tensor memory: S_0, S_1 (PT columns each) and D_0, D_1 (HD columns each).  QK: S_w = Q K^T,
 // Q from shared memory, the tile K-major.  The softmax thread overwrites its scores in place,
 // CH columns at a time, with the high halves of p (CH / 2 columns) and the low ones, the A
 // operand of PV: D_w = P V, the same tile layout read MN-major; D_w starts from zero for every
-// tile and joins the registers' output after the stream's next softmax.  QK runs one or two tiles
-// ahead of PV, so the tensor pipe works while a stream is in its softmax.
+// tile and joins the registers' output.  QK of tile i + 1 is issued before PV of tile i, so the
+// tensor pipe works while a stream is in its softmax.
 constexpr int TW_THREADS = 512;
 constexpr int TW_RT = 128;
 
@@ -791,11 +790,7 @@ struct WideCfg {
     // registers per thread of the softmax warpgroups and of the other two (512 in all, four
     // warpgroups of 128 at launch)
     static constexpr int REG_S = HD == 64 ? 144 : 192, REG_L = HD == 64 ? 112 : 64;
-    // score buffers in tensor memory (of PT columns; the two D of HD columns take the rest): with
-    // three a stream's next scores are there when it has written its probabilities
-    static constexpr int NS = KVT != KV_F32 && HD == 64 ? 3 : 2, D_COL = NS * PT;
-    static_assert(VS >= NS - 1, "a loader brings V of tile n + 1 before K of tile n + 2, and PV runs NS - 1 tiles behind");
-    static constexpr int CH = 16;                         // score columns a softmax thread takes at a time
+    static constexpr int CH = HD == 64 ? 32 : 16;         // score columns a softmax thread holds at a time
 };
 
 __device__ __forceinline__ uint64_t wide_desc(uint32_t saddr, uint32_t lbo) {
@@ -852,16 +847,6 @@ __device__ __forceinline__ void tmem_ld(uint32_t t, uint32_t (&r)[32]) {
 __device__ __forceinline__ void tmem_st(uint32_t t, const uint32_t (&r)[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(t), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]) : "memory");
 }
-// the same in two parts, so that other work runs in between
-__device__ __forceinline__ void tmem_ld_begin(uint32_t t, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(t)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_ld_end(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
-}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -879,11 +864,11 @@ struct WideShared {
     // mbarriers, initialised in order by count()
     uint64_t rawfull[8];                          // raw fp32 tiles, bf16 tiles in their operand stages
     uint64_t kfree[4], vfree[4];                  // operand stages: their MMAs are done
-    uint64_t sfull[3], dfull[2], done;
+    uint64_t sfull[2], dfull[2], done;
     uint64_t kfull[4], vfull[4], rawfree[2];      // one arrival per loader warp
     uint64_t pfull[2], qfull;
-    static constexpr int N_BARS = 35;
-    __device__ static uint32_t count(int i) { return i < 22 ? 1 : (i < 32 ? TW_LOADERS : (i < 34 ? 128 : 256)); }
+    static constexpr int N_BARS = 34;
+    __device__ static uint32_t count(int i) { return i < 21 ? 1 : (i < 31 ? TW_LOADERS : (i < 33 ? 128 : 256)); }
     uint32_t tmem;
     int abort;
     unsigned tmax[4];
@@ -936,7 +921,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
     tf_tree_attn_wide_kernel(const __grid_constant__ TreeAttnArgs a, const __grid_constant__ TreePlan pl,
                              const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
     using F = WideCfg<HD, KVT>;
-    constexpr int PT = F::PT, NLO = F::NLO, ESZ = F::ESZ, KS = F::KS, VS = F::VS, RS = F::RS, CH = F::CH, NS = F::NS;
+    constexpr int PT = F::PT, NLO = F::NLO, ESZ = F::ESZ, KS = F::KS, VS = F::VS, RS = F::RS, CH = F::CH;
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(16) WideShared sh;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, wg = warp >> 2;
@@ -1245,15 +1230,16 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         };
         while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             wait(&sh.qfull, seg);
-            // QK of tile t, then PV of tile t - (NS - 1)
+            // QK of tile t, then PV of tile t - 1 (one step more than there are tiles)
 #pragma unroll 1
-            for (int t = sg.t0; t < sg.t1 + NS - 1; ++t) {
+            for (int t = sg.t0; t <= sg.t1; ++t) {
+                const int w = (t - sg.t0) & 1;
                 if (t < sg.t1) {
                     const int os = n % KS;
                     wait(&sh.kfull[os], n / KS);
                     if (ok) {
                         tc_fence_after();
-                        const uint32_t d = tm + (n % NS) * PT;
+                        const uint32_t d = tm + w * 128;
                         const uint64_t kb = wide_desc(sb + F::K_OFF + os * NLO * F::HALF, 16), qb = wide_desc(sb + F::Q_OFF, 16);
 #pragma unroll
                         for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes along the rows of a 64-dim block
@@ -1264,19 +1250,19 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                             if (NLO == 2) wide_mma_ss(d, q, k + F::HALF / 16, iqk, 1, lead);
                         }
                         wide_commit(&sh.kfree[os], lead);
-                        wide_commit(&sh.sfull[n % NS], lead);
+                        wide_commit(&sh.sfull[w], lead);
                     }
                     ++n;
                 }
-                if (t >= sg.t0 + NS - 1) {
-                    const int pt = t - (NS - 1), mt = n - min(t + 1, sg.t1) + pt, v = (pt - sg.t0) & 1, os = mt % VS;  // tile, stream, stage
+                if (t > sg.t0) {
+                    const int mt = t < sg.t1 ? n - 2 : n - 1, v = w ^ 1, os = mt % VS;  // tile, stream, stage
                     wait(&sh.pfull[v], v ? cnt[1] : cnt[0]);
                     wait(&sh.vfull[os], mt / VS);
                     if (v) ++cnt[1];
                     else ++cnt[0];
                     if (ok) {
                         tc_fence_after();
-                        const uint32_t d = tm + F::D_COL + v * HD, p = tm + (mt % NS) * PT;
+                        const uint32_t d = tm + 256 + v * HD, p = tm + v * 128;
                         const uint64_t vh = wide_desc(sb + F::V_OFF + os * NLO * F::HALF, PT * 128);
 #pragma unroll
                         for (int j = 0; j < PT / 16; ++j) {  // 16 positions: 2048 bytes of rows; p's halves in blocks of CH columns
@@ -1298,7 +1284,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(F::REG_S));
         const int row = tid & 127;                                  // TMEM lane
         const uint32_t tl = tmem + ((uint32_t)(32 * (warp & 3)) << 16);
-        const uint32_t td = tl + F::D_COL + wg * HD;
+        const uint32_t ts = tl + wg * 128, td = tl + 256 + wg * HD;
         int n = 0, seg = 0, cnt = 0;
         while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
@@ -1348,115 +1334,72 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < HD; ++i) O[i] = 0.f;
             const int n0 = n - sg.t0;
-            // D of the stream's last tile joins the output: O = O * scale + D 2^ev
-            float scale = 0.f;
-            auto join = [&](int done) {  // its index among all tiles
-                tree_wait(&sh.dfull[wg], cnt - 1, a.err, ERR_WAIT_FULL, abort_flag);
+#pragma unroll 1
+            for (int t = sg.t0 + wg; t < sg.t1; t += 2, ++cnt) {
+                tree_wait(&sh.sfull[wg], cnt, a.err, ERR_WAIT_FULL, abort_flag);
                 __syncwarp();
                 tc_fence_after();
-                const float fv = KVT == KV_F16 ? 1.f : pow2i(sh.ev[done & 7]);
-                uint32_t x[2][CH];
-                tmem_ld_begin(td, x[0]);
+                const float f = KVT == KV_F16 ? qs : qs * pow2i(sh.ek[(n0 + t) & 7]);
+                const bool tail = (t + 1) * PT > s.n_ctx;
+                // (the loops over CH-column chunks stay loops: unrolled, the code outgrows the
+                // instruction cache and the one warp per scheduler waits for its fetches)
+                float mx = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < PT; c += CH) {
+                    uint32_t x[CH];
+                    tmem_ld(ts + c, x);
+                    if (tail) {
+                        const uint32_t seen = vis_window(vis, t * PT + c - s.n_ctx);
 #pragma unroll
-                for (int c = 0; c < HD / CH; ++c) {
-                    tmem_ld_end(x[c & 1]);
-                    if (c + 1 < HD / CH) tmem_ld_begin(td + CH * (c + 1), x[(c + 1) & 1]);
+                        for (int i = 0; i < CH; ++i) x[i] = (seen >> i) & 1 ? x[i] : 0xFF800000u;
+                        __syncwarp();
+                        tmem_st(ts + c, x);  // masked scores are -infinity from here on
+                    }
+                    float m0 = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+#pragma unroll
+                    for (int i = 2; i < CH; i += 2) m0 = fmaxf(m0, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+                    mx = fmaxf(mx, m0);
+                }
+                if (tail) tmem_wait_st();
+                mx = fmaxf(m, mx * f);
+                const float ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(m - ref), shift = kPShift - ref;
+                m = mx;
+                float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < PT; c += CH) {
+                    uint32_t x[CH], y[CH];
+                    tmem_ld(ts + c, x);
 #pragma unroll
                     for (int i = 0; i < CH; i += 2) {
-                        const float2 o = __ffma2_rn(make_float2(__uint_as_float(x[c & 1][i]), __uint_as_float(x[c & 1][i + 1])), make_float2(fv, fv),
-                                                    __fmul2_rn(make_float2(O[CH * c + i], O[CH * c + i + 1]), make_float2(scale, scale)));
+                        const float p0 = exp2_fast(fmaf(__uint_as_float(x[i]), f, shift));
+                        const float p1 = exp2_fast(fmaf(__uint_as_float(x[i + 1]), f, shift));
+                        sum0 += p0;
+                        sum1 += p1;
+                        split2t(make_float2(p0, p1), y[i / 2], y[CH / 2 + i / 2]);
+                    }
+                    tmem_st(ts + c, y);
+                }
+                l = fmaf(l, alpha, sum0 + sum1);
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&sh.pfull[wg]);
+                tree_wait(&sh.dfull[wg], cnt, a.err, ERR_WAIT_FULL, abort_flag);
+                __syncwarp();
+                tc_fence_after();
+                const float fv = KVT == KV_F16 ? 1.f : pow2i(sh.ev[(n0 + t) & 7]);
+#pragma unroll
+                for (int c = 0; c < HD / CH; ++c) {
+                    uint32_t x[CH];
+                    tmem_ld(td + CH * c, x);
+#pragma unroll
+                    for (int i = 0; i < CH; i += 2) {
+                        const float2 o = __ffma2_rn(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), make_float2(fv, fv),
+                                                    __fmul2_rn(make_float2(O[CH * c + i], O[CH * c + i + 1]), make_float2(alpha, alpha)));
                         O[CH * c + i] = o.x;
                         O[CH * c + i + 1] = o.y;
                     }
                 }
                 tc_fence_before();
-            };
-#pragma unroll 1
-            for (int t = sg.t0 + wg;; t += 2) {
-                if (t >= sg.t1) {
-                    if (t - 2 >= sg.t0) join(n0 + t - 2);
-                    break;
-                }
-                const int nt = n0 + t;
-                const uint32_t ts = tl + (nt % NS) * PT;
-                tree_wait(&sh.sfull[nt % NS], nt / NS, a.err, ERR_WAIT_FULL, abort_flag);
-                __syncwarp();
-                tc_fence_after();
-                const float f = KVT == KV_F16 ? qs : qs * pow2i(sh.ek[nt & 7]);
-                const bool tail = (t + 1) * PT > s.n_ctx;
-                // (the loops over CH-column chunks stay loops: unrolled, the code outgrows the
-                // instruction cache and the one warp per scheduler waits for its fetches; the next
-                // chunk is on its way while one is worked on)
-                uint32_t x[CH], x2[CH], y[CH];
-                float mx = -INFINITY, mx2 = -INFINITY;
-                if (tail) {
-#pragma unroll 1
-                    for (int c = 0; c < PT; c += CH) {
-                        tmem_ld_begin(ts + c, x);
-                        const uint32_t seen = vis_window(vis, t * PT + c - s.n_ctx);
-                        tmem_ld_end(x);
-#pragma unroll
-                        for (int i = 0; i < CH; ++i) {
-                            x[i] = (seen >> i) & 1 ? x[i] : 0xFF800000u;
-                            mx = fmaxf(mx, __uint_as_float(x[i]));
-                        }
-                        __syncwarp();
-                        tmem_st(ts + c, x);  // masked scores are -infinity from here on
-                    }
-                    tmem_wait_st();
-                } else {
-                    tmem_ld_begin(ts, x);
-#pragma unroll 1
-                    for (int c = 0; c < PT; c += 2 * CH) {
-                        tmem_ld_end(x);
-                        tmem_ld_begin(ts + c + CH, x2);
-#pragma unroll
-                        for (int i = 0; i < CH; i += 2) {
-                            mx = fmaxf(mx, __uint_as_float(x[i]));
-                            mx2 = fmaxf(mx2, __uint_as_float(x[i + 1]));
-                        }
-                        tmem_ld_end(x2);
-                        if (c + 2 * CH < PT) tmem_ld_begin(ts + c + 2 * CH, x);
-#pragma unroll
-                        for (int i = 0; i < CH; i += 2) {
-                            mx = fmaxf(mx, __uint_as_float(x2[i]));
-                            mx2 = fmaxf(mx2, __uint_as_float(x2[i + 1]));
-                        }
-                    }
-                }
-                tmem_ld_begin(ts, x);
-                mx = fmaxf(m, fmaxf(mx, mx2) * f);
-                const float ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(m - ref), shift = kPShift - ref;
-                m = mx;
-                float2 sum = make_float2(0.f, 0.f);
-                auto probs = [&](const uint32_t (&v)[CH]) {
-#pragma unroll
-                    for (int i = 0; i < CH; i += 2) {
-                        const float2 e = __ffma2_rn(make_float2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), make_float2(f, f),
-                                                    make_float2(shift, shift));
-                        const float2 p = make_float2(exp2_fast(e.x), exp2_fast(e.y));
-                        sum = __fadd2_rn(sum, p);
-                        split2t(p, y[i / 2], y[CH / 2 + i / 2]);
-                    }
-                };
-#pragma unroll 1
-                for (int c = 0; c < PT; c += 2 * CH) {
-                    tmem_ld_end(x);
-                    tmem_ld_begin(ts + c + CH, x2);
-                    probs(x);
-                    tmem_st(ts + c, y);
-                    tmem_ld_end(x2);
-                    if (c + 2 * CH < PT) tmem_ld_begin(ts + c + 2 * CH, x);
-                    probs(x2);
-                    tmem_st(ts + c + CH, y);
-                }
-                l = fmaf(l, alpha, sum.x + sum.y);
-                if (t - 2 >= sg.t0) join(nt - 2);
-                scale = alpha;
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sh.pfull[wg]);
-                ++cnt;
             }
             n += sg.t1 - sg.t0;
             // The streams meet in Q's shared memory (every QK of the segment is done), half of the
