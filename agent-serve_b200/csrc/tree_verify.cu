@@ -60,7 +60,6 @@ struct TvShared {
 
 struct TvPlan {
     int slice, piece;                  // elements of a CTA, of a warp (multiples of 4)
-    int prefetch;                      // few sequences: bring the first child's rows into L2 ahead
     int stats;                         // walk: the rows' statistics are in the workspace
 };
 
@@ -236,14 +235,6 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
             const bool kid = tid > cur && tid < n && sh.par[tid] == cur;
             const unsigned m = __ballot_sync(0xFFFFFFFFu, kid);
             if (lane == 0) sh.kids[warp] = m;
-            if (pl.prefetch && !pl.stats && m) {
-                const size_t t = (size_t)b * a.T + 32 * warp + __ffs(m) - 1;
-#pragma unroll 1
-                for (int i = s0 + 32 * lane; i < s1; i += 32 * 32) {
-                    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.logits + t * a.ld + i));
-                    if (DRAFT) asm volatile("prefetch.global.L2 [%0];" ::"l"(a.draft + t * a.ld_draft + i));
-                }
-            }
         }
         int best = 0;
         TvRow P, Q;
@@ -527,7 +518,6 @@ template <bool VEC, bool DRAFT>
 static cudaError_t verify_run(const TreeVerifyArgs& a, cudaStream_t st) {
     TvPlan pl = {};
     const int C = TV_MAX_CLUSTER;
-    pl.prefetch = a.B <= 8;
     pl.stats = a.T > 1 && a.B * a.T <= TV_MAX_STATS;
     if (pl.stats) {
         const cudaError_t e = verify_launch<VEC, DRAFT, true>(a, C, pl, st, false);
