@@ -20,9 +20,9 @@
 // contiguous slice of the vocabulary, each warp a contiguous piece of the slice, which it brings
 // into shared memory by a bulk copy of its own.  A visited row takes two passes (maximum, then
 // weights, in place, and sums), a rejection with a draft distribution and the final pick one more
-// each over the weights.  After a pass every warp writes its value into every CTA's shared memory,
-// one cluster barrier, and every warp adds the C x 16 values in the same order: all CTAs hold the
-// same sums and take the same decisions.  A walk is a chain of such rows, so its latency bounds
+// each over the weights.  After a pass each CTA joins its warps' values and writes the result into
+// every CTA's shared memory; behind one cluster barrier every warp joins those in the same order:
+// all CTAs hold the same sums and take the same decisions.  A walk is a chain of such rows, so its latency bounds
 // it: when all rows of all trees fit on the GPU at once, one cluster per row finds every row's
 // maximum and sum first (ROWS), and the walk behind it takes passes for rejections and picks only.
 #include <cooperative_groups.h>
@@ -37,8 +37,8 @@ namespace tfb {
 
 constexpr int TV_THREADS = 512;
 constexpr int TV_WARPS = TV_THREADS / 32;
-constexpr int TV_MAX_CLUSTER = 16;
-constexpr int TV_SLOTS = TV_MAX_CLUSTER * TV_WARPS;  // one value per warp of the cluster
+constexpr int TV_CLUSTER = 16;
+static_assert(TV_WARPS == 16 && TV_CLUSTER == 16, "values are joined and searched sixteen at a time");
 
 struct TvStats {                       // of a node's rows: maxima, and 1 / sum of the weights relative to them
     double ip, iq;
@@ -48,7 +48,8 @@ struct TvStats {                       // of a node's rows: maxima, and 1 / sum 
 constexpr int TV_MAX_STATS = 18;       // rows whose clusters fit the GPU at once (16 CTAs each, two per SM)
 
 struct TvShared {
-    double2 ex[2][TV_SLOTS];           // exchanged values, [rank][warp], of the last two exchanges
+    double2 warps[2][TV_WARPS];        // this CTA's values, one per warp, of the last two exchanges
+    double2 ex[2][TV_CLUSTER];     // every CTA's
     uint64_t landed[TV_WARPS];
     int par[TREE_MAX_NODES], tok[TREE_MAX_NODES];
     float u[TREE_MAX_NODES];
@@ -68,32 +69,44 @@ struct TvPlan {
 struct TvRow {
     float mx, inv_temp;
     bool inf;
-    __device__ __forceinline__ float weight(float l) const {
-        const float e = fmaxf(expf(__fmul_rn(__fsub_rn(l, mx), inv_temp)), 0.f);
-        return inf ? (l == mx ? 1.f : 0.f) : e;
+    __device__ __forceinline__ float finite_weight(float l) const {
+        return fmaxf(expf(__fmul_rn(__fsub_rn(l, mx), inv_temp)), 0.f);
     }
+    __device__ __forceinline__ float weight(float l) const { return inf ? (l == mx ? 1.f : 0.f) : finite_weight(l); }
 };
 __device__ __forceinline__ TvRow tv_row(float mx, float inv_temp) { return TvRow{mx, inv_temp, !(fabsf(mx) < INFINITY)}; }
 
+// A weight in 64 bits by integer instructions (a conversion shares the exponentials' pipe, which
+// bounds the pass): exact from 2^-126 on, off by 2^-127 at most below it and at zero, which no sum
+// of weights sees: its largest term is 1.  (Not for residuals: there a zero has to be one.)
+__device__ __forceinline__ double weight_wide(float x) {
+    const unsigned long long b = (unsigned long long)__float_as_uint(x) * (1u << 29);
+    return __hiloint2double((int)(b >> 32) + (896 << 20), (int)b);
+}
+
 // A warp's piece of logits into weights, in place, and their sums; elements behind its end become
-// weights of zero.  (One copy of the code: it is fetched anew by each CTA.)
-template <bool DRAFT>
+// weights of zero (FULL: pieces end at a multiple of four).  One copy of the code: it is fetched
+// anew by each CTA.
+template <bool DRAFT, bool FULL>
 __device__ __noinline__ double2 tv_weights(float* rp, float* rq, int wn, TvRow P, TvRow Q) {
     double2 s = make_double2(0.0, 0.0);
+    auto vec = [](float4 x, int k, const TvRow& R, double& sum, auto weight) {  // k: elements left
+        x = make_float4(weight(R, x.x), FULL || k > 1 ? weight(R, x.y) : 0.f, FULL || k > 2 ? weight(R, x.z) : 0.f,
+                        FULL || k > 3 ? weight(R, x.w) : 0.f);
+        sum += (weight_wide(x.x) + weight_wide(x.y)) + (weight_wide(x.z) + weight_wide(x.w));
+        return x;
+    };
+    auto pass = [&](auto weight) {
 #pragma unroll 2
-    for (int i = (threadIdx.x & 31) * 4; i < wn; i += 128) {
-        const int k = wn - i;  // elements left
-        float4 x = *reinterpret_cast<const float4*>(rp + i), y = x;
-        if (DRAFT) y = *reinterpret_cast<const float4*>(rq + i);
-        x = make_float4(P.weight(x.x), k > 1 ? P.weight(x.y) : 0.f, k > 2 ? P.weight(x.z) : 0.f, k > 3 ? P.weight(x.w) : 0.f);
-        *reinterpret_cast<float4*>(rp + i) = x;
-        s.x += ((double)x.x + (double)x.y) + ((double)x.z + (double)x.w);
-        if (DRAFT) {
-            y = make_float4(Q.weight(y.x), k > 1 ? Q.weight(y.y) : 0.f, k > 2 ? Q.weight(y.z) : 0.f, k > 3 ? Q.weight(y.w) : 0.f);
-            *reinterpret_cast<float4*>(rq + i) = y;
-            s.y += ((double)y.x + (double)y.y) + ((double)y.z + (double)y.w);
+        for (int i = (threadIdx.x & 31) * 4; i < wn; i += 128) {
+            const float4 x = *reinterpret_cast<const float4*>(rp + i);
+            const float4 y = DRAFT ? *reinterpret_cast<const float4*>(rq + i) : x;
+            *reinterpret_cast<float4*>(rp + i) = vec(x, wn - i, P, s.x, weight);
+            if (DRAFT) *reinterpret_cast<float4*>(rq + i) = vec(y, wn - i, Q, s.y, weight);
         }
-    }
+    };
+    if (P.inf || (DRAFT && Q.inf)) pass([](const TvRow& R, float l) { return R.weight(l); });
+    else pass([](const TvRow& R, float l) { return R.finite_weight(l); });
     __syncwarp();
     return make_double2(warp_sum_d(s.x), DRAFT ? warp_sum_d(s.y) : 0.0);
 }
@@ -126,7 +139,8 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
     extern __shared__ __align__(16) float rows[];  // the slice of the target's row, of the draft's
     __shared__ __align__(16) TvShared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    constexpr int C = TV_CLUSTER;
+    const int rank = (int)cluster.block_rank();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, V = a.V;
     const int b = ROWS ? blockIdx.x / C / a.T : blockIdx.x / C;
     pdl_trigger();
@@ -206,24 +220,28 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
         }
         __syncwarp();
     };
-    // one value pair per warp to every CTA of the cluster
-    auto exchange = [&](double x, double y) {
+    // Joins one value pair per warp over the cluster, in the same order in every warp; on the way the
+    // warps' pairs stay in sh.warps[parity], the CTAs' in sh.ex[parity].
+    auto exchange = [&](double x, double y, auto join) {
         parity ^= 1;
-        if (lane < C) *cluster.map_shared_rank(&sh.ex[parity][rank * TV_WARPS + warp], lane) = make_double2(x, y);
-        cluster.sync();
-    };
-    // the sums of what was exchanged (in the same order in every warp)
-    auto collect = [&](double& x, double& y) {
-        x = y = 0.0;
-#pragma unroll 2
-        for (int i = lane; i < C * TV_WARPS; i += 32) {
-            const double2 v = sh.ex[parity][i];
-            x += v.x;
-            y += v.y;
+        auto join16 = [&](double2 v) {
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) {
+                const double2 z = make_double2(__shfl_xor_sync(0xFFFFFFFFu, v.x, o), DRAFT ? __shfl_xor_sync(0xFFFFFFFFu, v.y, o) : 0.0);
+                v = make_double2(join(v.x, z.x), DRAFT ? join(v.y, z.y) : 0.0);
+            }
+            return v;
+        };
+        if (lane == 0) sh.warps[parity][warp] = make_double2(x, y);
+        __syncthreads();
+        if (warp == 0) {
+            const double2 v = join16(sh.warps[parity][lane % TV_WARPS]);
+            if (lane < TV_CLUSTER) *cluster.map_shared_rank(&sh.ex[parity][rank], lane) = v;
         }
-        x = warp_sum_d(x);
-        if (DRAFT) y = warp_sum_d(y);
+        cluster.sync();
+        return join16(sh.ex[parity][lane % TV_CLUSTER]);
     };
+    auto add = [](double x, double y) { return x + y; };
 
     int count = 1;
     for (;;) {
@@ -259,21 +277,15 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
                         key = k > key ? k : key;
                     }
                 });
-                auto key_max = [&]() {
 #pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, key, o);
-                        key = k > key ? k : key;
-                    }
-                };
-                key_max();
-                exchange(__longlong_as_double((long long)key), 0.0);
-#pragma unroll 1
-                for (int i = lane; i < C * TV_WARPS; i += 32) {
-                    const unsigned long long k = (unsigned long long)__double_as_longlong(sh.ex[parity][i].x);
+                for (int o = 16; o > 0; o >>= 1) {
+                    const unsigned long long k = __shfl_xor_sync(0xFFFFFFFFu, key, o);
                     key = k > key ? k : key;
                 }
-                key_max();
+                key = (unsigned long long)__double_as_longlong(
+                    exchange(__longlong_as_double((long long)key), 0.0, [](double x, double y) {
+                        return (unsigned long long)__double_as_longlong(x) > (unsigned long long)__double_as_longlong(y) ? x : y;
+                    }).x);
                 best = (int)key_index(key);
             } else {
                 float mp = -INFINITY, mq = -INFINITY;
@@ -292,22 +304,14 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
                 });
                 mp = warp_max(mp);
                 if (DRAFT) mq = warp_max(mq);
-                exchange((double)mp, (double)mq);
-#pragma unroll 1
-                for (int i = lane; i < C * TV_WARPS; i += 32) {
-                    const double2 v = sh.ex[parity][i];
-                    mp = fmaxf(mp, (float)v.x);
-                    mq = fmaxf(mq, (float)v.y);
-                }
-                P = tv_row(warp_max(mp), a.inv_temp);
-                Q = DRAFT ? tv_row(warp_max(mq), a.inv_temp) : P;
-                const double2 ws = tv_weights<DRAFT>(rp, rq, wn, P, Q);
+                const double2 m = exchange((double)mp, (double)mq, [](double x, double y) { return x > y ? x : y; });
+                P = tv_row((float)m.x, a.inv_temp);
+                Q = DRAFT ? tv_row((float)m.y, a.inv_temp) : P;
+                const double2 ws = tv_weights<DRAFT, VEC>(rp, rq, wn, P, Q);
                 weights = true;
-                exchange(ws.x, ws.y);
-                double Sp, Sq;
-                collect(Sp, Sq);
-                ip = 1.0 / Sp;
-                if (DRAFT) iq = 1.0 / Sq;
+                const double2 S = exchange(ws.x, ws.y, add);
+                ip = 1.0 / S.x;
+                if (DRAFT) iq = 1.0 / S.y;
             }
         }
         if (ROWS) {
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
             if (weights) return;
             load_begin();
             load_end();
-            tv_weights<DRAFT>(rp, rq, wn, P, Q);
+            tv_weights<DRAFT, VEC>(rp, rq, wn, P, Q);
             weights = true;
         };
         double c = 0.0, W = 1.0;
@@ -352,9 +356,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
                 } else {
                     need_weights();
                     c += W;
-                    double z;
-                    exchange(tv_rest<DRAFT>(rp, rq, wn, ip, c * iq), 0.0);
-                    collect(W, z);
+                    W = exchange(tv_rest<DRAFT>(rp, rq, wn, ip, c * iq), 0.0, add).x;
                     if (!(W > 0.0)) {
                         c = 0.0;
                         W = 1.0;
@@ -397,43 +399,30 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
             }
             __syncwarp();
         }
-        exchange(tv_rest<DRAFT>(rp, rq, wn, ip, cq), 0.0);
-        // the warp whose piece holds the limit: lane i has the 8 pieces from 8 i on (pieces of rank
-        // r's warp w are number r * 16 + w); the last piece with mass if rounding leaves none
-        double v[8], inc = 0.0;
+        const double lim = (double)sh.u[0] * exchange(tv_rest<DRAFT>(rp, rq, wn, ip, cq), 0.0, add).x;
+        // Of 16 masses, lane i (and i + 16) holding the i-th, the first whose running sum passes the
+        // limit, or the last with mass if rounding leaves none; `at` moves up to its start.  -1: no mass.
+        double at = 0.0;
+        auto find16 = [&](double v) {
+            double run = v;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            v[k] = 8 * lane + k < C * TV_WARPS ? sh.ex[parity][8 * lane + k].x : 0.0;
-            inc += v[k];
-        }
-        const double own = inc;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double z = __shfl_up_sync(0xFFFFFFFFu, inc, o);
-            if (lane >= o) inc += z;
-        }
-        const double lim = (double)sh.u[0] * __shfl_sync(0xFFFFFFFFu, inc, 31);
-        double at = inc - own, hit_at = 0.0;
-        int hit = -1;   // the lane's piece: the first that passes the limit, else its last with mass
-        bool over = false;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            if (v[k] > 0.0 && !over) {
-                hit = 8 * lane + k;
-                hit_at = at;
-                over = at + v[k] > lim;
+            for (int o = 1; o < 16; o <<= 1) {
+                const double z = __shfl_up_sync(0xFFFFFFFFu, run, o, 16);
+                if (lane % 16 >= o) run += z;
             }
-            at += v[k];
-        }
-        const unsigned any = __ballot_sync(0xFFFFFFFFu, over), some = __ballot_sync(0xFFFFFFFFu, hit >= 0);
-        if (!some) {  // a row without mass
+            const unsigned some = __ballot_sync(0xFFFFFFFFu, v > 0.0) & 0xFFFFu;
+            const unsigned over = __ballot_sync(0xFFFFFFFFu, v > 0.0 && at + run > lim) & 0xFFFFu;
+            if (!some) return -1;
+            const int src = over ? __ffs(over) - 1 : 31 - __clz(some);
+            at += __shfl_sync(0xFFFFFFFFu, run - v, src);
+            return src;
+        };
+        const int hit = find16(sh.ex[parity][lane % TV_CLUSTER].x);
+        if (hit < 0) {  // a row without mass
             if (rank == 0 && tid == 0) a.next[b] = 0;
             return;
         }
-        const int src = any ? __ffs(any) - 1 : 31 - __clz(some);
-        hit = __shfl_sync(0xFFFFFFFFu, hit, src);
-        at = __shfl_sync(0xFFFFFFFFu, hit_at, src);
-        if (hit != rank * TV_WARPS + warp) return;
+        if (hit != rank || find16(sh.warps[parity][lane % TV_WARPS].x) != warp) return;
         // 128 elements at a time, four per lane: prefix sums, the first that passes the limit
         int last = -1;
 #pragma unroll 1
@@ -478,11 +467,12 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
 
 size_t tree_verify_ws_bytes(int B, int T, int) { return 256 + (size_t)B * T * sizeof(TvStats); }
 
-int tree_verify_max_vocab(bool draft) { return (TV_MAX_CLUSTER * (200 * 1024 / (draft ? 8 : 4))) / 1024 * 1024; }
+int tree_verify_max_vocab(bool draft) { return (TV_CLUSTER * (200 * 1024 / (draft ? 8 : 4))) / 1024 * 1024; }
 
 template <bool VEC, bool DRAFT, bool ROWS>
-static cudaError_t verify_launch(const TreeVerifyArgs& a, int C, TvPlan pl, cudaStream_t st, bool pdl) {
+static cudaError_t verify_launch(const TreeVerifyArgs& a, TvPlan pl, cudaStream_t st, bool pdl) {
     auto fn = tf_tree_verify_kernel<VEC, DRAFT, ROWS>;
+    constexpr int C = TV_CLUSTER;
     pl.piece = ((a.V + C * TV_WARPS - 1) / (C * TV_WARPS) + 3) / 4 * 4;
     pl.slice = pl.piece * TV_WARPS;
     const size_t smem = (size_t)pl.slice * (DRAFT ? 8 : 4);
@@ -505,7 +495,7 @@ static cudaError_t verify_launch(const TreeVerifyArgs& a, int C, TvPlan pl, cuda
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)C;
+    attr[0].val.clusterDim.x = C;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
@@ -517,13 +507,12 @@ static cudaError_t verify_launch(const TreeVerifyArgs& a, int C, TvPlan pl, cuda
 template <bool VEC, bool DRAFT>
 static cudaError_t verify_run(const TreeVerifyArgs& a, cudaStream_t st) {
     TvPlan pl = {};
-    const int C = TV_MAX_CLUSTER;
     pl.stats = a.T > 1 && a.B * a.T <= TV_MAX_STATS;
     if (pl.stats) {
-        const cudaError_t e = verify_launch<VEC, DRAFT, true>(a, C, pl, st, false);
+        const cudaError_t e = verify_launch<VEC, DRAFT, true>(a, pl, st, false);
         if (e != cudaSuccess) return e;
     }
-    return verify_launch<VEC, DRAFT, false>(a, C, pl, st, pl.stats);
+    return verify_launch<VEC, DRAFT, false>(a, pl, st, pl.stats);
 }
 
 cudaError_t tree_verify_launch(const TreeVerifyArgs& a, cudaStream_t st) {
