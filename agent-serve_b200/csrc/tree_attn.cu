@@ -421,7 +421,6 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
     const int rep_inv = pl.rep_inv;
     auto div_rep = [&](int x) { return (x * rep_inv) >> 16; };
     const int wm = warp % MT, wg = warp / MT;  // row block, position group
-    const bool active = wg < NG;
     const int g8 = lane >> 2, q4 = lane & 3;
 
     pdl_trigger();
@@ -438,6 +437,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
         const TreeSeq s = sg.s;
         const int b = sg.b, kvh = sg.kvh, rtile = sg.rtile, t0 = sg.t0, t1 = sg.t1;
         const int end = s.n_ctx + s.n_node, rows = s.n_node * rep;
+        const bool active = wg < NG && rtile * RT + wm * 16 < rows;  // (a row block behind the last row is left out)
         const size_t off = (size_t)s.slot * a.slot_stride + (size_t)kvh * a.cap * hd;
         const uint8_t* kp = static_cast<const uint8_t*>(a.kc) + off * ESZ;
         const uint8_t* vp = static_cast<const uint8_t*>(a.vc) + off * ESZ;
