@@ -23,8 +23,8 @@
 // each over the weights.  After a pass each CTA joins its warps' values and writes the result into
 // every CTA's shared memory; behind one cluster barrier every warp joins those in the same order:
 // all CTAs hold the same sums and take the same decisions.  A walk is a chain of such rows, so its latency bounds
-// it: when all rows of all trees fit on the GPU at once, one cluster per row finds every row's
-// maximum and sum first (ROWS), and the walk behind it takes passes for rejections and picks only.
+// it: when all rows of all trees fit on the GPU at once, and there is a draft distribution, one
+// cluster per row finds every row's maximum and sum first (ROWS), and the walk behind it takes passes for rejections and picks only.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -43,9 +43,14 @@ static_assert(TV_WARPS == 16 && TV_CLUSTER == 16, "values are joined and searche
 struct TvStats {                       // of a node's rows: maxima, and 1 / sum of the weights relative to them
     double ip, iq;
     float mp, mq;
-    int best, pad;                     // temperature 0: the argmax
 };
-constexpr int TV_MAX_STATS = 18;       // rows whose clusters fit the GPU at once (16 CTAs each, two per SM)
+// Rows whose clusters fit the GPU at once (16 CTAs each, two per SM).  With a draft distribution their
+// statistics are found ahead of the walk; mean over 16 chains of 128256 tokens without / with it:
+// 2 nodes (1.8 rows visited) 15.9 / 16.2 us, 6 nodes (3.3) 26.3 / 20.1, 12 nodes (4.2) 32.6 / 24.7, 18
+// nodes 33.1 / 30.5; 32 nodes in two waves 33 / 50.  Without a distribution, or greedy, a row of the walk
+// is cheaper and fewer are visited: 12 nodes 11.4 / 15.1 and 10.5 / 10.1, 18 nodes 11.4 / 17.8 and
+// 10.4 / 12.5, so those walk at once.
+constexpr int TV_MAX_STATS = 18;
 
 struct TvShared {
     double2 warps[2][TV_WARPS];        // this CTA's values, one per warp, of the last two exchanges
@@ -259,7 +264,6 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
         double ip = 0.0, iq = 0.0;
         bool weights = false;  // the slice holds weights
         if (!ROWS && pl.stats) {
-            best = sh.st[cur].best;
             P = tv_row(sh.st[cur].mp, a.inv_temp);
             Q = tv_row(sh.st[cur].mq, a.inv_temp);
             ip = sh.st[cur].ip;
@@ -267,7 +271,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
             __syncthreads();
         } else {
             load_end();
-            if (greedy) {  // the maximum with its first place
+            if (!DRAFT && greedy) {  // the maximum with its first place
                 unsigned long long key = 0;
                 each([&](float4 x, float4, int i) {
                     const float v[4] = {x.x, x.y, x.z, x.w};
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
         }
         if (ROWS) {
             if (rank == 0 && tid == 0)
-                stats[(size_t)b * a.T + cur] = greedy ? TvStats{0.0, 0.0, 0.f, 0.f, best, 0} : TvStats{ip, iq, P.mx, DRAFT ? Q.mx : 0.f, 0, 0};
+                stats[(size_t)b * a.T + cur] = TvStats{ip, iq, P.mx, Q.mx};
             return;
         }
         auto need_weights = [&]() {
@@ -342,7 +346,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
                 if (tid == 0 && rank == 0) atomicCAS(a.err, 0, ERR_BAD_TOKEN);
                 continue;
             }
-            if (greedy) {
+            if (!DRAFT && greedy) {
                 if (x == best) taken = t;
                 continue;
             }
@@ -386,7 +390,7 @@ __global__ void __launch_bounds__(TV_THREADS, 2)
         }
         // no child: the next token
         if (rank == 0 && tid == 0) a.n_path[b] = count;
-        if (greedy) {
+        if (!DRAFT && greedy) {
             if (rank == 0 && tid == 0) a.next[b] = best;
             return;
         }
@@ -507,10 +511,12 @@ static cudaError_t verify_launch(const TreeVerifyArgs& a, TvPlan pl, cudaStream_
 template <bool VEC, bool DRAFT>
 static cudaError_t verify_run(const TreeVerifyArgs& a, cudaStream_t st) {
     TvPlan pl = {};
-    pl.stats = a.T > 1 && a.B * a.T <= TV_MAX_STATS;
-    if (pl.stats) {
-        const cudaError_t e = verify_launch<VEC, DRAFT, true>(a, pl, st, false);
-        if (e != cudaSuccess) return e;
+    pl.stats = DRAFT && a.T > 1 && a.B * a.T <= TV_MAX_STATS;
+    if constexpr (DRAFT) {
+        if (pl.stats) {
+            const cudaError_t e = verify_launch<VEC, DRAFT, true>(a, pl, st, false);
+            if (e != cudaSuccess) return e;
+        }
     }
     return verify_launch<VEC, DRAFT, false>(a, pl, st, pl.stats);
 }
