@@ -71,7 +71,7 @@ __device__ __forceinline__ int seq_units(int n_kv, int rep, const TreeSeq& s) {
 }
 
 // A CTA's place in its range of tiles [g0, g1): the sequence it is in and the global index of
-// that sequence's first tile.  (32 bits: a call has fewer than 2^31 tiles, tree_attn_launch.)
+// that sequence's first tile.  (32 bits: tree_attn_fits.)
 struct TreeIter {
     int g0, g1, per, base, b;
 };
@@ -1527,10 +1527,29 @@ static int tree_sms() {
     return sms < 1 ? 1 : (2 * sms > TA_MAX_GRID ? TA_MAX_GRID / 2 : sms);
 }
 
+// Rows of a unit's row tile, which chooses the kernel too: TW_RT the wide one, fewer the narrow one.
+// Device time, narrow / wide (f32 unless said; B trees of T nodes, positions, heads x kv heads x dims):
+//   up to 32 rows:   1 x 8, 100, 32x8x64: 9.9 / 19.2 us;  32 x 8, 1144, 32x8x64 f16: 33.8 / 43.1;
+//                    the same in f32: 62.1 / 60.7;  1 x 8, 8000: 28.3 / 26.3
+//   33 to 64 rows:   1 x 12, 100, 32x8x64 (0.4 MB of K and V): 12.3 / 18.5;  1 x 5, 1733, 14x2x64
+//                    (1.8 MB): 15.3 / 16.6;  2 x 14, 700, 32x8x64 f16 (2.9 MB): 14.7 / 14.5;
+//                    1 x 9, 2000, 12x2x128 (4.1 MB): 23.0 / 21.5;  1 x 9, 16000, the same in
+//                    bf16: 50.4 / 35.5;  32 x 8, 1144, 12x2x128: 40.7 / 38.2;  32 x 16, 1144,
+//                    32x8x64: 59.6 / 52.5
+// so 64 rows stay with the narrow kernel only where the whole cache is too small to repay the wide
+// one's set-up (lengths are on the device: the capacity stands for them).
+constexpr double TN_MAX_BYTES = 4e6;
+static int tree_row_tile(int rows, double kv_bytes) {
+    if (rows <= 32) return rows <= 16 ? 16 : 32;
+    return rows <= 64 && kv_bytes < TN_MAX_BYTES ? 64 : TW_RT;
+}
+static int tree_grid(int rt) { return rt == TW_RT ? tree_sms() : 2 * tree_sms(); }
+
 size_t tree_attn_ws_bytes(int B, int T, int n_head, int n_kv, int hd) {
     (void)B;
-    const int rows = T * (n_head / n_kv), rt = rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
-    return 65536 + (size_t)2 * tree_sms() * 2 * tree_part_floats(rt, hd) * sizeof(float);  // wide: half the CTAs, twice the rows
+    static_assert(TW_RT == 2 * 64, "half the CTAs, twice the rows: a tile of 64 rows needs as much as a wide one");
+    const int rt = tree_row_tile(T * (n_head / n_kv), TN_MAX_BYTES);
+    return 65536 + (size_t)tree_grid(rt) * 2 * tree_part_floats(rt, hd) * sizeof(float);
 }
 
 static cudaError_t tree_launch(const void* fn, dim3 grid, int threads, size_t smem, void** args, cudaStream_t st, bool pdl) {
@@ -1563,7 +1582,7 @@ static cudaError_t narrow_launch(const TreeAttnArgs& a, cudaStream_t st, bool pd
         ready[dev].store(true);
     }
     TreePlan pl;
-    pl.grid = 2 * tree_sms();
+    pl.grid = tree_grid(F::RT);
     pl.rt = F::RT;
     pl.rep = a.n_head / a.n_kv;
     pl.rep_inv = (65536 + pl.rep - 1) / pl.rep;
@@ -1616,7 +1635,7 @@ static cudaError_t wide_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl)
         ready[dev].store(true);
     }
     TreePlan pl;
-    pl.grid = tree_sms();
+    pl.grid = tree_grid(TW_RT);
     pl.rt = TW_RT;
     pl.rep = a.n_head / a.n_kv;
     pl.rep_inv = (65536 + pl.rep - 1) / pl.rep;
@@ -1632,24 +1651,31 @@ static cudaError_t wide_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl)
 }
 
 template <int HD, int KVT>
-static cudaError_t narrow_rows(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
-    const int rows = a.T * (a.n_head / a.n_kv);
-    if (rows <= 16) return narrow_launch<HD, 1, KVT>(a, st, pdl);
-    if (rows <= 32) return narrow_launch<HD, 2, KVT>(a, st, pdl);
-    if (rows > 64) return wide_launch<HD, KVT>(a, st, pdl);
-    return narrow_launch<HD, 4, KVT>(a, st, pdl);
+static cudaError_t rows_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
+    const double kv_bytes = 2.0 * a.B * a.n_kv * a.cap * a.hd * (KVT == KV_F32 ? 4 : 2);
+    const int rt = tree_row_tile(a.T * (a.n_head / a.n_kv), kv_bytes);
+    if (rt == 16) return narrow_launch<HD, 1, KVT>(a, st, pdl);
+    if (rt == 32) return narrow_launch<HD, 2, KVT>(a, st, pdl);
+    if (rt == 64) return narrow_launch<HD, 4, KVT>(a, st, pdl);
+    return wide_launch<HD, KVT>(a, st, pdl);
 }
 template <int HD>
-static cudaError_t narrow_type(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
-    if (a.kv_type == KV_F32) return narrow_rows<HD, KV_F32>(a, st, pdl);
-    if (a.kv_type == KV_F16) return narrow_rows<HD, KV_F16>(a, st, pdl);
-    return narrow_rows<HD, KV_BF16>(a, st, pdl);
+static cudaError_t type_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
+    if (a.kv_type == KV_F32) return rows_launch<HD, KV_F32>(a, st, pdl);
+    if (a.kv_type == KV_F16) return rows_launch<HD, KV_F16>(a, st, pdl);
+    return rows_launch<HD, KV_BF16>(a, st, pdl);
+}
+
+// Tiles of 32 positions or more and a unit's cost, of units of 16 rows or more.
+bool tree_attn_fits(int B, int T, int n_head, int n_kv, int cap) {
+    static_assert(TN_UNIT_COST < 8 && TW_UNIT_COST < 8, "a unit's cost is within the bound");
+    const long long rows = (long long)T * (n_head / n_kv);
+    return (double)B * n_kv * ((rows + 15) / 16) * ((double)cap / 32 + 8) < 2147483648.0;
 }
 
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
-    const long long rows = (long long)a.T * (a.n_head / a.n_kv);
-    if ((long long)a.B * a.n_kv * ((rows + 15) / 16) * ((long long)a.cap / 32 + 1) > 0x7FFFFFFFll - 4096) return cudaErrorInvalidValue;
-    return a.hd <= 64 ? narrow_type<64>(a, st, pdl) : narrow_type<128>(a, st, pdl);
+    if (!tree_attn_fits(a.B, a.T, a.n_head, a.n_kv, a.cap)) return cudaErrorInvalidValue;
+    return a.hd <= 64 ? type_launch<64>(a, st, pdl) : type_launch<128>(a, st, pdl);
 }
 
 }  // namespace tfb

@@ -77,6 +77,8 @@ int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, const void
     if (!aligned(out, 16) || !aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(ws, 256))
         return set_error("out, q and the caches must be 16-byte aligned, the workspace 256-byte aligned");
     if (ws_bytes < tree_attn_ws_bytes(B, T, n_heads, n_kv_heads, head_dim)) return set_error("workspace too small");
+    if (!tree_attn_fits(B, T, n_heads, n_kv_heads, cap))
+        return set_error("B * n_kv_heads * ceil(T * (n_heads / n_kv_heads) / 16) * (cap / 32 + 8) must be below 2^31");
     TreeAttnArgs a = {};
     if (op_err_word(&a.err)) return -1;
     a.out = out;
@@ -122,7 +124,7 @@ int tf_op_verify_tree(int* path, int* n_path, int* next, const float* logits, lo
     if (!(inv < INFINITY) || (temperature > 0.0f && inv == 0.0f)) return set_error("temperature out of range");
     if (ld < V || (draft && ld_draft < V)) return set_error("ld must be at least V");
     if (!aligned(ws, 256)) return set_error("the workspace must be 256-byte aligned");
-    if (V > tree_verify_max_vocab(draft && temperature > 0.0f)) return set_error("V is above the limit (409600 with draft, 655360 without)");
+    if (V > tree_verify_max_vocab(draft && temperature > 0.0f)) return set_error("V is above the limit (409600 with draft, 819200 without)");
     if (ws_bytes < tree_verify_ws_bytes(B, T, V)) return set_error("workspace too small");
     TreeVerifyArgs a = {};
     if (op_err_word(&a.err)) return -1;

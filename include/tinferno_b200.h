@@ -282,8 +282,9 @@ TF_API int tf_op_argmax(const float* logits, int n, int rows, int* out, void* st
  * n_ctx committed rows, its ancestors and itself.  Counts, lengths, slots and paths live on
  * the device, so a whole step needs no host round trip and can be captured in a CUDA graph.
  *
- * Workspaces: the caller allocates `bytes` of device memory (256-byte aligned), zeroes it once
- * and may use it for any number of calls of at most those sizes, one call in flight at a time.
+ * Workspaces: the caller allocates `bytes` of device memory (256-byte aligned, its contents do
+ * not matter) and may use it for any number of calls of at most those sizes, one call in flight
+ * at a time.
  * The calls allocate nothing and do not synchronise.  What a kernel finds wrong on the device
  * (a slot outside the cache, a context that does not fit, a token outside the vocabulary) goes
  * to tf_op_device_error. */
@@ -301,7 +302,8 @@ TF_API int tf_tree_mask(const int* parents, int n, int T, unsigned long long* ma
  * sees nothing, like the rows from n_node on, is zero.  Rows that a node does not see do not
  * reach its output, whatever they hold.  T <= 256, head_dim a multiple of 8 up to 128, at most
  * 8 query heads per kv head; B = 1, T = 1 is decode attention.  Scores, softmax and sums are
- * fp32-equivalent for every kv_type. */
+ * fp32-equivalent for every kv_type.  Work is counted in 32 bits: B * n_kv_heads *
+ * ceil(T * (n_heads / n_kv_heads) / 16) * (cap / 32 + 8) must be below 2^31. */
 TF_API int tf_op_attn_tree_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
 TF_API int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, const void* k_cache, const void* v_cache,
                            int kv_type, long long slot_stride, int cap, int n_slots, const int* slots,
@@ -321,7 +323,8 @@ TF_API int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, con
  * first i whose cumulative r exceeds u[b][0] times r's total (temperature 0: the argmax).  The
  * tokens then follow the target's own distribution.  Outputs: path[b][T] the kept nodes from
  * the root on (-1 behind them), n_path[b] their count (0 when n_node[b] is 0), next[b].
- * NaN logits weigh nothing; sums are held in 64 bits. */
+ * NaN logits weigh nothing; sums are held in 64 bits.  V is at most 409600 with draft, 819200
+ * without (the rows that a sequence works on stay in shared memory). */
 TF_API int tf_op_verify_tree_workspace(int B, int T, int V, size_t* bytes);
 TF_API int tf_op_verify_tree(int* path, int* n_path, int* next, const float* logits, long long ld,
                              const float* draft, long long ld_draft, const int* tokens, const int* parents,

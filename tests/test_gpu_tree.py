@@ -342,6 +342,28 @@ def test_attention_refusals():
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("kv", TYPES)
+@pytest.mark.parametrize("heads,T", [((12, 2, 128), 8), ((14, 2, 64), 9), ((6, 1, 80), 6), ((32, 8, 64), 16)])
+@pytest.mark.parametrize("cap", [80, 16384])
+def test_attention_kernel_choice_by_capacity(cap, heads, T, kv):
+    """33 to 64 rows per kv head: a small and a large cache are read by different kernels, from the
+    same workspace, whatever it holds."""
+    c = Case([60, 0, 33], [T, T - 1, 1], T, *heads, kv, seed=cap + T, cap=cap)
+    ws = workspace(native.lib().tf_op_attn_tree_workspace, 3, T, *heads).fill_(255)
+    c.check(c.call(ws=ws))
+    assert device_error() == 0
+
+
+def test_attention_refuses_too_many_tiles():
+    """Tiles are counted in 32 bits: 65535 x 8 units of 2^30 positions are not."""
+    c = Case([10], [3], 3, 8, 2, 64, native.TF_KV_F32, seed=1)
+    ws = workspace(native.lib().tf_op_attn_tree_workspace, 1, 3, 8, 2, 64)
+    with pytest.raises(native.TFError, match=r"2\^31"):
+        native.check(native.lib().tf_op_attn_tree(
+            ptr(c.out), c.ld_out, ptr(c.q), c.ld_q, ptr(c.k), ptr(c.v), c.kv, 8 * 64 << 30, 1 << 30, 1, None, ptr(i32([10])),
+            None, None, 65535, 3, 8, 8, 64, ptr(ws), ws.numel(), None))
+
+
 # ---- verification ---------------------------------------------------------------------------------
 
 def weights(l, inv):
@@ -585,6 +607,20 @@ def test_verify_refusals():
         with pytest.raises(native.TFError, match=text):
             native.check(L.tf_op_verify_tree(*{**good, **bad}.values()))
     native.check(L.tf_op_verify_tree(*{**good, "B": 0}.values()))
+
+
+@pytest.mark.parametrize("V,with_draft,text", [(409601, True, "409600"), (819201, False, "819200")])
+def test_verify_refuses_a_vocabulary_that_does_not_fit(V, with_draft, text):
+    t = torch.zeros(4096, device="cuda")
+    with pytest.raises(native.TFError, match=text):
+        native.check(native.lib().tf_op_verify_tree(ptr(t), ptr(t), ptr(t), ptr(t), V, ptr(t) if with_draft else None, V, ptr(t),
+                                                    ptr(t), None, ptr(t), 1.0, 1, 2, V, ptr(t), 1 << 30, None))
+
+
+@pytest.mark.parametrize("V,with_draft", [(409600, True), (819200, False)])
+def test_verify_largest_vocabulary(V, with_draft):
+    logits, draft, tokens, parents, u = problem(1, 3, V, seed=6, with_draft=with_draft, chain=True)
+    check_verify((logits, draft, tokens, parents, u), [3], 0.9)
 
 
 # ---- commit ---------------------------------------------------------------------------------------
