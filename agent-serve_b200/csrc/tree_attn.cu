@@ -42,7 +42,7 @@ struct TreePlan {
     int rep_inv;             // (x * rep_inv) >> 16 = x / rep for x < 2048 and rep <= 8
 };
 struct TreeDesc {            // a unit split over CTAs c0..c1, found at slot c0
-    int b, kvh, rtile, c1;   // b < 0: none
+    int b, kvh, tile, c1;    // b < 0: none; tile: row tile, and its rows in the high half
 };
 
 __host__ __device__ inline size_t tree_part_floats(int rt, int hd) { return (size_t)rt * (hd + 2); }
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
             }
         }
         if (!whole && t0 == 0 && tid == 0)
-            desc[blockIdx.x] = TreeDesc{b, kvh, rtile, sg.last_cta};
+            desc[blockIdx.x] = TreeDesc{b, kvh, rtile | min(RT, rows - rtile * RT) << 16, sg.last_cta};
         __syncthreads();
         if (anybad) {
             tree_fix_rows<KVT>(a, sg, RT, rep, badrow, &vis[0][0], part, whole, tid, TN_THREADS);
@@ -1443,7 +1443,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                 wide_rows_out<HD>(sb + F::Q_OFF, sh.ml[0], sh.dst, h, hd);
                 named_bar<1, 256>();  // the shared memory takes the next half, or the next segment's queries
             }
-            if (!whole && sg.t0 == 0 && tid == 0) desc[blockIdx.x] = TreeDesc{sg.b, sg.kvh, sg.rtile, sg.last_cta};
+            if (!whole && sg.t0 == 0 && tid == 0)
+                desc[blockIdx.x] =
+                    TreeDesc{sg.b, sg.kvh, sg.rtile | min(TW_RT, sg.s.n_node * rep - sg.rtile * TW_RT) << 16, sg.last_cta};
             if (badrow_any(sh.badrow[seg & 7])) {
                 if (!*abort_flag)
                     tree_fix_rows<KVT>(a, sg, TW_RT, rep, sh.badrow[seg & 7], &sh.vis[0][0], part, whole, tid, 256);
@@ -1471,42 +1473,50 @@ __global__ void __launch_bounds__(TC_THREADS) tf_tree_combine_kernel(const TreeA
     pdl_trigger();
     pdl_wait();
     const int c0 = blockIdx.x, lane = threadIdx.x & 31;
+    const int r = blockIdx.y * (TC_THREADS / 32) + (threadIdx.x >> 5);
     const TreeDesc de = static_cast<const TreeDesc*>(a.ws)[c0];
-    if (de.b < 0) return;
+    if (de.b < 0 || r >= de.tile >> 16) return;
     const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + 65536);
     const int rep = a.n_head / a.n_kv, hd = a.hd, rt = pl.rt, n = de.c1 - c0 + 1;
+    const int rr = (de.tile & 0xFFFF) * rt + r;
     const size_t pf = tree_part_floats(rt, hd);
-    const int n_node = tree_seq(a, de.b).n_node;
-    const int r = blockIdx.y * (TC_THREADS / 32) + (threadIdx.x >> 5), rr = de.rtile * rt + r;
-    if (r >= rt || rr >= n_node * rep) return;
     auto part = [&](int i) { return parts + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * pf; };
-    float M = -INFINITY;
-#pragma unroll 1
-    for (int i = lane; i < n; i += 32) M = fmaxf(M, part(i)[(size_t)rt * hd + r]);
-    M = warp_max(M);
-    const float ref = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
+    // 32 parts at a time, a lane per part for the weights and per four dims for the sums; eight
+    // parts' loads in flight
+    float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     const int d = lane * 4;
 #pragma unroll 1
     for (int i0 = 0; i0 < n; i0 += 32) {
-        float w = 0.f, lw = 0.f;
-        if (i0 + lane < n) {
-            const float* p = part(i0 + lane);
-            w = exp2_fast(p[(size_t)rt * hd + r] - ref);
-            lw = p[(size_t)rt * hd + rt + r] * w;
-        }
-        L += warp_sum(lw);
         const int k = min(32, n - i0);
-#pragma unroll 4
-        for (int i = 0; i < k; ++i) {
-            const float wi = __shfl_sync(0xFFFFFFFFu, w, i);
-            if (d < hd) {
-                const float4 x = *reinterpret_cast<const float4*>(part(i0 + i) + (size_t)r * hd + d);
-                o.x = fmaf(x.x, wi, o.x);
-                o.y = fmaf(x.y, wi, o.y);
-                o.z = fmaf(x.z, wi, o.z);
-                o.w = fmaf(x.w, wi, o.w);
+        float m = -INFINITY, l = 0.f;
+        if (lane < k) {
+            const float* p = part(i0 + lane) + (size_t)rt * hd + r;
+            m = p[0];
+            l = p[rt];
+        }
+        float w = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < k; i += 8) {
+            float4 x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = i + j < k && d < hd ? *reinterpret_cast<const float4*>(part(i0 + i + j) + (size_t)r * hd + d)
+                                           : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i == 0) {
+                const float mx = fmaxf(M, warp_max(m)), ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(M - ref);
+                M = mx;
+                w = exp2_fast(m - ref);
+                L = fmaf(L, alpha, warp_sum(l * w));
+                o = make_float4(o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float wi = __shfl_sync(0xFFFFFFFFu, w, i + j);
+                o.x = fmaf(x[j].x, wi, o.x);
+                o.y = fmaf(x[j].y, wi, o.y);
+                o.z = fmaf(x[j].z, wi, o.z);
+                o.w = fmaf(x[j].w, wi, o.w);
             }
         }
     }
