@@ -15,12 +15,12 @@ constexpr int KC_VEC = 8;  // 16-byte vectors in flight per lane
 
 __global__ void __launch_bounds__(KC_THREADS) tf_kv_commit_kernel(const KvCommitArgs a) {
     const int lane = threadIdx.x & 31;
-    const long long unit = ((long long)blockIdx.x * KC_THREADS + threadIdx.x) >> 5;  // layer, sequence, kv head, K / V
-    if (unit >= (long long)a.n_layer * a.B * a.n_kv * 2) return;
-    const int kv = (int)(unit & 1);
-    const int h = (int)((unit >> 1) % a.n_kv);
-    const int b = (int)((unit >> 1) / a.n_kv % a.B);
-    const int layer = (int)((unit >> 1) / a.n_kv / a.B);
+    const unsigned unit = (unsigned)(((unsigned long long)blockIdx.x * KC_THREADS + threadIdx.x) >> 5);
+    if (unit >= (unsigned)a.n_layer * a.B * a.n_kv * 2u) return;
+    const int kv = (int)(unit & 1);                                  // layer, sequence, kv head, K / V
+    const unsigned seq = (unit >> 1) / (unsigned)a.n_kv;
+    const int h = (int)((unit >> 1) - seq * a.n_kv);
+    const int layer = (int)(seq / (unsigned)a.B), b = (int)(seq - (unsigned)layer * a.B);
     const int slot = a.slots ? a.slots[b] : b, n_ctx = a.n_ctx[b], n = a.n_path[b];
     const int* path = a.path + (long long)b * a.ld_path;
     bool bad = slot < 0 || slot >= a.n_slots || n_ctx < 0 || n_ctx > a.cap || n < 0 || n > a.ld_path;
@@ -30,7 +30,7 @@ __global__ void __launch_bounds__(KC_THREADS) tf_kv_commit_kernel(const KvCommit
             bad |= p < i || p >= a.cap - n_ctx || (i > 0 && p <= path[i - 1]);
         }
     bad = __any_sync(0xFFFFFFFFu, bad);
-    if (unit < 2ll * a.n_kv * a.B && kv == 0 && h == 0 && lane == 0) {
+    if (layer == 0 && kv == 0 && h == 0 && lane == 0) {
         if (bad) atomicCAS(a.err, 0, ERR_POS);
         if (a.n_new) a.n_new[b] = bad ? n_ctx : n_ctx + n;
     }
@@ -39,26 +39,31 @@ __global__ void __launch_bounds__(KC_THREADS) tf_kv_commit_kernel(const KvCommit
     uint4* base = reinterpret_cast<uint4*>(static_cast<uint8_t*>(kv ? a.vc : a.kc) +
                                            ((long long)layer * a.layer_stride + (long long)slot * a.slot_stride +
                                             ((long long)h * a.cap + n_ctx) * a.hd) * a.elem_bytes);
-    const int total = n * vpr;
+    const int total = n * vpr, rows_step = 32 / vpr, rest = 32 - rows_step * vpr;
+    int i = lane / vpr, c = lane - i * vpr;  // row and vector of this lane's next one
     for (int v0 = 0; v0 < total; v0 += 32 * KC_VEC) {
         uint4 r[KC_VEC];
+        unsigned moved = 0;
 #pragma unroll
         for (int u = 0; u < KC_VEC; ++u) {
-            const int v = v0 + u * 32 + lane;
-            if (v < total) {
-                const int i = v / vpr, p = path[i];
-                if (p != i) r[u] = base[(long long)p * vpr + v % vpr];
+            if (v0 + u * 32 + lane < total) {
+                const int p = path[i];
+                if (p != i) {
+                    r[u] = base[(long long)p * vpr + c];
+                    moved |= 1u << u;
+                }
+            }
+            i += rows_step;
+            c += rest;
+            if (c >= vpr) {
+                c -= vpr;
+                ++i;
             }
         }
         __syncwarp();
 #pragma unroll
-        for (int u = 0; u < KC_VEC; ++u) {
-            const int v = v0 + u * 32 + lane;
-            if (v < total) {
-                const int i = v / vpr;
-                if (path[i] != i) base[v] = r[u];
-            }
-        }
+        for (int u = 0; u < KC_VEC; ++u)
+            if (moved >> u & 1) base[v0 + u * 32 + lane] = r[u];
         __syncwarp();
     }
 }
@@ -115,7 +120,7 @@ cudaError_t tree_rope_store_launch(const AttnArgs& a, const int* depth, int M, c
 
 cudaError_t kv_commit_launch(const KvCommitArgs& a, cudaStream_t st) {
     const long long warps = (long long)a.n_layer * a.B * a.n_kv * 2, per = KC_THREADS / 32;
-    if ((warps + per - 1) / per > 0x7FFFFFFFll) return cudaErrorInvalidValue;
+    if (warps > 0xFFFFFFFFll - KC_THREADS) return cudaErrorInvalidValue;
     tf_kv_commit_kernel<<<(unsigned)((warps + per - 1) / per), KC_THREADS, 0, st>>>(a);
     return cudaGetLastError();
 }
