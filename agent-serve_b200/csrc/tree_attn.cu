@@ -26,7 +26,11 @@
 namespace tfb {
 
 constexpr int TN_THREADS = 256;
-constexpr int TN_UNIT_COST = 2;       // tiles that a unit's start and end take the time of: narrow, wide kernel
+// Tiles that a unit's start and end (queries, partial results, output) take the time of in the narrow
+// and the wide kernel.  Without them / with them, device time: 1 tree of 8, 8000 positions, 32x8x64 f32
+// (narrow) 28.7 / 22.9 us; 12 trees of 31, 4001 positions, 32x8x128 bf16 (wide) 113 / 97 us; 32 trees
+// of 64, 8128 positions, 32x8x64 f16 (wide) 257 / 212 us; 1 tree of 64, 16000 positions 48.8 / 50.7 us.
+constexpr int TN_UNIT_COST = 2;
 constexpr int TW_UNIT_COST = 5;
 constexpr int TN_TILE_BYTES = 32768;  // K and V bytes of a tile in the cache's type: 32 registers per thread
 constexpr float kLog2e = 1.4426950408889634f;
@@ -379,6 +383,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 // ---- narrow trees: mma.sync, up to 64 rows per row tile ----------------------------------------------
+// (16 rows do not fill a tcgen05 product, and its set-up costs more than a short context takes.)
 // One CTA of 8 warps per range of tiles, two CTAs per SM.  A tile is 32 KB of cache (K and V),
 // copied into shared memory by cp.async one tile ahead while the current one is computed; fp32
 // and bf16 tiles are then split into f16 halves in a second buffer, each thread taking the
@@ -386,6 +391,14 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // buffers.  Operand rows are HD halves, 16-byte chunk c of row r at c ^ (r & 7).
 // Warp (m, g): 16 rows of row block m, the positions of group g of the tile; each keeps its own
 // running maximum, sum and output, and the groups meet through shared memory when a unit ends.
+// 32 KB tiles, because two CTAs of two buffers and the queries fill an SM's shared memory.
+//
+// Bound by the latency of a tile's chain (copy, split, scores, softmax, P V: about 6000 cycles per
+// tile and CTA, two CTAs per SM) and, in short calls, by the unit's start (queries behind the
+// lengths, 5000 cycles) and the launches.  Device time, both launches: 1 tree of 1, 96 positions,
+// 32x8x64 f32 8.6 us; 1 tree of 5, 1733 positions, 14x2x64 f32 12.7 us; 1 tree of 8, 8000 positions,
+// 32x8x64 f32 22.9 us (33 MB: 1.4 TB/s); 32 trees of 8, 1144 positions, the same 61.9 us (151 MB: 2.4
+// TB/s).
 template <int HD, int MT, int KVT>
 struct NarrowCfg {
     static constexpr int ESZ = KVT == KV_F32 ? 4 : 2;
@@ -528,7 +541,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
             }
             if (KVT != KV_F16) {
                 if (t > t0) __syncthreads();  // the last tile's operands are free
-                // split after the last tile's scale; when the maximum turns out not to fit it
+                // split by the last tile's scale; when the maximum turns out not to fit it
                 // (seldom), once more after its own
                 for (;;) {
 #pragma unroll 1
@@ -753,18 +766,35 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
 }
 
 // ---- wide trees: tcgen05, 128 rows per row tile -------------------------------------------------------
-// One CTA per SM and range of tiles, four warpgroups:
-//   0, 1  softmax streams: even and odd tiles of a segment, a thread per row with a running
-//         maximum, sum and output of its own (registers); no shuffles, no exchange until the end;
-//   2     loaders: a tile's K and V rows arrive by one 1-D bulk copy each, are split into f16
-//         halves and written as MMA operands (rows of 64 dims, 128-byte swizzle);
-//   3     MMA issue (one thread).
+// One CTA per SM and range of tiles, sixteen warps:
+//   0-7       softmax streams (two warpgroups): even and odd tiles of a segment, a thread per row with
+//             a running maximum, sum and output of its own (registers); no shuffles, no exchange
+//             until the end;
+//   8-11, 14, loaders: a tile is split into f16 halves and written as MMA operands (rows of 64 dims,
+//   15        128-byte swizzle): fp32 from raw buffers, bf16 in place, and of either type the last
+//             tiles, whose rows may end inside;
+//   12        MMA issue;
+//   13        copies ahead of the loaders: fp32 rows by bulk copies into raw buffers, bf16 tiles
+//             through a tensor map into their operand stages.  (f16 tiles need no loader at all.)
 // Tensor memory: S_0, S_1 (PT columns each) and D_0, D_1 (HD columns each).  QK: S_w = Q K^T,
 // Q from shared memory, the tile K-major.  The softmax thread overwrites its scores in place,
 // CH columns at a time, with the high halves of p (CH / 2 columns) and the low ones, the A
 // operand of PV: D_w = P V, the same tile layout read MN-major; D_w starts from zero for every
 // tile and joins the registers' output.  QK of tile i + 1 is issued before PV of tile i, so the
 // tensor pipe works while a stream is in its softmax.
+// 128 positions per tile (64 where fp32 rows of 128 dims would not fit): the costs per tile (waits,
+// reductions, the output's join) are spread over most scores.  Registers: HD output sums per softmax
+// thread decide the split between the warpgroups.
+//
+// Bound, 16-bit caches of 64 dims: by the instructions of the two softmax streams, one warp of each
+// per scheduler (per 128 x 128 tile about 750 cycles for the maximum, 2700 for exponentials and their
+// split, 550 for the join); issue slots 53 %, tensor pipe 38 %, DRAM 35 % of their peaks.  fp32 and
+// bf16: by the loaders' split (tensor pipe 16 to 29 %), and for heads of 128 dims by the 22000 cycles
+// of a segment's start and end.  Device time, both launches: 32 trees of 64, 8128 positions, 32x8x64
+// f16 212 us (342 MB of rows read: 1.6 TB/s; 155 GF in two products: 733 TF/s); 12 trees of 31, 4001
+// positions, 32x8x128 bf16 97 us; 1 tree of 64, 16000 positions, 32x8x64 f32 51 us (25 GF in three
+// products: 497 TF/s).  A third score buffer (QK two tiles ahead) and chunks of scores fetched ahead
+// made no difference and were left out.
 constexpr int TW_THREADS = 512;
 constexpr int TW_RT = 128;
 
@@ -1056,7 +1086,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         }
                     }
                     if (KVT != KV_F16) {
-                        // split after the last tile's scale; when the maximum turns out not to fit it
+                        // split by the last tile's scale; when the maximum turns out not to fit it
                         // (seldom), once more after its own.  bf16 tiles are converted in place, so
                         // their maximum is found first.
                         unsigned* tm = &sh.tmax[2 * (n & 1) + which];
@@ -1468,6 +1498,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
 
 // ---- joins the partial results of units that were split over CTAs ------------------------------------
 // Block (c, y): the unit that starts in CTA c's range and ends in a later one; a warp per row.
+// out = sum_i w_i o_i / sum_i w_i l_i, w_i = exp2(m_i - max m).  Bound by the latency of its loads
+// (descriptor; maxima and sums; rows): eight rows in flight took 15.2 us of a tree of 5 at 1733
+// positions to 12.7, and 35.2 us of one of 9 at 16000 to 25.4.
 constexpr int TC_THREADS = 256;
 __global__ void __launch_bounds__(TC_THREADS) tf_tree_combine_kernel(const TreeAttnArgs a, const TreePlan pl) {
     pdl_trigger();
@@ -1539,13 +1572,13 @@ static int tree_sms() {
 
 // Rows of a unit's row tile, which chooses the kernel too: TW_RT the wide one, fewer the narrow one.
 // Device time, narrow / wide (f32 unless said; B trees of T nodes, positions, heads x kv heads x dims):
-//   up to 32 rows:   1 x 8, 100, 32x8x64: 9.9 / 19.2 us;  32 x 8, 1144, 32x8x64 f16: 33.8 / 43.1;
-//                    the same in f32: 62.1 / 60.7;  1 x 8, 8000: 28.3 / 26.3
-//   33 to 64 rows:   1 x 12, 100, 32x8x64 (0.4 MB of K and V): 12.3 / 18.5;  1 x 5, 1733, 14x2x64
-//                    (1.8 MB): 15.3 / 16.6;  2 x 14, 700, 32x8x64 f16 (2.9 MB): 14.7 / 14.5;
-//                    1 x 9, 2000, 12x2x128 (4.1 MB): 23.0 / 21.5;  1 x 9, 16000, the same in
-//                    bf16: 50.4 / 35.5;  32 x 8, 1144, 12x2x128: 40.7 / 38.2;  32 x 16, 1144,
-//                    32x8x64: 59.6 / 52.5
+//   17 to 32 rows:   1 x 8, 100, 32x8x64: 10.4 / 19.3 us;  32 x 8, 1144, 32x8x64 f16: 34.1 / 42.3;
+//                    the same in f32: 61.9 / 60.7;  1 x 8, 8000: 22.9 / 22.8
+//   33 to 64 rows:   1 x 12, 100, 32x8x64 (0.4 MB of K and V): 12.8 / 19.2;  1 x 5, 1733, 14x2x64
+//                    (1.8 MB): 12.7 / 15.2;  2 x 14, 700, 32x8x64 f16 (2.9 MB): 14.3 / 14.0;
+//                    1 x 9, 2000, 12x2x128 (4.1 MB): 17.8 / 18.6;  1 x 9, 16000, the same in
+//                    bf16: 34.5 / 25.6;  32 x 8, 1144, 12x2x128: 39.1 / 37.1, in f16 28.7 / 34.0;
+//                    32 x 10, 1144, 32x8x64: 59.1 / 52.1;  16 x 12, 4000, the same in f16: 50.1 / 40.3
 // so 64 rows stay with the narrow kernel only where the whole cache is too small to repay the wide
 // one's set-up (lengths are on the device: the capacity stands for them).
 constexpr double TN_MAX_BYTES = 4e6;

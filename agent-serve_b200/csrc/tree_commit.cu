@@ -4,8 +4,10 @@
 //
 // One warp per (layer, sequence, kv head, K or V).  The path is strictly increasing, so
 // path[i] >= i: taking the rows in ascending groups, each group loaded into registers before it
-// is stored, never reads a row that an earlier group has overwritten.  Bound by latency (a few
-// rows of 128 to 512 bytes per warp); rows that stay where they are (the root's) are not moved.
+// is stored, never reads a row that an earlier group has overwritten.  Rows that stay where they
+// are (the root's) are not moved.  Bound by latency (lengths and path, then a few rows of 128 to 512
+// bytes per warp): 16 layers of 8 kv heads, one path of 5 rows 2.2 us; 28 layers of 2 kv heads of 128
+// dims fp32, 64 paths of 7 rows 9.4 us (44 MB read and written: 4.7 TB/s).
 #include "tree.cuh"
 
 namespace tfb {
@@ -71,7 +73,8 @@ __global__ void __launch_bounds__(KC_THREADS) tf_kv_commit_kernel(const KvCommit
 // ---- the drafted nodes' rows: RoPE of q (in place) and k at the node's depth, K / V store -------------
 // Node m of the sequence in slots[m] stands at position pos[slot] + depth[m] and takes cache row
 // pos[slot] + m (siblings share a position).  One CTA per (node, head), a thread per rotation pair,
-// as the prefill chunk's kernel.
+// as the prefill chunk's kernel.  (A launch's latency: q, k and v of a step's 64 nodes are 1 to 2 MB,
+// which the attention behind it reads from L2.)
 __global__ void tf_tree_rope_store_kernel(const AttnArgs a, const int* depth) {
     pdl_trigger();
     pdl_wait();
