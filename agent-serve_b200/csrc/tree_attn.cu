@@ -1271,14 +1271,17 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         tc_fence_after();
                         const uint32_t d = tm + w * 128;
                         const uint64_t kb = wide_desc(sb + F::K_OFF + os * NLO * F::HALF, 16), qb = wide_desc(sb + F::Q_OFF, 16);
+                        // the products with a low half first: each step truncates at the size of the
+                        // sum so far, which the high halves' products bring up only then
 #pragma unroll
-                        for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes along the rows of a 64-dim block
-                            const uint64_t q = qb + ((j / 4) * (TW_RT * 128) + (j % 4) * 32) / 16;
-                            const uint64_t k = kb + ((j / 4) * (PT * 128) + (j % 4) * 32) / 16;
-                            wide_mma_ss(d, q, k, iqk, j > 0, lead);
-                            wide_mma_ss(d, q + F::QH / 16, k, iqk, 1, lead);
-                            if (NLO == 2) wide_mma_ss(d, q, k + F::HALF / 16, iqk, 1, lead);
-                        }
+                        for (int hi = 0; hi < 2; ++hi)
+#pragma unroll
+                            for (int j = 0; j < HD / 16; ++j) {  // 16 dims: 32 bytes along the rows of a 64-dim block
+                                const uint64_t q = qb + ((j / 4) * (TW_RT * 128) + (j % 4) * 32) / 16;
+                                const uint64_t k = kb + ((j / 4) * (PT * 128) + (j % 4) * 32) / 16;
+                                wide_mma_ss(d, hi ? q : q + F::QH / 16, k, iqk, hi || j > 0, lead);
+                                if (NLO == 2 && !hi) wide_mma_ss(d, q, k + F::HALF / 16, iqk, 1, lead);
+                            }
                         wide_commit(&sh.kfree[os], lead);
                         wide_commit(&sh.sfull[w], lead);
                     }
@@ -1295,12 +1298,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         const uint32_t d = tm + 256 + v * HD, p = tm + v * 128;
                         const uint64_t vh = wide_desc(sb + F::V_OFF + os * NLO * F::HALF, PT * 128);
 #pragma unroll
-                        for (int j = 0; j < PT / 16; ++j) {  // 16 positions: 2048 bytes of rows; p's halves in blocks of CH columns
-                            const uint32_t ph = CH == 32 ? p + 32 * (j / 2) + 8 * (j % 2) : p + 16 * j;
-                            wide_mma_ts(d, ph, vh + 128u * j, ipv, j > 0, lead);
-                            wide_mma_ts(d, ph + CH / 2, vh + 128u * j, ipv, 1, lead);
-                            if (NLO == 2) wide_mma_ts(d, ph, vh + F::HALF / 16 + 128u * j, ipv, 1, lead);
-                        }
+                        for (int hi = 0; hi < 2; ++hi)
+#pragma unroll
+                            for (int j = 0; j < PT / 16; ++j) {  // 16 positions: 2048 bytes of rows; p's halves in blocks of CH columns
+                                const uint32_t ph = CH == 32 ? p + 32 * (j / 2) + 8 * (j % 2) : p + 16 * j;
+                                wide_mma_ts(d, hi ? ph : ph + CH / 2, vh + 128u * j, ipv, hi || j > 0, lead);
+                                if (NLO == 2 && !hi) wide_mma_ts(d, ph, vh + F::HALF / 16 + 128u * j, ipv, 1, lead);
+                            }
                         wide_commit(&sh.vfree[os], lead);
                         wide_commit(&sh.dfull[v], lead);
                     }
