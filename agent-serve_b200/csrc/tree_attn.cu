@@ -1580,22 +1580,32 @@ static int tree_sms() {
 //                    the same in f32: 61.9 / 60.7;  1 x 8, 8000: 22.9 / 22.8
 //   33 to 64 rows:   1 x 12, 100, 32x8x64 (0.4 MB of K and V): 12.8 / 19.2;  1 x 5, 1733, 14x2x64
 //                    (1.8 MB): 12.7 / 15.2;  2 x 14, 700, 32x8x64 f16 (2.9 MB): 14.3 / 14.0;
-//                    1 x 9, 2000, 12x2x128 (4.1 MB): 17.8 / 18.6;  1 x 9, 16000, the same in
-//                    bf16: 34.5 / 25.6;  32 x 8, 1144, 12x2x128: 39.1 / 37.1, in f16 28.7 / 34.0;
-//                    32 x 10, 1144, 32x8x64: 59.1 / 52.1;  16 x 12, 4000, the same in f16: 50.1 / 40.3
-// so 64 rows stay with the narrow kernel only where the whole cache is too small to repay the wide
-// one's set-up (lengths are on the device: the capacity stands for them).
+//                    1 x 9, 2000, 12x2x128 (4.1 MB): 17.8 / 18.6;  32 x 8, 1144, 12x2x128: 39.1 /
+//                    37.1;  32 x 10, 1144, 32x8x64: 59.1 / 52.1;  16 x 12, 4000, in f16: 50.1 / 40.3
+//   the same, 16-bit rows of 128 dims (12x2x128, f16; bf16; positions):  1 x 9, 2000: 16.3 / 16.7;
+//                    18.2 / 21.7;  32 x 8, 1144: 25.1 / 29.2; 29.2 / 40.3;  64 x 7, 600: 30.3 / 31.4;
+//                    35.5 / 43.9;  4 x 10, 4000: 24.6 / 19.2; 26.9 / 24.0;  32 x 9, 4000: 78.1 /
+//                    44.7; 97.4 / 73.7;  1 x 9, 16000: 32.1 / 21.6; 34.4 / 25.9
+// So up to 64 rows stay with the narrow kernel where the cache is too small to repay the wide one's
+// set-up; for 16-bit rows of 128 dims, where a segment's start and end take as long as three or more
+// tiles of 128 positions, where sequences are short.  (Lengths are on the device: the capacity stands
+// for them.)
 constexpr double TN_MAX_BYTES = 4e6;
-static int tree_row_tile(int rows, double kv_bytes) {
+constexpr int TN_MAX_CAP = 3000;
+static bool tree_short(const TreeAttnArgs& a) {
+    if (a.hd > 64 && a.kv_type != KV_F32) return a.cap < TN_MAX_CAP;
+    return 2.0 * a.B * a.n_kv * a.cap * a.hd * (a.kv_type == KV_F32 ? 4 : 2) < TN_MAX_BYTES;
+}
+static int tree_row_tile(int rows, bool short_cache) {
     if (rows <= 32) return rows <= 16 ? 16 : 32;
-    return rows <= 64 && kv_bytes < TN_MAX_BYTES ? 64 : TW_RT;
+    return rows <= 64 && short_cache ? 64 : TW_RT;
 }
 static int tree_grid(int rt) { return rt == TW_RT ? tree_sms() : 2 * tree_sms(); }
 
 size_t tree_attn_ws_bytes(int B, int T, int n_head, int n_kv, int hd) {
     (void)B;
     static_assert(TW_RT == 2 * 64, "half the CTAs, twice the rows: a tile of 64 rows needs as much as a wide one");
-    const int rt = tree_row_tile(T * (n_head / n_kv), TN_MAX_BYTES);
+    const int rt = tree_row_tile(T * (n_head / n_kv), false);
     return 65536 + (size_t)tree_grid(rt) * 2 * tree_part_floats(rt, hd) * sizeof(float);
 }
 
@@ -1699,8 +1709,7 @@ static cudaError_t wide_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl)
 
 template <int HD, int KVT>
 static cudaError_t rows_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl) {
-    const double kv_bytes = 2.0 * a.B * a.n_kv * a.cap * a.hd * (KVT == KV_F32 ? 4 : 2);
-    const int rt = tree_row_tile(a.T * (a.n_head / a.n_kv), kv_bytes);
+    const int rt = tree_row_tile(a.T * (a.n_head / a.n_kv), tree_short(a));
     if (rt == 16) return narrow_launch<HD, 1, KVT>(a, st, pdl);
     if (rt == 32) return narrow_launch<HD, 2, KVT>(a, st, pdl);
     if (rt == 64) return narrow_launch<HD, 4, KVT>(a, st, pdl);
