@@ -354,7 +354,9 @@ int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk, 
     };
     auto matmul = [&](const Mm& q, int r0, int rows) -> int {
         const WeightRef& w = *q.w;
-        if (gemm_weight_ok(w) && rows >= GM_MIN_M) {
+        // (a model whose layers are mostly of other types has no GEMM buffers: a tree of 16 nodes or
+        // more gets here for its few Q8_0 / Q4_0 matrices all the same)
+        if (m->xh && gemm_weight_ok(w) && rows >= GM_MIN_M) {
             XPrepArgs p;
             memset(&p, 0, sizeof(p));
             p.x = q.x + (size_t)r0 * q.ldx;
