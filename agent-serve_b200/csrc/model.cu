@@ -166,12 +166,15 @@ struct tf_model {
     std::vector<int> gvt_meta;
     // speculative steps: drafted trees of up to tree_rows nodes (device words; pinned staging)
     int tree_rows = 0, tree_tile = 1;
-    int tree_n = 0, tree_seq = -1;  // the tree of the last tree step, until it is accepted
+    // the tree of the last tree step, until it is accepted or another step or a changed position of its
+    // sequence takes away what it was scored with (logits, context)
+    int tree_n = 0, tree_seq = -1;
     int *d_ttok = nullptr, *d_tpar = nullptr, *d_tdepth = nullptr;  // tokens, parents, depths
     unsigned long long* d_tmask = nullptr;
     float* d_tu = nullptr;
     int* d_tout = nullptr;          // [tree_rows] path | n_path | next | new position
-    int* d_tpos = nullptr;          // positions the step's finish kernel may advance (not used)
+    int* d_tpos = nullptr;          // positions the step's finish kernel may advance (not used) | the tree's
+                                    // context length, slot
     uint8_t* d_tws = nullptr;       // workspaces: attention, then verification
     size_t tws_attn = 0, tws_verify = 0;
     int* h_tree = nullptr;
@@ -457,7 +460,7 @@ int enqueue_step_gemm(tf_model* m, int M, bool head, int* n_launch, bool chunk, 
                 t.slot_stride = m->slot_elems;
                 t.cap = m->opt.max_seq;
                 t.n_slots = m->opt.max_batch;
-                t.slots = m->d_slots;
+                t.slots = m->d_tpos + m->opt.max_batch + 1;
                 t.n_ctx = m->d_tpos + m->opt.max_batch;
                 t.mask = m->d_tmask;
                 t.B = 1;
@@ -674,6 +677,7 @@ int enqueue_step(tf_model* m, int M, bool head, bool pdl, int* n_launch, int fus
 
 // Run one step for M rows (tokens in d_tokens[0..M), slots in d_slots[0..M)).
 int run_step(tf_model* m, int M, bool head, int fused, bool chunk = false, bool from_key = false, bool tree = false) {
+    if (!tree) m->tree_n = 0;  // its logits are overwritten
     if (!m->opt.use_graph) return enqueue_step(m, M, head, true, nullptr, fused, chunk, from_key, tree);
     // graphs are keyed by everything that changes the launch sequence or its arguments
     const bool split = head && m->split_step && M == 1;
@@ -781,6 +785,7 @@ int build_pk_plan(tf_model* m) {
 int run_pk(tf_model* m, int seq, const int* d_prompt, int n_prompt, int n_steps, int first_head, int ws_prompt,
            int hist_cap) {
     const PkPlan& p = m->pk_plan;
+    m->tree_n = 0;  // its logits are overwritten
     PkArgs a;
     memset(&a, 0, sizeof(a));
     a.mats = m->d_pkmats;
@@ -1347,6 +1352,7 @@ int tf_cuda_reset(tf_model* m, int seq) {
     const int s0 = seq < 0 ? 0 : seq, s1 = seq < 0 ? m->opt.max_batch : seq + 1;
     if (seq >= m->opt.max_batch) return fail(m, "sequence slot out of range");
     const size_t esz = m->opt.kv_type == TF_KV_F32 ? 4 : 2;
+    if (m->tree_seq >= s0 && m->tree_seq < s1) m->tree_n = 0;
     for (int s = s0; s < s1; ++s) {
         m->hpos[s] = 0;
         for (int li = 0; li < m->hp.n_layer; ++li) {  // KVCache::clear (src/kvcache.cpp:16-19)
@@ -1686,9 +1692,9 @@ int tree_init(tf_model* m) {
     if (!m->d_tmask) CK(cudaMalloc(&m->d_tmask, sizeof(unsigned long long) * R * ((R + 63) / 64)));
     if (!m->d_tu) CK(cudaMalloc(&m->d_tu, sizeof(float) * R));
     if (!m->d_tout) CK(cudaMalloc(&m->d_tout, sizeof(int) * (R + 3)));
-    if (!m->d_tpos) CK(cudaMalloc(&m->d_tpos, sizeof(int) * (m->opt.max_batch + 1)));
+    if (!m->d_tpos) CK(cudaMalloc(&m->d_tpos, sizeof(int) * (m->opt.max_batch + 2)));
     if (!m->d_tws) CK(cudaMalloc(&m->d_tws, m->tws_attn + m->tws_verify));
-    CK(cudaMemsetAsync(m->d_tpos, 0, sizeof(int) * (m->opt.max_batch + 1), m->stream));
+    CK(cudaMemsetAsync(m->d_tpos, 0, sizeof(int) * (m->opt.max_batch + 2), m->stream));
     CK(cudaMemsetAsync(m->d_tws, 0, m->tws_attn + m->tws_verify, m->stream));
     CK(cudaMallocHost(&m->h_tree, sizeof(int) * 5 * R + sizeof(unsigned long long) * R * ((R + 63) / 64) + 64));
     return 0;
@@ -1707,7 +1713,7 @@ int tf_cuda_tree_step(tf_model* m, int seq, const int* tokens, const int* parent
     for (int i = 0; i < n; ++i)
         if (tokens[i] < 0 || tokens[i] >= m->V) return fail(m, "token id out of range");
     if (tree_init(m)) return -1;
-    // staging: masks | tokens, parents, depths, slots, position
+    // staging: masks | tokens, parents, depths, slots, context length, slot
     unsigned long long* mask = reinterpret_cast<unsigned long long*>(m->h_tree);
     const size_t words = (size_t)n * ((n + 63) / 64);
     int* st = reinterpret_cast<int*>(mask + words);
@@ -1718,13 +1724,14 @@ int tf_cuda_tree_step(tf_model* m, int seq, const int* tokens, const int* parent
     memcpy(st + n, parents, sizeof(int) * n);
     for (int i = 0; i < n; ++i) st[3 * n + i] = seq;
     st[4 * n] = m->hpos[seq];
+    st[4 * n + 1] = seq;
     CK(cudaMemcpyAsync(m->d_tmask, mask, sizeof(unsigned long long) * words, cudaMemcpyHostToDevice, m->stream));
     CK(cudaMemcpyAsync(m->d_ttok, st, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
     CK(cudaMemcpyAsync(m->d_tokens, st, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
     CK(cudaMemcpyAsync(m->d_tpar, st + n, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
     CK(cudaMemcpyAsync(m->d_tdepth, st + 2 * n, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
     CK(cudaMemcpyAsync(m->d_slots, st + 3 * n, sizeof(int) * n, cudaMemcpyHostToDevice, m->stream));
-    CK(cudaMemcpyAsync(m->d_tpos + m->opt.max_batch, st + 4 * n, sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    CK(cudaMemcpyAsync(m->d_tpos + m->opt.max_batch, st + 4 * n, sizeof(int) * 2, cudaMemcpyHostToDevice, m->stream));
     if (run_step(m, n, true, 0, false, false, true)) return -1;
     const int rc = read_outputs(m, n, logits, argmax_out);
     if (rc) return rc;
@@ -1752,7 +1759,7 @@ int tf_cuda_tree_accept(tf_model* m, int seq, const float* draft, float temperat
         return fail(m, last_error_tls());
     const int* n_ctx = m->d_tpos + m->opt.max_batch;
     if (tf_op_kv_commit(m->kc, m->vc, m->opt.kv_type, m->hp.n_layer, m->layer_elems, m->slot_elems, m->opt.max_seq,
-                        m->opt.max_batch, m->d_slots, n_ctx, path, n, n_path, pos, 1, m->hp.n_kv_head, m->hd, m->stream))
+                        m->opt.max_batch, n_ctx + 1, n_ctx, path, n, n_path, pos, 1, m->hp.n_kv_head, m->hd, m->stream))
         return fail(m, last_error_tls());
     CK(cudaMemcpyAsync(m->d_pos + seq, pos, sizeof(int), cudaMemcpyDeviceToDevice, m->stream));
     int* back = m->h_tree + m->tree_rows;

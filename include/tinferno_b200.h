@@ -175,7 +175,9 @@ TF_API int tf_cuda_reset(tf_model* m, int seq);
  *                        or nullptr; u, host, n uniform numbers, for temperature > 0), moves the
  *                        kept path's K/V rows up in every layer and advances the position by the
  *                        path's length.  nodes (host, n ints) receives the kept nodes, the root
- *                        first, *n_nodes their count, *next the token after them: the next root;
+ *                        first, *n_nodes their count, *next the token after them: the next root.
+ *                        Another step of the engine (of any sequence), or a reset or rewind of
+ *                        this one, ends the tree: accepting it is then refused;
  *   tf_cuda_rewind       takes a sequence back to an earlier position (a draft model's cache after
  *                        a refused draft);
  *   tf_cuda_tree_capacity  nodes per tree (64, or the prefill chunk's rows);

@@ -45,3 +45,63 @@ def test_tree_step_of_a_model_without_gemm_buffers(cfg, n, model_cache):
             want = m.decode(tokens[i])
             assert np.abs(lg[i] - want).max() < LOGIT_TOL, (leaf, i, np.abs(lg[i] - want).max())
     m.close()
+
+
+@pytest.fixture(scope="module")
+def path(model_cache):
+    return synth.model_path(CFG, model_cache)
+
+
+def prompts(n=2):
+    return [[int(t) for t in synth.prompt_tokens(CFG, 18 + i, stream=3 + i)] for i in range(n)]
+
+
+def started(path, **kw):
+    """Two sequences behind their prompts; the greedy tokens after them."""
+    m = Model(path, RunConfig(max_seq=96, max_batch=2, **kw))
+    return m, [int(np.argmax(m.prefill(p, seq=i))) for i, p in enumerate(prompts())]
+
+
+STEPS = {
+    "decode another": lambda m, t: m.decode(t[1], seq=1),
+    "decode the same": lambda m, t: m.decode(t[0], seq=0),
+    "decode both": lambda m, t: m.decode_batch([1, 0], [t[1], t[0]]),
+    "short prompt of another": lambda m, t: m.prefill([5, 6, 7], seq=1),
+    "long prompt of another": lambda m, t: m.prefill(list(range(20, 60)), seq=1),
+    "prompts of both": lambda m, t: m.prefill_batch([0, 1], [[3, 4], [5, 6]]),
+    "generation of another": lambda m, t: m.generate_greedy(t[1], 3, seq=1),
+    "sharded step of another": lambda m, t: (m.set_vocab_shard(0, 1), m.decode_shard(t[1], seq=1)),
+    "reset": lambda m, t: m.reset(0),
+    "reset of all": lambda m, t: m.reset(),
+}
+
+
+@pytest.mark.parametrize("step", list(STEPS))
+def test_a_step_in_between_ends_the_tree(step, path):
+    """The logits and the context that a tree was scored with are gone after another step: accepting it
+    is refused, and every sequence goes on as if the tree had never been drafted."""
+    m, t = started(path)
+    m.tree_step([t[0], 11, 12, 13], [-1, 0, 1, 0], seq=0)
+    STEPS[step](m, t)
+    with pytest.raises(native.TFError, match="no tree step"):
+        m.tree_accept(seq=0)
+    plain, _ = started(path)
+    STEPS[step](plain, t)
+    for s in (0, 1):
+        assert m.n_pos(seq=s) == plain.n_pos(seq=s)
+        assert np.array_equal(m.decode(9, seq=s), plain.decode(9, seq=s))
+    m.close()
+    plain.close()
+
+
+@pytest.mark.parametrize("what", ["reset", "rewind"])
+def test_another_sequences_position_does_not_end_the_tree(what, path):
+    m, t = started(path)
+    am = m.tree_step([t[0], 11], [-1, 0], seq=0)
+    if what == "reset":
+        m.reset(1)
+    else:
+        m.rewind(4, seq=1)
+    kept, nxt = m.tree_accept(seq=0)
+    assert nxt == am[len(kept)] and m.n_pos(seq=0) == len(prompts()[0]) + 1 + len(kept)
+    m.close()
