@@ -1748,28 +1748,59 @@ int tf_cuda_tree_accept(tf_model* m, int seq, const float* draft, float temperat
     if (!nodes || !n_nodes || !next) return fail(m, "null outputs");
     if (m->tree_n < 1 || m->tree_seq != seq) return fail(m, "no tree step of this sequence to accept");
     const int n = m->tree_n;
+    TreeVerifyArgs v = {};
+    if (const char* refusal = tree_verify_refusal(temperature, draft != nullptr, m->V, &v.inv_temp)) return fail(m, refusal);
     if (temperature > 0.0f) {
         if (!u) return fail(m, "u must not be null at a positive temperature");
         memcpy(m->h_tree, u, sizeof(float) * n);
         CK(cudaMemcpyAsync(m->d_tu, m->h_tree, sizeof(float) * n, cudaMemcpyHostToDevice, m->stream));
     }
     int *path = m->d_tout, *n_path = path + m->tree_rows, *nx = n_path + 1, *pos = nx + 1;
-    if (tf_op_verify_tree(path, n_path, nx, m->logits, m->V, draft, m->V, m->d_ttok, m->d_tpar, nullptr, m->d_tu, temperature, 1,
-                          n, m->V, m->d_tws + m->tws_attn, m->tws_verify, m->stream))
-        return fail(m, last_error_tls());
-    const int* n_ctx = m->d_tpos + m->opt.max_batch;
-    if (tf_op_kv_commit(m->kc, m->vc, m->opt.kv_type, m->hp.n_layer, m->layer_elems, m->slot_elems, m->opt.max_seq,
-                        m->opt.max_batch, n_ctx + 1, n_ctx, path, n, n_path, pos, 1, m->hp.n_kv_head, m->hd, m->stream))
-        return fail(m, last_error_tls());
-    CK(cudaMemcpyAsync(m->d_pos + seq, pos, sizeof(int), cudaMemcpyDeviceToDevice, m->stream));
+    // the operators' kernels with the engine's own error word
+    v.path = path;
+    v.n_path = n_path;
+    v.next = nx;
+    v.logits = m->logits;
+    v.ld = m->V;
+    v.draft = temperature > 0.0f ? draft : nullptr;
+    v.ld_draft = m->V;
+    v.tokens = m->d_ttok;
+    v.parents = m->d_tpar;
+    v.u = m->d_tu;
+    v.B = 1;
+    v.T = n;
+    v.V = m->V;
+    v.ws = m->d_tws + m->tws_attn;
+    v.err = m->d_err;
+    KvCommitArgs c = {};
+    c.kc = m->kc;
+    c.vc = m->vc;
+    c.elem_bytes = m->opt.kv_type == TF_KV_F32 ? 4 : 2;
+    c.n_layer = m->hp.n_layer;
+    c.layer_stride = m->layer_elems;
+    c.slot_stride = m->slot_elems;
+    c.cap = m->opt.max_seq;
+    c.n_slots = m->opt.max_batch;
+    c.n_ctx = m->d_tpos + m->opt.max_batch;
+    c.slots = c.n_ctx + 1;
+    c.path = path;
+    c.ld_path = n;
+    c.n_path = n_path;
+    c.n_new = pos;
+    c.B = 1;
+    c.n_kv = m->hp.n_kv_head;
+    c.hd = m->hd;
+    c.err = m->d_err;
+    CK(tree_verify_launch(v, m->stream));
+    CK(kv_commit_launch(c, m->stream));
     int* back = m->h_tree + m->tree_rows;
     CK(cudaMemcpyAsync(back, m->d_tout, sizeof(int) * (m->tree_rows + 3), cudaMemcpyDeviceToHost, m->stream));
     m->tree_n = 0;
+    // the position moves, on both sides, only when nothing failed: the rows in front of it are untouched
+    // then, and the step can be taken again
     const int rc = finish_call(m);
     if (rc) return rc;
-    int code = 0;
-    if (tf_op_device_error(m->stream, &code)) return fail(m, last_error_tls());
-    if (code) return fail(m, err_code_text(code));
+    CK(cudaMemcpyAsync(m->d_pos + seq, pos, sizeof(int), cudaMemcpyDeviceToDevice, m->stream));
     const int k = back[m->tree_rows];
     memcpy(nodes, back, sizeof(int) * k);
     *n_nodes = k;

@@ -54,6 +54,8 @@ struct TreeVerifyArgs {
 };
 size_t tree_verify_ws_bytes(int B, int T, int V);
 int tree_verify_max_vocab(bool draft);  // a row's slices fit the shared memory of a cluster
+// What a caller's temperature and vocabulary are refused for (nullptr: nothing); inv_temp: 0 for greedy.
+const char* tree_verify_refusal(float temperature, bool draft, int V, float* inv_temp);
 cudaError_t tree_verify_launch(const TreeVerifyArgs& a, cudaStream_t st);
 
 struct KvCommitArgs {

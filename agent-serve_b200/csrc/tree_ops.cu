@@ -34,6 +34,16 @@ int verify_shape(int B, int T, int V) {
 }
 }  // namespace
 
+namespace tfb {
+const char* tree_verify_refusal(float temperature, bool draft, int V, float* inv_temp) {
+    if (temperature != temperature) return "temperature is NaN";
+    *inv_temp = temperature <= 0.0f ? 0.0f : (float)(1.0 / (double)temperature);
+    if (!(*inv_temp < INFINITY) || (temperature > 0.0f && *inv_temp == 0.0f)) return "temperature out of range";
+    if (V > tree_verify_max_vocab(draft && temperature > 0.0f)) return "V is above the limit (409600 with draft, 819200 without)";
+    return nullptr;
+}
+}  // namespace tfb
+
 extern "C" {
 
 int tf_tree_mask(const int* parents, int n, int T, unsigned long long* mask, int* depth) {
@@ -119,12 +129,11 @@ int tf_op_verify_tree(int* path, int* n_path, int* next, const float* logits, lo
     if (B == 0) return 0;
     if (!path || !n_path || !next || !logits || !tokens || !parents || !ws) return set_error("null pointer");
     if (!(temperature <= 0.0f) && !u) return set_error("u must not be null at a positive temperature");
-    if (temperature != temperature) return set_error("temperature is NaN");
-    const float inv = temperature <= 0.0f ? 0.0f : (float)(1.0 / (double)temperature);
-    if (!(inv < INFINITY) || (temperature > 0.0f && inv == 0.0f)) return set_error("temperature out of range");
+    float inv = 0.0f;
+    const char* refusal = tree_verify_refusal(temperature, draft != nullptr, V, &inv);
+    if (refusal) return set_error(refusal);
     if (ld < V || (draft && ld_draft < V)) return set_error("ld must be at least V");
     if (!aligned(ws, 256)) return set_error("the workspace must be 256-byte aligned");
-    if (V > tree_verify_max_vocab(draft && temperature > 0.0f)) return set_error("V is above the limit (409600 with draft, 819200 without)");
     if (ws_bytes < tree_verify_ws_bytes(B, T, V)) return set_error("workspace too small");
     TreeVerifyArgs a = {};
     if (op_err_word(&a.err)) return -1;

@@ -105,3 +105,41 @@ def test_another_sequences_position_does_not_end_the_tree(what, path):
     kept, nxt = m.tree_accept(seq=0)
     assert nxt == am[len(kept)] and m.n_pos(seq=0) == len(prompts()[0]) + 1 + len(kept)
     m.close()
+
+
+def test_an_operator_calls_error_is_not_the_engines(path):
+    """The operator level's error word belongs to its callers: a code that waits there fails no
+    acceptance and stays to be read."""
+    torch = pytest.importorskip("torch")
+    L = native.lib()
+    m, t = started(path)
+    want = m.generate_greedy(t[0], 12)
+    m.rewind(len(prompts()[0]))
+    k = torch.zeros((1, 1, 1, 8, 8), device="cuda")
+    one = lambda v: torch.tensor([v], dtype=torch.int32, device="cuda")
+    n_ctx, p, n = one(0), one(5), one(1)
+    slot = one(7)  # outside the cache
+    native.check(L.tf_op_kv_commit(k.data_ptr(), k.data_ptr(), native.TF_KV_F32, 1, 64, 64, 8, 1, slot.data_ptr(), n_ctx.data_ptr(),
+                                   p.data_ptr(), 1, n.data_ptr(), None, 1, 1, 8, None))
+    torch.cuda.synchronize()
+    m.tree_step(want[:3], [-1, 0, 1])
+    kept, nxt = m.tree_accept()
+    assert kept == want[1:3] and nxt == want[3] and m.n_pos() == len(prompts()[0]) + 3
+    assert m.generate_greedy(nxt, 8) == want[3:11]  # device and host positions agree
+    code = native.C.c_int(0)
+    native.check(L.tf_op_device_error(None, native.C.byref(code)))
+    assert code.value == 4  # TF_DEV_ERR_POS of the operator call
+    m.close()
+
+
+def test_a_refused_acceptance_leaves_the_tree(path):
+    m, t = started(path)
+    am = m.tree_step([t[0], 11], [-1, 0], seq=0)
+    for temperature, text in ((float("nan"), "NaN"), (1e-45, "range"), (float("inf"), "range")):
+        with pytest.raises(native.TFError, match=text):
+            m.tree_accept(temperature, [0.5, 0.5], seq=0)
+    with pytest.raises(native.TFError, match="no tree step"):
+        m.tree_accept(seq=1)
+    kept, nxt = m.tree_accept(seq=0)
+    assert nxt == am[len(kept)] and m.n_pos(seq=0) == len(prompts()[0]) + 1 + len(kept)
+    m.close()
