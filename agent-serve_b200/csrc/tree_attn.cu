@@ -1373,7 +1373,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                 tree_wait(&sh.sfull[wg], cnt, a.err, ERR_WAIT_FULL, abort_flag);
                 __syncwarp();
                 tc_fence_after();
-                const float f = KVT == KV_F16 ? qs : qs * pow2i(sh.ek[(n0 + t) & 7]);
+                // (not below the smallest normal number: a query of zeros over small keys would make it zero, and
+                // the masked scores' -infinity a NaN; scores that small are equal)
+                const float f = KVT == KV_F16 ? qs : fmaxf(qs * pow2i(sh.ek[(n0 + t) & 7]), 1.17549435e-38f);
                 const bool tail = (t + 1) * PT > s.n_ctx;
                 // (the loops over CH-column chunks stay loops: unrolled, the code outgrows the
                 // instruction cache and the one warp per scheduler waits for its fetches)
