@@ -1334,7 +1334,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
 #pragma unroll
                     for (int i = 0; i < U; ++i) {
                         const int r = ((i0 + i) * 8 + warp) * RPW + lane / LPR, q = sg.rtile * TW_RT + r, nd = (q * rep_inv) >> 16;
-                        const float* qp = qb + (nd * a.ld_q + (q - nd * rep) * hd);
+                        const float* qp = qb + ((long long)nd * a.ld_q + (q - nd * rep) * hd);
                         x[i][0] = x[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
                         if (q < rows && c * 8 < hd) {
                             x[i][0] = reinterpret_cast<const float4*>(qp)[0];

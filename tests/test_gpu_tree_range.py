@@ -7,7 +7,7 @@ bits of what a row sees, whatever lies beside it."""
 import pytest
 
 from tinferno_b200 import native
-from test_gpu_tree import TYPES, Case, device_error
+from test_gpu_tree import TYPES, Case, device_error, torch
 
 pytestmark = pytest.mark.gpu
 
@@ -39,4 +39,16 @@ def test_small_queries_over_small_keys(kv, T):
     c = Case([70, 0], [T, T - 1], T, 8, 2, 64, kv, seed=T)
     c.k *= 1e-20
     c.q *= 1e-25
+    c.check(c.call())
+
+
+def test_query_offsets_beyond_32_bits():
+    """Query rows so far apart that the last one starts beyond 2^31 elements."""
+    T, H, HK, hd = 256, 8, 8, 64
+    c = Case([40], [T], T, H, HK, hd, native.TF_KV_F32, seed=7)
+    ld = (1 << 23) + (1 << 16)
+    assert (T - 1) * ld > 2 ** 31
+    q = torch.empty((1, T, ld), device="cuda")
+    q[..., :H * hd] = c.q[..., :H * hd]
+    c.q, c.ld_q = q, ld
     c.check(c.call())
