@@ -12,9 +12,13 @@
 // Arithmetic (fp32-equivalent on the f16 tensor pipe): an operand is split into two f16 halves
 // after a power-of-two scale (q: per row; fp32 K and V: per tile; p: fixed), 22 bits or more of
 // it; the product of the two low halves (2^-22 relative) is dropped.  An f16 cache is its own
-// exact half; a bf16 row fits one half after the scale (8 bits, and 2^-39 of the tile's maximum
-// where f16 runs out of exponents).  Every tile's P V product starts from zero and joins the
-// running output by an fp32 fma, so its rounding does not grow with the context.
+// exact half; a bf16 row fits one half after the scale (8 bits; f16 runs out of exponents 2^-24
+// below 1).  Every tile's P V product starts from zero and joins the running output by an fp32
+// fma, so its rounding does not grow with the context.
+// One scale serves a tile whose rows' maxima lie within 2^12 of each other.  Beyond that the small
+// rows would lose their bits to a large one, which need not have a reader in common with them: a
+// segment with such a tile is computed once more from the cache, in fp32 and row by row
+// (tree_exact_rows).  A probability below 2^-39 of its row's largest counts as zero.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -251,16 +255,20 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // 2^e for -126 <= e <= 127
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 // Whether a tile whose largest |x| is maxbits may be split after the scale 2^-e: its maximum within
-// [2^-4, 2^15), so that nothing overflows and the low halves keep 21 bits below it; and an exponent
-// that puts it in the middle.
+// [2^8, 2^15), so that nothing overflows and the low halves keep 20 bits of every row whose own
+// maximum is at most 2^TILE_SPREAD below it; and an exponent that puts it in the middle.
+constexpr int TILE_SPREAD = 12;
+constexpr int TILE_FIRST = -9;  // the exponent before the first tile
 __device__ __forceinline__ bool tile_fits(uint32_t maxbits, int e) {
     const int x = (int)(maxbits >> 23) - 127 - e;
-    return maxbits == 0 || (x >= -4 && x < 15);
+    return maxbits == 0 || (x < 15 && (x >= 8 || e == -126));
 }
 __device__ __forceinline__ int tile_exponent(uint32_t maxbits) {
-    const int e = (int)(maxbits >> 23) - 127 - 6;
+    const int e = (int)(maxbits >> 23) - 127 - 11;
     return e < -126 ? -126 : (e > 126 ? 126 : e);
 }
+// Whether a vector whose largest |x| is `bits` leaves open that its row keeps fewer bits.
+__device__ __forceinline__ bool may_be_low(uint32_t bits, int e) { return (int)(bits >> 23) - 127 < e + 8 - TILE_SPREAD; }
 // exponent e such that |x| 2^-e lies in [2^14, 2^15) for the largest finite |x| (its bits
 // without sign), kept where 2^e and 2^-e are normal numbers
 __device__ __forceinline__ int half_exponent(uint32_t maxbits) {
@@ -335,7 +343,6 @@ __device__ __forceinline__ uint32_t abs_bits(const uint4& x) {
     const uint32_t v = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
     return max(v << 16, v & 0xFFFF0000u);
 }
-// largest |x| of eight values (NaN aside), as fp32 bits
 // running maximum of |x| over vectors, cheaper: fp32 as a float, bf16 as two packed values whose
 // signs are not meaningful; NaN aside
 template <int KVT>
@@ -351,6 +358,7 @@ template <int KVT>
 __device__ __forceinline__ uint32_t abs_max_bits(uint32_t m) {
     return KVT == KV_F32 ? m : max((m << 16) & 0x7FFF0000u, m & 0x7FFF0000u);
 }
+// largest |x| of eight values (NaN aside), as fp32 bits
 __device__ __forceinline__ uint32_t max8(const float4& x, const float4& y) {
     return __float_as_uint(fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))),
                                  fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
@@ -380,6 +388,100 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// four consecutive elements of the cache
+template <int KVT>
+__device__ __forceinline__ float4 kv_load4(const void* p, long long i) {
+    if (KVT == KV_F32) return *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i);
+    return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+}
+// Whether a tile of the segment has rows whose maxima lie further apart than its scale allows (rows of
+// zeros aside): a warp's share of the tiles, a lane per row.
+template <int KVT, int PT>
+__device__ __forceinline__ bool tree_rows_apart(const TreeAttnArgs& a, const TreeSeg& sg, int warp, int warps) {
+    const int hd = a.hd, end = sg.s.n_ctx + sg.s.n_node, lane = threadIdx.x & 31;
+    const long long base = (long long)sg.s.slot * a.slot_stride + (long long)sg.kvh * a.cap * hd;
+    bool apart = false;
+#pragma unroll 1
+    for (int i = 2 * sg.t0 + warp; i < 2 * sg.t1; i += warps) {  // tile, K / V
+        const void* c = i & 1 ? a.vc : a.kc;
+        uint32_t hi = 0, lo = 0xFFFFFFFFu;
+#pragma unroll 1
+        for (int p = (i >> 1) * PT + lane; p < min(((i >> 1) + 1) * PT, end); p += 32) {
+            uint32_t m = 0;
+#pragma unroll 1
+            for (int d = 0; d < hd; d += 4) {
+                const float4 x = kv_load4<KVT>(c, base + (long long)p * hd + d);
+                m = max(m, max(max(finite_abs_bits(x.x), finite_abs_bits(x.y)), max(finite_abs_bits(x.z), finite_abs_bits(x.w))));
+            }
+            hi = max(hi, m);
+            if (m) lo = min(lo, m);
+        }
+        hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+        lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+        apart |= hi && (int)(hi >> 23) - (int)(lo >> 23) > TILE_SPREAD;
+    }
+    return apart;
+}
+// A segment's rows in fp32, over what has been written of them (after a barrier): for tiles whose rows
+// lie too far apart for one scale.  A warp per row; 32 positions at a time, a lane per position for the
+// scores and per dim (d, d + 32, ...) for the sums.  (fp32 and bf16 caches.)  Such a segment takes some
+// ten times as long as another.
+template <int KVT, int PT>
+__device__ __forceinline__ void tree_exact_rows(const TreeAttnArgs& a, const TreeSeg& sg, int rt, int rep, const uint32_t* vis, float* part,
+                                                bool whole, int warp, int warps) {
+    const int hd = a.hd, rows = sg.s.n_node * rep, lane = threadIdx.x & 31;
+    const int p1 = min(sg.t1 * PT, sg.s.n_ctx + sg.s.n_node);
+    const long long base = (long long)sg.s.slot * a.slot_stride + (long long)sg.kvh * a.cap * hd;
+    const float scale = kLog2e / sqrtf((float)hd);
+#pragma unroll 1
+    for (int r = warp; r < rt; r += warps) {
+        const int rr = sg.rtile * rt + r, node = rr / rep;
+        if (rr >= rows) return;
+        const int head = sg.kvh * rep + rr - node * rep;
+        const float* q = a.q + ((size_t)sg.b * a.T + node) * a.ld_q + (size_t)head * hd;
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+        for (int p0 = sg.t0 * PT; p0 < p1; p0 += 32) {
+            const int p = p0 + lane;
+            const bool seen = p < p1 && (vis_window(vis + r * VIS_WORDS, p0 - sg.s.n_ctx) >> lane & 1);
+            float s = -INFINITY;
+            if (seen) {
+                s = 0.f;
+#pragma unroll 2
+                for (int d = 0; d < hd; d += 4) {
+                    const float4 x = *reinterpret_cast<const float4*>(q + d), k = kv_load4<KVT>(a.kc, base + (long long)p * hd + d);
+                    s = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s))));
+                }
+                s *= scale;
+            }
+            const float mx = fmaxf(m, warp_max(s)), ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(m - ref);
+            const float w = seen ? exp2_fast(s - ref + kPShift) : 0.f;
+            m = mx;
+            l = fmaf(l, alpha, warp_sum(w));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] *= alpha;
+#pragma unroll 1
+            for (unsigned bits = __ballot_sync(0xFFFFFFFFu, seen); bits; bits &= bits - 1) {
+                const int j = __ffs(bits) - 1;
+                const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (lane + 32 * i < hd) o[i] = fmaf(wj, kv_load(a.vc, base + (long long)(p0 + j) * hd + lane + 32 * i, KVT), o[i]);
+            }
+        }
+        const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        float* dst = whole ? a.out + ((size_t)sg.b * a.T + node) * a.ld_out + (size_t)head * hd : part + (size_t)r * hd;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (lane + 32 * i < hd) dst[lane + 32 * i] = o[i] * inv;
+        if (!whole && lane == 0) {
+            part[(size_t)rt * hd + r] = m;
+            part[(size_t)rt * hd + rt + r] = l;
+        }
+    }
 }
 
 // ---- narrow trees: mma.sync, up to 64 rows per row tile ----------------------------------------------
@@ -426,6 +528,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
     __shared__ float qscale[RT];
     __shared__ uint32_t vis[RT][VIS_WORDS];
     __shared__ unsigned tmax[4];                      // maxima of K, V (bits) of this tile and the next
+    __shared__ int low;                               // the segment may have a tile whose rows one scale does not hold
     __shared__ unsigned badrow[TREE_MAX_NODES / 32];  // drafted rows of the unit with non-finite values
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rep = pl.rep, hd = a.hd;
@@ -445,7 +548,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
     if (tid == 0) desc[blockIdx.x].b = -1;
 
     TreeSeg sg;
-    int ek = 0, ev = 0;  // scale exponents of K and V, kept from tile to tile
+    int ek = KVT == KV_F16 ? 0 : TILE_FIRST, ev = ek;  // scale exponents of K and V, kept from tile to tile
     while (tree_next<PT, RT, TN_UNIT_COST>(a, rep, it, sg)) {
         const TreeSeq s = sg.s;
         const int b = sg.b, kvh = sg.kvh, rtile = sg.rtile, t0 = sg.t0, t1 = sg.t1;
@@ -513,6 +616,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
         }
         if (tid < TREE_MAX_NODES / 32) badrow[tid] = 0;
         if (tid < 4) tmax[tid] = 0;
+        if (tid == 0) low = 0;
         __syncthreads();
 
         float O[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
@@ -541,14 +645,14 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
             }
             if (KVT != KV_F16) {
                 if (t > t0) __syncthreads();  // the last tile's operands are free
-                // split by the last tile's scale; when the maximum turns out not to fit it
-                // (seldom), once more after its own
+                // split by the last tile's scale; when the values turn out not to fit it
+                // (seldom), once more after their own
                 for (;;) {
 #pragma unroll 1
                     for (int which = 0; which < 2; ++which) {
                         const float f = pow2i(which ? -ev : -ek);
                         const uint32_t dst = which ? vh : kh;
-                        uint32_t mb = 0;
+                        uint32_t mb = 0, mn = 0xFFFFFFFFu;
                         uint4 xs[NV];  // (all loads before the first store: the compiler keeps their order)
 #pragma unroll
                         for (int i = 0; i < NV; ++i) xs[i] = ld_shared16(mine + i * OSTEP + which * HALF_TILE);
@@ -556,7 +660,9 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
                         for (int i = 0; i < NV; ++i) {
                             const int r = r0 + i * RSTEP;
                             const uint4 x = xs[i];
-                            mb = max(mb, abs_bits<KVT>(x));
+                            const uint32_t top = abs_bits<KVT>(x);
+                            mb = max(mb, top);
+                            mn = __viaddmin_u32(top, 0xFFFFFFFFu, mn);
                             if (KVT == KV_F32) {
                                 uint32_t h0, l0, h1, l1;
                                 split2t(__fmul2_rn(make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), make_float2(f, f)), h0, l0);
@@ -579,6 +685,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
                         }
                         mb = __reduce_max_sync(0xFFFFFFFFu, mb);
                         if (lane == 0) atomicMax(&tmax[2 * (t & 1) + which], mb);
+                        if (may_be_low(mn, which ? ev : ek)) low = 1;
                     }
                     __syncthreads();
                     const uint32_t mk = tmax[2 * (t & 1)], mv = tmax[2 * (t & 1) + 1];
@@ -699,6 +806,7 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
         }
         // the position groups' results meet in shared memory: per row m, l, O
         __syncthreads();
+        bool exact = KVT != KV_F16 && low;
         float* fin = reinterpret_cast<float*>(smem);  // [NG][RT][HD + 4]
         if (active) {
 #pragma unroll
@@ -757,7 +865,11 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
         if (!whole && t0 == 0 && tid == 0)
             desc[blockIdx.x] = TreeDesc{b, kvh, rtile | min(RT, rows - rtile * RT) << 16, sg.last_cta};
         __syncthreads();
-        if (anybad) {
+        if (KVT != KV_F16 && exact) exact = __syncthreads_or(tree_rows_apart<KVT, PT>(a, sg, warp, TN_THREADS / 32));
+        if (KVT != KV_F16 && exact) {
+            tree_exact_rows<KVT, PT>(a, sg, RT, rep, &vis[0][0], part, whole, warp, TN_THREADS / 32);
+            __syncthreads();
+        } else if (anybad) {
             tree_fix_rows<KVT>(a, sg, RT, rep, badrow, &vis[0][0], part, whole, tid, TN_THREADS);
             __syncthreads();
         }
@@ -902,6 +1014,8 @@ struct WideShared {
     uint32_t tmem;
     int abort;
     unsigned tmax[4];
+    int low[8];                                   // by segment: as in the narrow kernel
+    int apart;                                    // what is found then
     int ek[8], ev[8];                             // scale exponents of the last eight tiles
     unsigned badrow[8][TREE_MAX_NODES / 32];      // drafted rows with non-finite values, by segment
     float qscale[TW_RT];
@@ -1010,11 +1124,13 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         int n = 0, nr = 0, nd = 0, seg = 0;  // running tile, raw buffer, direct tile, segment
         constexpr int VPR = HD * ESZ / 16, RSTEP = LT / VPR;  // 16-byte vectors per row, rows per step of all loaders
         constexpr int UNR = 6;               // vectors in flight per thread
-        int ek = 0, ev = 0;                  // scale exponents of K and V, kept from tile to tile
+        int ek = TILE_FIRST, ev = TILE_FIRST;  // scale exponents of K and V, kept from tile to tile
         const int r0 = lt / VPR, c0 = lt % VPR;
         // where this thread's vectors of a whole tile go: row r0 + k * RSTEP at rel[k % NB] + k * RSTEP * 128
         // (the swizzle depends on the row modulo 8)
         constexpr int NVT = (PT + RSTEP - 1) / RSTEP, NB = RSTEP % 8 == 0 ? 1 : (RSTEP % 4 == 0 ? 2 : 4);
+        // the vector of row lt that this thread looks at (fp32: from the thread's first one on)
+        const int look_c = lt % (hd * ESZ / 16), look = lt * hd * 4 + look_c * 16 - (r0 * hd * 4 + c0 * 16);
         uint32_t rel[NB];
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
@@ -1025,6 +1141,7 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
         while (tree_next<PT, TW_RT, TW_UNIT_COST>(a, rep, it, sg)) {
             const TreeSeq s = sg.s;
             if (lt < TREE_MAX_NODES / 32) sh.badrow[seg & 7][lt] = 0;  // read by others long ago
+            if (lt == 0) sh.low[seg & 7] = 0;
             named_bar<2, LT>();
 #pragma unroll 1
             for (int t = sg.t0; t < sg.t1; ++t, ++n) {
@@ -1086,9 +1203,9 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                         }
                     }
                     if (KVT != KV_F16) {
-                        // split by the last tile's scale; when the maximum turns out not to fit it
-                        // (seldom), once more after its own.  bf16 tiles are converted in place, so
-                        // their maximum is found first.
+                        // split by the last tile's scale; when the values turn out not to fit it
+                        // (seldom), once more after their own.  bf16 tiles are converted in place, so
+                        // their range is found first.
                         unsigned* tm = &sh.tmax[2 * (n & 1) + which];
                         // a whole tile's vectors lie at compile-time distances; this thread's last one
                         // may not exist
@@ -1113,10 +1230,14 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
                             }
                             st_shared16(o, w);
                         };
+                        if (KVT == KV_F32 ? tail : !dir) named_bar<2, LT>();  // (the others' stores, for the look at a row)
                         for (;;) {
                             const int e = which ? ev : ek;
                             const float2 f = make_float2(pow2i(-e), pow2i(-e));
                             uint32_t mb = 0;
+                            // one vector of a row, a row per thread, tells most tiles whose rows share a scale
+                            if (lt < rows && may_be_low(abs_bits<KVT>(ld_shared16(KVT == KV_F32 ? src + look : dst + wide_off(PT, lt, look_c))), e))
+                                sh.low[seg & 7] = 1;
                             if (whole_tile) {
 #pragma unroll
                                 for (int k0 = 0; k0 < NVT; k0 += UNR) {  // (all loads before the first store: the compiler keeps their order)
@@ -1482,7 +1603,18 @@ __global__ void __launch_bounds__(TW_THREADS, 1)
             if (!whole && sg.t0 == 0 && tid == 0)
                 desc[blockIdx.x] =
                     TreeDesc{sg.b, sg.kvh, sg.rtile | min(TW_RT, sg.s.n_node * rep - sg.rtile * TW_RT) << 16, sg.last_cta};
-            if (badrow_any(sh.badrow[seg & 7])) {
+            bool exact = KVT != KV_F16 && sh.low[seg & 7];
+            if (KVT != KV_F16 && exact) {
+                if (tid == 0) sh.apart = 0;
+                named_bar<1, 256>();
+                if (tree_rows_apart<KVT, PT>(a, sg, warp, 8)) sh.apart = 1;
+                named_bar<1, 256>();
+                exact = sh.apart;
+            }
+            if (KVT != KV_F16 && exact) {
+                if (!*abort_flag) tree_exact_rows<KVT, PT>(a, sg, TW_RT, rep, &sh.vis[0][0], part, whole, warp, 8);
+                named_bar<1, 256>();
+            } else if (badrow_any(sh.badrow[seg & 7])) {
                 if (!*abort_flag)
                     tree_fix_rows<KVT>(a, sg, TW_RT, rep, sh.badrow[seg & 7], &sh.vis[0][0], part, whole, tid, 256);
                 named_bar<1, 256>();  // (its reads of vis end before the next segment's)
