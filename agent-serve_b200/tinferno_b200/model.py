@@ -178,6 +178,7 @@ class Model:
         self.weight_bytes = int(self.L.tf_cuda_weight_bytes(self.h))
         self.kernels_per_step = int(self.L.tf_cuda_kernels_per_step(self.h))
         self.arch = self.gguf.str("general.architecture", "llama")
+        self._tree = np.zeros(0, np.int32)  # tokens of the last tree step
 
     def describe(self) -> str:
         return describe(self.arch, self.hp, self.weight_bytes, self.cfg)
@@ -297,7 +298,7 @@ class Model:
         from, 0 for drafts without a distribution; u: one uniform number per node).  Returns
         (accepted tokens, next token); the accepted path stays in the cache, next is the next root."""
         n = len(self._tree)
-        nodes, k, nxt = np.zeros(n, np.int32), C.c_int(0), C.c_int(0)
+        nodes, k, nxt = np.zeros(max(1, n), np.int32), C.c_int(0), C.c_int(0)
         uu = np.zeros(n, np.float32) if u is None else np.ascontiguousarray(u, dtype=np.float32)
         if len(uu) < n:
             raise ValueError("u needs one number per node")

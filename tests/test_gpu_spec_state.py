@@ -143,3 +143,10 @@ def test_a_refused_acceptance_leaves_the_tree(path):
     kept, nxt = m.tree_accept(seq=0)
     assert nxt == am[len(kept)] and m.n_pos(seq=0) == len(prompts()[0]) + 1 + len(kept)
     m.close()
+
+
+def test_accept_without_a_step(path):
+    m, _ = started(path)
+    with pytest.raises(native.TFError, match="no tree step"):
+        m.tree_accept()
+    m.close()
