@@ -295,15 +295,16 @@ class Model:
     def tree_accept(self, temperature: float = 0.0, u: Optional[Sequence[float]] = None, draft_ptr: int = 0, seq: int = 0):
         """Verifies the last tree_step's tree against the model's distribution at `temperature`
         (draft_ptr: device address of the [nodes][n_vocab] logits that each node's children were drawn
-        from, 0 for drafts without a distribution; u: one uniform number per node).  Returns
-        (accepted tokens, next token); the accepted path stays in the cache, next is the next root."""
+        from, 0 for drafts without a distribution; u: one uniform number per node, needed at a positive
+        temperature).  Returns (accepted tokens, next token); the accepted path stays in the cache, next
+        is the next root."""
         n = len(self._tree)
         nodes, k, nxt = np.zeros(max(1, n), np.int32), C.c_int(0), C.c_int(0)
-        uu = np.zeros(n, np.float32) if u is None else np.ascontiguousarray(u, dtype=np.float32)
-        if len(uu) < n:
+        uu = None if u is None else np.ascontiguousarray(u, dtype=np.float32)
+        if uu is not None and len(uu) < n:
             raise ValueError("u needs one number per node")
         native.check(self.L.tf_cuda_tree_accept(self.h, seq, C.c_void_p(draft_ptr) if draft_ptr else None, float(temperature),
-                                                uu.ctypes.data_as(native.f32p), nodes.ctypes.data_as(native.i32p),
+                                                None if uu is None else uu.ctypes.data_as(native.f32p), nodes.ctypes.data_as(native.i32p),
                                                 C.byref(k), C.byref(nxt)), self.h)
         return [int(self._tree[i]) for i in nodes[1:k.value]], nxt.value
 

@@ -150,3 +150,15 @@ def test_accept_without_a_step(path):
     with pytest.raises(native.TFError, match="no tree step"):
         m.tree_accept()
     m.close()
+
+
+def test_accept_without_random_numbers(path):
+    """Numbers of zero in their place would keep every draft."""
+    m, t = started(path)
+    m.tree_step([t[0], 11], [-1, 0])
+    with pytest.raises(native.TFError, match="u must not be null"):
+        m.tree_accept(0.8)
+    with pytest.raises(ValueError):
+        m.tree_accept(0.8, [0.5])
+    m.tree_accept(0.8, [0.5, 0.5])
+    m.close()
