@@ -289,7 +289,7 @@ class Model:
         native.check(self.L.tf_cuda_tree_step(self.h, seq, t.ctypes.data_as(native.i32p), p.ctypes.data_as(native.i32p),
                                               len(t), lg.ctypes.data_as(native.f32p) if want_logits else None,
                                               am.ctypes.data_as(native.i32p)), self.h)
-        self._tree = t
+        self._tree = t.copy()  # (t may be the caller's array)
         return (am, lg) if want_logits else am
 
     def tree_accept(self, temperature: float = 0.0, u: Optional[Sequence[float]] = None, draft_ptr: int = 0, seq: int = 0):

@@ -162,3 +162,15 @@ def test_accept_without_random_numbers(path):
         m.tree_accept(0.8, [0.5])
     m.tree_accept(0.8, [0.5, 0.5])
     m.close()
+
+
+def test_accepted_tokens_are_the_stepped_ones(path):
+    """The caller may reuse its array between the step and the acceptance."""
+    m, t = started(path)
+    want = m.generate_greedy(t[0], 4)
+    m.rewind(len(prompts()[0]))
+    tokens = np.array(want[:3], np.int32)
+    m.tree_step(tokens, [-1, 0, 1])
+    tokens[:] = 0
+    assert m.tree_accept() == (want[1:3], want[3])
+    m.close()
