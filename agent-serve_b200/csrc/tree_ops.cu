@@ -168,7 +168,12 @@ int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_layer, long
         return set_error("bad cache strides");
     if (B == 0) return 0;
     if (!k_cache || !v_cache || !n_ctx || !path || !n_path) return set_error("null pointer");
-    if (n_new == n_ctx) return set_error("n_new must not be n_ctx (every block of the launch reads n_ctx)");
+    auto in_n_new = [&](const int* p, long long n) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(n_new), y = reinterpret_cast<uintptr_t>(p);
+        return n_new && p && x < y + sizeof(int) * n && y < x + sizeof(int) * B;
+    };
+    if (in_n_new(n_ctx, B) || in_n_new(n_path, B) || in_n_new(slots, B) || in_n_new(path, (long long)B * ld_path))
+        return set_error("n_new must not overlap n_ctx, n_path, slots or path (every block of the launch reads them)");
     if (!aligned(k_cache, 16) || !aligned(v_cache, 16)) return set_error("the caches must be 16-byte aligned");
     KvCommitArgs a = {};
     if (op_err_word(&a.err)) return -1;

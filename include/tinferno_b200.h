@@ -335,9 +335,9 @@ TF_API int tf_op_verify_tree(int* path, int* n_path, int* next, const float* log
 
 /* Commit: cache row n_ctx[b] + path[b][i] becomes row n_ctx[b] + i for i < n_path[b], in place,
  * K and V of n_layer layers (layer_stride elements apart) and every kv head; n_new[b]
- * (optional, not n_ctx itself) = n_ctx[b] + n_path[b].  path[b] (ld_path ints apart) strictly
- * increasing, slots distinct; a path that is not moves nothing and records
- * TF_DEV_ERR_POS. */
+ * (optional, in memory of its own: every block of the launch reads the other arrays) = n_ctx[b]
+ * + n_path[b].  path[b] (ld_path ints apart) strictly increasing, slots distinct; a path that is
+ * not moves nothing and records TF_DEV_ERR_POS. */
 TF_API int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_layer, long long layer_stride,
                            long long slot_stride, int cap, int n_slots, const int* slots, const int* n_ctx,
                            const int* path, int ld_path, const int* n_path, int* n_new, int B, int n_kv_heads,
