@@ -146,3 +146,22 @@ def test_large_rows_in_a_batch_leave_the_others(T):
     sees_inf = torch.from_numpy(c.bits[2][:, 3]).cuda()
     assert not got[2][sees_inf].isfinite().any()
     assert torch.equal(got, c.call())
+
+
+@pytest.mark.parametrize("T", [4, 64])
+@pytest.mark.parametrize("kv", TYPES)
+def test_a_row_does_not_depend_on_its_batch_beyond_rounding(kv, T):
+    """A sequence alone, with others, and with others in another order: the split over CTAs differs, the
+    values by the rounding of either (twice the bound of one)."""
+    lens = [900, 33, 2000, 1]
+    c = Case(lens, [T] * 4, T, 8, 2, 64, kv, seed=13)
+    full = c.call().clone()
+    q, mask, slots, bits = c.q, c.mask, c.slots, c.bits
+    for order in ([0], [1], [2], [3], [2, 0], [3, 2, 1, 0]):
+        c.B, c.lens, c.nodes, c.slots = len(order), [lens[b] for b in order], [T] * len(order), [slots[b] for b in order]
+        c.q, c.mask, c.out = q[order].contiguous(), mask[order].contiguous(), torch.full((len(order), T, c.ld_out), 7.0, device="cuda")
+        c.bits = [bits[b] for b in order]
+        got = c.call()
+        for i, b in enumerate(order):
+            assert (got[i] - full[b]).norm() <= 1e-5 * full[b].norm()
+            assert ((got[i] - full[b]).abs() <= 2 * c.want(i)[1]).all()
