@@ -398,9 +398,11 @@ __device__ __forceinline__ float4 kv_load4(const void* p, long long i) {
     return make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u), __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
 }
 // Whether a tile of the segment has rows whose maxima lie further apart than its scale allows (rows of
-// zeros aside): a warp's share of the tiles, a lane per row.
+// zeros aside): a warp's share of the tiles, a lane per row.  (The look at one vector of a row finds
+// channels of small values too: with 16 of 64 at 10^-9 a call of 1 tree of 64, 16000 positions takes
+// 91 us instead of 58.)
 template <int KVT, int PT>
-__device__ __forceinline__ bool tree_rows_apart(const TreeAttnArgs& a, const TreeSeg& sg, int warp, int warps) {
+__device__ __noinline__ bool tree_rows_apart(const TreeAttnArgs& a, const TreeSeg sg, int warp, int warps) {
     const int hd = a.hd, end = sg.s.n_ctx + sg.s.n_node, lane = threadIdx.x & 31;
     const long long base = (long long)sg.s.slot * a.slot_stride + (long long)sg.kvh * a.cap * hd;
     bool apart = false;
@@ -411,7 +413,7 @@ __device__ __forceinline__ bool tree_rows_apart(const TreeAttnArgs& a, const Tre
 #pragma unroll 1
         for (int p = (i >> 1) * PT + lane; p < min(((i >> 1) + 1) * PT, end); p += 32) {
             uint32_t m = 0;
-#pragma unroll 1
+#pragma unroll 4
             for (int d = 0; d < hd; d += 4) {
                 const float4 x = kv_load4<KVT>(c, base + (long long)p * hd + d);
                 m = max(m, max(max(finite_abs_bits(x.x), finite_abs_bits(x.y)), max(finite_abs_bits(x.z), finite_abs_bits(x.w))));
@@ -426,60 +428,87 @@ __device__ __forceinline__ bool tree_rows_apart(const TreeAttnArgs& a, const Tre
     return apart;
 }
 // A segment's rows in fp32, over what has been written of them (after a barrier): for tiles whose rows
-// lie too far apart for one scale.  A warp per row; 32 positions at a time, a lane per position for the
-// scores and per dim (d, d + 32, ...) for the sums.  (fp32 and bf16 caches.)  Such a segment takes some
-// ten times as long as another.
+// lie too far apart for one scale.  Four rows per warp, which share the cache's loads; 32 positions
+// at a time, a lane per position for the scores and per dim (d, d + 32, ...) for the sums.  (fp32
+// and bf16 caches.)  Bound by the latency of its loads; calls without / with one row 10^6 times the
+// others: 1 tree of 8, 8000 positions, 32x8x64 f32 30 / 119 us; 32 trees of 8, 1144 positions,
+// 12x2x128 f32 54 / 500 us; 1 tree of 64, 16000 positions, 32x8x64 f32 58 / 2150 us; 12 trees of 31,
+// 4001 positions, 32x8x128 bf16 122 / 7000 us.  A function of its own, so that the kernels' loops keep
+// their registers.
 template <int KVT, int PT>
-__device__ __forceinline__ void tree_exact_rows(const TreeAttnArgs& a, const TreeSeg& sg, int rt, int rep, const uint32_t* vis, float* part,
+__device__ __noinline__ void tree_exact_rows(const TreeAttnArgs& a, const TreeSeg sg, int rt, int rep, const uint32_t* vis, float* part,
                                                 bool whole, int warp, int warps) {
-    const int hd = a.hd, rows = sg.s.n_node * rep, lane = threadIdx.x & 31;
+    constexpr int R = 4;
+    const int hd = a.hd, rows = min(rt, sg.s.n_node * rep - sg.rtile * rt), lane = threadIdx.x & 31;
     const int p1 = min(sg.t1 * PT, sg.s.n_ctx + sg.s.n_node);
     const long long base = (long long)sg.s.slot * a.slot_stride + (long long)sg.kvh * a.cap * hd;
     const float scale = kLog2e / sqrtf((float)hd);
 #pragma unroll 1
-    for (int r = warp; r < rt; r += warps) {
-        const int rr = sg.rtile * rt + r, node = rr / rep;
-        if (rr >= rows) return;
-        const int head = sg.kvh * rep + rr - node * rep;
-        const float* q = a.q + ((size_t)sg.b * a.T + node) * a.ld_q + (size_t)head * hd;
-        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r0 = warp * R; r0 < rows; r0 += warps * R) {
+        const float* q[R];
+        float m[R], l[R], o[R][4];
+#pragma unroll
+        for (int i = 0; i < R; ++i) {  // (the last row stands in for rows behind it)
+            const int rr = sg.rtile * rt + min(r0 + i, rows - 1), node = rr / rep;
+            q[i] = a.q + ((size_t)sg.b * a.T + node) * a.ld_q + (size_t)(sg.kvh * rep + rr - node * rep) * hd;
+            m[i] = -INFINITY;
+            l[i] = o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+        }
 #pragma unroll 1
         for (int p0 = sg.t0 * PT; p0 < p1; p0 += 32) {
-            const int p = p0 + lane;
-            const bool seen = p < p1 && (vis_window(vis + r * VIS_WORDS, p0 - sg.s.n_ctx) >> lane & 1);
-            float s = -INFINITY;
-            if (seen) {
-                s = 0.f;
-#pragma unroll 2
-                for (int d = 0; d < hd; d += 4) {
-                    const float4 x = *reinterpret_cast<const float4*>(q + d), k = kv_load4<KVT>(a.kc, base + (long long)p * hd + d);
-                    s = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s))));
+            const int p = min(p0 + lane, p1 - 1);
+            float s[R] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+            for (int d = 0; d < hd; d += 4) {
+                const float4 k = kv_load4<KVT>(a.kc, base + (long long)p * hd + d);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float4 x = *reinterpret_cast<const float4*>(q[i] + d);
+                    s[i] = fmaf(x.x, k.x, fmaf(x.y, k.y, fmaf(x.z, k.z, fmaf(x.w, k.w, s[i]))));
                 }
-                s *= scale;
             }
-            const float mx = fmaxf(m, warp_max(s)), ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(m - ref);
-            const float w = seen ? exp2_fast(s - ref + kPShift) : 0.f;
-            m = mx;
-            l = fmaf(l, alpha, warp_sum(w));
+            unsigned seen[R];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] *= alpha;
-#pragma unroll 1
-            for (unsigned bits = __ballot_sync(0xFFFFFFFFu, seen); bits; bits &= bits - 1) {
-                const int j = __ffs(bits) - 1;
-                const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
+            for (int i = 0; i < R; ++i) {
+                const uint32_t bits = vis_window(vis + min(r0 + i, rows - 1) * VIS_WORDS, p0 - sg.s.n_ctx);
+                seen[i] = p1 - p0 < 32 ? bits & ((1u << (p1 - p0)) - 1) : bits;
+                const bool mine = seen[i] >> lane & 1;
+                const float x = mine ? s[i] * scale : -INFINITY;
+                const float mx = fmaxf(m[i], warp_max(x)), ref = mx == -INFINITY ? 0.f : mx, alpha = exp2_fast(m[i] - ref);
+                s[i] = mine ? exp2_fast(x - ref + kPShift) : 0.f;  // the weight from here on
+                m[i] = mx;
+                l[i] = fmaf(l[i], alpha, warp_sum(s[i]));
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (lane + 32 * i < hd) o[i] = fmaf(wj, kv_load(a.vc, base + (long long)(p0 + j) * hd + lane + 32 * i, KVT), o[i]);
+                for (int e = 0; e < 4; ++e) o[i][e] *= alpha;
+            }
+#pragma unroll 4
+            for (int j = 0; j < 32; ++j) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    v[e] = lane + 32 * e < hd ? kv_load(a.vc, base + (long long)min(p0 + j, p1 - 1) * hd + lane + 32 * e, KVT) : 0.f;
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float w = __shfl_sync(0xFFFFFFFFu, s[i], j);
+                    if (seen[i] >> j & 1)  // (what is not seen may not be finite)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[i][e] = fmaf(w, v[e], o[i][e]);
+                }
             }
         }
-        const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
-        float* dst = whole ? a.out + ((size_t)sg.b * a.T + node) * a.ld_out + (size_t)head * hd : part + (size_t)r * hd;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < hd) dst[lane + 32 * i] = o[i] * inv;
-        if (!whole && lane == 0) {
-            part[(size_t)rt * hd + r] = m;
-            part[(size_t)rt * hd + rt + r] = l;
+        for (int i = 0; i < R; ++i) {
+            const int r = r0 + i, rr = sg.rtile * rt + r, node = rr / rep;
+            if (r >= rows) continue;
+            const float inv = !whole ? 1.f : (l[i] == 0.f ? 0.f : 1.f / l[i]);
+            float* dst = whole ? a.out + ((size_t)sg.b * a.T + node) * a.ld_out + (size_t)(sg.kvh * rep + rr - node * rep) * hd : part + (size_t)r * hd;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (lane + 32 * e < hd) dst[lane + 32 * e] = o[i][e] * inv;
+            if (!whole && lane == 0) {
+                part[(size_t)rt * hd + r] = m[i];
+                part[(size_t)rt * hd + rt + r] = l[i];
+            }
         }
     }
 }
