@@ -332,13 +332,13 @@ __device__ __forceinline__ uint32_t max_bits(const uint4& x) {
     }
     return m;
 }
-// |x| of a vector's largest value, as fp32 bits (fp32 or bf16; 0x7F800000 and more: not all finite)
+// |x| of a vector's largest value, as fp32 bits (fp32 or bf16; 0x7F800000 and more: not all finite;
+// fp32: NaN aside where there is another value)
 template <int KVT>
 __device__ __forceinline__ uint32_t abs_bits(const uint4& x) {
-    if (KVT == KV_F32) {
-        const uint32_t m = 0x7FFFFFFFu;
-        return max(max(x.x & m, x.y & m), max(x.z & m, x.w & m));
-    }
+    if (KVT == KV_F32)
+        return __float_as_uint(fmaxf(fmaxf(fabsf(__uint_as_float(x.x)), fabsf(__uint_as_float(x.y))),
+                                     fmaxf(fabsf(__uint_as_float(x.z)), fabsf(__uint_as_float(x.w)))));
     const uint32_t m = 0x7FFF7FFFu;
     const uint32_t v = __vmaxu2(__vmaxu2(x.x & m, x.y & m), __vmaxu2(x.z & m, x.w & m));
     return max(v << 16, v & 0xFFFF0000u);
