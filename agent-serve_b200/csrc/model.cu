@@ -1684,7 +1684,7 @@ int tree_init(tf_model* m) {
     if (m->h_tree) return 0;
     const size_t R = (size_t)m->tree_rows;
     auto round = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    m->tws_attn = round(tree_attn_ws_bytes(1, m->tree_rows, m->hp.n_head, m->hp.n_kv_head, m->hd));
+    m->tws_attn = round(tree_attn_ws_bytes(m->tree_rows, m->hp.n_head, m->hp.n_kv_head, m->hd));
     m->tws_verify = round(tree_verify_ws_bytes(1, m->tree_rows, m->V));
     if (!m->d_ttok) CK(cudaMalloc(&m->d_ttok, sizeof(int) * R));
     if (!m->d_tpar) CK(cudaMalloc(&m->d_tpar, sizeof(int) * R));

@@ -31,7 +31,7 @@ struct TreeAttnArgs {
     void* ws;
     int* err;
 };
-size_t tree_attn_ws_bytes(int B, int T, int n_head, int n_kv, int hd);
+size_t tree_attn_ws_bytes(int T, int n_head, int n_kv, int hd);  // any B
 bool tree_attn_fits(int B, int T, int n_head, int n_kv, int cap);  // tiles are counted in 32 bits
 cudaError_t tree_attn_launch(const TreeAttnArgs& a, cudaStream_t st, bool pdl);
 

@@ -527,9 +527,9 @@ __device__ __noinline__ void tree_exact_rows(const TreeAttnArgs& a, const TreeSe
 // Bound by the latency of a tile's chain (copy, split, scores, softmax, P V: about 6000 cycles per
 // tile and CTA, two CTAs per SM) and, in short calls, by the unit's start (queries behind the
 // lengths, 5000 cycles) and the launches.  Device time, both launches: 1 tree of 1, 96 positions,
-// 32x8x64 f32 8.6 us; 1 tree of 5, 1733 positions, 14x2x64 f32 12.7 us; 1 tree of 8, 8000 positions,
-// 32x8x64 f32 22.9 us (33 MB: 1.4 TB/s); 32 trees of 8, 1144 positions, the same 61.9 us (151 MB: 2.4
-// TB/s).
+// 32x8x64 f32 8.8 us; 1 tree of 5, 1733 positions, 14x2x64 f32 13.3 us; 1 tree of 8, 8000 positions,
+// 32x8x64 f32 23.3 us (33 MB: 1.4 TB/s); 32 ragged trees of 8, 1144 positions, the same 46.0 us (91
+// MB: 2.0 TB/s).  The look at the range of a tile's rows (TILE_SPREAD) is 1 to 4 % of that.
 template <int HD, int MT, int KVT>
 struct NarrowCfg {
     static constexpr int ESZ = KVT == KV_F32 ? 4 : 2;
@@ -932,9 +932,9 @@ __global__ void __launch_bounds__(TN_THREADS, 2)
 // split, 550 for the join); issue slots 53 %, tensor pipe 38 %, DRAM 35 % of their peaks.  fp32 and
 // bf16: by the loaders' split (tensor pipe 16 to 29 %), and for heads of 128 dims by the 22000 cycles
 // of a segment's start and end.  Device time, both launches: 32 trees of 64, 8128 positions, 32x8x64
-// f16 212 us (342 MB of rows read: 1.6 TB/s; 155 GF in two products: 733 TF/s); 12 trees of 31, 4001
-// positions, 32x8x128 bf16 97 us; 1 tree of 64, 16000 positions, 32x8x64 f32 51 us (25 GF in three
-// products: 497 TF/s).  A third score buffer (QK two tiles ahead) and chunks of scores fetched ahead
+// f16 215 us (342 MB of rows read: 1.6 TB/s; 155 GF in two products: 722 TF/s); 12 trees of 31, 4001
+// positions, 32x8x128 bf16 95 us; 1 tree of 64, 16000 positions, 32x8x64 f32 51.4 us (25 GF in three
+// products: 490 TF/s).  The look at the range of a tile's rows is 0 to 2 % of that.  A third score buffer (QK two tiles ahead) and chunks of scores fetched ahead
 // made no difference and were left out.
 constexpr int TW_THREADS = 512;
 constexpr int TW_RT = 128;
@@ -1738,7 +1738,9 @@ static int tree_sms() {
 }
 
 // Rows of a unit's row tile, which chooses the kernel too: TW_RT the wide one, fewer the narrow one.
-// Device time, narrow / wide (f32 unless said; B trees of T nodes, positions, heads x kv heads x dims):
+// Device time, narrow / wide (f32 unless said; B trees of T nodes, positions, heads x kv heads x dims),
+// measured before the look at the rows' range, which costs the narrow kernel 1 to 4 % and the wide
+// one 0 to 2 %:
 //   17 to 32 rows:   1 x 8, 100, 32x8x64: 10.4 / 19.3 us;  32 x 8, 1144, 32x8x64 f16: 34.1 / 42.3;
 //                    the same in f32: 61.9 / 60.7;  1 x 8, 8000: 22.9 / 22.8
 //   33 to 64 rows:   1 x 12, 100, 32x8x64 (0.4 MB of K and V): 12.8 / 19.2;  1 x 5, 1733, 14x2x64
@@ -1765,8 +1767,7 @@ static int tree_row_tile(int rows, bool short_cache) {
 }
 static int tree_grid(int rt) { return rt == TW_RT ? tree_sms() : 2 * tree_sms(); }
 
-size_t tree_attn_ws_bytes(int B, int T, int n_head, int n_kv, int hd) {
-    (void)B;
+size_t tree_attn_ws_bytes(int T, int n_head, int n_kv, int hd) {
     static_assert(TW_RT == 2 * 64, "half the CTAs, twice the rows: a tile of 64 rows needs as much as a wide one");
     const int rt = tree_row_tile(T * (n_head / n_kv), false);
     return 65536 + (size_t)tree_grid(rt) * 2 * tree_part_floats(rt, hd) * sizeof(float);

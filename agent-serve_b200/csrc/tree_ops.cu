@@ -68,7 +68,7 @@ int tf_op_attn_tree_workspace(int B, int T, int n_heads, int n_kv_heads, int hea
     if (!bytes) return set_error("bytes is null");
     *bytes = 0;
     if (attn_shape(B, T, n_heads, n_kv_heads, head_dim)) return -1;
-    *bytes = tree_attn_ws_bytes(B, T, n_heads, n_kv_heads, head_dim);
+    *bytes = tree_attn_ws_bytes(T, n_heads, n_kv_heads, head_dim);
     return 0;
 }
 
@@ -86,7 +86,7 @@ int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, const void
         return set_error("bad cache shape (cap, n_slots, slot_stride)");
     if (!aligned(out, 16) || !aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(ws, 256))
         return set_error("out, q and the caches must be 16-byte aligned, the workspace 256-byte aligned");
-    if (ws_bytes < tree_attn_ws_bytes(B, T, n_heads, n_kv_heads, head_dim)) return set_error("workspace too small");
+    if (ws_bytes < tree_attn_ws_bytes(T, n_heads, n_kv_heads, head_dim)) return set_error("workspace too small");
     if (!tree_attn_fits(B, T, n_heads, n_kv_heads, cap))
         return set_error("B * n_kv_heads * ceil(T * (n_heads / n_kv_heads) / 16) * (cap / 32 + 8) must be below 2^31");
     TreeAttnArgs a = {};

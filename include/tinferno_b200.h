@@ -287,7 +287,7 @@ TF_API int tf_op_argmax(const float* logits, int n, int rows, int* out, void* st
  * Workspaces: the caller allocates `bytes` of device memory (256-byte aligned, its contents do
  * not matter) and may use it for any number of calls of at most those sizes, one call in flight
  * at a time.
- * The calls allocate nothing and do not synchronise.  What a kernel finds wrong on the device
+ * The calls allocate nothing and do not synchronise.  Outputs are in memory of their own.  What a kernel finds wrong on the device
  * (a slot outside the cache, a context that does not fit, a token outside the vocabulary) goes
  * to tf_op_device_error. */
 
@@ -304,7 +304,9 @@ TF_API int tf_tree_mask(const int* parents, int n, int T, unsigned long long* ma
  * sees nothing, like the rows from n_node on, is zero.  Rows that a node does not see do not
  * reach its output, whatever they hold.  T <= 256, head_dim a multiple of 8 up to 128, at most
  * 8 query heads per kv head; B = 1, T = 1 is decode attention.  Scores, softmax and sums are
- * fp32-equivalent for every kv_type.  Work is counted in 32 bits: B * n_kv_heads *
+ * fp32-equivalent for every kv_type: errors are relative to the largest key and value that a row
+ * sees.  (fp32 and bf16 caches: among 32 to 128 neighbouring positions whose rows' maxima lie more
+ * than 2^12 apart the work is done once more in plain fp32, many times slower.)  Work is counted in 32 bits: B * n_kv_heads *
  * ceil(T * (n_heads / n_kv_heads) / 16) * (cap / 32 + 8) must be below 2^31. */
 TF_API int tf_op_attn_tree_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
 TF_API int tf_op_attn_tree(float* out, int ld_out, const float* q, int ld_q, const void* k_cache, const void* v_cache,
