@@ -294,7 +294,7 @@ def _run_own(s):
                                _ptr(qkv, (h + hk) * d), ld, _ptr(s["q_w"]), _ptr(s["k_w"]), EPS, _ptr(s["freq"]), s["rot"], rows,
                                h, hk, d, stream))
     ok(lib.tf_op_kv_dequant(_ptr(s["k_rows"]), hk * d, _ptr(s["v_rows"]), hk * d, *cache, *where, rows, hk, d, stream))
-    return (s["q_out"],) * (op == "store") + (s["k_rows"], s["v_rows"])
+    return ((s["q_out"],) if op == "store" else ()) + (s["k_rows"], s["v_rows"])
 
 
 # ---- the plain forms -----------------------------------------------------------------------------
