@@ -19,7 +19,7 @@ i32p = C.POINTER(C.c_int)
 u64p = C.POINTER(C.c_ulonglong)
 
 TF_F32, TF_F16, TF_Q4_0, TF_Q4_1, TF_Q8_0, TF_Q6_K = 0, 1, 2, 3, 8, 14
-TF_KV_F32, TF_KV_F16, TF_KV_BF16 = 0, 1, 2
+TF_KV_F32, TF_KV_F16, TF_KV_BF16, TF_KV_Q4_0, TF_KV_Q8_0 = range(5)
 TF_DECODE_KERNELS, TF_DECODE_PERSISTENT = 0, 1
 (TF_DEV_ERR_NONE, TF_DEV_ERR_WAIT_FULL, TF_DEV_ERR_WAIT_EMPTY, TF_DEV_ERR_BAD_INDEX, TF_DEV_ERR_POS,
  TF_DEV_ERR_GRID_SYNC) = range(6)
@@ -102,6 +102,18 @@ SIGNATURES = [
                                     C.c_int, C.c_int, _V, C.c_size_t, _V]),
     ("tf_op_kv_commit", C.c_int, [_V, _V, C.c_int, C.c_int, C.c_longlong, C.c_longlong, C.c_int, C.c_int, _V, _V, _V,
                                   C.c_int, _V, _V, C.c_int, C.c_int, C.c_int, _V]),
+    ("tf_op_qk_norm_rope", C.c_int, [_V, C.c_int, _V, C.c_int, _V, C.c_int, _V, C.c_int, _V, _V, C.c_float, _V, C.c_int,
+                                     _V, C.c_int, C.c_int, C.c_int, C.c_int, _V]),
+    ("tf_op_kv_quant", C.c_int, [_V, _V, C.c_int, C.c_longlong, C.c_int, C.c_int, _V, _V, _V, C.c_int, _V, C.c_int,
+                                 C.c_int, C.c_int, C.c_int, _V]),
+    ("tf_op_kv_dequant", C.c_int, [_V, C.c_int, _V, C.c_int, _V, _V, C.c_int, C.c_longlong, C.c_int, C.c_int, _V, _V,
+                                   C.c_int, C.c_int, C.c_int, _V]),
+    ("tf_op_qkv_store", C.c_int, [_V, C.c_int, _V, _V, C.c_int, C.c_longlong, C.c_int, C.c_int, _V, _V, _V, C.c_int, _V,
+                                  C.c_int, _V, C.c_int, _V, _V, C.c_float, _V, C.c_int, C.c_int, C.c_int, C.c_int,
+                                  C.c_int, _V]),
+    ("tf_op_attn_quant_workspace", C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    ("tf_op_attn_quant", C.c_int, [_V, C.c_int, _V, C.c_int, _V, _V, C.c_int, C.c_longlong, C.c_int, C.c_int, _V, _V, _V,
+                                   C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, _V, C.c_size_t, _V]),
 ]
 
 _lib = None

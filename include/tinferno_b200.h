@@ -32,6 +32,9 @@ enum { TF_F32 = 0, TF_F16 = 1, TF_Q4_0 = 2, TF_Q4_1 = 3, TF_Q8_0 = 8, TF_Q6_K = 
 
 /* KV cache element type.  F32 is the reference's own cache type (src/kvcache.hpp:26-27). */
 enum { TF_KV_F32 = 0, TF_KV_F16 = 1, TF_KV_BF16 = 2 };
+/* Quantised cache types of the operators below (tf_op_kv_quant and its neighbours); the engine's own
+ * cache and the other operators take the three above. */
+enum { TF_KV_Q4_0 = 3, TF_KV_Q8_0 = 4 };
 
 /* One GGUF tensor as the reference's Tensor describes it (src/tensor.hpp:7-23): ne[0] is
  * the innermost dimension (K for 2-D weights), data points at the tensor's bytes in their
@@ -344,6 +347,83 @@ TF_API int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_laye
                            long long slot_stride, int cap, int n_slots, const int* slots, const int* n_ctx,
                            const int* path, int ld_path, const int* n_path, int* n_new, int B, int n_kv_heads,
                            int head_dim, void* stream);
+
+/* ---- a KV cache in Q4_0 or Q8_0 -----------------------------------------------------------
+ * No reference counterpart (its cache is fp32, src/kvcache.hpp:26-27).  Values are those of the
+ * ggml block types of the same names: groups of 32 dims of one position, a scale in f16 and a
+ * code per value; value = (code - 8) scale or (code - 128) scale.
+ *   Q4_0  scale = f16(m / -8), m the group's first value of largest magnitude;
+ *         code = clamp(rint(x / scale), -8, 7) + 8
+ *   Q8_0  scale = f16(max|x| r), r = 1 / 127 in fp32;  code = clamp(rint(x / scale), -127, 127) + 128
+ * rint rounds halves to even; a scale beyond f16 is held at +-65504; where it is zero the group
+ * is; a group with a NaN or an infinity reads back as NaN.
+ *
+ * A cache of n_slots sequences of up to cap positions (a multiple of 16) is
+ * [n_slots][n_kv_heads][cap / 16][block], a block being 16 positions: 16 head_dim / 32 times 18
+ * bytes (Q4_0) or 34 (Q8_0).  slot_stride counts elements, as for the other caches (a multiple of
+ * 16 * head_dim): slots lie slot_stride / 32 * 18 (34) bytes apart.  A block's codes come first,
+ * as 32-bit words: word i of lane l at byte 512 (i / 4) + 16 l + 4 (i % 4), or, for the last two
+ * where 4 does not divide the words per lane, 512 (i / 4) + 8 l + 4 (i % 4):
+ *   K, position p, dim e   l = 4 (p % 8) + e % 32 / 8
+ *        Q4_0  i = (p / 8) (head_dim / 32) + e / 32, nibble e % 8 (the lowest first)
+ *        Q8_0  i = 2 ((p / 8) (head_dim / 32) + e / 32) + e % 8 / 4, byte e % 4
+ *   V, position p, dim e   l = 4 (e % 16 / 2) + p % 8 / 2, byte 2 (p % 2) + p / 8
+ *        Q4_0  i = e / 16, the low nibble for even e;  Q8_0  i = 2 (e / 16) + e % 2
+ * then the scales: position p, group k at index (2 (p % 8) + p / 8) head_dim / 32 + k.
+ *
+ * Rows: row r of an operand is ld floats from the next, heads * head_dim of them are used; rows are
+ * 16-byte aligned and strides multiples of 4.  Row r belongs to position pos[r] of slot slots[r]
+ * (slots nullptr: slot r).  A row whose slot is negative (a padded batch) is left out: nothing of
+ * it is read or written.  A slot or a position outside the cache leaves the row out too and goes to
+ * tf_op_device_error.  Rows written by one call name distinct places.  head_dim: 32, 64, 96 or 128.
+ * The calls allocate nothing and do not synchronise. */
+
+/* Per-head RMS norm of queries and keys and the rotation of both, in one pass:
+ *   y = (x / sqrt(mean x^2 + eps)) * weight   (rmsnorm, src/layers.hpp:7, on each head; weight
+ *                                              [head_dim], nullptr: no norm)
+ *   pairs (j, j + rope_dim / 2) of the first rope_dim dims turned by the angle pos[r] freq[j]
+ *                                             (apply_rope, src/attention.hpp:25; freq nullptr: none)
+ * The angle is a product in 64 bits (tf_op_rope keeps the reference's fp32 product, off by 2^-24 of
+ * itself); cosine and sine are fp32, their two products are summed in 64 bits and rounded once.
+ * q (or k) may be nullptr together with its output; outputs may be the inputs themselves (same
+ * pointer and stride), else in memory of their own.  pos [rows]: a negative one leaves its row as it
+ * is; nullptr where nothing is rotated.  head_dim and rope_dim: multiples of 8, head_dim up to 128. */
+TF_API int tf_op_qk_norm_rope(float* q_out, int ld_qo, float* k_out, int ld_ko, const float* q, int ld_q,
+                              const float* k, int ld_k, const float* q_weight, const float* k_weight, float eps,
+                              const float* freq, int rope_dim, const int* pos, int rows, int n_heads,
+                              int n_kv_heads, int head_dim, void* stream);
+
+/* Rows of keys and values into the cache, and cache rows as fp32 (k or v may be nullptr). */
+TF_API int tf_op_kv_quant(void* k_cache, void* v_cache, int kv_type, long long slot_stride, int cap, int n_slots,
+                          const int* slots, const int* pos, const float* k, int ld_k, const float* v, int ld_v,
+                          int rows, int n_kv_heads, int head_dim, void* stream);
+TF_API int tf_op_kv_dequant(float* k, int ld_k, float* v, int ld_v, const void* k_cache, const void* v_cache,
+                            int kv_type, long long slot_stride, int cap, int n_slots, const int* slots,
+                            const int* pos, int rows, int n_kv_heads, int head_dim, void* stream);
+
+/* The step's form of both in one launch: queries normed and rotated to q_out (q itself is allowed),
+ * keys normed, rotated and written, values written.  The results are those of tf_op_qk_norm_rope
+ * followed by tf_op_kv_quant, bit for bit. */
+TF_API int tf_op_qkv_store(float* q_out, int ld_qo, void* k_cache, void* v_cache, int kv_type, long long slot_stride,
+                           int cap, int n_slots, const int* slots, const int* pos, const float* q, int ld_q,
+                           const float* k, int ld_k, const float* v, int ld_v, const float* q_weight,
+                           const float* k_weight, float eps, const float* freq, int rope_dim, int rows, int n_heads,
+                           int n_kv_heads, int head_dim, void* stream);
+
+/* Attention of up to T new rows of B sequences over the cache, their own keys and values written
+ * before: row t < n_new[b] (nullptr: T) of sequence b, in slot slots[b] (nullptr: b), sees cache
+ * rows 0 .. n_ctx[b] + t.  B = 1, T = 1 is decode attention.  q and out: row b * T + t.  Rows from
+ * n_new[b] on are zero, and so are all rows of a sequence whose slot, n_ctx or n_new does not fit
+ * the cache (which goes to tf_op_device_error).  Cache rows that a row does not see do not reach it,
+ * whatever they hold.  Scores, softmax and sums are fp32-equivalent: errors are relative to the
+ * largest key and value that a row sees.  T <= 64, any number of query heads per kv head, up to 1024
+ * heads.  Workspace: as for tf_op_attn_tree.  Work is counted in 32 bits: B * n_kv_heads *
+ * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 8) must be below 2^31. */
+TF_API int tf_op_attn_quant_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
+TF_API int tf_op_attn_quant(float* out, int ld_out, const float* q, int ld_q, const void* k_cache, const void* v_cache,
+                            int kv_type, long long slot_stride, int cap, int n_slots, const int* slots,
+                            const int* n_ctx, const int* n_new, int B, int T, int n_heads, int n_kv_heads,
+                            int head_dim, void* ws, size_t ws_bytes, void* stream);
 
 /* Pipeline trace of the tensor-core GEMM, no reference counterpart (a finer-grained companion
  * of the reference's --profile timings, src/main.cpp): while `buf` (device memory, 968
