@@ -993,6 +993,10 @@ int tf_cuda_create(const tf_tensor_desc* t, int nt, const tf_hparams* hp_in, con
         delete m;
         return set_error("max_seq and max_batch must be positive");
     }
+    if (o.kv_type < TF_KV_F32 || o.kv_type > TF_KV_BF16) {
+        delete m;
+        return set_error("unknown kv_type (the engine's cache is F32, F16 or BF16)");
+    }
     m->opt = o;
     m->device = o.device;
     const tf_hparams& hp = m->hp;

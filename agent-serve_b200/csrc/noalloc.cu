@@ -79,6 +79,7 @@ extern "C" {
 int tf_op_attn_decode_noalloc(float* out, const float* q, const void* k_cache, const void* v_cache, int kv_type,
                               int cap, int n_pos, int n_heads, int n_kv_heads, int head_dim, void* stream) {
     using namespace tfb;
+    if (kv_type < KV_F32 || kv_type > KV_BF16) return set_error("unknown kv_type");
     if (n_pos <= 0 || n_pos > cap) return set_error("n_pos must be in [1, cap]");
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads)
         return set_error("n_heads must be a positive multiple of n_kv_heads");
