@@ -5,11 +5,12 @@
 //
 // Bound by the cache's bytes: a position of one kv head is 2 hd codes (144 bytes with its scales for 128 dims in
 // 4 bits), so every warp instruction per position counts: at 6.5 TB/s an SM has 6.2 cycles for those 144 bytes,
-// 25 issue slots.  Hence mma.sync m16n8k16 with the positions as M (K, then V transposed, is the A operand; a
-// decode step has too few rows to fill M) and the rows as N, codes stored in the order of its fragments:
-// a 32-bit word of eight codes is a shift, four LOP3 and four HADD2 away from four A registers, and no
-// shared-memory pass or transpose is needed.  tcgen05 would want the codes unpacked through shared memory and 64 rows
-// or more.
+// 25 issue slots.  Hence mma.sync m16n8k16 with the codes in the order of its fragments: a 32-bit word of eight
+// codes is a shift, four LOP3 and four HADD2 away from four operand registers, and no shared-memory pass or
+// transpose is needed.  Scores have the rows as M and the positions as N (K is the B operand), the second product
+// the dims as M and the rows as N (V transposed is the A operand), so that the scores' registers are the
+// probabilities' operand as they stand.  Up to 8 rows, the M of 16 holds q's high and low halves; up to 4, the N of 8
+// holds p's.  tcgen05 would want the codes unpacked through shared memory and 64 rows or more.
 //
 // Arithmetic (fp32-equivalent).  Codes less their zero are exact in f16: (code | 0x6400) is 1024 + code, and
 // the high nibble in place 1024 + 16 code; the 16 is taken out of q (K) or of the output row (V).  q is split
@@ -26,6 +27,7 @@
 // in the loop), and join at the range's end.  A unit that a range cuts leaves partial results for
 // tf_kvq_combine_kernel, in a fixed order: results repeat bit for bit.
 #include <atomic>
+#include <type_traits>
 
 #include "kvq.cuh"
 
@@ -95,18 +97,44 @@ __device__ __forceinline__ uint32_t ka_centre(uint32_t x) {
     const __half2 y = __hadd2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(-1024.0f - Z));
     return *reinterpret_cast<const uint32_t*>(&y);
 }
+// (w & MASK) | magic in one instruction: of two constants one has to lie in a register, which the caller sees to
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t ka_field(uint32_t w, uint32_t magic) {
+    uint32_t y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(w), "n"(MASK), "r"(magic));
+    return y;
+}
 // the eight codes of a Q4_0 word, pairs 16 bits apart: codes 0 and 4, 1 and 5 (times 16), 2 and 6, 3 and 7 (times 16)
-__device__ __forceinline__ void ka_nibbles(uint32_t w, uint32_t (&f)[4]) {
+__device__ __forceinline__ void ka_nibbles(uint32_t w, uint32_t magic, uint32_t (&f)[4]) {
     const uint32_t v = w >> 8;
-    f[0] = ka_centre<8>((w & 0x000F000Fu) | 0x64006400u);
-    f[1] = ka_centre<128>((w & 0x00F000F0u) | 0x64006400u);
-    f[2] = ka_centre<8>((v & 0x000F000Fu) | 0x64006400u);
-    f[3] = ka_centre<128>((v & 0x00F000F0u) | 0x64006400u);
+    f[0] = ka_centre<8>(ka_field<0x000F000Fu>(w, magic));
+    f[1] = ka_centre<128>(ka_field<0x00F000F0u>(w, magic));
+    f[2] = ka_centre<8>(ka_field<0x000F000Fu>(v, magic));
+    f[3] = ka_centre<128>(ka_field<0x00F000F0u>(v, magic));
 }
 // the four codes of a Q8_0 word: codes 0 and 2, 1 and 3
-__device__ __forceinline__ void ka_bytes(uint32_t w, uint32_t& f0, uint32_t& f1) {
-    f0 = ka_centre<128>((w & 0x00FF00FFu) | 0x64006400u);
-    f1 = ka_centre<128>((w >> 8 & 0x00FF00FFu) | 0x64006400u);
+__device__ __forceinline__ void ka_bytes(uint32_t w, uint32_t magic, uint32_t& f0, uint32_t& f1) {
+    f0 = ka_centre<128>(ka_field<0x00FF00FFu>(w, magic));
+    f1 = ka_centre<128>(ka_field<0x00FF00FFu>(w >> 8, magic));
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 ka_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 ka_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\t"
+        "mov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 __device__ __forceinline__ void ka_copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -131,23 +159,29 @@ __device__ __forceinline__ void ka_words(uint32_t at, int lane, uint32_t (&w)[N]
                      : "r"(at + N / 4 * 512 + lane * 8)
                      : "memory");
 }
-// the scales of positions g and g + 8, HD / 32 groups each
-template <int HD>
-__device__ __forceinline__ void ka_scales(uint32_t at, int g, uint32_t (&s)[HD / 32]) {
-    if (HD == 128)
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(s[0]), "=r"(s[HD / 32 > 1 ? 1 : 0]), "=r"(s[HD / 32 > 2 ? 2 : 0]), "=r"(s[HD / 32 > 3 ? 3 : 0])
-                     : "r"(at + g * 16)
-                     : "memory");
-    else
+// the scales of positions 2 tq, 2 tq + 8, 2 tq + 1, 2 tq + 9: NG = HD / 32 groups each, two to a word
+template <int NG>
+__device__ __forceinline__ void ka_scales(uint32_t at, int tq, uint32_t (&s)[2 * NG]) {
+    const uint32_t p = at + tq * (8 * NG);
+    if (NG % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) s[i] = ka_lds(at + g * (HD / 8) + 4 * i);
+        for (int i = 0; i < 2 * NG; i += 4)
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(s[i]), "=r"(s[i + 1]), "=r"(s[(i + 2) % (2 * NG)]), "=r"(s[(i + 3) % (2 * NG)])
+                         : "r"(p + 4 * i)
+                         : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i += 2)
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(s[i]), "=r"(s[i + 1]) : "r"(p + 4 * i) : "memory");
+    }
 }
-// scale of group k of position g (half 0) or g + 8 (half 1)
+// Scale of group k of position 2 tq + e (e = 0, 1) or 2 tq + 8 + e - 2 (e = 2, 3).
 template <int N>
-__device__ __forceinline__ float ka_scale(const uint32_t (&s)[N], int half, int k) {
-    const int i = half * N + k;
-    return h2f(i & 1 ? s[i >> 1] >> 16 : s[i >> 1]);
+__device__ __forceinline__ float ka_scale(const uint32_t (&s)[N], int e, int k) {
+    const int i = ((e & 1) * 2 + (e >> 1)) * (N / 2) + k;
+    const __half2 h = *reinterpret_cast<const __half2*>(&s[i >> 1]);
+    return i & 1 ? __high2float(h) : __low2float(h);
 }
 
 // ---- the split of the blocks over the CTAs ------------------------------------------------------------
@@ -204,13 +238,14 @@ template <int BITS, int HD, int MODE>
 __global__ void __launch_bounds__(KA_THREADS, KvqCfg<BITS, HD, MODE>::CTAS)
 tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     using F = KvqCfg<BITS, HD, MODE>;
-    constexpr int RT = F::RT, NT = MODE == 2 ? 2 : 1, NG = HD / 32, W = HD * BITS / 64, CODES = kvq_code_bytes(BITS, HD);
-    constexpr int QP = MODE == 0 ? 1 : 2;  // parts of q and p that are products of their own
+    constexpr int RT = F::RT, NG = HD / 32, W = HD * BITS / 64, CODES = kvq_code_bytes(BITS, HD);
+    constexpr int NR = MODE == 2 ? 2 : 1;  // rows of a thread: g, and g + 8
+    constexpr int QP = MODE == 2 ? 2 : 1;  // products of q's halves: side by side in M, or one after the other
+    constexpr int PP = MODE == 0 ? 1 : 2;  // products of p's halves: side by side in N, or one after the other
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    uint8_t* ring_p = smem + warp * (F::ST * F::STAGE);
-    const uint32_t ring = smem_u32(ring_p);
+    const uint32_t ring = smem_u32(smem + warp * (F::ST * F::STAGE));
     float* slot_all = reinterpret_cast<float*>(smem + KA_WARPS * F::ST * F::STAGE);
     float* stat = slot_all + KA_WARPS * RT * HD;  // [warp][RT] exponents, then sums
     KvqDesc* desc = static_cast<KvqDesc*>(a.ws);
@@ -220,6 +255,8 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     KvqDesc open = {-1, 0, 0, 0};  // the unit that begins here and ends in a later CTA
     int b = range.b, base = range.base;
     const float log2e_d = 1.4426950408889634f * rsqrtf((float)HD);
+    uint32_t magic;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
 
 #pragma unroll 1
     for (int gpos = range.g0; gpos < range.g1;) {
@@ -238,32 +275,37 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
         const int tiles = sq.units / a.n_kv, kvh = unit / tiles, tile = unit - kvh * tiles;
         const int r0 = tile * RT, rows = min(RT, sq.n_new * pl.rep - r0);
 
-        const long long where = sq.slot * a.slot_bytes + kvh * a.head_bytes;
-        const uint8_t *kc = a.kc + where, *vc = a.vc + where;
+        // this warp's blocks: blk0 + warp, and every KA_WARPS-th from there
         const int n_mine = blk1 - blk0 > warp ? (blk1 - blk0 - warp + KA_WARPS - 1) / KA_WARPS : 0;
-        auto fetch = [&](int i) {  // block i of this warp's, in stage i % ST
-            if (i < n_mine) {
-                const long long off = (long long)(blk0 + warp + i * KA_WARPS) * F::BLOCK;
-                const uint32_t dst = ring + i % F::ST * F::STAGE;
+        const long long where = sq.slot * a.slot_bytes + kvh * a.head_bytes + (long long)(blk0 + warp) * F::BLOCK + lane * 16;
+        const uint8_t *kc = a.kc + where, *vc = a.vc + where;
+        int left = n_mine;
+        uint32_t fill = ring + lane * 16;
+        auto fetch = [&]() {  // the next block into the next stage
+            if (left > 0) {
 #pragma unroll
-                for (int c = 0; c < (2 * F::BLOCK / 16 + 31) / 32; ++c) {
-                    const int e = (c * 32 + lane) * 16;
-                    if (e < F::BLOCK) ka_copy16(dst + e, kc + off + e);
-                    else if (e < 2 * F::BLOCK) ka_copy16(dst + e, vc + off + (e - F::BLOCK));
-                }
+                for (int c = 0; c < F::BLOCK; c += 512)
+                    if (c + 512 <= F::BLOCK || lane * 16 < F::BLOCK - c) {
+                        ka_copy16(fill + c, kc + c);
+                        ka_copy16(fill + F::BLOCK + c, vc + c);
+                    }
+                --left;
+                kc += KA_WARPS * F::BLOCK;
+                vc += KA_WARPS * F::BLOCK;
+                fill = fill + F::STAGE >= ring + F::ST * F::STAGE ? ring + lane * 16 : fill + F::STAGE;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
-        for (int i = 0; i < F::ST - 1; ++i) fetch(i);
+        for (int i = 0; i < F::ST - 1; ++i) fetch();
 
-        // q as B fragments: column g is row g of the tile (packed: rows 0 .. 3 high, then rows 0 .. 3 low)
-        uint32_t qf[NT][QP][NG][4];
-        float fr[NT][2];  // of columns 2 tq and 2 tq + 1: out of q's scale, to powers of two
-        int lim[NT][2];   // last position that they see
+        // q as A fragments.  Rows g and g + 8 of M: the tile's rows (MODE 2), or the high and the low half of one.
+        uint32_t qf[QP][NG][8];  // [..][4 u + i]: register i of the product's half u of a group
+        float fr[NR];            // out of q's scale, to powers of two
+        int lim[NR];             // last position that the row sees
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            const int row = MODE == 0 ? g & 3 : nt * 8 + g, rr = r0 + row;
+        for (int nr = 0; nr < NR; ++nr) {
+            const int row = MODE == 0 ? g & 3 : nr * 8 + g, rr = r0 + row;
             const bool valid = row < rows;
             const int t = valid ? rr / pl.rep : 0, h = valid ? kvh * pl.rep + rr - t * pl.rep : 0;
             const float* qp = a.q + ((long long)b * a.T + t) * a.ld_q + h * HD + tq * 8;
@@ -283,231 +325,231 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
             const int sh = ex <= -127 || ex == 128 ? 0 : max(-120, min(120, 13 - ex));
             const float sc = __int_as_float((sh + 127) << 23);
-            const float back = __int_as_float((127 - sh) << 23) * log2e_d;
+            fr[nr] = __int_as_float((127 - sh) << 23) * log2e_d;
+            lim[nr] = sq.n_ctx + (r0 + row) / pl.rep;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                uint32_t hi[4], lo[4];
+            for (int k = 0; k < NG; ++k)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     // codes 4 apart share a register in 4 bits (odd ones times 16), codes 2 apart in 8
                     const int e0 = BITS == 4 ? i : (i >> 1) * 4 + (i & 1), e1 = BITS == 4 ? i + 4 : e0 + 2;
                     const float down = BITS == 4 && (i & 1) ? sc * 0.0625f : sc;
                     const float u = x[k][e0] * down, v = x[k][e1] * down;
-                    hi[i] = ka_pack(u, v);
-                    const float2 f = ka_unpack(hi[i]);
-                    lo[i] = ka_pack(u - f.x, v - f.y);
-                    if (MODE == 0) qf[nt][0][k][i] = g < 4 ? hi[i] : lo[i];
-                    else { qf[nt][0][k][i] = hi[i]; qf[nt][QP - 1][k][i] = lo[i]; }
+                    const uint32_t hi = ka_pack(u, v);
+                    const float2 f = ka_unpack(hi);
+                    const uint32_t lo = ka_pack(u - f.x, v - f.y);
+                    const int at = (i >> 1) * 4 + (i & 1) * 2;
+                    if (MODE == 2) {
+                        qf[0][k][at + nr] = hi;
+                        qf[QP - 1][k][at + nr] = lo;
+                    } else {
+                        qf[0][k][at] = hi;
+                        qf[0][k][at + 1] = lo;
+                    }
                 }
-            }
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                fr[nt][j] = __shfl_sync(0xFFFFFFFFu, back, (2 * tq + j) * 4);
-                const int c = MODE == 0 ? (2 * tq + j) & 3 : nt * 8 + 2 * tq + j;
-                lim[nt][j] = sq.n_ctx + (r0 + c) / pl.rep;
-            }
         }
         const int open_to = sq.n_ctx + r0 / pl.rep;  // every row sees the positions up to here
 
-        float o[NT][HD / 16][4];
-        float m[NT][2], ref[NT][2], l[NT][2];
-        uint32_t top[NT][2];  // largest V scale that the column saw, rounded up within its binary order
+        // Columns 2 tq and 2 tq + 1 of the output; dims 16 d + 2 g and one on.
+        float o[NR][HD / 16][4];
+        // Row g (and g + 8): largest score and the one that moves it (both in q's scale), exponent that p is
+        // relative to, sum
+        float m[NR], ref[NR], thr[NR], l[NR];
+        uint32_t top[NR];          // largest V scale that the row saw, rounded up within its binary order
+        uint32_t top_all = 0;      // the least of all rows' tops, twice
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
-            for (int j = 0; j < HD / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                m[nt][j] = -INFINITY;
-                ref[nt][j] = 0.f;
-                l[nt][j] = 0.f;
-                top[nt][j] = 0;
-            }
+            for (int j = 0; j < HD / 16; ++j) o[nr][j][0] = o[nr][j][1] = o[nr][j][2] = o[nr][j][3] = 0.f;
+            m[nr] = thr[nr] = -INFINITY;
+            ref[nr] = l[nr] = 0.f;
+            top[nr] = 0;
         }
 
-#pragma unroll 1
-        for (int i = 0; i < n_mine; ++i) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(F::ST - 2) : "memory");
-            __syncwarp();  // everyone's copies of this stage are visible, and the stage before is read
-            fetch(i + F::ST - 1);
-            const uint32_t at = ring + i % F::ST * F::STAGE;
-            const int p0 = (blk0 + warp + i * KA_WARPS) * 16;
-            const bool masked = p0 + 15 > open_to;
-
-            // scores: positions g and g + 8 (rows of C), columns 2 tq and 2 tq + 1
-            float x[NT][4];
+        // One block at shared address `at`, from position p0 on.
+        auto block = [&](auto masked_c, const uint32_t at, const int p0) {
+            constexpr bool MASKED = decltype(masked_c)::value;
+            // scores of row g (and g + 8) against positions 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9
+            float2 x[NR][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) x[nt][0] = x[nt][1] = x[nt][2] = x[nt][3] = 0.f;
+            for (int nr = 0; nr < NR; ++nr) x[nr][0] = x[nr][1] = make_float2(0.f, 0.f);
             {
-                uint32_t w[W], s[NG];
+                uint32_t w[W], s[2 * NG];
                 ka_words<W>(at, lane, w);
-                ka_scales<HD>(at + CODES, g, s);
+                ka_scales<NG>(at + CODES, tq, s);
 #pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    uint32_t a0[4], a1[4];
-                    if (BITS == 4) {
-                        uint32_t u[4], v[4];
-                        ka_nibbles(w[k], u);
-                        ka_nibbles(w[W / 2 + k], v);
-                        a0[0] = u[0]; a0[1] = v[0]; a0[2] = u[1]; a0[3] = v[1];
-                        a1[0] = u[2]; a1[1] = v[2]; a1[2] = u[3]; a1[3] = v[3];
-                    } else {
-                        ka_bytes(w[2 * k], a0[0], a0[2]);
-                        ka_bytes(w[W / 2 + 2 * k], a0[1], a0[3]);
-                        ka_bytes(w[2 * k + 1], a1[0], a1[2]);
-                        ka_bytes(w[W / 2 + 2 * k + 1], a1[1], a1[3]);
-                    }
-                    const float s0 = ka_scale(s, 0, k), s1 = ka_scale(s, 1, k);
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
+                    for (int k = 0; k < NG; ++k) {
+                        uint32_t f[4];
+                        if (BITS == 4) {
+                            ka_nibbles(w[half * (W / 2) + k], magic, f);
+                        } else {
+                            ka_bytes(w[half * (W / 2) + 2 * k], magic, f[0], f[1]);
+                            ka_bytes(w[half * (W / 2) + 2 * k + 1], magic, f[2], f[3]);
+                        }
                         float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int part = QP - 1; part >= 0; --part) {  // the low halves first
-                            ka_mma(c, a0, qf[nt][part][k][0], qf[nt][part][k][1]);
-                            ka_mma(c, a1, qf[nt][part][k][2], qf[nt][part][k][3]);
+                            ka_mma(c, reinterpret_cast<const uint32_t(&)[4]>(qf[part][k][0]), f[0], f[1]);
+                            ka_mma(c, reinterpret_cast<const uint32_t(&)[4]>(qf[part][k][4]), f[2], f[3]);
                         }
-                        x[nt][0] = fmaf(c[0], s0, x[nt][0]);
-                        x[nt][1] = fmaf(c[1], s0, x[nt][1]);
-                        x[nt][2] = fmaf(c[2], s1, x[nt][2]);
-                        x[nt][3] = fmaf(c[3], s1, x[nt][3]);
+                        const float2 sc = make_float2(ka_scale(s, half * 2, k), ka_scale(s, half * 2 + 1, k));
+                        x[NR - 1][half] = ka_fma2(make_float2(c[2], c[3]), sc, x[NR - 1][half]);
+                        x[0][half] = ka_fma2(make_float2(c[0], c[1]), sc, x[0][half]);
                     }
-                }
             }
-            if (MODE == 0) {  // column c holds the high half's part of row c, column c + 4 the low half's
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[0][e] += __shfl_xor_sync(0xFFFFFFFFu, x[0][e], 2);
+            uint32_t vs[2 * NG];
+            ka_scales<NG>(at + F::BLOCK + CODES, tq, vs);
+            auto seen = [&](int nr, int e) { return !MASKED || p0 + 2 * tq + (e & 1) + (e >> 1) * 8 <= lim[nr]; };
+            bool raise;
+            {  // a lane looks at one word of V's scales
+                const uint32_t word = ka_lds(at + F::BLOCK + CODES + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
+                raise = (word & 0xFFFFu) > top_all || word >> 16 > top_all;
             }
-            uint32_t vs[NG];
-            ka_scales<HD>(at + F::BLOCK + CODES, g, vs);
-            // largest |scale| of V at positions g and g + 8; NaN and infinity have no say
-            uint32_t big0 = 0, big1 = 0;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                const int i0 = k, i1 = NG + k;
-                const uint32_t e0 = (i0 & 1 ? vs[i0 >> 1] >> 16 : vs[i0 >> 1]) & 0x7FFFu;
-                const uint32_t e1 = (i1 & 1 ? vs[i1 >> 1] >> 16 : vs[i1 >> 1]) & 0x7FFFu;
-                if (e0 < 0x7C00u) big0 = max(big0, e0);
-                if (e1 < 0x7C00u) big1 = max(big1, e1);
-            }
-            bool raise = false;
+            for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int j = e & 1;
-                    const bool seen = !masked || p0 + g + (e >> 1) * 8 <= lim[nt][j];
-                    x[nt][e] = seen ? x[nt][e] * fr[nt][j] : -INFINITY;
-                    raise |= x[nt][e] > m[nt][j] + (float)KA_SLACK || (seen && (e >> 1 ? big1 : big0) > top[nt][j]);
+                for (int e = 0; e < 2; ++e) {
+                    if (!seen(nr, 2 * e)) x[nr][e].x = -INFINITY;
+                    if (!seen(nr, 2 * e + 1)) x[nr][e].y = -INFINITY;
+                    raise |= x[nr][e].x > thr[nr] || x[nr][e].y > thr[nr];
                 }
             if (__any_sync(0xFFFFFFFFu, raise)) {
+                uint32_t least = 0xFFFFu;
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int nr = 0; nr < NR; ++nr) {
+                    float mx = m[nr];
+                    uint32_t tp = top[nr];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float mx = fmaxf(m[nt][j], fmaxf(x[nt][j], x[nt][2 + j]));
-                        uint32_t tp = top[nt][j];
-                        if (!masked || p0 + g <= lim[nt][j]) tp = max(tp, big0);
-                        if (!masked || p0 + g + 8 <= lim[nt][j]) tp = max(tp, big1);
+                    for (int e = 0; e < 4; ++e) {
+                        mx = fmaxf(mx, e & 1 ? x[nr][e >> 1].y : x[nr][e >> 1].x);
+                        if (seen(nr, e)) {
 #pragma unroll
-                        for (int s = 4; s < 32; s <<= 1) {
-                            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, s));
-                            tp = max(tp, __shfl_xor_sync(0xFFFFFFFFu, tp, s));
-                        }
-                        // a column moves by what it sees alone, whichever column asked
-                        const bool move = mx > m[nt][j] + (float)KA_SLACK || tp > top[nt][j];
-                        if (!move) continue;
-                        tp |= 0x3FFu;  // scales are below 2^(tp / 1024 - 14)
-                        const float nref = mx == -INFINITY ? 0.f : mx - (float)(15 - KA_SLACK + 14 - (int)(tp >> 10));
-                        const float f = m[nt][j] == -INFINITY ? 0.f : ka_exp2(ref[nt][j] - nref);
-                        // (a row that saw nothing yet has sums of zero, or NaN, which stays)
-                        m[nt][j] = mx;
-                        ref[nt][j] = nref;
-                        top[nt][j] = tp;
-                        l[nt][j] *= f;
-#pragma unroll
-                        for (int d = 0; d < HD / 16; ++d) {
-                            o[nt][d][j] *= f;
-                            o[nt][d][2 + j] *= f;
+                            for (int k = 0; k < NG; ++k) {  // NaN and infinity have no say
+                                const uint32_t v = __half_as_ushort(__float2half_rn(fabsf(ka_scale(vs, e, k))));
+                                if (v < 0x7C00u) tp = max(tp, v);
+                            }
                         }
                     }
+#pragma unroll
+                    for (int s = 1; s < 4; s <<= 1) {
+                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, s));
+                        tp = max(tp, __shfl_xor_sync(0xFFFFFFFFu, tp, s));
+                    }
+                    // a row moves by what it sees alone, whichever row asked
+                    float f = 1.0f;
+                    if (mx > thr[nr] || tp > top[nr]) {
+                        tp |= 0x3FFu;  // scales are below 2^(tp / 1024 - 14)
+                        const float nref = mx == -INFINITY ? 0.f : mx * fr[nr] - (float)(15 - KA_SLACK + 14 - (int)(tp >> 10));
+                        // (a row that saw nothing yet has sums of zero, or NaN, which stays)
+                        f = m[nr] == -INFINITY ? 0.f : ka_exp2(ref[nr] - nref);
+                        m[nr] = mx;
+                        thr[nr] = mx + (float)KA_SLACK / fr[nr];
+                        ref[nr] = nref;
+                        top[nr] = tp;
+                        l[nr] *= f;
+                    }
+                    least = min(least, top[nr]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float fc = __shfl_sync(0xFFFFFFFFu, f, (2 * tq + j) * 4);
+#pragma unroll
+                        for (int d = 0; d < HD / 16; ++d) {
+                            o[nr][d][j] *= fc;
+                            o[nr][d][2 + j] *= fc;
+                        }
+                    }
+                }
+                top_all = __reduce_min_sync(0xFFFFFFFFu, least);
             }
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[nt][e] = ka_exp2(x[nt][e] - ref[nt][e & 1]);
-                    l[nt][e & 1] += x[nt][e];
+                for (int e = 0; e < 2; ++e) {
+                    const float2 y = ka_fma2(x[nr][e], make_float2(fr[nr], fr[nr]), make_float2(-ref[nr], -ref[nr]));
+                    x[nr][e] = make_float2(ka_exp2(y.x), ka_exp2(y.y));
+                    l[nr] += x[nr][e].x + x[nr][e].y;
                 }
             uint32_t w[W];
             ka_words<W>(at + F::BLOCK, lane, w);
+            // the low half is what the high one leaves; MODE 0: columns 0 .. 3 take the high half, 4 .. 7 the low
+            const float low = MODE == 0 && g < 4 ? 0.f : -1.f;
 #pragma unroll
             for (int k = 0; k < NG; ++k) {
-                const float s0 = ka_scale(vs, 0, k), s1 = ka_scale(vs, 1, k);
-                uint32_t pf[NT][QP][2];
+                uint32_t pf[NR][PP][2];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float y[4] = {x[nt][0] * s0, x[nt][1] * s0, x[nt][2] * s1, x[nt][3] * s1};
-                    if (masked) {  // an unseen position's scale may be NaN
+                for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (p0 + g + (e >> 1) * 8 > lim[nt][e & 1]) y[e] = 0.f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t hi = ka_pack(y[2 * e], y[2 * e + 1]);
-                        const float2 f = ka_unpack(hi);
-                        const uint32_t lo = ka_pack(y[2 * e] - f.x, y[2 * e + 1] - f.y);
-                        if (MODE == 0) {
-                            pf[nt][0][e] = ka_trans(tq < 2 ? hi : lo);
-                        } else {
-                            pf[nt][0][e] = ka_trans(hi);
-                            pf[nt][QP - 1][e] = ka_trans(lo);
+                    for (int half = 0; half < 2; ++half) {
+                        float2 y = ka_mul2(x[nr][half], make_float2(ka_scale(vs, 2 * half, k), ka_scale(vs, 2 * half + 1, k)));
+                        if (MASKED) {  // an unseen position's scale may be NaN
+                            if (!seen(nr, 2 * half)) y.x = 0.f;
+                            if (!seen(nr, 2 * half + 1)) y.y = 0.f;
                         }
+                        const uint32_t hi = ka_pack(y.x, y.y);
+                        const float2 z = ka_fma2(ka_unpack(hi), make_float2(low, low), y);
+                        if (MODE != 0) pf[nr][0][half] = hi;
+                        pf[nr][PP - 1][half] = ka_pack(z.x, z.y);
                     }
-                }
 #pragma unroll
                 for (int d = 2 * k; d < 2 * k + 2; ++d) {
                     uint32_t v[4];
                     if (BITS == 4) {
-                        ka_nibbles(w[d], v);
+                        ka_nibbles(w[d], magic, v);
                     } else {
-                        ka_bytes(w[2 * d], v[0], v[2]);
-                        ka_bytes(w[2 * d + 1], v[1], v[3]);
+                        ka_bytes(w[2 * d], magic, v[0], v[2]);
+                        ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
                     }
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                        for (int part = QP - 1; part >= 0; --part) ka_mma(o[nt][d], v, pf[nt][part][0], pf[nt][part][1]);
+                        for (int part = PP - 1; part >= 0; --part) ka_mma(o[nr][d], v, pf[nr][part][0], pf[nr][part][1]);
                 }
             }
+        };
+
+        uint32_t at = ring;
+        int p0 = (blk0 + warp) * 16;
+#pragma unroll 1
+        for (int i = 0; i < n_mine; ++i) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(F::ST - 2) : "memory");
+            __syncwarp();  // everyone's copies of this stage are visible, and the stage before is read
+            fetch();
+            if (p0 + 15 <= open_to) block(std::false_type(), at, p0);
+            else block(std::true_type(), at, p0);
+            p0 += KA_WARPS * 16;
+            at = at + F::STAGE >= ring + F::ST * F::STAGE ? ring : at + F::STAGE;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
         // the warp's rows into its slot: dims 16 d + 2 g and one on, rows 2 tq and one on
         __syncthreads();  // the slots of the segment before are read
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                for (int s = 4; s < 32; s <<= 1) l[nt][j] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][j], s);
-                const int row = nt * 8 + 2 * tq + j;
+                const int row = nr * 8 + 2 * tq + j;
 #pragma unroll
                 for (int d = 0; d < HD / 16; ++d) {
-                    float2 y = make_float2(o[nt][d][j], o[nt][d][2 + j] * (BITS == 4 ? 0.0625f : 1.0f));
+                    float2 y = make_float2(o[nr][d][j], o[nr][d][2 + j] * (BITS == 4 ? 0.0625f : 1.0f));
                     if (MODE == 0) {
                         y.x += __shfl_xor_sync(0xFFFFFFFFu, y.x, 2);
                         y.y += __shfl_xor_sync(0xFFFFFFFFu, y.y, 2);
                     }
                     if (row < RT) *reinterpret_cast<float2*>(slot_all + (warp * RT + row) * HD + 16 * d + 2 * g) = y;
                 }
-                if (g == 0 && row < RT) {
-                    // a warp without blocks, or whose rows saw nothing: its exponent says so
-                    const bool none = n_mine == 0 || (m[nt][j] == -INFINITY && l[nt][j] == 0.f);
-                    stat[warp * RT + row] = none ? -INFINITY : ref[nt][j];
-                    stat[(KA_WARPS + warp) * RT + row] = l[nt][j];
-                }
             }
+            l[nr] += __shfl_xor_sync(0xFFFFFFFFu, l[nr], 1);
+            l[nr] += __shfl_xor_sync(0xFFFFFFFFu, l[nr], 2);
+            const int row = nr * 8 + g;
+            if (tq == 0 && row < RT) {
+                // a warp without blocks, or whose rows saw nothing: its exponent says so
+                const bool none = n_mine == 0 || (m[nr] == -INFINITY && l[nr] == 0.f);
+                stat[warp * RT + row] = none ? -INFINITY : ref[nr];
+                stat[(KA_WARPS + warp) * RT + row] = l[nr];
+            }
+        }
         __syncthreads();
         const bool begins = blk0 == 0, ends = blk1 == sq.blocks;
         float* part = parts + (blockIdx.x * 2 + (begins ? 1 : 0)) * kvq_part_floats(RT, HD);
