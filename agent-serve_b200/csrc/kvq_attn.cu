@@ -33,7 +33,7 @@
 
 namespace tfb {
 
-constexpr int KA_THREADS = 256;
+constexpr int KA_THREADS = 128;
 constexpr int KA_WARPS = KA_THREADS / 32;
 constexpr int KA_UNIT_COST = 8;    // blocks that a unit's start and end take the time of
 constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
@@ -54,19 +54,23 @@ __host__ __device__ inline size_t kvq_part_floats(int rt, int hd) { return (size
 // 0: up to 4 rows (both halves of q and p side by side in the 8 columns), 1: up to 8, 2: up to 16
 __host__ __device__ constexpr int kvq_rt(int mode) { return mode == 0 ? 4 : mode == 1 ? 8 : 16; }
 
+__host__ __device__ constexpr int kvq_ctas(int mode) { return mode == 2 ? 3 : 5; }  // 168 or 96 registers a thread
+
 template <int BITS, int HD, int MODE>
 struct KvqCfg {
     static constexpr int RT = kvq_rt(MODE);
-    static constexpr int CTAS = MODE == 2 ? 1 : 2;                 // per SM
+    static constexpr int CTAS = kvq_ctas(MODE);                    // per SM
     static constexpr int BLOCK = kvq_block_bytes(BITS, HD);
     static constexpr int STAGE = 2 * BLOCK;                        // K and V of 16 positions
     static constexpr int SLOT = RT * HD * 4;                       // a warp's output rows
-    static constexpr int STAT = KA_WARPS * RT * 8;
-    static constexpr int ROOM = (CTAS == 2 ? 112 : 224) * 1024 - KA_WARPS * SLOT - STAT;
+    static constexpr int QF = (MODE == 2 ? 2 : 1) * HD / 32 * 1024;  // q's fragments
+    static constexpr int STAT = KA_WARPS * RT * 12;
+    static constexpr int ROOM = 227 * 1024 / CTAS - 1024 - STAT - QF;
     static constexpr int FIT = ROOM / (KA_WARPS * STAGE);
     static constexpr int ST = FIT > 8 ? 8 : FIT;                   // stages of a warp's ring
-    static constexpr int SMEM = KA_WARPS * (ST * STAGE + SLOT) + STAT;
-    static_assert(ST >= 2, "two stages at least");
+    static constexpr int RING = ST * STAGE > SLOT ? ST * STAGE : SLOT;  // output rows take the rings' place
+    static constexpr int SMEM = KA_WARPS * RING + STAT + QF;
+    static_assert(ST >= 2 && KA_WARPS * RING + STAT + QF <= 227 * 1024 / CTAS - 1024, "two stages at least");
 };
 
 __device__ __forceinline__ float ka_exp2(float x) {
@@ -75,15 +79,10 @@ __device__ __forceinline__ float ka_exp2(float x) {
     return y;
 }
 __device__ __forceinline__ void ka_mma(float (&c)[4], const uint32_t (&a)[4], const uint32_t b0, const uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t ka_trans(uint32_t x) {
-    uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
 }
 __device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
     uint32_t y;
@@ -139,41 +138,32 @@ __device__ __forceinline__ float2 ka_mul2(float2 a, float2 b) {
 __device__ __forceinline__ void ka_copy16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint32_t ka_lds(uint32_t at) {
-    uint32_t x;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
-    return x;
+__device__ __forceinline__ void ka_lds4(const uint8_t* p, uint32_t* x) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    x[0] = v.x;
+    x[1] = v.y;
+    x[2] = v.z;
+    x[3] = v.w;
+}
+__device__ __forceinline__ void ka_lds2(const uint8_t* p, uint32_t* x) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = v.x;
+    x[1] = v.y;
 }
 // N words that lie as kvq_word() places them for this lane
 template <int N>
-__device__ __forceinline__ void ka_words(uint32_t at, int lane, uint32_t (&w)[N]) {
+__device__ __forceinline__ void ka_words(const uint8_t* p, int lane, uint32_t (&w)[N]) {
 #pragma unroll
-    for (int c = 0; c < N / 4; ++c)
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                     : "=r"(w[4 * c]), "=r"(w[4 * c + 1]), "=r"(w[4 * c + 2]), "=r"(w[4 * c + 3])
-                     : "r"(at + c * 512 + lane * 16)
-                     : "memory");
-    if (N % 4)
-        asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
-                     : "=r"(w[N - 2]), "=r"(w[N - 1])
-                     : "r"(at + N / 4 * 512 + lane * 8)
-                     : "memory");
+    for (int c = 0; c < N / 4; ++c) ka_lds4(p + c * 512 + lane * 16, &w[4 * c]);
+    if (N % 4) ka_lds2(p + N / 4 * 512 + lane * 8, &w[N - 2]);
 }
 // the scales of positions 2 tq, 2 tq + 8, 2 tq + 1, 2 tq + 9: NG = HD / 32 groups each, two to a word
 template <int NG>
-__device__ __forceinline__ void ka_scales(uint32_t at, int tq, uint32_t (&s)[2 * NG]) {
-    const uint32_t p = at + tq * (8 * NG);
-    if (NG % 2 == 0) {
+__device__ __forceinline__ void ka_scales(const uint8_t* p, int tq, uint32_t (&s)[2 * NG]) {
 #pragma unroll
-        for (int i = 0; i < 2 * NG; i += 4)
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                         : "=r"(s[i]), "=r"(s[i + 1]), "=r"(s[(i + 2) % (2 * NG)]), "=r"(s[(i + 3) % (2 * NG)])
-                         : "r"(p + 4 * i)
-                         : "memory");
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2 * NG; i += 2)
-            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(s[i]), "=r"(s[i + 1]) : "r"(p + 4 * i) : "memory");
+    for (int i = 0; i < 2 * NG; i += NG % 2 ? 2 : 4) {
+        if (NG % 2) ka_lds2(p + tq * (8 * NG) + 4 * i, &s[i]);
+        else ka_lds4(p + tq * (8 * NG) + 4 * i, &s[i]);
     }
 }
 // Scale of group k of position 2 tq + e (e = 0, 1) or 2 tq + 8 + e - 2 (e = 2, 3).
@@ -245,9 +235,13 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    const uint32_t ring = smem_u32(smem + warp * (F::ST * F::STAGE));
-    float* slot_all = reinterpret_cast<float*>(smem + KA_WARPS * F::ST * F::STAGE);
-    float* stat = slot_all + KA_WARPS * RT * HD;  // [warp][RT] exponents, then sums
+    const uint8_t* ring_p = smem + warp * (F::ST * F::STAGE);
+    const uint32_t ring = smem_u32(ring_p);
+    uint8_t* qs = smem + KA_WARPS * F::RING;  // [QP][NG][2][lane] four registers
+    const uint8_t* q_at = qs + lane * 16;
+    float* slot_all = reinterpret_cast<float*>(smem);  // where the rings are, once a segment's blocks are done
+    float* stat = reinterpret_cast<float*>(qs + F::QF);  // [warp][RT] exponents, then sums, then q's maxima
+    float* q_max = stat + 2 * KA_WARPS * RT;
     KvqDesc* desc = static_cast<KvqDesc*>(a.ws);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + KA_DESC_BYTES);
 
@@ -299,54 +293,75 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
 #pragma unroll
         for (int i = 0; i < F::ST - 1; ++i) fetch();
 
-        // q as A fragments.  Rows g and g + 8 of M: the tile's rows (MODE 2), or the high and the low half of one.
-        uint32_t qf[QP][NG][8];  // [..][4 u + i]: register i of the product's half u of a group
-        float fr[NR];            // out of q's scale, to powers of two
-        int lim[NR];             // last position that the row sees
+        // q as A fragments in shared memory.  Rows g and g + 8 of M: the tile's rows (MODE 2), or the high and the low
+        // half of one.  Each warp lays out every KA_WARPS-th group.
+        constexpr int NQ = (NG + KA_WARPS - 1) / KA_WARPS;
+        float fr[NR];  // out of q's scale, to powers of two
+        int lim[NR];   // last position that the row sees
+        {
+            float x[NR][NQ][8];
 #pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-            const int row = MODE == 0 ? g & 3 : nr * 8 + g, rr = r0 + row;
-            const bool valid = row < rows;
-            const int t = valid ? rr / pl.rep : 0, h = valid ? kvh * pl.rep + rr - t * pl.rep : 0;
-            const float* qp = a.q + ((long long)b * a.T + t) * a.ld_q + h * HD + tq * 8;
-            float x[NG][8], mx = 0.f;
+            for (int nr = 0; nr < NR; ++nr) {
+                const int row = MODE == 0 ? g & 3 : nr * 8 + g, rr = r0 + row;
+                const bool valid = row < rows;
+                const int t = valid ? rr / pl.rep : 0, h = valid ? kvh * pl.rep + rr - t * pl.rep : 0;
+                const float* qp = a.q + ((long long)b * a.T + t) * a.ld_q + h * HD + tq * 8;
+                float mx = 0.f;
 #pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                const float4 u = valid ? *reinterpret_cast<const float4*>(qp + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-                const float4 v = valid ? *reinterpret_cast<const float4*>(qp + k * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                x[k][0] = u.x; x[k][1] = u.y; x[k][2] = u.z; x[k][3] = u.w;
-                x[k][4] = v.x; x[k][5] = v.y; x[k][6] = v.z; x[k][7] = v.w;
+                for (int i = 0; i < NQ; ++i) {
+                    const int k = i * KA_WARPS + warp;
+                    const bool in = valid && k < NG;
+                    const float4 u = in ? *reinterpret_cast<const float4*>(qp + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    const float4 v = in ? *reinterpret_cast<const float4*>(qp + k * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    float* y = x[nr][i];
+                    y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w;
+                    y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, fabsf(x[k][i]));
+                    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(y[j]));
+                }
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+                if (tq == 0 && row < RT) q_max[warp * RT + row] = mx;
+                lim[nr] = sq.n_ctx + (r0 + row) / pl.rep;
             }
-            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-            // the row's largest value goes to [2^13, 2^14); rows of zeros, subnormals and infinities as they are
-            const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-            const int sh = ex <= -127 || ex == 128 ? 0 : max(-120, min(120, 13 - ex));
-            const float sc = __int_as_float((sh + 127) << 23);
-            fr[nr] = __int_as_float((127 - sh) << 23) * log2e_d;
-            lim[nr] = sq.n_ctx + (r0 + row) / pl.rep;
+            __syncthreads();
 #pragma unroll
-            for (int k = 0; k < NG; ++k)
+            for (int nr = 0; nr < NR; ++nr) {
+                const int row = MODE == 0 ? g & 3 : nr * 8 + g;
+                float mx = q_max[row];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    // codes 4 apart share a register in 4 bits (odd ones times 16), codes 2 apart in 8
-                    const int e0 = BITS == 4 ? i : (i >> 1) * 4 + (i & 1), e1 = BITS == 4 ? i + 4 : e0 + 2;
-                    const float down = BITS == 4 && (i & 1) ? sc * 0.0625f : sc;
-                    const float u = x[k][e0] * down, v = x[k][e1] * down;
-                    const uint32_t hi = ka_pack(u, v);
-                    const float2 f = ka_unpack(hi);
-                    const uint32_t lo = ka_pack(u - f.x, v - f.y);
-                    const int at = (i >> 1) * 4 + (i & 1) * 2;
-                    if (MODE == 2) {
-                        qf[0][k][at + nr] = hi;
-                        qf[QP - 1][k][at + nr] = lo;
-                    } else {
-                        qf[0][k][at] = hi;
-                        qf[0][k][at + 1] = lo;
+                for (int i = 1; i < KA_WARPS; ++i) mx = fmaxf(mx, q_max[i * RT + row]);
+                // the row's largest value goes to [2^13, 2^14); rows of zeros, subnormals and infinities as they are
+                const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+                const int sh = ex <= -127 || ex == 128 ? 0 : max(-120, min(120, 13 - ex));
+                const float sc = __int_as_float((sh + 127) << 23);
+                fr[nr] = __int_as_float((127 - sh) << 23) * log2e_d;
+#pragma unroll
+                for (int i = 0; i < NQ; ++i) {
+                    const int k = i * KA_WARPS + warp;
+                    if (k >= NG) continue;
+                    uint32_t* dst = reinterpret_cast<uint32_t*>(qs + k * 1024 + lane * 16);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        // codes 4 apart share a register in 4 bits (odd ones times 16), codes 2 apart in 8
+                        const int e0 = BITS == 4 ? j : (j >> 1) * 4 + (j & 1), e1 = BITS == 4 ? j + 4 : e0 + 2;
+                        const float down = BITS == 4 && (j & 1) ? sc * 0.0625f : sc;
+                        const float u = x[nr][i][e0] * down, v = x[nr][i][e1] * down;
+                        const uint32_t hi = ka_pack(u, v);
+                        const float2 f = ka_unpack(hi);
+                        const uint32_t lo = ka_pack(u - f.x, v - f.y);
+                        uint32_t* d = dst + (j >> 1) * 128 + (j & 1) * 2;
+                        if (MODE == 2) {
+                            d[nr] = hi;
+                            d[NG * 256 + nr] = lo;
+                        } else {
+                            d[0] = hi;
+                            d[1] = lo;
+                        }
                     }
                 }
+            }
+            __syncthreads();
         }
         const int open_to = sq.n_ctx + r0 / pl.rep;  // every row sees the positions up to here
 
@@ -366,8 +381,8 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             top[nr] = 0;
         }
 
-        // One block at shared address `at`, from position p0 on.
-        auto block = [&](auto masked_c, const uint32_t at, const int p0) {
+        // One block at `at`, from position p0 on.
+        auto block = [&](auto masked_c, const uint8_t* at, const int p0) {
             constexpr bool MASKED = decltype(masked_c)::value;
             // scores of row g (and g + 8) against positions 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9
             float2 x[NR][2];
@@ -378,9 +393,15 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                 ka_words<W>(at, lane, w);
                 ka_scales<NG>(at + CODES, tq, s);
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int k = 0; k < NG; ++k) {
+                    uint32_t qf[QP][2][4];
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) {
+                    for (int part = 0; part < QP; ++part) {
+                        ka_lds4(q_at + (part * NG + k) * 1024, qf[part][0]);
+                        ka_lds4(q_at + (part * NG + k) * 1024 + 512, qf[part][1]);
+                    }
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
                         uint32_t f[4];
                         if (BITS == 4) {
                             ka_nibbles(w[half * (W / 2) + k], magic, f);
@@ -391,20 +412,21 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                         float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int part = QP - 1; part >= 0; --part) {  // the low halves first
-                            ka_mma(c, reinterpret_cast<const uint32_t(&)[4]>(qf[part][k][0]), f[0], f[1]);
-                            ka_mma(c, reinterpret_cast<const uint32_t(&)[4]>(qf[part][k][4]), f[2], f[3]);
+                            ka_mma(c, qf[part][0], f[0], f[1]);
+                            ka_mma(c, qf[part][1], f[2], f[3]);
                         }
                         const float2 sc = make_float2(ka_scale(s, half * 2, k), ka_scale(s, half * 2 + 1, k));
                         x[NR - 1][half] = ka_fma2(make_float2(c[2], c[3]), sc, x[NR - 1][half]);
                         x[0][half] = ka_fma2(make_float2(c[0], c[1]), sc, x[0][half]);
                     }
+                }
             }
             uint32_t vs[2 * NG];
             ka_scales<NG>(at + F::BLOCK + CODES, tq, vs);
             auto seen = [&](int nr, int e) { return !MASKED || p0 + 2 * tq + (e & 1) + (e >> 1) * 8 <= lim[nr]; };
             bool raise;
             {  // a lane looks at one word of V's scales
-                const uint32_t word = ka_lds(at + F::BLOCK + CODES + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
+                const uint32_t word = *reinterpret_cast<const uint32_t*>(at + F::BLOCK + CODES + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
                 raise = (word & 0xFFFFu) > top_all || word >> 16 > top_all;
             }
 #pragma unroll
@@ -509,7 +531,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             }
         };
 
-        uint32_t at = ring;
+        const uint8_t* at = ring_p;
         int p0 = (blk0 + warp) * 16;
 #pragma unroll 1
         for (int i = 0; i < n_mine; ++i) {
@@ -519,12 +541,12 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             if (p0 + 15 <= open_to) block(std::false_type(), at, p0);
             else block(std::true_type(), at, p0);
             p0 += KA_WARPS * 16;
-            at = at + F::STAGE >= ring + F::ST * F::STAGE ? ring : at + F::STAGE;
+            at = at + F::STAGE >= ring_p + F::ST * F::STAGE ? ring_p : at + F::STAGE;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
+        __syncthreads();
         // the warp's rows into its slot: dims 16 d + 2 g and one on, rows 2 tq and one on
-        __syncthreads();  // the slots of the segment before are read
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -584,6 +606,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                 }
             }
         }
+        __syncthreads();
         if (begins && !ends) open = KvqDesc{b, kvh, tile | rows << 16, (ub + sq.blocks - 1) / range.per};
     }
     if (threadIdx.x == 0) desc[blockIdx.x] = open;
@@ -655,13 +678,13 @@ static int kvq_sms() {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms < 1 ? 1 : (2 * sms > KA_MAX_GRID ? KA_MAX_GRID / 2 : sms);
+    return sms < 1 ? 1 : (5 * sms > KA_MAX_GRID ? KA_MAX_GRID / 5 : sms);
 }
 static int kvq_mode(int rows) { return rows <= 4 ? 0 : rows <= 8 ? 1 : 2; }
 
 size_t kvq_attn_ws_bytes(int T, int n_head, int n_kv, int hd) {
     const int mode = kvq_mode(T * (n_head / n_kv));
-    return KA_DESC_BYTES + (size_t)kvq_sms() * (mode == 2 ? 1 : 2) * 2 * kvq_part_floats(kvq_rt(mode), hd) * sizeof(float);
+    return KA_DESC_BYTES + (size_t)kvq_sms() * kvq_ctas(mode) * 2 * kvq_part_floats(kvq_rt(mode), hd) * sizeof(float);
 }
 
 // Units of 4 rows or more, blocks of 16 positions and a unit's cost.
