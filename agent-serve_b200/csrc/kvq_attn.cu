@@ -36,17 +36,21 @@ namespace tfb {
 constexpr int KA_THREADS = 128;
 constexpr int KA_WARPS = KA_THREADS / 32;
 constexpr int KA_UNIT_COST = 8;    // blocks that a unit's start and end take the time of
+constexpr int KA_MIN_RANGE = 16;   // blocks of a CTA's range at least
+constexpr int KA_SNAP = 6;         // a cut this near to a unit's first or last block moves there
 constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
-constexpr int KA_MAX_GRID = 1024;  // descriptors of 16 bytes in the workspace's first 16 KB
-constexpr size_t KA_DESC_BYTES = 16384;
+constexpr int KA_MAX_GRID = 1024;  // descriptors of 32 bytes in the workspace's first 32 KB
+constexpr size_t KA_DESC_BYTES = 32768;
 
 struct KvqPlan {
     int grid;
     int rt;        // rows per row tile
     int rep;       // query heads per kv head
+    int tiles;     // row tiles of T rows
+    int by_unit;   // descriptors are found by unit (there are at most `grid`), else by the CTA that begins it
 };
-struct KvqDesc {   // a unit split over CTAs c0 .. c1, found at slot c0
-    int b, kvh, tile, c1;  // b < 0: none; tile: row tile, and its rows in the high half
+struct alignas(32) KvqDesc {  // a unit split over CTAs c0 .. c1
+    int b, kvh, tile, rows, c0, c1;  // b < 0: no unit, or one that was not split
 };
 
 __host__ __device__ inline size_t kvq_part_floats(int rt, int hd) { return (size_t)rt * (hd + 2); }
@@ -192,7 +196,12 @@ __device__ __forceinline__ KvqSeq kvq_seq(const KvqAttnArgs& a, const KvqPlan& p
 }
 __device__ __forceinline__ int kvq_len(const KvqSeq& s) { return s.n_new ? s.units * (s.blocks + KA_UNIT_COST) : 0; }
 
-// A CTA's range [g0, g1) of the flattened blocks: `b` is the sequence it begins in, `base` that one's start.
+// Where the cut at offset t of a unit of n blocks falls: near a unit's ends it would cost a partial result for
+// next to nothing.
+__device__ __forceinline__ int kvq_cut(int t, int n) { return t < KA_SNAP ? 0 : n - t < KA_SNAP ? max(t, n) : t; }
+
+// A CTA's range [g0, g1) of the flattened blocks, before its ends are moved (kvq_cut): `b` is the sequence it
+// begins in, `base` that one's start.
 struct KvqRange {
     int g0, g1, per, b, base;
 };
@@ -214,7 +223,7 @@ __device__ __forceinline__ KvqRange kvq_range(const KvqAttnArgs& a, const KvqPla
     }
     const int total = __shfl_sync(0xFFFFFFFFu, inc, 31);
     KvqRange r;
-    r.per = max(1, (int)(((unsigned)total + pl.grid - 1) / pl.grid));
+    r.per = max(KA_MIN_RANGE, (int)(((unsigned)total + pl.grid - 1) / pl.grid));
     r.g0 = (int)min((long long)total, (long long)blockIdx.x * r.per);
     r.g1 = min(total, r.g0 + min(r.per, total - r.g0));
     const unsigned at = __ballot_sync(0xFFFFFFFFu, r.g0 >= inc - mine && r.g0 < inc);
@@ -246,7 +255,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + KA_DESC_BYTES);
 
     const KvqRange range = kvq_range(a, pl);
-    KvqDesc open = {-1, 0, 0, 0};  // the unit that begins here and ends in a later CTA
+    KvqDesc open = {-1, 0, 0, 0, 0, 0};  // the unit that begins here and ends in a later CTA
     int b = range.b, base = range.base;
     const float log2e_d = 1.4426950408889634f * rsqrtf((float)HD);
     uint32_t magic;
@@ -263,7 +272,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
         }
         if (gpos >= base + len) break;
         const int per_unit = sq.blocks + KA_UNIT_COST, unit = (gpos - base) / per_unit, ub = base + unit * per_unit;
-        const int blk0 = gpos - ub, blk1 = min(sq.blocks, range.g1 - ub);
+        const int blk0 = kvq_cut(gpos - ub, sq.blocks), blk1 = min(sq.blocks, range.g1 - ub < per_unit ? kvq_cut(range.g1 - ub, sq.blocks) : per_unit);
         gpos = min(range.g1, ub + per_unit);
         if (blk0 >= blk1) continue;
         const int tiles = sq.units / a.n_kv, kvh = unit / tiles, tile = unit - kvh * tiles;
@@ -607,9 +616,15 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             }
         }
         __syncthreads();
-        if (begins && !ends) open = KvqDesc{b, kvh, tile | rows << 16, (ub + sq.blocks - 1) / range.per};
+        if (begins) {
+            const int last = (ub + sq.blocks - 1) / range.per;  // the CTA with the last block, if its cut stays
+            const int c1 = kvq_cut(last * range.per - ub, sq.blocks) >= sq.blocks ? last - 1 : last;
+            const KvqDesc de = {ends ? -1 : b, kvh, tile, rows, (int)blockIdx.x, c1};
+            if (!ends) open = de;
+            if (pl.by_unit && threadIdx.x == 0) desc[(b * a.n_kv + kvh) * pl.tiles + tile] = de;
+        }
     }
-    if (threadIdx.x == 0) desc[blockIdx.x] = open;
+    if (!pl.by_unit && threadIdx.x == 0) desc[blockIdx.x] = open;
 
     // rows behind a sequence's new ones, and rows of a sequence that was refused, are zero
     for (int s = blockIdx.x; s < a.B; s += pl.grid) {
@@ -622,40 +637,54 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
 }
 
 // ---- joins the partial results of units that were split over CTAs ------------------------------------
-// Block (c, y): the unit that begins in CTA c's range and ends in a later one; a warp per row.
-constexpr int KC_WARPS = 4;
-__global__ void __launch_bounds__(KC_WARPS * 32) tf_kvq_combine_kernel(const KvqAttnArgs a, const KvqPlan pl) {
+// Block (x, y): descriptor x, rows y ROWS on; WAYS warps per row share its parts, a lane per part for the weights
+// and per four dims for the sums, eight parts' rows in flight.
+template <int ROWS, int WAYS>
+__global__ void __launch_bounds__(ROWS * WAYS * 32) tf_kvq_combine_kernel(const KvqAttnArgs a, const KvqPlan pl) {
+    __shared__ float4 sum[ROWS][WAYS][32];
+    __shared__ float2 stat[ROWS][WAYS];
     pdl_wait();
-    const int c0 = blockIdx.x, lane = threadIdx.x & 31, r = blockIdx.y * KC_WARPS + (threadIdx.x >> 5);
-    const KvqDesc de = static_cast<const KvqDesc*>(a.ws)[c0];
-    if (de.b < 0 || r >= de.tile >> 16) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lr = warp / WAYS, way = warp % WAYS, r = blockIdx.y * ROWS + lr;
+    if (pl.by_unit) {  // a unit that does not exist has no descriptor
+        const KvqSeq sq = kvq_seq(a, pl, blockIdx.x / (a.n_kv * pl.tiles));
+        if ((int)(blockIdx.x % pl.tiles) * a.n_kv >= sq.units) return;
+    }
+    const KvqDesc de = static_cast<const KvqDesc*>(a.ws)[blockIdx.x];
+    if (de.b < 0 || (int)blockIdx.y * ROWS >= de.rows) return;
     const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + KA_DESC_BYTES);
-    const int hd = a.hd, rt = pl.rt, n = de.c1 - c0 + 1, d = lane * 4;
+    const int hd = a.hd, rt = pl.rt, n = de.c1 - de.c0 + 1, d = lane * 4;
     const size_t pf = kvq_part_floats(rt, hd);
-    auto part = [&](int i) { return parts + ((size_t)(c0 + i) * 2 + (i == 0 ? 1 : 0)) * pf; };
+    auto part = [&](int i) { return parts + ((size_t)(de.c0 + i) * 2 + (i == 0 ? 1 : 0)) * pf; };
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    // this warp's parts: way, way + WAYS, ...; 32 of them at a time
+    const int mine = r < de.rows ? (n - way + WAYS - 1) / WAYS : 0;
 #pragma unroll 1
-    for (int i0 = 0; i0 < n; i0 += 32) {  // 32 parts at a time, eight parts' rows in flight
-        const int k = min(32, n - i0);
+    for (int i0 = 0; i0 < mine; i0 += 32) {
+        const int k = min(32, mine - i0);
+        auto at = [&](int i) { return part((i0 + i) * WAYS + way); };
         float m = -INFINITY, l = 0.f;
         if (lane < k) {
-            const float* p = part(i0 + lane) + (size_t)rt * hd + r;
+            const float* p = at(lane) + (size_t)rt * hd + r;
             m = p[0];
             l = p[rt];
         }
-        const float mx = fmaxf(M, warp_max(m)), at = mx == -INFINITY ? 0.f : mx;
-        const float alpha = ka_exp2(M - at), w = m == -INFINITY ? 0.f : ka_exp2(m - at);
-        M = mx;
-        L = fmaf(L, alpha, warp_sum(m == -INFINITY ? 0.f : l * w));
-        o = make_float4(o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha);
+        float w = 0.f;
 #pragma unroll 1
         for (int i = 0; i < k; i += 8) {
             float4 x[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                x[j] = i + j < k && d < hd ? *reinterpret_cast<const float4*>(part(i0 + i + j) + (size_t)r * hd + d)
+                x[j] = i + j < k && d < hd ? *reinterpret_cast<const float4*>(at(i + j) + (size_t)r * hd + d)
                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+            if (i == 0) {
+                const float mx = fmaxf(M, warp_max(m)), to = mx == -INFINITY ? 0.f : mx, alpha = ka_exp2(M - to);
+                w = m == -INFINITY ? 0.f : ka_exp2(m - to);
+                M = mx;
+                L = fmaf(L, alpha, warp_sum(m == -INFINITY ? 0.f : l * w));
+                o = make_float4(o.x * alpha, o.y * alpha, o.z * alpha, o.w * alpha);
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float wi = __shfl_sync(0xFFFFFFFFu, w, i + j);
@@ -666,8 +695,30 @@ __global__ void __launch_bounds__(KC_WARPS * 32) tf_kvq_combine_kernel(const Kvq
             }
         }
     }
-    if (d >= hd) return;
-    const int rep = pl.rep, rr = (de.tile & 0xFFFF) * rt + r, t = rr / rep, h = de.kvh * rep + rr - t * rep;
+    if (WAYS > 1) {
+        sum[lr][way][lane] = o;
+        if (lane == 0) stat[lr][way] = make_float2(M, L);
+        __syncthreads();
+        if (way != 0) return;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < WAYS; ++i) mx = fmaxf(mx, stat[lr][i].x);
+        L = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < WAYS; ++i) {
+            if (stat[lr][i].x == -INFINITY) continue;
+            const float f = ka_exp2(stat[lr][i].x - mx);
+            const float4 u = sum[lr][i][lane];
+            L = fmaf(stat[lr][i].y, f, L);
+            o.x = fmaf(u.x, f, o.x);
+            o.y = fmaf(u.y, f, o.y);
+            o.z = fmaf(u.z, f, o.z);
+            o.w = fmaf(u.w, f, o.w);
+        }
+    }
+    if (r >= de.rows || d >= hd) return;
+    const int rep = pl.rep, rr = de.tile * rt + r, t = rr / rep, h = de.kvh * rep + rr - t * rep;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     *reinterpret_cast<float4*>(a.out + ((long long)de.b * a.T + t) * a.ld_out + h * hd + d) =
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -726,11 +777,17 @@ static cudaError_t mode_launch(const KvqAttnArgs& a, cudaStream_t st) {
     pl.grid = kvq_sms() * F::CTAS;
     pl.rt = F::RT;
     pl.rep = a.n_head / a.n_kv;
+    pl.tiles = (a.T * pl.rep + F::RT - 1) / F::RT;
+    const long long units = (long long)a.B * a.n_kv * pl.tiles;
+    pl.by_unit = units <= pl.grid;
     KvqAttnArgs aa = a;
     void* args[] = {&aa, &pl};
     cudaError_t e = kvq_launch(fn, dim3(pl.grid), KA_THREADS, F::SMEM, args, st, false);
     if (e != cudaSuccess) return e;
-    return kvq_launch((const void*)tf_kvq_combine_kernel, dim3(pl.grid, F::RT / KC_WARPS), KC_WARPS * 32, 0, args, st, true);
+    const int found = pl.by_unit ? (int)units : pl.grid;
+    // few units have many parts each: eight warps to a row
+    if (found * F::RT <= 1024) return kvq_launch((const void*)tf_kvq_combine_kernel<1, 8>, dim3(found, F::RT), 256, 0, args, st, true);
+    return kvq_launch((const void*)tf_kvq_combine_kernel<4, 1>, dim3(found, F::RT / 4), 128, 0, args, st, true);
 }
 template <int BITS, int HD>
 static cudaError_t hd_launch(const KvqAttnArgs& a, cudaStream_t st) {
