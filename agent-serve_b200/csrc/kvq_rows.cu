@@ -4,16 +4,22 @@
 //   norm    y = (x inv) w, inv = 1 / sqrt(mean x^2 + eps), the mean in 64 bits (the row norm's own order)
 //   rotate  pairs (j, j + rot / 2): (a, b) -> (a c - b s, a s + b c), c and s the cosine and sine of
 //           pos freq[j].  The angle is a product in 64 bits: in fp32 a far position's angle is off by
-//           2^-24 of itself, 0.004 at 65536.  The two products are summed in 64 bits and rounded once, so that a
-//           key next to the border of two codes takes the same code wherever it is computed.
+//           2^-24 of itself, 0.004 at 65536.  Queries: a product and an fma.  Keys: the two products and their
+//           sum are carried with their rounding errors (Dekker's product by fma, Knuth's sum) and rounded once, so
+//           that a key next to the border of two codes takes the same code wherever it is computed.  (In 64 bits:
+//           12 conversions a vector through a pipe of 4 lanes a cycle; 9001 rows of 32 + 8 heads of 128, 135 us.)
 //   Q4_0    scale = f16(m / -8), m the group's first value of largest magnitude; code = rint(x / scale) in [-8, 7]
 //   Q8_0    scale = f16(max|x| r), r = 1 / 127 in fp32; code = rint(x / scale) in [-127, 127]
-// (x / scale is IEEE's quotient: none rounds to a half that it is not, since a half times an f16 scale
-// fits 19 bits.)  A group with an infinity or NaN gets a NaN for its scale and reads back as NaN; a
-// scale beyond f16 is held at 65504, and a zero scale reads back as zeros.
+// A group with an infinity or NaN gets a NaN for its scale and reads back as NaN; a scale beyond f16 is held at
+// 65504, and a zero scale reads back as zeros.
 //
 // One warp per row and share of its heads; 8, 16 or 32 lanes per head, four dims each, so that a group of
-// 32 is eight lanes.
+// 32 is eight lanes.  A word of V's codes holds four positions of a block (a "quad": 2 t, 2 t + 8, 2 t + 1,
+// 2 t + 9), so values are taken four rows at a time: neighbouring rows of the call that lie in one block at
+// rising positions (a run) share their quads out over the run's warps.  Row by row, the bytes of a head's V
+// touch 16 lines an instruction.
+#include <type_traits>
+
 #include "kvq.cuh"
 
 namespace tfb {
@@ -21,175 +27,372 @@ namespace tfb {
 constexpr int KR_THREADS = 256;
 constexpr int KR_VEC = 4;  // vectors of a warp in flight
 
-__device__ __forceinline__ int kvq_slot(const int* slots, int row) { return slots ? slots[row] : row; }
+__device__ __forceinline__ float2 kr_mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 kr_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "add.rn.f32x2 rd, ra, rb;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 kr_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+// y c + m s, rounded once (but for cases within 2^-46 of a tie)
+__device__ __forceinline__ float2 kr_turn(float2 y, float2 c, float2 m, float2 s) {
+    const float2 m1 = make_float2(-1.f, -1.f);
+    const float2 p = kr_mul2(y, c), np = kr_mul2(p, m1), q = kr_mul2(m, s), nq = kr_mul2(q, m1);
+    const float2 e = kr_add2(kr_fma2(y, c, np), kr_fma2(m, s, nq));  // what the products' roundings left out
+    const float2 t = kr_add2(p, q), b = kr_add2(t, np), z = kr_fma2(b, m1, t);
+    const float2 et = kr_add2(kr_fma2(z, m1, p), kr_fma2(b, m1, q));  // p + q = t + et
+    return kr_add2(t, kr_add2(e, et));
+}
+__device__ __forceinline__ float kr_max_nan(float a, float b) {  // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 
-// Codes and scale of a group of 32 over eight neighbouring lanes, four values each.
+// Codes and scale of a group of 32 over eight neighbouring lanes, four values each.  A code is the low 16 bits of
+// code[i]; above them lies what packing drops.
+//
+// rint(x / scale) without a quotient: rint of the product with the reciprocal is right unless the product is
+// next to a half; there (one vector in 500 of random values) the remainder x - q scale, which is exact, says which
+// integer is nearest.  Adding 1.5 2^23 rounds to an integer, ties to even, in the low bits.
 template <int BITS>
-__device__ __forceinline__ void quantise(const float4& x, int lane, int (&code)[4], __half& scale) {
+__device__ __forceinline__ void quantise(const float4& x, int lane, uint32_t (&code)[4], __half& scale) {
+    constexpr float LO = BITS == 4 ? -8.0f : -127.0f, HI = BITS == 4 ? 7.0f : 127.0f, Z = BITS == 4 ? 8.0f : 128.0f;
+    constexpr float M = 12582912.0f + Z;
     const float v[4] = {x.x, x.y, x.z, x.w};
-    unsigned top = 0;
+    const float mine = kr_max_nan(kr_max_nan(fabsf(v[0]), fabsf(v[1])), kr_max_nan(fabsf(v[2]), fabsf(v[3])));
+    float top = mine;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-    const unsigned mine = top;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+    for (int o = 1; o < 8; o <<= 1) top = kr_max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
     float d;
     if (BITS == 4) {
         float m = v[3];
 #pragma unroll
         for (int i = 2; i >= 0; --i)
-            if ((__float_as_uint(v[i]) & 0x7FFFFFFFu) == top) m = v[i];
+            if (fabsf(v[i]) == top) m = v[i];
         const unsigned has = __ballot_sync(0xFFFFFFFFu, mine == top) >> (lane & 24) & 0xFFu;
-        m = __shfl_sync(0xFFFFFFFFu, m, (lane & 24) + __ffs(has) - 1);
+        m = __shfl_sync(0xFFFFFFFFu, m, (lane & 24) + __ffs(has) - 1);  // (NaN: no lane has it, any will do)
         d = __fmul_rn(m, -0.125f);
     } else {
-        d = __fmul_rn(__uint_as_float(top), 1.0f / 127.0f);
+        d = __fmul_rn(top, 1.0f / 127.0f);
     }
-    const bool bad = top >= 0x7F800000u;
+    const bool bad = !(top < INFINITY);
     scale = bad ? __ushort_as_half(0x7FFF) : __float2half_rn(fminf(fmaxf(d, -65504.0f), 65504.0f));
-    const float s = __half2float(scale);
-    const float lo = BITS == 4 ? -8.0f : -127.0f, hi = BITS == 4 ? 7.0f : 127.0f;
+    const float s = __half2float(scale), inv = s == 0.0f ? 0.0f : __frcp_rn(s);
+    bool doubt = bad;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        code[i] = (bad || s == 0.0f ? 0 : (int)fminf(fmaxf(rintf(__fdiv_rn(v[i], s)), lo), hi)) + (BITS == 4 ? 8 : 128);
+    for (int i = 0; i < 4; ++i) {
+        const float r = fminf(fmaxf(__fmul_rn(v[i], inv), LO), HI);
+        const float t = __fadd_rn(r, M);
+        doubt |= fabsf(__fadd_rn(r, -__fadd_rn(t, -M))) > 0.49999f;
+        code[i] = __float_as_uint(t);
+    }
+    if (__any_sync(0xFFFFFFFFu, doubt)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float r = fminf(fmaxf(__fmul_rn(v[i], inv), LO), HI);
+            const float q = __fadd_rn(__fadd_rn(r, M), -M), e = __fmaf_rn(-q, s, v[i]), e2 = fabsf(e + e);
+            const bool next = e2 > fabsf(s) || (e2 == fabsf(s) && ((int)q & 1));
+            const float to = next ? (__float_as_int(e) ^ __float_as_int(s)) < 0 ? q - 1.0f : q + 1.0f : q;
+            code[i] = __float_as_uint((bad || s == 0.0f ? 0.0f : fminf(fmaxf(to, LO), HI)) + M);
+        }
+    }
+}
+// four codes of 8 bits to a word
+__device__ __forceinline__ uint32_t kr_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
 // Four dims 4 hl .. 4 hl + 3 of position p of a block.
 template <int BITS>
-__device__ __forceinline__ void store_k(uint8_t* blk, int hd, int p, int hl, const int (&c)[4]) {
+__device__ __forceinline__ int k_place(int hd, int p, int hl) {
     const int half = p >> 3, lane = (p & 7) * 4 + (hl >> 1 & 3), words = hd * BITS / 64, grp = hl >> 3;
-    if (BITS == 4)
-        *reinterpret_cast<uint16_t*>(blk + kvq_word(words, half * (hd >> 5) + grp, lane) + (hl & 1) * 2) =
-            (uint16_t)(c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12);
-    else
-        *reinterpret_cast<uint32_t*>(blk + kvq_word(words, half * (hd >> 4) + grp * 2 + (hl & 1), lane)) =
-            (uint32_t)c[0] | (uint32_t)c[1] << 8 | (uint32_t)c[2] << 16 | (uint32_t)c[3] << 24;
+    return BITS == 4 ? kvq_word(words, half * (hd >> 5) + grp, lane) + (hl & 1) * 2
+                     : kvq_word(words, half * (hd >> 4) + grp * 2 + (hl & 1), lane);
 }
+// The words of quad t that hold dims 4 hl and 4 hl + 1 (Q8_0: the second 4 bytes on); those of dims 4 hl + 2 and
+// 4 hl + 3 lie *next bytes on.
 template <int BITS>
-__device__ __forceinline__ void store_v(uint8_t* blk, int hd, int p, int hl, const int (&c)[4]) {
-    const int words = hd * BITS / 64, byte = (p & 1) * 2 + (p >> 3), tile = hl >> 2;
-    const int lane = (hl & 3) * 8 + ((p & 7) >> 1);  // of dims 0 and 1; dims 2 and 3: four lanes on
-    if (BITS == 4) {
-        uint8_t* w = blk + kvq_word(words, tile, lane) + byte;
-        const int next = tile < (words & ~3) ? 64 : 32;
-        w[0] = (uint8_t)(c[0] | c[1] << 4);
-        w[next] = (uint8_t)(c[2] | c[3] << 4);
-    } else {
-        uint8_t* w = blk + kvq_word(words, tile * 2, lane) + byte;
-        w[0] = (uint8_t)c[0];
-        w[4] = (uint8_t)c[1];
-        w[64] = (uint8_t)c[2];
-        w[68] = (uint8_t)c[3];
-    }
+__device__ __forceinline__ int v_place(int hd, int t, int hl, int* next) {
+    const int words = hd * BITS / 64, tile = hl >> 2;
+    *next = BITS == 8 || tile < (words & ~3) ? 64 : 32;
+    return kvq_word(words, BITS == 4 ? tile : tile * 2, (hl & 3) * 8 + t);
+}
+__device__ __forceinline__ int scale_place(int bits, int hd, int p, int grp) {
+    return kvq_code_bytes(bits, hd) + 2 * (((p & 7) * 2 + (p >> 3)) * (hd >> 5) + grp);
 }
 
-// LH lanes per head.  A warp takes vectors (32 / LH heads) first, first + split, ... of its row's
-// n_head + 2 n_kv heads.
-template <int LH, int BITS>
-__global__ void __launch_bounds__(KR_THREADS) tf_kvq_rows_kernel(const KvqRowsArgs a, int split) {
+// Which rows share a block with a warp's own: the run's first row, its length, this row's index in it, and the
+// block's positions that it holds (rows in rising order of position).
+struct Run {
+    int first, len, index;
+    unsigned mask;
+    __device__ __forceinline__ int row(int p) const {  // the row of position p of the block, or -1
+        return mask >> p & 1 ? first + __popc(mask & ((1u << p) - 1)) : -1;
+    }
+    __device__ __forceinline__ int quads() const {  // bit t: quad t holds a row
+        const unsigned m = mask | mask >> 8;
+        return (m & 3 ? 1 : 0) | (m & 12 ? 2 : 0) | (m & 48 ? 4 : 0) | (m & 192 ? 8 : 0);
+    }
+};
+// The n-th quad of a set.
+__device__ __forceinline__ int nth_quad(unsigned quads, int n) {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        if (i < n) quads &= quads - 1;
+    return __ffs(quads) - 1;
+}
+// Position of byte i of a quad's words.
+__device__ __forceinline__ int quad_pos(int t, int i) { return 2 * t + (i >> 1) + (i & 1) * 8; }
+
+template <class A>
+__device__ __forceinline__ int row_slot(const A& a, int row) { return a.slots ? a.slots[row] : row; }
+
+// The run of `row`, which lies in the cache.  A warp looks 15 rows back and 16 on.
+template <class A>
+__device__ __forceinline__ Run find_run(const A& a, int row) {
+    const int lane = threadIdx.x & 31, q = row - 15 + lane;
+    int slot = -1, pos = -1;
+    if (q >= 0 && q < a.rows) {
+        slot = row_slot(a, q);
+        pos = a.pos[q];
+    }
+    const int slot0 = __shfl_up_sync(0xFFFFFFFFu, slot, 1), pos0 = __shfl_up_sync(0xFFFFFFFFu, pos, 1);
+    const bool on = lane > 0 && slot >= 0 && slot == slot0 && pos0 >= 0 && pos > pos0 && pos >> 4 == pos0 >> 4;
+    const unsigned c = __ballot_sync(0xFFFFFFFFu, on);  // rows that go on with the run of the row before
+    const int back = __clz(~(c << 16)), ahead = __ffs(~(c >> 16)) - 1;
+    Run r;
+    r.first = row - back;
+    r.len = back + 1 + ahead;
+    r.index = back;
+    const bool in = lane >= 15 - back && lane <= 15 + ahead;
+    r.mask = __reduce_or_sync(0xFFFFFFFFu, in ? 1u << (pos & 15) : 0u);
+    return r;
+}
+
+// LH lanes per head.  A row has `split` warps for its queries and keys (vectors of 32 / LH heads: first, first +
+// split, ...) and `vsplit` for its share of the run's values.
+// TURN: with a rotation.
+template <int LH, int BITS, bool TURN>
+__global__ void __launch_bounds__(KR_THREADS, TURN ? 4 : 5) tf_kvq_rows_kernel(const KvqRowsArgs a, int split, int vsplit) {
     constexpr int HPW = 32 / LH;
-    const int lane = threadIdx.x & 31, hl = lane & (LH - 1);
-    const long long task = ((long long)blockIdx.x * KR_THREADS + threadIdx.x) >> 5;
-    const int row = (int)(task / split), first = (int)(task - (long long)row * split);
-    if (row >= a.rows) return;
+    const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
+    const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
+    const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
+    if ((unsigned)row >= (unsigned)a.rows) return;
     const int pos = a.pos ? a.pos[row] : 0;
-    uint8_t *kblk = nullptr, *vblk = nullptr;
+    long long off = 0;
     if (a.kc) {
-        const int slot = kvq_slot(a.slots, row);
+        const int slot = row_slot(a, row);
         if (slot < 0) return;
         if (slot >= a.n_slots || pos < 0 || pos >= a.cap) {
             if (first == 0 && lane == 0) atomicCAS(a.err, 0, slot >= a.n_slots ? ERR_BAD_TOKEN : ERR_POS);
             return;
         }
-        const long long off = slot * a.slot_bytes + (long long)(pos >> 4) * kvq_block_bytes(BITS, a.hd);
-        kblk = a.kc + off;
-        vblk = a.vc + off;
+        off = slot * a.slot_bytes + (long long)(pos >> 4) * kvq_block_bytes(BITS, a.hd);
     } else if (pos < 0) {
         return;
     }
-    const int nq = a.q ? a.n_head : 0, nk = nq + (a.k ? a.n_kv : 0), nv = nk + (a.v ? a.n_kv : 0);
     const int d0 = hl * 4, half = a.rot >> 1;
-    const bool live = d0 < a.hd, turn = a.freq && d0 < a.rot;
-    // cosines and sines of the lane's four dims; the second half's sign
-    double c[4], s[4];
-    int mate = lane;
-    if (turn) {
-        const int j0 = d0 < half ? d0 : d0 - half;
-        mate = d0 < half ? lane + (half >> 2) : lane - (half >> 2);
+    const bool live = d0 < a.hd;
+    if (first < split) {
+        // cosines and sines of the row's angles (a lane computes one or two), then of the lane's four dims
+        const bool turn = TURN && d0 < a.rot;
+        float4 c = make_float4(0.f, 0.f, 0.f, 0.f), s = c;
+        int mate = lane;
+        if (TURN) {
+            float cs[2] = {0.f, 0.f}, sn[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            double sn, cs;
-            sincos((double)pos * (double)a.freq[j0 + i], &sn, &cs);
-            c[i] = (double)(float)cs;
-            s[i] = d0 < half ? -(double)(float)sn : (double)(float)sn;
+            for (int i = 0; i < 2; ++i)
+                if (lane + 32 * i < half) {
+                    double u, v;
+                    sincos((double)pos * (double)a.freq[lane + 32 * i], &u, &v);
+                    sn[i] = (float)u;
+                    cs[i] = (float)v;
+                }
+            const bool upper = d0 >= half;  // the pair's second element
+            const int j0 = turn ? (upper ? d0 - half : d0) : 0, from = j0 & 31;
+            float t[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                t[i] = __shfl_sync(0xFFFFFFFFu, cs[0], from + i);
+                t[4 + i] = __shfl_sync(0xFFFFFFFFu, sn[0], from + i);
+                if (half > 32) {
+                    const float c1 = __shfl_sync(0xFFFFFFFFu, cs[1], from + i), s1 = __shfl_sync(0xFFFFFFFFu, sn[1], from + i);
+                    if (j0 >= 32) {
+                        t[i] = c1;
+                        t[4 + i] = s1;
+                    }
+                }
+                if (!upper) t[4 + i] = -t[4 + i];
+            }
+            c = make_float4(t[0], t[1], t[2], t[3]);
+            s = make_float4(t[4], t[5], t[6], t[7]);
+            if (turn) mate = upper ? lane - (half >> 2) : lane + (half >> 2);
         }
+        const double inv_n = 1.0 / a.hd;
+        // Vectors of one kind: the warp's, of `heads` heads from `in` on (its dims), to `out` and to the cache (`blk`)
+        auto vectors_of = [&](auto is_k, const float* in, float* out, int heads, const float* weight, uint8_t* blk, int begin) {
+            constexpr bool IS_K = decltype(is_k)::value;
+            float4 w = make_float4(1.f, 1.f, 1.f, 1.f);
+            if (weight && live) w = *reinterpret_cast<const float4*>(weight + d0);
+            const int step = split * HPW;
+            int h = begin * HPW + sub;
+            const int kat = k_place<BITS>(a.hd, pos & 15, hl), sat = scale_place(BITS, a.hd, pos & 15, hl >> 3);
+            for (int left = (heads + HPW - 1) / HPW - begin; left > 0; left -= split * KR_VEC, h += step * KR_VEC) {
+                float4 x[KR_VEC];
+#pragma unroll
+                for (int u = 0; u < KR_VEC; ++u) {
+                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (h + u * step < heads && live) x[u] = *reinterpret_cast<const float4*>(in + (h + u * step) * a.hd);
+                }
+                // The squares of the four vectors are summed together: at each of the first two steps a lane hands on
+                // the half of its sums that its partner keeps, so that a lane ends with the sum of one of them.
+                float inv = 1.0f;
+                if (weight) {
+                    double ss[KR_VEC];
+#pragma unroll
+                    for (int u = 0; u < KR_VEC; ++u) {
+                        const float4 y = x[u];
+                        ss[u] = fma((double)y.x, (double)y.x,
+                                    fma((double)y.y, (double)y.y, fma((double)y.z, (double)y.z, (double)y.w * (double)y.w)));
+                    }
+                    const bool hi = lane & LH / 2, odd = lane & LH / 4;
+                    const double e0 = hi ? ss[0] : ss[2], e1 = hi ? ss[1] : ss[3];
+                    const double k0 = (hi ? ss[2] : ss[0]) + __shfl_xor_sync(0xFFFFFFFFu, e0, LH / 2);
+                    const double k1 = (hi ? ss[3] : ss[1]) + __shfl_xor_sync(0xFFFFFFFFu, e1, LH / 2);
+                    double sum = (odd ? k1 : k0) + __shfl_xor_sync(0xFFFFFFFFu, odd ? k0 : k1, LH / 4);
+#pragma unroll
+                    for (int o = LH / 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+                    inv = __fdiv_rn(1.0f, __fsqrt_rn((float)(sum * inv_n) + a.eps));
+                }
+#pragma unroll
+                for (int u = 0; u < KR_VEC; ++u) {
+                    if (left - u * split <= 0) continue;
+                    const bool mine = h + u * step < heads && live;
+                    float4 y = x[u];
+                    if (weight) {
+                        const float f = __shfl_sync(0xFFFFFFFFu, inv, (lane & ~(LH / 2 + LH / 4)) + (u >> 1) * (LH / 2) + (u & 1) * (LH / 4));
+                        y.x = __fmul_rn(__fmul_rn(y.x, f), w.x);
+                        y.y = __fmul_rn(__fmul_rn(y.y, f), w.y);
+                        y.z = __fmul_rn(__fmul_rn(y.z, f), w.z);
+                        y.w = __fmul_rn(__fmul_rn(y.w, f), w.w);
+                    }
+                    if (TURN) {
+                        float4 m;
+                        m.x = __shfl_sync(0xFFFFFFFFu, y.x, mate);
+                        m.y = __shfl_sync(0xFFFFFFFFu, y.y, mate);
+                        m.z = __shfl_sync(0xFFFFFFFFu, y.z, mate);
+                        m.w = __shfl_sync(0xFFFFFFFFu, y.w, mate);
+                        if (turn) {
+                            const float4 z = make_float4(__fmaf_rn(y.x, c.x, __fmul_rn(m.x, s.x)), __fmaf_rn(y.y, c.y, __fmul_rn(m.y, s.y)),
+                                                         __fmaf_rn(y.z, c.z, __fmul_rn(m.z, s.z)), __fmaf_rn(y.w, c.w, __fmul_rn(m.w, s.w)));
+                            if (IS_K) {
+                                const float2 r0 = kr_turn(make_float2(y.x, y.y), make_float2(c.x, c.y), make_float2(m.x, m.y), make_float2(s.x, s.y));
+                                const float2 r1 = kr_turn(make_float2(y.z, y.w), make_float2(c.z, c.w), make_float2(m.z, m.w), make_float2(s.z, s.w));
+                                // an infinity's rounding error is NaN
+                                y = make_float4(fabsf(r0.x) < INFINITY ? r0.x : z.x, fabsf(r0.y) < INFINITY ? r0.y : z.y,
+                                                fabsf(r1.x) < INFINITY ? r1.x : z.z, fabsf(r1.y) < INFINITY ? r1.y : z.w);
+                            } else {
+                                y = z;
+                            }
+                        }
+                    }
+                    if (out && mine) *reinterpret_cast<float4*>(out + (h + u * step) * a.hd) = y;
+                    if (IS_K && blk) {
+                        uint32_t code[4];
+                        __half scale;
+                        quantise<BITS>(y, lane, code, scale);
+                        if (mine) {
+                            uint8_t* to = blk + (h + u * step) * a.head_bytes;
+                            if (BITS == 4) *reinterpret_cast<uint16_t*>(to + kat) = (uint16_t)(code[0] + 16 * code[1] + 256 * code[2] + 4096 * code[3]);
+                            else *reinterpret_cast<uint32_t*>(to + kat) = kr_bytes(code[0], code[1], code[2], code[3]);
+                            if ((hl & 7) == 0) *reinterpret_cast<__half*>(to + sat) = scale;
+                        }
+                    }
+                }
+            }
+        };
+        if (a.q)
+            vectors_of(std::false_type(), a.q + (long long)row * a.ld_q + d0, a.q_out + (long long)row * a.ld_qo + d0, a.n_head, a.q_weight,
+                       nullptr, first);
+        // keys go on where the queries' share ended, so that a row's warps have equal shares
+        if (a.k) {
+            const int q_vectors = a.q ? (a.n_head + HPW - 1) / HPW : 0, begin = (first + split - q_vectors % split) % split;
+            vectors_of(std::true_type(), a.k + (long long)row * a.ld_k + d0, a.k_out ? a.k_out + (long long)row * a.ld_ko + d0 : nullptr, a.n_kv,
+                       a.k_weight, a.kc ? a.kc + off : nullptr, begin);
+        }
+        return;
     }
-    float4 wq = make_float4(1.f, 1.f, 1.f, 1.f), wk = wq;
-    if (a.q_weight && live) wq = *reinterpret_cast<const float4*>(a.q_weight + d0);
-    if (a.k_weight && live) wk = *reinterpret_cast<const float4*>(a.k_weight + d0);
-    const double inv_n = 1.0 / a.hd;
-    const int vectors = (nv + HPW - 1) / HPW, sub = lane / LH;
-    for (int i0 = first; i0 < vectors; i0 += split * KR_VEC) {
-        float4 x[KR_VEC];
+
+    // values: (quad, vector) pairs of the run, dealt out to its warps
+    const Run run = find_run(a, row);
+    const int quads = run.quads(), nquad = __popc(quads), vv = (a.n_kv + HPW - 1) / HPW;
+    for (int i = run.index * vsplit + first - split; i < nquad * vv; i += run.len * vsplit) {
+        const int vec = i / nquad, t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
+        float4 x[4];
+        bool all = true;
 #pragma unroll
-        for (int u = 0; u < KR_VEC; ++u) {
-            const int h = (i0 + u * split) * HPW + sub;
-            x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (h < nv && live) {
-                const float* p = h < nq   ? a.q + (long long)row * a.ld_q + (long long)h * a.hd
-                                 : h < nk ? a.k + (long long)row * a.ld_k + (long long)(h - nq) * a.hd
-                                          : a.v + (long long)row * a.ld_v + (long long)(h - nk) * a.hd;
-                x[u] = *reinterpret_cast<const float4*>(p + d0);
-            }
+        for (int j = 0; j < 4; ++j) {
+            const int r = run.row(quad_pos(t, j));
+            x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            all = all && r >= 0;
+            if (r >= 0 && h < a.n_kv && live) x[j] = *reinterpret_cast<const float4*>(a.v + (long long)r * a.ld_v + h * a.hd + d0);
         }
+        uint8_t* blk = a.vc + off + h * a.head_bytes;
+        uint32_t w[4] = {0, 0, 0, 0};  // bytes of dims 0 and 1, and 2 and 3 (Q8_0: a word each)
 #pragma unroll
-        for (int u = 0; u < KR_VEC; ++u) {
-            if (i0 + u * split >= vectors) break;
-            const int h = (i0 + u * split) * HPW + sub;
-            const bool isq = h < nq, isk = !isq && h < nk, rotated = h < nk;
-            float4 y = x[u];
-            if (a.q_weight || a.k_weight) {
-                double ss = fma((double)y.x, (double)y.x, fma((double)y.y, (double)y.y, fma((double)y.z, (double)y.z, (double)y.w * (double)y.w)));
+        for (int j = 0; j < 4; ++j) {
+            uint32_t code[4];
+            __half scale;
+            quantise<BITS>(x[j], lane, code, scale);
 #pragma unroll
-                for (int o = LH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-                if ((isq && a.q_weight) || (isk && a.k_weight)) {
-                    const float inv = __fdiv_rn(1.0f, __fsqrt_rn((float)(ss * inv_n) + a.eps));
-                    const float4 w = isq ? wq : wk;
-                    y.x = __fmul_rn(__fmul_rn(y.x, inv), w.x);
-                    y.y = __fmul_rn(__fmul_rn(y.y, inv), w.y);
-                    y.z = __fmul_rn(__fmul_rn(y.z, inv), w.z);
-                    y.w = __fmul_rn(__fmul_rn(y.w, inv), w.w);
-                }
+            for (int e = 0; e < (BITS == 4 ? 2 : 4); ++e)  // byte j of word e
+                w[e] = __byte_perm(w[e], BITS == 4 ? code[2 * e & 3] + 16 * code[(2 * e + 1) & 3] : code[e & 3], j == 0 ? 0x3214 : j == 1 ? 0x3240 : j == 2 ? 0x3410 : 0x4210);
+            const int p = quad_pos(t, j);
+            if ((run.mask >> p & 1) && h < a.n_kv && live && (hl & 7) == 0)
+                *reinterpret_cast<__half*>(blk + scale_place(BITS, a.hd, p, hl >> 3)) = scale;
+        }
+        if (h >= a.n_kv || !live) continue;
+        int next;
+        uint8_t* at = blk + v_place<BITS>(a.hd, t, hl, &next);
+        if (all) {
+            if (BITS == 4) {
+                *reinterpret_cast<uint32_t*>(at) = w[0];
+                *reinterpret_cast<uint32_t*>(at + next) = w[1];
+            } else {
+                *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+                *reinterpret_cast<uint2*>(at + next) = make_uint2(w[2], w[3]);
             }
-            if (a.freq) {
-                float4 m;
-                m.x = __shfl_sync(0xFFFFFFFFu, y.x, mate);
-                m.y = __shfl_sync(0xFFFFFFFFu, y.y, mate);
-                m.z = __shfl_sync(0xFFFFFFFFu, y.z, mate);
-                m.w = __shfl_sync(0xFFFFFFFFu, y.w, mate);
-                if (turn && rotated) {
-                    y.x = (float)fma((double)y.x, c[0], (double)m.x * s[0]);
-                    y.y = (float)fma((double)y.y, c[1], (double)m.y * s[1]);
-                    y.z = (float)fma((double)y.z, c[2], (double)m.z * s[2]);
-                    y.w = (float)fma((double)y.w, c[3], (double)m.w * s[3]);
-                }
-            }
-            if (isq) {
-                if (live) *reinterpret_cast<float4*>(a.q_out + (long long)row * a.ld_qo + (long long)h * a.hd + d0) = y;
-            } else if (isk && a.k_out && live) {
-                *reinterpret_cast<float4*>(a.k_out + (long long)row * a.ld_ko + (long long)(h - nq) * a.hd + d0) = y;
-            }
-            if (a.kc && __any_sync(0xFFFFFFFFu, !isq && h < nv)) {
-                int code[4];
-                __half scale;
-                quantise<BITS>(y, lane, code, scale);
-                if (!isq && h < nv && live) {
-                    uint8_t* blk = (isk ? kblk : vblk) + (long long)(isk ? h - nq : h - nk) * a.head_bytes;
-                    const int p = pos & 15;
-                    if (isk) store_k<BITS>(blk, a.hd, p, hl, code);
-                    else store_v<BITS>(blk, a.hd, p, hl, code);
-                    if ((hl & 7) == 0)
-                        reinterpret_cast<__half*>(blk + kvq_code_bytes(BITS, a.hd))[((p & 7) * 2 + (p >> 3)) * (a.hd >> 5) + (hl >> 3)] = scale;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!(run.mask >> quad_pos(t, j) & 1)) continue;
+                if (BITS == 4) {
+                    at[j] = (uint8_t)(w[0] >> 8 * j);
+                    at[next + j] = (uint8_t)(w[1] >> 8 * j);
+                } else {
+                    at[j] = (uint8_t)(w[0] >> 8 * j);
+                    at[4 + j] = (uint8_t)(w[1] >> 8 * j);
+                    at[next + j] = (uint8_t)(w[2] >> 8 * j);
+                    at[next + 4 + j] = (uint8_t)(w[3] >> 8 * j);
                 }
             }
         }
@@ -197,60 +400,82 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_rows_kernel(const KvqRowsAr
 }
 
 // ---- reading back -------------------------------------------------------------------------------------
+template <int BITS>
+__device__ __forceinline__ float4 kr_values(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, float s) {
+    constexpr float Z = BITS == 4 ? 8.0f : 128.0f;
+    // a code as the low bits of 2^23 + code: exact, without a conversion
+    auto f = [](uint32_t c) { return __uint_as_float(0x4B000000u | c) - (8388608.0f + Z); };
+    return make_float4(f(c0) * s, f(c1) * s, f(c2) * s, f(c3) * s);
+}
+
 template <int LH, int BITS>
-__global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadArgs a, int split) {
+__global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadArgs a, int split, int vsplit) {
     constexpr int HPW = 32 / LH;
-    const int lane = threadIdx.x & 31, hl = lane & (LH - 1);
-    const long long task = ((long long)blockIdx.x * KR_THREADS + threadIdx.x) >> 5;
-    const int row = (int)(task / split), first = (int)(task - (long long)row * split);
-    if (row >= a.rows) return;
-    const int pos = a.pos[row], slot = kvq_slot(a.slots, row);
+    constexpr uint32_t M = (1u << BITS) - 1;
+    const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
+    const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
+    const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
+    if ((unsigned)row >= (unsigned)a.rows) return;
+    const int pos = a.pos[row], slot = row_slot(a, row);
     if (slot < 0) return;
     if (slot >= a.n_slots || pos < 0 || pos >= a.cap) {
         if (first == 0 && lane == 0) atomicCAS(a.err, 0, slot >= a.n_slots ? ERR_BAD_TOKEN : ERR_POS);
         return;
     }
     const long long off = slot * a.slot_bytes + (long long)(pos >> 4) * kvq_block_bytes(BITS, a.hd);
-    const int nk = a.k ? a.n_kv : 0, nv = nk + (a.v ? a.n_kv : 0);
-    const int words = a.hd * BITS / 64, p = pos & 15, phalf = p >> 3, d0 = hl * 4;
-    // where the lane's four codes lie in a block of K and of V
-    const int kat = BITS == 4 ? kvq_word(words, phalf * (a.hd >> 5) + (hl >> 3), (p & 7) * 4 + (hl >> 1 & 3)) + (hl & 1) * 2
-                              : kvq_word(words, phalf * (a.hd >> 4) + (hl >> 3) * 2 + (hl & 1), (p & 7) * 4 + (hl >> 1 & 3));
-    const int vtile = hl >> 2, vlane = (hl & 3) * 8 + ((p & 7) >> 1);
-    const int vat = kvq_word(words, BITS == 4 ? vtile : vtile * 2, vlane) + (p & 1) * 2 + phalf;
-    const int vnext = BITS == 4 && vtile >= (words & ~3) ? 32 : 64;
-    const int sat = kvq_code_bytes(BITS, a.hd) + 2 * (((p & 7) * 2 + phalf) * (a.hd >> 5) + (hl >> 3));
-    if (d0 >= a.hd) return;
-    for (int i0 = first; i0 * HPW < nv; i0 += split * KR_VEC) {
-        uint32_t code[KR_VEC];
-        float s[KR_VEC];
+    const int d0 = hl * 4, vectors = (a.n_kv + HPW - 1) / HPW;
+    const bool live = d0 < a.hd;
+    if (first < split) {
+        const int kat = k_place<BITS>(a.hd, pos & 15, hl), sat = scale_place(BITS, a.hd, pos & 15, hl >> 3);
+        for (int i0 = first; i0 < vectors; i0 += split * KR_VEC) {
+            uint32_t code[KR_VEC];
+            float s[KR_VEC];
 #pragma unroll
-        for (int u = 0; u < KR_VEC; ++u) {
-            const int h = (i0 + u * split) * HPW + lane / LH;
-            if (h >= nv) continue;
-            const bool isk = h < nk;
-            const uint8_t* blk = (isk ? a.kc : a.vc) + off + (long long)(isk ? h : h - nk) * a.head_bytes;
-            s[u] = __half2float(*reinterpret_cast<const __half*>(blk + sat));
-            if (isk)
+            for (int u = 0; u < KR_VEC; ++u) {
+                const int h = (i0 + u * split) * HPW + sub;
+                if (h >= a.n_kv || !live) continue;
+                const uint8_t* blk = a.kc + off + h * a.head_bytes;
+                s[u] = __half2float(*reinterpret_cast<const __half*>(blk + sat));
                 code[u] = BITS == 4 ? *reinterpret_cast<const uint16_t*>(blk + kat) : *reinterpret_cast<const uint32_t*>(blk + kat);
-            else if (BITS == 4)
-                code[u] = blk[vat] | blk[vat + vnext] << 8;
-            else
-                code[u] = blk[vat] | blk[vat + 4] << 8 | blk[vat + 64] << 16 | (uint32_t)blk[vat + 68] << 24;
-        }
+            }
 #pragma unroll
-        for (int u = 0; u < KR_VEC; ++u) {
-            const int h = (i0 + u * split) * HPW + lane / LH;
-            if (h >= nv) continue;
-            const bool isk = h < nk;
-            float4 y;
-            constexpr int Z = BITS == 4 ? 8 : 128, M = BITS == 4 ? 15 : 255;
-            y.x = (float)((int)(code[u] & M) - Z) * s[u];
-            y.y = (float)((int)(code[u] >> BITS & M) - Z) * s[u];
-            y.z = (float)((int)(code[u] >> 2 * BITS & M) - Z) * s[u];
-            y.w = (float)((int)(code[u] >> 3 * BITS & M) - Z) * s[u];
-            float* o = isk ? a.k + (long long)row * a.ld_k + (long long)h * a.hd : a.v + (long long)row * a.ld_v + (long long)(h - nk) * a.hd;
-            *reinterpret_cast<float4*>(o + d0) = y;
+            for (int u = 0; u < KR_VEC; ++u) {
+                const int h = (i0 + u * split) * HPW + sub;
+                if (h >= a.n_kv || !live) continue;
+                const uint32_t c = code[u];
+                *reinterpret_cast<float4*>(a.k + (long long)row * a.ld_k + h * a.hd + d0) =
+                    kr_values<BITS>(c & M, c >> BITS & M, c >> 2 * BITS & M, c >> 3 * BITS & M, s[u]);
+            }
+        }
+        return;
+    }
+    const Run run = find_run(a, row);
+    const int quads = run.quads(), nquad = __popc(quads);
+    for (int i = run.index * vsplit + first - split; i < nquad * vectors; i += run.len * vsplit) {
+        const int vec = i / nquad, t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
+        if (h >= a.n_kv || !live) continue;
+        const uint8_t* blk = a.vc + off + h * a.head_bytes;
+        int next;
+        const uint8_t* at = blk + v_place<BITS>(a.hd, t, hl, &next);
+        uint32_t w[4];
+        if (BITS == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(at);
+            w[1] = *reinterpret_cast<const uint32_t*>(at + next);
+        } else {
+            const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + next);
+            w[0] = u.x; w[1] = u.y; w[2] = v.x; w[3] = v.y;
+        }
+        float s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = __half2float(*reinterpret_cast<const __half*>(blk + scale_place(BITS, a.hd, quad_pos(t, j), hl >> 3)));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int r = run.row(quad_pos(t, j));
+            if (r < 0) continue;
+            const int b = 8 * j;
+            *reinterpret_cast<float4*>(a.v + (long long)r * a.ld_v + h * a.hd + d0) =
+                BITS == 4 ? kr_values<4>(w[0] >> b & 15, w[0] >> (b + 4) & 15, w[1] >> b & 15, w[1] >> (b + 4) & 15, s[j])
+                          : kr_values<8>(w[0] >> b & 255, w[1] >> b & 255, w[2] >> b & 255, w[3] >> b & 255, s[j]);
         }
     }
 }
@@ -265,18 +490,19 @@ static int kvq_split(int rows, int vectors) {
 
 template <int LH, int BITS>
 static cudaError_t rows_launch(const KvqRowsArgs& a, cudaStream_t st) {
-    const int heads = (a.q ? a.n_head : 0) + (a.k ? a.n_kv : 0) + (a.v ? a.n_kv : 0);
-    const int split = kvq_split(a.rows, (heads * LH + 31) / 32);
-    const long long warps = (long long)a.rows * split, per = KR_THREADS / 32;
-    tf_kvq_rows_kernel<LH, BITS><<<(unsigned)((warps + per - 1) / per), KR_THREADS, 0, st>>>(a, split);
+    const int hpw = 32 / LH, vectors = (a.q ? (a.n_head + hpw - 1) / hpw : 0) + (a.k ? (a.n_kv + hpw - 1) / hpw : 0);
+    const int split = vectors ? kvq_split(a.rows, vectors) : 0, vsplit = a.v ? kvq_split(a.rows, (a.n_kv * LH + 31) / 32) : 0;
+    const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;  // below 2^32: kvq_split
+    const unsigned grid = (unsigned)((warps + per - 1) / per);
+    if (a.freq) tf_kvq_rows_kernel<LH, BITS, true><<<grid, KR_THREADS, 0, st>>>(a, split, vsplit);
+    else tf_kvq_rows_kernel<LH, BITS, false><<<grid, KR_THREADS, 0, st>>>(a, split, vsplit);
     return cudaGetLastError();
 }
 template <int LH, int BITS>
 static cudaError_t read_launch(const KvqReadArgs& a, cudaStream_t st) {
-    const int heads = (a.k ? a.n_kv : 0) + (a.v ? a.n_kv : 0);
-    const int split = kvq_split(a.rows, (heads * LH + 31) / 32);
-    const long long warps = (long long)a.rows * split, per = KR_THREADS / 32;
-    tf_kvq_read_kernel<LH, BITS><<<(unsigned)((warps + per - 1) / per), KR_THREADS, 0, st>>>(a, split);
+    const int each = kvq_split(a.rows, (a.n_kv * LH + 31) / 32), split = a.k ? each : 0, vsplit = a.v ? each : 0;
+    const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;
+    tf_kvq_read_kernel<LH, BITS><<<(unsigned)((warps + per - 1) / per), KR_THREADS, 0, st>>>(a, split, vsplit);
     return cudaGetLastError();
 }
 
