@@ -165,15 +165,23 @@ __device__ __forceinline__ int quad_pos(int t, int i) { return 2 * t + (i >> 1) 
 template <class A>
 __device__ __forceinline__ int row_slot(const A& a, int row) { return a.slots ? a.slots[row] : row; }
 
-// The run of `row`, which lies in the cache.  A warp looks 15 rows back and 16 on.
+// Slots and positions of the rows 15 back to 16 on, a lane each; the row's own are lane 15's.
+struct Window {
+    int slot, pos;
+};
 template <class A>
-__device__ __forceinline__ Run find_run(const A& a, int row) {
-    const int lane = threadIdx.x & 31, q = row - 15 + lane;
-    int slot = -1, pos = -1;
+__device__ __forceinline__ Window load_window(const A& a, int row) {
+    const int q = row - 15 + (int)(threadIdx.x & 31);
+    Window w = {-1, -1};
     if (q >= 0 && q < a.rows) {
-        slot = row_slot(a, q);
-        pos = a.pos[q];
+        w.slot = row_slot(a, q);
+        w.pos = a.pos[q];
     }
+    return w;
+}
+// The run of `row`, which lies in the cache.
+__device__ __forceinline__ Run find_run(int row, int slot, int pos) {
+    const int lane = threadIdx.x & 31;
     const int slot0 = __shfl_up_sync(0xFFFFFFFFu, slot, 1), pos0 = __shfl_up_sync(0xFFFFFFFFu, pos, 1);
     const bool on = lane > 0 && slot >= 0 && slot == slot0 && pos0 >= 0 && pos > pos0 && pos >> 4 == pos0 >> 4;
     const unsigned c = __ballot_sync(0xFFFFFFFFu, on);  // rows that go on with the run of the row before
@@ -191,16 +199,33 @@ __device__ __forceinline__ Run find_run(const A& a, int row) {
 // split, ...) and `vsplit` for its share of the run's values.
 // TURN: with a rotation.
 template <int LH, int BITS, bool TURN>
-__global__ void __launch_bounds__(KR_THREADS, TURN ? 4 : 5) tf_kvq_rows_kernel(const KvqRowsArgs a, int split, int vsplit) {
+__global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(const KvqRowsArgs a, int split, int vsplit) {
     constexpr int HPW = 32 / LH;
     const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
     const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
     if ((unsigned)row >= (unsigned)a.rows) return;
-    const int pos = a.pos ? a.pos[row] : 0;
+    Window win = {0, 0};
+    int pos = 0, slot = 0;
+    float4 ahead[KR_VEC];  // the first vectors of the warp's share, on their way while the position is
+    if (first < split) {
+        const float* in = a.q ? a.q + (long long)row * a.ld_q : a.k + (long long)row * a.ld_k;
+        const int heads = a.q ? a.n_head : a.n_kv;
+#pragma unroll
+        for (int u = 0; u < KR_VEC; ++u) {
+            const int h = (first + u * split) * HPW + sub;
+            ahead[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (h < heads && hl * 4 < a.hd) ahead[u] = *reinterpret_cast<const float4*>(in + h * a.hd + hl * 4);
+        }
+        if (a.pos) pos = a.pos[row];
+        if (a.kc) slot = row_slot(a, row);
+    } else {
+        win = load_window(a, row);
+        pos = __shfl_sync(0xFFFFFFFFu, win.pos, 15);
+        slot = __shfl_sync(0xFFFFFFFFu, win.slot, 15);
+    }
     long long off = 0;
     if (a.kc) {
-        const int slot = row_slot(a, row);
         if (slot < 0) return;
         if (slot >= a.n_slots || pos < 0 || pos >= a.cap) {
             if (first == 0 && lane == 0) atomicCAS(a.err, 0, slot >= a.n_slots ? ERR_BAD_TOKEN : ERR_POS);
@@ -249,20 +274,26 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 4 : 5) tf_kvq_rows_kernel(c
         }
         const double inv_n = 1.0 / a.hd;
         // Vectors of one kind: the warp's, of `heads` heads from `in` on (its dims), to `out` and to the cache (`blk`)
-        auto vectors_of = [&](auto is_k, const float* in, float* out, int heads, const float* weight, uint8_t* blk, int begin) {
+        auto vectors_of = [&](auto is_k, const float* in, float* out, int heads, const float* weight, uint8_t* blk, int begin, bool loaded) {
             constexpr bool IS_K = decltype(is_k)::value;
             float4 w = make_float4(1.f, 1.f, 1.f, 1.f);
             if (weight && live) w = *reinterpret_cast<const float4*>(weight + d0);
             const int step = split * HPW;
             int h = begin * HPW + sub;
             const int kat = k_place<BITS>(a.hd, pos & 15, hl), sat = scale_place(BITS, a.hd, pos & 15, hl >> 3);
+            auto load = [&](int h0) {
+#pragma unroll
+                for (int u = 0; u < KR_VEC; ++u) {
+                    ahead[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (h0 + u * step < heads && live) ahead[u] = *reinterpret_cast<const float4*>(in + (h0 + u * step) * a.hd);
+                }
+            };
+            if (!loaded) load(h);
             for (int left = (heads + HPW - 1) / HPW - begin; left > 0; left -= split * KR_VEC, h += step * KR_VEC) {
                 float4 x[KR_VEC];
 #pragma unroll
-                for (int u = 0; u < KR_VEC; ++u) {
-                    x[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (h + u * step < heads && live) x[u] = *reinterpret_cast<const float4*>(in + (h + u * step) * a.hd);
-                }
+                for (int u = 0; u < KR_VEC; ++u) x[u] = ahead[u];
+                load(h + step * KR_VEC);
                 // The squares of the four vectors are summed together: at each of the first two steps a lane hands on
                 // the half of its sums that its partner keeps, so that a lane ends with the sum of one of them.
                 float inv = 1.0f;
@@ -332,18 +363,18 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 4 : 5) tf_kvq_rows_kernel(c
         };
         if (a.q)
             vectors_of(std::false_type(), a.q + (long long)row * a.ld_q + d0, a.q_out + (long long)row * a.ld_qo + d0, a.n_head, a.q_weight,
-                       nullptr, first);
+                       nullptr, first, true);
         // keys go on where the queries' share ended, so that a row's warps have equal shares
         if (a.k) {
             const int q_vectors = a.q ? (a.n_head + HPW - 1) / HPW : 0, begin = (first + split - q_vectors % split) % split;
             vectors_of(std::true_type(), a.k + (long long)row * a.ld_k + d0, a.k_out ? a.k_out + (long long)row * a.ld_ko + d0 : nullptr, a.n_kv,
-                       a.k_weight, a.kc ? a.kc + off : nullptr, begin);
+                       a.k_weight, a.kc ? a.kc + off : nullptr, begin, !a.q);
         }
         return;
     }
 
     // values: (quad, vector) pairs of the run, dealt out to its warps
-    const Run run = find_run(a, row);
+    const Run run = find_run(row, win.slot, win.pos);
     const int quads = run.quads(), nquad = __popc(quads), vv = (a.n_kv + HPW - 1) / HPW;
     for (int i = run.index * vsplit + first - split; i < nquad * vv; i += run.len * vsplit) {
         const int vec = i / nquad, t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
@@ -416,7 +447,16 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
     const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
     if ((unsigned)row >= (unsigned)a.rows) return;
-    const int pos = a.pos[row], slot = row_slot(a, row);
+    Window win = {0, 0};
+    int pos, slot;
+    if (first < split) {
+        pos = a.pos[row];
+        slot = row_slot(a, row);
+    } else {
+        win = load_window(a, row);
+        pos = __shfl_sync(0xFFFFFFFFu, win.pos, 15);
+        slot = __shfl_sync(0xFFFFFFFFu, win.slot, 15);
+    }
     if (slot < 0) return;
     if (slot >= a.n_slots || pos < 0 || pos >= a.cap) {
         if (first == 0 && lane == 0) atomicCAS(a.err, 0, slot >= a.n_slots ? ERR_BAD_TOKEN : ERR_POS);
@@ -449,7 +489,7 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
         }
         return;
     }
-    const Run run = find_run(a, row);
+    const Run run = find_run(row, win.slot, win.pos);
     const int quads = run.quads(), nquad = __popc(quads);
     for (int i = run.index * vsplit + first - split; i < nquad * vectors; i += run.len * vsplit) {
         const int vec = i / nquad, t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
@@ -481,17 +521,20 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
 }
 
 // ---- host ---------------------------------------------------------------------------------------------
-// Warps per row: one when rows alone fill the device (16 warps on each of its SMs), else a row's vectors are
-// shared out so that few rows finish in one round of loads.
-static int kvq_split(int rows, int vectors) {
-    const int want = (148 * 16 + rows - 1) / rows;
+// Warps per row: one when rows alone fill the device (`fill` warps on each of its SMs), else a row's vectors are
+// shared out so that few rows finish in one round of loads.  16 warps, and twice what an SM holds where they carry
+// a whole row of queries and keys, whose last round would else be long: 5003 rows of 32 + 8 + 8 heads of 128, 71 us
+// with 16, FILL48 with 48.
+constexpr int KR_FILL = 16, KR_FILL_TURN = 48;
+static int kvq_split(int rows, int vectors, int fill = KR_FILL) {
+    const int want = (int)((148ll * fill + rows - 1) / rows);
     return want < 1 ? 1 : want > vectors ? vectors : want;
 }
 
 template <int LH, int BITS>
 static cudaError_t rows_launch(const KvqRowsArgs& a, cudaStream_t st) {
     const int hpw = 32 / LH, vectors = (a.q ? (a.n_head + hpw - 1) / hpw : 0) + (a.k ? (a.n_kv + hpw - 1) / hpw : 0);
-    const int split = vectors ? kvq_split(a.rows, vectors) : 0, vsplit = a.v ? kvq_split(a.rows, (a.n_kv * LH + 31) / 32) : 0;
+    const int split = vectors ? kvq_split(a.rows, vectors, a.freq ? KR_FILL_TURN : KR_FILL) : 0, vsplit = a.v ? kvq_split(a.rows, (a.n_kv * LH + 31) / 32) : 0;
     const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;  // below 2^32: kvq_split
     const unsigned grid = (unsigned)((warps + per - 1) / per);
     if (a.freq) tf_kvq_rows_kernel<LH, BITS, true><<<grid, KR_THREADS, 0, st>>>(a, split, vsplit);
