@@ -37,6 +37,7 @@ constexpr int KA_THREADS = 128;
 constexpr int KA_WARPS = KA_THREADS / 32;
 constexpr int KA_UNIT_COST = 8;    // blocks that a unit's start and end take the time of
 constexpr int KA_MIN_RANGE = 16;   // blocks of a CTA's range at least
+constexpr int KA_MAX_SPLIT = 8;    // CTAs of a cluster
 constexpr int KA_SNAP = 6;         // a cut this near to a unit's first or last block moves there
 constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
 constexpr int KA_MAX_GRID = 1024;  // descriptors of 32 bytes in the workspace's first 32 KB
@@ -47,6 +48,7 @@ struct KvqPlan {
     int rt;        // rows per row tile
     int rep;       // query heads per kv head
     int tiles;     // row tiles of T rows
+    int split;     // CTAs of a unit, one cluster; 0: ranges of all units' blocks
     int by_unit;   // descriptors are found by unit (there are at most `grid`), else by the CTA that begins it
 };
 struct alignas(32) KvqDesc {  // a unit split over CTAs c0 .. c1
@@ -58,18 +60,19 @@ __host__ __device__ inline size_t kvq_part_floats(int rt, int hd) { return (size
 // 0: up to 4 rows (both halves of q and p side by side in the 8 columns), 1: up to 8, 2: up to 16
 __host__ __device__ constexpr int kvq_rt(int mode) { return mode == 0 ? 4 : mode == 1 ? 8 : 16; }
 
-__host__ __device__ constexpr int kvq_ctas(int mode) { return mode == 2 ? 3 : 5; }  // 168 or 96 registers a thread
+__host__ __device__ constexpr int kvq_ctas(int mode) { return mode == 2 ? 3 : 4; }  // 168 or 128 registers a thread
 
 template <int BITS, int HD, int MODE>
 struct KvqCfg {
     static constexpr int RT = kvq_rt(MODE);
     static constexpr int CTAS = kvq_ctas(MODE);                    // per SM
     static constexpr int BLOCK = kvq_block_bytes(BITS, HD);
-    static constexpr int STAGE = 2 * BLOCK;                        // K and V of 16 positions
     static constexpr int SLOT = RT * HD * 4;                       // a warp's output rows
     static constexpr int QF = (MODE == 2 ? 2 : 1) * HD / 32 * 1024;  // q's fragments
     static constexpr int STAT = KA_WARPS * RT * 12;
     static constexpr int ROOM = 227 * 1024 / CTAS - 1024 - STAT - QF;
+    static constexpr int PB = HD < 128 && ROOM >= 8 * KA_WARPS * BLOCK ? 2 : 1;  // neighbouring blocks of a warp's turn: two where two stages fit
+    static constexpr int STAGE = 2 * PB * BLOCK;                   // K, then V
     static constexpr int FIT = ROOM / (KA_WARPS * STAGE);
     static constexpr int ST = FIT > 8 ? 8 : FIT;                   // stages of a warp's ring
     static constexpr int RING = ST * STAGE > SLOT ? ST * STAGE : SLOT;  // output rows take the rings' place
@@ -87,6 +90,11 @@ __device__ __forceinline__ void ka_mma(float (&c)[4], const uint32_t (&a)[4], co
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t ka_pack_rz(float lo, float hi) {  // towards zero
+    uint32_t y;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
 }
 __device__ __forceinline__ uint32_t ka_pack(float lo, float hi) {
     uint32_t y;
@@ -233,7 +241,32 @@ __device__ __forceinline__ KvqRange kvq_range(const KvqAttnArgs& a, const KvqPla
     return r;
 }
 
-template <int BITS, int HD, int MODE>
+// Every thread of the cluster arrives; shared memory written before is visible after.
+__device__ __forceinline__ void ka_cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t ka_remote(const void* p, int rank) {  // the same place in another CTA of the cluster
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float ka_remote1(const float* p, int rank) {
+    float x;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(ka_remote(p, rank)) : "memory");
+    return x;
+}
+__device__ __forceinline__ float4 ka_remote4(const float* p, int rank) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(ka_remote(p, rank))
+                 : "memory");
+    return x;
+}
+
+// CLUSTER: a cluster of pl.split CTAs per unit (all of them, from the sequences' T rows), which join over distributed
+// shared memory; else ranges, and a second launch.
+template <int BITS, int HD, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(KA_THREADS, KvqCfg<BITS, HD, MODE>::CTAS)
 tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     using F = KvqCfg<BITS, HD, MODE>;
@@ -242,10 +275,9 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     constexpr int QP = MODE == 2 ? 2 : 1;  // products of q's halves: side by side in M, or one after the other
     constexpr int PP = MODE == 0 ? 1 : 2;  // products of p's halves: side by side in N, or one after the other
     extern __shared__ __align__(128) uint8_t smem[];
-    pdl_trigger();
+    if (!CLUSTER) pdl_trigger();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
-    const uint8_t* ring_p = smem + warp * (F::ST * F::STAGE);
-    const uint32_t ring = smem_u32(ring_p);
+    const uint32_t ring_at = warp * (F::ST * F::STAGE), ring = smem_u32(smem) + ring_at;
     uint8_t* qs = smem + KA_WARPS * F::RING;  // [QP][NG][2][lane] four registers
     const uint8_t* q_at = qs + lane * 16;
     float* slot_all = reinterpret_cast<float*>(smem);  // where the rings are, once a segment's blocks are done
@@ -254,9 +286,17 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     KvqDesc* desc = static_cast<KvqDesc*>(a.ws);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + KA_DESC_BYTES);
 
-    const KvqRange range = kvq_range(a, pl);
+    KvqRange range = {0, 1, 0, 0, 0};
+    int b = 0, base = 0, rank = 0;
+    if (CLUSTER) {
+        rank = blockIdx.x % pl.split;
+        b = blockIdx.x / (pl.split * pl.tiles * a.n_kv);
+    } else {
+        range = kvq_range(a, pl);
+        b = range.b;
+        base = range.base;
+    }
     KvqDesc open = {-1, 0, 0, 0, 0, 0};  // the unit that begins here and ends in a later CTA
-    int b = range.b, base = range.base;
     const float log2e_d = 1.4426950408889634f * rsqrtf((float)HD);
     uint32_t magic;
     asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
@@ -264,38 +304,74 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
 #pragma unroll 1
     for (int gpos = range.g0; gpos < range.g1;) {
         KvqSeq sq = kvq_seq(a, pl, b);
-        int len = kvq_len(sq);
-        while (gpos >= base + len && b + 1 < a.B) {  // gpos is below the total: a sequence with work follows
-            base += len;
-            sq = kvq_seq(a, pl, ++b);
-            len = kvq_len(sq);
+        int blk0, blk1, kvh, tile, rows, r0, ub = 0;
+        if (CLUSTER) {
+            gpos = range.g1;
+            const int unit = blockIdx.x / pl.split - b * (pl.tiles * a.n_kv);
+            kvh = unit / pl.tiles;
+            tile = unit - kvh * pl.tiles;
+            if (sq.bad && unit == 0 && rank == 0 && threadIdx.x == 0) atomicCAS(a.err, 0, ERR_POS);
+            const int each = (sq.blocks + pl.split - 1) / pl.split;
+            blk0 = min(rank * each, sq.blocks);
+            blk1 = min(blk0 + each, sq.blocks);
+            r0 = tile * RT;
+            // the tile's rows behind the new ones are zero
+            const int all = min(RT, a.T * pl.rep - r0), first = max(0, sq.n_new * pl.rep - r0);
+            for (int i = first * (HD / 4) + rank * KA_THREADS + threadIdx.x; i < all * (HD / 4); i += pl.split * KA_THREADS) {
+                const int row = i / (HD / 4), rr = r0 + row, t = rr / pl.rep, h = kvh * pl.rep + rr - t * pl.rep;
+                *reinterpret_cast<float4*>(a.out + ((long long)b * a.T + t) * a.ld_out + h * HD + (i - row * (HD / 4)) * 4) =
+                    make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            rows = min(RT, sq.n_new * pl.rep - r0);
+            if (rows <= 0) return;  // the whole cluster
+        } else {
+            int len = kvq_len(sq);
+            while (gpos >= base + len && b + 1 < a.B) {  // gpos is below the total: a sequence with work follows
+                base += len;
+                sq = kvq_seq(a, pl, ++b);
+                len = kvq_len(sq);
+            }
+            if (gpos >= base + len) break;
+            const int per_unit = sq.blocks + KA_UNIT_COST, unit = (gpos - base) / per_unit;
+            ub = base + unit * per_unit;
+            blk0 = kvq_cut(gpos - ub, sq.blocks);
+            blk1 = min(sq.blocks, range.g1 - ub < per_unit ? kvq_cut(range.g1 - ub, sq.blocks) : per_unit);
+            gpos = min(range.g1, ub + per_unit);
+            if (blk0 >= blk1) continue;
+            const int tiles = sq.units / a.n_kv;
+            kvh = unit / tiles;
+            tile = unit - kvh * tiles;
+            r0 = tile * RT;
+            rows = min(RT, sq.n_new * pl.rep - r0);
         }
-        if (gpos >= base + len) break;
-        const int per_unit = sq.blocks + KA_UNIT_COST, unit = (gpos - base) / per_unit, ub = base + unit * per_unit;
-        const int blk0 = kvq_cut(gpos - ub, sq.blocks), blk1 = min(sq.blocks, range.g1 - ub < per_unit ? kvq_cut(range.g1 - ub, sq.blocks) : per_unit);
-        gpos = min(range.g1, ub + per_unit);
-        if (blk0 >= blk1) continue;
-        const int tiles = sq.units / a.n_kv, kvh = unit / tiles, tile = unit - kvh * tiles;
-        const int r0 = tile * RT, rows = min(RT, sq.n_new * pl.rep - r0);
 
-        // this warp's blocks: blk0 + warp, and every KA_WARPS-th from there
-        const int n_mine = blk1 - blk0 > warp ? (blk1 - blk0 - warp + KA_WARPS - 1) / KA_WARPS : 0;
-        const long long where = sq.slot * a.slot_bytes + kvh * a.head_bytes + (long long)(blk0 + warp) * F::BLOCK + lane * 16;
+        // this warp's turns of PB blocks: warp, and every KA_WARPS-th from there
+        const int turns = (blk1 - blk0 + F::PB - 1) / F::PB, n_mine = turns > warp ? (turns - warp + KA_WARPS - 1) / KA_WARPS : 0;
+        const long long where = sq.slot * a.slot_bytes + kvh * a.head_bytes + (long long)(blk0 + warp * F::PB) * F::BLOCK + lane * 16;
         const uint8_t *kc = a.kc + where, *vc = a.vc + where;
-        int left = n_mine;
-        uint32_t fill = ring + lane * 16;
-        auto fetch = [&]() {  // the next block into the next stage
+        int left = blk1 - blk0 - warp * F::PB;  // blocks from the next turn on
+        uint32_t fill = ring;
+        auto fetch = [&]() {  // the next turn into the next stage
             if (left > 0) {
+                const uint32_t dst = fill + lane * 16;
+                const int bytes = left >= F::PB ? F::PB * F::BLOCK : F::BLOCK;  // (a segment's last turn may lack a block)
+                if (F::PB == 1 || left >= F::PB) {
 #pragma unroll
-                for (int c = 0; c < F::BLOCK; c += 512)
-                    if (c + 512 <= F::BLOCK || lane * 16 < F::BLOCK - c) {
-                        ka_copy16(fill + c, kc + c);
-                        ka_copy16(fill + F::BLOCK + c, vc + c);
+                    for (int c = 0; c < F::PB * F::BLOCK; c += 512)
+                        if (c + 512 <= F::PB * F::BLOCK || lane * 16 < F::PB * F::BLOCK - c) {
+                            ka_copy16(dst + c, kc + c);
+                            ka_copy16(dst + F::PB * F::BLOCK + c, vc + c);
+                        }
+                } else {
+                    for (int c = 0; c + lane * 16 < bytes; c += 512) {
+                        ka_copy16(dst + c, kc + c);
+                        ka_copy16(dst + F::PB * F::BLOCK + c, vc + c);
                     }
-                --left;
-                kc += KA_WARPS * F::BLOCK;
-                vc += KA_WARPS * F::BLOCK;
-                fill = fill + F::STAGE >= ring + F::ST * F::STAGE ? ring + lane * 16 : fill + F::STAGE;
+                }
+                left -= KA_WARPS * F::PB;
+                kc += KA_WARPS * F::PB * F::BLOCK;
+                vc += KA_WARPS * F::PB * F::BLOCK;
+                fill = fill == ring + (F::ST - 1) * F::STAGE ? ring : fill + F::STAGE;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
@@ -390,17 +466,21 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             top[nr] = 0;
         }
 
-        // One block at `at`, from position p0 on.
-        auto block = [&](auto masked_c, const uint8_t* at, const int p0) {
+        // One turn at `at` (its K, then its V), from position p0 on.
+        constexpr int PB = F::PB;
+        auto turn = [&](auto masked_c, const uint8_t* at, const int p0) {
             constexpr bool MASKED = decltype(masked_c)::value;
-            // scores of row g (and g + 8) against positions 2 tq, 2 tq + 1, 2 tq + 8, 2 tq + 9
-            float2 x[NR][2];
+            const int end = MASKED ? min(p0 + 16 * PB, blk1 * 16) : 0;
+            // scores of row g (and g + 8) against positions 2 tq, 2 tq + 1 (x, y), and 8 on, of each block
+            float2 x[PB][NR][2];
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) x[nr][0] = x[nr][1] = make_float2(0.f, 0.f);
-            {
+            for (int pb = 0; pb < PB; ++pb) {
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) x[pb][nr][0] = x[pb][nr][1] = make_float2(0.f, 0.f);
+                const uint8_t* kb = at + pb * F::BLOCK;
                 uint32_t w[W], s[2 * NG];
-                ka_words<W>(at, lane, w);
-                ka_scales<NG>(at + CODES, tq, s);
+                ka_words<W>(kb, lane, w);
+                ka_scales<NG>(kb + CODES, tq, s);
 #pragma unroll
                 for (int k = 0; k < NG; ++k) {
                     uint32_t qf[QP][2][4];
@@ -425,27 +505,31 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                             ka_mma(c, qf[part][1], f[2], f[3]);
                         }
                         const float2 sc = make_float2(ka_scale(s, half * 2, k), ka_scale(s, half * 2 + 1, k));
-                        x[NR - 1][half] = ka_fma2(make_float2(c[2], c[3]), sc, x[NR - 1][half]);
-                        x[0][half] = ka_fma2(make_float2(c[0], c[1]), sc, x[0][half]);
+                        x[pb][NR - 1][half] = ka_fma2(make_float2(c[2], c[3]), sc, x[pb][NR - 1][half]);
+                        x[pb][0][half] = ka_fma2(make_float2(c[0], c[1]), sc, x[pb][0][half]);
                     }
                 }
             }
-            uint32_t vs[2 * NG];
-            ka_scales<NG>(at + F::BLOCK + CODES, tq, vs);
-            auto seen = [&](int nr, int e) { return !MASKED || p0 + 2 * tq + (e & 1) + (e >> 1) * 8 <= lim[nr]; };
-            bool raise;
-            {  // a lane looks at one word of V's scales
-                const uint32_t word = *reinterpret_cast<const uint32_t*>(at + F::BLOCK + CODES + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
-                raise = (word & 0xFFFFu) > top_all || word >> 16 > top_all;
+            const uint8_t* vb = at + PB * F::BLOCK;
+            auto seen = [&](int pb, int nr, int e) {
+                const int pos = p0 + 16 * pb + 2 * tq + (e & 1) + (e >> 1) * 8;
+                return !MASKED || (pos <= lim[nr] && pos < end);
+            };
+            bool raise = false;
+#pragma unroll
+            for (int pb = 0; pb < PB; ++pb) {
+                // a lane looks at one word of V's scales
+                const uint32_t word = *reinterpret_cast<const uint32_t*>(vb + pb * F::BLOCK + CODES + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
+                raise |= (word & 0xFFFFu) > top_all || word >> 16 > top_all;
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        if (!seen(pb, nr, 2 * e)) x[pb][nr][e].x = -INFINITY;
+                        if (!seen(pb, nr, 2 * e + 1)) x[pb][nr][e].y = -INFINITY;
+                        raise |= x[pb][nr][e].x > thr[nr] || x[pb][nr][e].y > thr[nr];
+                    }
             }
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    if (!seen(nr, 2 * e)) x[nr][e].x = -INFINITY;
-                    if (!seen(nr, 2 * e + 1)) x[nr][e].y = -INFINITY;
-                    raise |= x[nr][e].x > thr[nr] || x[nr][e].y > thr[nr];
-                }
             if (__any_sync(0xFFFFFFFFu, raise)) {
                 uint32_t least = 0xFFFFu;
 #pragma unroll
@@ -453,13 +537,18 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                     float mx = m[nr];
                     uint32_t tp = top[nr];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        mx = fmaxf(mx, e & 1 ? x[nr][e >> 1].y : x[nr][e >> 1].x);
-                        if (seen(nr, e)) {
+                    for (int pb = 0; pb < PB; ++pb) {
+                        uint32_t vs[2 * NG];
+                        ka_scales<NG>(vb + pb * F::BLOCK + CODES, tq, vs);
 #pragma unroll
-                            for (int k = 0; k < NG; ++k) {  // NaN and infinity have no say
-                                const uint32_t v = __half_as_ushort(__float2half_rn(fabsf(ka_scale(vs, e, k))));
-                                if (v < 0x7C00u) tp = max(tp, v);
+                        for (int e = 0; e < 4; ++e) {
+                            mx = fmaxf(mx, e & 1 ? x[pb][nr][e >> 1].y : x[pb][nr][e >> 1].x);
+                            if (seen(pb, nr, e)) {
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) {  // NaN and infinity have no say
+                                    const uint32_t v = __half_as_ushort(__float2half_rn(fabsf(ka_scale(vs, e, k))));
+                                    if (v < 0x7C00u) tp = max(tp, v);
+                                }
                             }
                         }
                     }
@@ -495,62 +584,68 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                 top_all = __reduce_min_sync(0xFFFFFFFFu, least);
             }
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float2 y = ka_fma2(x[nr][e], make_float2(fr[nr], fr[nr]), make_float2(-ref[nr], -ref[nr]));
-                    x[nr][e] = make_float2(ka_exp2(y.x), ka_exp2(y.y));
-                    l[nr] += x[nr][e].x + x[nr][e].y;
-                }
-            uint32_t w[W];
-            ka_words<W>(at + F::BLOCK, lane, w);
-            // the low half is what the high one leaves; MODE 0: columns 0 .. 3 take the high half, 4 .. 7 the low
-            const float low = MODE == 0 && g < 4 ? 0.f : -1.f;
-#pragma unroll
-            for (int k = 0; k < NG; ++k) {
-                uint32_t pf[NR][PP][2];
+            for (int pb = 0; pb < PB; ++pb) {
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        float2 y = ka_mul2(x[nr][half], make_float2(ka_scale(vs, 2 * half, k), ka_scale(vs, 2 * half + 1, k)));
-                        if (MASKED) {  // an unseen position's scale may be NaN
-                            if (!seen(nr, 2 * half)) y.x = 0.f;
-                            if (!seen(nr, 2 * half + 1)) y.y = 0.f;
-                        }
-                        const uint32_t hi = ka_pack(y.x, y.y);
-                        const float2 z = ka_fma2(ka_unpack(hi), make_float2(low, low), y);
-                        if (MODE != 0) pf[nr][0][half] = hi;
-                        pf[nr][PP - 1][half] = ka_pack(z.x, z.y);
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 y = ka_fma2(x[pb][nr][e], make_float2(fr[nr], fr[nr]), make_float2(-ref[nr], -ref[nr]));
+                        x[pb][nr][e] = make_float2(ka_exp2(y.x), ka_exp2(y.y));
+                        l[nr] += x[pb][nr][e].x + x[pb][nr][e].y;
                     }
+                uint32_t w[W], vs[2 * NG];
+                ka_scales<NG>(vb + pb * F::BLOCK + CODES, tq, vs);
+                ka_words<W>(vb + pb * F::BLOCK, lane, w);
+                // p is cut after 11 bits, and what is left again; MODE 0: columns 0 .. 3 take the first part, 4 .. 7 the
+                // second (the cut of the others is to nothing)
+                const uint32_t cut = MODE == 0 && g < 4 ? 0u : 0xFFFFE000u;
 #pragma unroll
-                for (int d = 2 * k; d < 2 * k + 2; ++d) {
-                    uint32_t v[4];
-                    if (BITS == 4) {
-                        ka_nibbles(w[d], magic, v);
-                    } else {
-                        ka_bytes(w[2 * d], magic, v[0], v[2]);
-                        ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
-                    }
+                for (int k = 0; k < NG; ++k) {
+                    uint32_t pf[NR][PP][2];
 #pragma unroll
                     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                        for (int part = PP - 1; part >= 0; --part) ka_mma(o[nr][d], v, pf[nr][part][0], pf[nr][part][1]);
+                        for (int half = 0; half < 2; ++half) {
+                            float2 y = ka_mul2(x[pb][nr][half], make_float2(ka_scale(vs, 2 * half, k), ka_scale(vs, 2 * half + 1, k)));
+                            if (MASKED) {  // an unseen position's scale may be NaN
+                                if (!seen(pb, nr, 2 * half)) y.x = 0.f;
+                                if (!seen(pb, nr, 2 * half + 1)) y.y = 0.f;
+                            }
+                            const float2 h = make_float2(__uint_as_float(__float_as_uint(y.x) & cut), __uint_as_float(__float_as_uint(y.y) & cut));
+                            const float2 z = ka_fma2(h, make_float2(-1.f, -1.f), y);
+                            if (MODE != 0) pf[nr][0][half] = ka_pack_rz(y.x, y.y);
+                            pf[nr][PP - 1][half] = ka_pack_rz(z.x, z.y);
+                        }
+#pragma unroll
+                    for (int d = 2 * k; d < 2 * k + 2; ++d) {
+                        uint32_t v[4];
+                        if (BITS == 4) {
+                            ka_nibbles(w[d], magic, v);
+                        } else {
+                            ka_bytes(w[2 * d], magic, v[0], v[2]);
+                            ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
+                        }
+#pragma unroll
+                        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                            for (int part = PP - 1; part >= 0; --part) ka_mma(o[nr][d], v, pf[nr][part][0], pf[nr][part][1]);
+                    }
                 }
             }
         };
 
-        const uint8_t* at = ring_p;
-        int p0 = (blk0 + warp) * 16;
+        uint32_t at = ring_at;
+        int p0 = (blk0 + warp * PB) * 16;
+        const int last = min(open_to, blk1 * 16 - 1);  // up to here every position of a turn is seen
 #pragma unroll 1
         for (int i = 0; i < n_mine; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(F::ST - 2) : "memory");
             __syncwarp();  // everyone's copies of this stage are visible, and the stage before is read
             fetch();
-            if (p0 + 15 <= open_to) block(std::false_type(), at, p0);
-            else block(std::true_type(), at, p0);
-            p0 += KA_WARPS * 16;
-            at = at + F::STAGE >= ring_p + F::ST * F::STAGE ? ring_p : at + F::STAGE;
+            if (p0 + 16 * PB - 1 <= last) turn(std::false_type(), smem + at, p0);
+            else turn(std::true_type(), smem + at, p0);
+            p0 += KA_WARPS * PB * 16;
+            at = at == ring_at + (F::ST - 1) * F::STAGE ? ring_at : at + F::STAGE;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
@@ -582,8 +677,10 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             }
         }
         __syncthreads();
-        const bool begins = blk0 == 0, ends = blk1 == sq.blocks;
-        float* part = parts + (blockIdx.x * 2 + (begins ? 1 : 0)) * kvq_part_floats(RT, HD);
+        const bool begins = blk0 == 0, ends = blk1 == sq.blocks, whole = CLUSTER ? pl.split == 1 : begins && ends;
+        // what this CTA hands on: rows, then their exponents and sums (CLUSTER: in shared memory, where q was)
+        float* part = CLUSTER ? reinterpret_cast<float*>(qs) : parts + (blockIdx.x * 2 + (begins ? 1 : 0)) * kvq_part_floats(RT, HD);
+        float* part_stat = CLUSTER ? q_max : part + RT * HD;
         for (int i = threadIdx.x; i < rows * (HD / 4); i += KA_THREADS) {
             const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
             float mx = -INFINITY, L = 0.f;
@@ -602,7 +699,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                 y.z = fmaf(u.z, f, y.z);
                 y.w = fmaf(u.w, f, y.w);
             }
-            if (begins && ends) {
+            if (whole) {
                 const int rr = r0 + row, t = rr / pl.rep, h = kvh * pl.rep + rr - t * pl.rep;
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 *reinterpret_cast<float4*>(a.out + ((long long)b * a.T + t) * a.ld_out + h * HD + d) =
@@ -610,10 +707,45 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             } else {
                 *reinterpret_cast<float4*>(part + row * HD + d) = y;
                 if (d == 0) {
-                    part[RT * HD + row] = mx;
-                    part[RT * HD + RT + row] = L;
+                    part_stat[row] = mx;
+                    part_stat[RT + row] = L;
                 }
             }
+        }
+        if (CLUSTER) {
+            if (whole) return;
+            ka_cluster_sync();
+            for (int i = rank * KA_THREADS + threadIdx.x; i < rows * (HD / 4); i += pl.split * KA_THREADS) {
+                const int row = i / (HD / 4), d = (i - row * (HD / 4)) * 4;
+                float e[KA_MAX_SPLIT], l1[KA_MAX_SPLIT], mx = -INFINITY, L = 0.f;
+                float4 u[KA_MAX_SPLIT], y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int c = 0; c < KA_MAX_SPLIT; ++c)
+                    if (c < pl.split) {
+                        e[c] = ka_remote1(part_stat + row, c);
+                        l1[c] = ka_remote1(part_stat + RT + row, c);
+                        u[c] = ka_remote4(part + row * HD + d, c);
+                    }
+#pragma unroll
+                for (int c = 0; c < KA_MAX_SPLIT; ++c)
+                    if (c < pl.split) mx = fmaxf(mx, e[c]);
+#pragma unroll
+                for (int c = 0; c < KA_MAX_SPLIT; ++c)
+                    if (c < pl.split && e[c] != -INFINITY) {
+                        const float f = ka_exp2(e[c] - mx);
+                        L = fmaf(l1[c], f, L);
+                        y.x = fmaf(u[c].x, f, y.x);
+                        y.y = fmaf(u[c].y, f, y.y);
+                        y.z = fmaf(u[c].z, f, y.z);
+                        y.w = fmaf(u[c].w, f, y.w);
+                    }
+                const int rr = r0 + row, t = rr / pl.rep, h = kvh * pl.rep + rr - t * pl.rep;
+                const float inv = L == 0.f ? 0.f : 1.0f / L;
+                *reinterpret_cast<float4*>(a.out + ((long long)b * a.T + t) * a.ld_out + h * HD + d) =
+                    make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+            }
+            ka_cluster_sync();  // no CTA leaves while another reads its shared memory
+            return;
         }
         __syncthreads();
         if (begins) {
@@ -729,7 +861,15 @@ static int kvq_sms() {
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms < 1 ? 1 : (5 * sms > KA_MAX_GRID ? KA_MAX_GRID / 5 : sms);
+    return sms < 1 ? 1 : (4 * sms > KA_MAX_GRID ? KA_MAX_GRID / 4 : sms);
+}
+// CTAs per unit where a cluster takes each unit: as many as leave all units resident, while a warp has no more than
+// KA_TURNS blocks at the cache's capacity (lengths are on the device; longer ones are balanced better by ranges).
+constexpr int KA_TURNS = 10;
+static int kvq_split_of(long long units, int cap, int slots) {
+    for (int s = KA_MAX_SPLIT; s >= 1; s >>= 1)
+        if (units * s <= slots) return cap / 16 <= s * KA_WARPS * KA_TURNS ? s : 0;
+    return 0;
 }
 static int kvq_mode(int rows) { return rows <= 4 ? 0 : rows <= 8 ? 1 : 2; }
 
@@ -744,50 +884,67 @@ bool kvq_attn_fits(int B, int T, int n_head, int n_kv, int cap) {
     return (double)B * n_kv * ((rows + rt - 1) / rt) * ((double)cap / 16 + KA_UNIT_COST) < 2147483648.0;
 }
 
-static cudaError_t kvq_launch(const void* fn, dim3 grid, int threads, size_t smem, void** args, cudaStream_t st, bool pdl) {
+static cudaError_t kvq_launch(const void* fn, dim3 grid, int threads, size_t smem, int cluster, void** args, cudaStream_t st, bool pdl) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = pdl ? 1 : 0;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+template <int BITS, int HD, int MODE, bool CLUSTER>
+static cudaError_t kvq_ready() {  // set once per device; twice is harmless
+    const void* fn = (const void*)tf_kvq_attn_kernel<BITS, HD, MODE, CLUSTER>;
+    static std::atomic<bool> ready[64] = {};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64) dev = 0;
+    if (ready[dev]) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, KvqCfg<BITS, HD, MODE>::SMEM);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    ready[dev].store(true);
+    return cudaSuccess;
 }
 
 template <int BITS, int HD, int MODE>
 static cudaError_t mode_launch(const KvqAttnArgs& a, cudaStream_t st) {
     using F = KvqCfg<BITS, HD, MODE>;
-    const void* fn = (const void*)tf_kvq_attn_kernel<BITS, HD, MODE>;
-    static std::atomic<bool> ready[64] = {};  // set once per device; twice is harmless
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev < 0 || dev >= 64) dev = 0;
-    if (!ready[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, F::SMEM);
-        if (e != cudaSuccess) return e;
-        e = cudaFuncSetAttribute(fn, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        if (e != cudaSuccess) return e;
-        ready[dev].store(true);
-    }
     KvqPlan pl;
-    pl.grid = kvq_sms() * F::CTAS;
+    const int slots = kvq_sms() * F::CTAS;
     pl.rt = F::RT;
     pl.rep = a.n_head / a.n_kv;
     pl.tiles = (a.T * pl.rep + F::RT - 1) / F::RT;
     const long long units = (long long)a.B * a.n_kv * pl.tiles;
-    pl.by_unit = units <= pl.grid;
+    pl.by_unit = units <= slots;
+    pl.split = kvq_split_of(units, a.cap, slots);
     KvqAttnArgs aa = a;
     void* args[] = {&aa, &pl};
-    cudaError_t e = kvq_launch(fn, dim3(pl.grid), KA_THREADS, F::SMEM, args, st, false);
+    if (pl.split) {
+        pl.grid = (int)units * pl.split;
+        const cudaError_t e = kvq_ready<BITS, HD, MODE, true>();
+        if (e != cudaSuccess) return e;
+        return kvq_launch((const void*)tf_kvq_attn_kernel<BITS, HD, MODE, true>, dim3(pl.grid), KA_THREADS, F::SMEM, pl.split, args, st, false);
+    }
+    pl.grid = slots;
+    cudaError_t e = kvq_ready<BITS, HD, MODE, false>();
+    if (e != cudaSuccess) return e;
+    e = kvq_launch((const void*)tf_kvq_attn_kernel<BITS, HD, MODE, false>, dim3(pl.grid), KA_THREADS, F::SMEM, 1, args, st, false);
     if (e != cudaSuccess) return e;
     const int found = pl.by_unit ? (int)units : pl.grid;
     // few units have many parts each: eight warps to a row
-    if (found * F::RT <= 1024) return kvq_launch((const void*)tf_kvq_combine_kernel<1, 8>, dim3(found, F::RT), 256, 0, args, st, true);
-    return kvq_launch((const void*)tf_kvq_combine_kernel<4, 1>, dim3(found, F::RT / 4), 128, 0, args, st, true);
+    if (found * F::RT <= 1024) return kvq_launch((const void*)tf_kvq_combine_kernel<1, 8>, dim3(found, F::RT), 256, 0, 1, args, st, true);
+    return kvq_launch((const void*)tf_kvq_combine_kernel<4, 1>, dim3(found, F::RT / 4), 128, 0, 1, args, st, true);
 }
 template <int BITS, int HD>
 static cudaError_t hd_launch(const KvqAttnArgs& a, cudaStream_t st) {
