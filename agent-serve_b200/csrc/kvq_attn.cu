@@ -3,14 +3,18 @@
 //
 // Row (b, t, h): s_j = q . k_j / sqrt(hd), p_j = exp(s_j - max s), out = sum p_j v_j / sum p_j.
 //
-// Bound by the cache's bytes: a position of one kv head is 2 hd codes (144 bytes with its scales for 128 dims in
-// 4 bits), so every warp instruction per position counts: at 6.5 TB/s an SM has 6.2 cycles for those 144 bytes,
-// 25 issue slots.  Hence mma.sync m16n8k16 with the codes in the order of its fragments: a 32-bit word of eight
-// codes is a shift, four LOP3 and four HADD2 away from four operand registers, and no shared-memory pass or
-// transpose is needed.  Scores have the rows as M and the positions as N (K is the B operand), the second product
-// the dims as M and the rows as N (V transposed is the A operand), so that the scores' registers are the
-// probabilities' operand as they stand.  Up to 8 rows, the M of 16 holds q's high and low halves; up to 4, the N of 8
-// holds p's.  tcgen05 would want the codes unpacked through shared memory and 64 rows or more.
+// Bound by the cache's bytes, then by instructions: a position of one kv head is 2 hd codes (144 bytes with its scales
+// for 128 dims in 4 bits), and at 6.5 TB/s an SM has 6.2 cycles for those, 25 issue slots.  Hence mma.sync m16n8k16
+// with the codes in the order of its fragments: a 32-bit word of eight codes is a shift, four LOP3 and four HADD2 away
+// from four operand registers, and no shared-memory pass is needed.  tcgen05 would want the codes unpacked through
+// shared memory, and 64 rows or more.  The output has the dims as M and the rows as N (V transposed is the A operand).
+// The scores, by the rows of a kv head (times the new rows):
+//   up to 4 (FewRows)   positions as M, rows as N: the 8 columns hold the high and the low half of q, and of p, side by
+//                       side; probabilities go to the second product's operand by movmatrix;
+//   more (ManyRows)     rows as M, positions as N: the scores' registers are the second product's operand as they
+//                       stand; up to 8 rows, the 16 rows of M hold q's two halves.
+// 64 sequences over 16384 positions, 8 kv heads of 128, 4 rows each: 267 us as FewRows, 309 as ManyRows; 16 sequences of 16
+// new rows over 4000 positions, 64 dims: 61 and 56.
 //
 // Arithmetic (fp32-equivalent).  Codes less their zero are exact in f16: (code | 0x6400) is 1024 + code, and
 // the high nibble in place 1024 + 16 code; the 16 is taken out of q (K) or of the output row (V).  q is split
@@ -21,11 +25,13 @@
 // stays below 2^15 and its low half keeps 2^-24 / 2^7 of the largest; it is a row's own, since a row's bits must
 // not hang on what only another row sees.
 //
-// Work is cut into units (sequence, kv head, row tile) and each unit into blocks of 16 positions; the
-// blocks of all units, in order, are dealt out to the CTAs in equal contiguous ranges (lengths are read on the
-// device), a CTA's warps take a range's blocks in turn, each with its own ring of cp.async copies (no barrier
-// in the loop), and join at the range's end.  A unit that a range cuts leaves partial results for
-// tf_kvq_combine_kernel, in a fixed order: results repeat bit for bit.
+// Work is cut into units (sequence, kv head, row tile) and each unit into blocks of 16 positions.  A CTA's warps take
+// its blocks in turn, each with its own ring of cp.async copies (no barrier in the loop), and join at the end.
+//   Short caches: a cluster of 1 to 8 CTAs per unit, which join over distributed shared memory: one launch.
+//   Else the blocks of all units, in order, are dealt out to the CTAs in equal contiguous ranges (lengths are read on
+//   the device, so ragged batches stay balanced); a unit that a range cuts leaves partial results for
+//   tf_kvq_combine_kernel.
+// All joins are in a fixed order: results repeat bit for bit.
 #include <atomic>
 #include <type_traits>
 
@@ -67,17 +73,17 @@ struct KvqCfg {
     static constexpr int RT = kvq_rt(MODE);
     static constexpr int CTAS = kvq_ctas(MODE);                    // per SM
     static constexpr int BLOCK = kvq_block_bytes(BITS, HD);
+    static constexpr int STAGE = 2 * BLOCK;                        // K, then V, of 16 positions
     static constexpr int SLOT = RT * HD * 4;                       // a warp's output rows
-    static constexpr int QF = (MODE == 2 ? 2 : 1) * HD / 32 * 1024;  // q's fragments
+    static constexpr int QF = (MODE == 2 ? 2 : 1) * HD / 32 * (MODE == 0 ? 512 : 1024);  // q's fragments
+    static constexpr int QS = QF > SLOT ? QF : SLOT;               // later a CTA's output rows
     static constexpr int STAT = KA_WARPS * RT * 12;
-    static constexpr int ROOM = 227 * 1024 / CTAS - 1024 - STAT - QF;
-    static constexpr int PB = HD < 128 && ROOM >= 8 * KA_WARPS * BLOCK ? 2 : 1;  // neighbouring blocks of a warp's turn: two where two stages fit
-    static constexpr int STAGE = 2 * PB * BLOCK;                   // K, then V
+    static constexpr int ROOM = 227 * 1024 / CTAS - 1024 - STAT - QS;
     static constexpr int FIT = ROOM / (KA_WARPS * STAGE);
     static constexpr int ST = FIT > 8 ? 8 : FIT;                   // stages of a warp's ring
     static constexpr int RING = ST * STAGE > SLOT ? ST * STAGE : SLOT;  // output rows take the rings' place
-    static constexpr int SMEM = KA_WARPS * RING + STAT + QF;
-    static_assert(ST >= 2 && KA_WARPS * RING + STAT + QF <= 227 * 1024 / CTAS - 1024, "two stages at least");
+    static constexpr int SMEM = KA_WARPS * RING + STAT + QS;
+    static_assert(ST >= 2 && SMEM <= 227 * 1024 / CTAS - 1024, "two stages at least");
 };
 
 __device__ __forceinline__ float ka_exp2(float x) {
@@ -90,6 +96,12 @@ __device__ __forceinline__ void ka_mma(float (&c)[4], const uint32_t (&a)[4], co
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 8 x 8 halves, row g in the lanes 4 g .. 4 g + 3, to their transpose
+__device__ __forceinline__ uint32_t ka_trans(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 __device__ __forceinline__ uint32_t ka_pack_rz(float lo, float hi) {  // towards zero
     uint32_t y;
@@ -169,19 +181,23 @@ __device__ __forceinline__ void ka_words(const uint8_t* p, int lane, uint32_t (&
     for (int c = 0; c < N / 4; ++c) ka_lds4(p + c * 512 + lane * 16, &w[4 * c]);
     if (N % 4) ka_lds2(p + N / 4 * 512 + lane * 8, &w[N - 2]);
 }
-// the scales of positions 2 tq, 2 tq + 8, 2 tq + 1, 2 tq + 9: NG = HD / 32 groups each, two to a word
+// the scales of positions g and g + 8: NG = HD / 32 groups each, two to a word
 template <int NG>
-__device__ __forceinline__ void ka_scales(const uint8_t* p, int tq, uint32_t (&s)[2 * NG]) {
+__device__ __forceinline__ void ka_scales(const uint8_t* p, int g, uint32_t (&s)[NG]) {
+    const uint8_t* q = p + g * (4 * NG);
+    if (NG % 4 == 0) {
+        ka_lds4(q, s);
+    } else if (NG % 2 == 0) {
+        ka_lds2(q, s);
+    } else {
 #pragma unroll
-    for (int i = 0; i < 2 * NG; i += NG % 2 ? 2 : 4) {
-        if (NG % 2) ka_lds2(p + tq * (8 * NG) + 4 * i, &s[i]);
-        else ka_lds4(p + tq * (8 * NG) + 4 * i, &s[i]);
+        for (int i = 0; i < NG; ++i) s[i] = *reinterpret_cast<const uint32_t*>(q + 4 * i);
     }
 }
-// Scale of group k of position 2 tq + e (e = 0, 1) or 2 tq + 8 + e - 2 (e = 2, 3).
-template <int N>
-__device__ __forceinline__ float ka_scale(const uint32_t (&s)[N], int e, int k) {
-    const int i = ((e & 1) * 2 + (e >> 1)) * (N / 2) + k;
+// Scale of group k of position g + 8 half.
+template <int NG>
+__device__ __forceinline__ float ka_scale(const uint32_t (&s)[NG], int half, int k) {
+    const int i = half * NG + k;
     const __half2 h = *reinterpret_cast<const __half2*>(&s[i >> 1]);
     return i & 1 ? __high2float(h) : __low2float(h);
 }
@@ -264,24 +280,560 @@ __device__ __forceinline__ float4 ka_remote4(const float* p, int rank) {
     return x;
 }
 
+// ---- a warp's work on a unit's blocks --------------------------------------------------------------------
+// What a segment of a unit is to its warps.
+struct KvqSeg {
+    int b, kvh, r0, rows, rep, T, n_ctx;  // rows r0 .. r0 + rows - 1 of the unit's (new row, head) pairs
+    int open_to;                          // every row sees the positions up to here
+};
+__device__ __forceinline__ const float* kvq_query(const KvqAttnArgs& a, const KvqSeg& sg, int row, int hd) {
+    const int rr = sg.r0 + row, t = rr / sg.rep, h = sg.kvh * sg.rep + rr - t * sg.rep;
+    return a.q + ((long long)sg.b * sg.T + t) * a.ld_q + h * hd;
+}
+// A row's largest value goes to [2^13, 2^14); rows of zeros, subnormals and infinities stay as they are.
+__device__ __forceinline__ int kvq_shift(float mx) {
+    const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
+    return ex <= -127 || ex == 128 ? 0 : max(-120, min(120, 13 - ex));
+}
+template <int RT>
+__device__ __forceinline__ float kvq_row_max(const float* q_max, int row) {  // over the warps' groups
+    float mx = q_max[row];
+#pragma unroll
+    for (int i = 1; i < KA_WARPS; ++i) mx = fmaxf(mx, q_max[i * RT + row]);
+    return mx;
+}
+// Eight dims of q from 8 tq on of group k, as f16 halves in the order of a word's codes: registers 0 .. 3 pair codes 4
+// apart in 4 bits (odd ones times 16), 2 apart in 8.
+template <int BITS>
+__device__ __forceinline__ void kvq_split_q(const float (&x)[8], float sc, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e0 = BITS == 4 ? j : (j >> 1) * 4 + (j & 1), e1 = BITS == 4 ? j + 4 : e0 + 2;
+        const float down = BITS == 4 && (j & 1) ? sc * 0.0625f : sc;
+        const float u = x[e0] * down, v = x[e1] * down;
+        hi[j] = ka_pack(u, v);
+        const float2 f = ka_unpack(hi[j]);
+        lo[j] = ka_pack(u - f.x, v - f.y);
+    }
+}
+// A row's running state: largest score and the one that moves it (both in q's scale), minus the exponent that p is
+// relative to, sum, and the largest V scale that the row saw, rounded up within its binary order.
+struct KvqRow {
+    float m, thr, nref, l;
+    uint32_t top;
+    __device__ __forceinline__ void clear() {
+        m = thr = -INFINITY;
+        nref = l = 0.f;
+        top = 0;
+    }
+    // New largest score and V scale; returns what the row's sums are multiplied with.  A row moves by what it sees
+    // alone, whichever row asked.
+    __device__ __forceinline__ float move(float mx, uint32_t tp, float fr) {
+        if (!(mx > thr || tp > top)) return 1.0f;
+        tp |= 0x3FFu;  // scales are below 2^(tp / 1024 - 14)
+        const float r = mx == -INFINITY ? 0.f : (float)(15 - KA_SLACK + 14 - (int)(tp >> 10)) - mx * fr;
+        const float f = m == -INFINITY ? 0.f : ka_exp2(r - nref);  // (nothing seen yet: sums of zero, or NaN, which stays)
+        m = mx;
+        thr = mx + (float)KA_SLACK / fr;
+        nref = r;
+        top = tp;
+        l *= f;
+        return f;
+    }
+    __device__ __forceinline__ bool none() const { return m == -INFINITY && l == 0.f; }
+};
+__device__ __forceinline__ uint32_t ka_scale_bits(uint32_t v, uint32_t top) {  // NaN and infinity have no say
+    v &= 0x7FFFu;
+    return v < 0x7C00u ? max(v, top) : top;
+}
+// Whether a V scale of a block is above `top` (a lane looks at one word of them).
+template <int HD>
+__device__ __forceinline__ bool ka_scale_above(const uint8_t* scales, int lane, uint32_t top) {
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(scales + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
+    return (word & 0xFFFFu) > top || word >> 16 > top;
+}
+__device__ __forceinline__ uint32_t ka_magic() {
+    uint32_t m;
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(m));
+    return m;
+}
+
+// Up to 4 rows.  Column c of N is row c & 3: the high half below 4, the low half from 4 on.  A thread holds
+// columns 2 tq and 2 tq + 1, positions g and g + 8 of a block, and dims 16 d + 2 g and one on of the output.
+template <int BITS, int HD>
+struct FewRows {
+    static constexpr int RT = 4, NG = HD / 32, W = HD * BITS / 64, CODES = kvq_code_bytes(BITS, HD), BLOCK = kvq_block_bytes(BITS, HD);
+    static constexpr int NQ = (NG + KA_WARPS - 1) / KA_WARPS;
+    const uint8_t* q_at;
+    int lane, g, tq;
+    uint32_t magic;
+    float2 fr;  // out of q's scale, to powers of two
+    int2 lim;   // last position that the row sees
+    KvqRow r0, r1;
+    float o[HD / 16][4];
+    uint32_t top_all;  // the least of all rows' tops
+
+    // q to [NG][lane] four registers; each warp lays out every KA_WARPS-th group.
+    __device__ __forceinline__ void load_q(const KvqAttnArgs& a, const KvqSeg& sg, uint8_t* qs, float* q_max, int warp, float log2e_d) {
+        lane = threadIdx.x & 31;
+        g = lane >> 2;
+        tq = lane & 3;
+        magic = ka_magic();
+        q_at = qs + lane * 16;
+        float x[NQ][8], mx = 0.f;
+        const bool valid = (g & 3) < sg.rows;
+        const float* qp = kvq_query(a, sg, valid ? g & 3 : 0, HD) + tq * 8;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int k = i * KA_WARPS + warp;
+            const bool in = valid && k < NG;
+            const float4 u = in ? *reinterpret_cast<const float4*>(qp + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+            const float4 v = in ? *reinterpret_cast<const float4*>(qp + k * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+            float* y = x[i];
+            y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w;
+            y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(y[j]));
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+        if (tq == 0 && g < RT) q_max[warp * RT + g] = mx;
+        __syncthreads();
+        const float sc = __int_as_float((kvq_shift(kvq_row_max<RT>(q_max, g & 3)) + 127) << 23);
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int k = i * KA_WARPS + warp;
+            if (k >= NG) continue;
+            uint32_t hi[4], lo[4];
+            kvq_split_q<BITS>(x[i], sc, hi, lo);
+            *reinterpret_cast<uint4*>(qs + k * 512 + lane * 16) =
+                g < 4 ? make_uint4(hi[0], hi[1], hi[2], hi[3]) : make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        const int c = (2 * tq) & 3;
+        fr.x = __int_as_float((127 - kvq_shift(kvq_row_max<RT>(q_max, c))) << 23) * log2e_d;
+        fr.y = __int_as_float((127 - kvq_shift(kvq_row_max<RT>(q_max, c + 1))) << 23) * log2e_d;
+        lim.x = sg.n_ctx + (sg.r0 + c) / sg.rep;
+        lim.y = sg.n_ctx + (sg.r0 + c + 1) / sg.rep;
+        __syncthreads();
+        r0.clear();
+        r1.clear();
+        top_all = 0;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[d][0] = o[d][1] = o[d][2] = o[d][3] = 0.f;
+    }
+
+    // One block at `kb` (K, then V), from position p0 on.
+    template <bool MASKED>
+    __device__ __forceinline__ void block(const uint8_t* kb, int p0) {
+        const uint8_t* vb = kb + BLOCK;
+        const int pos = p0 + g;
+        auto seen = [&](int limit, int e) { return !MASKED || pos + 8 * e <= limit; };
+        float2 x[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        {
+            uint32_t w[W], s[NG];
+            ka_words<W>(kb, lane, w);
+            ka_scales<NG>(kb + CODES, g, s);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                uint32_t a0[4], a1[4], q[4];
+                if (BITS == 4) {
+                    uint32_t u[4], v[4];
+                    ka_nibbles(w[k], magic, u);
+                    ka_nibbles(w[W / 2 + k], magic, v);
+                    a0[0] = u[0]; a0[1] = v[0]; a0[2] = u[1]; a0[3] = v[1];
+                    a1[0] = u[2]; a1[1] = v[2]; a1[2] = u[3]; a1[3] = v[3];
+                } else {
+                    ka_bytes(w[2 * k], magic, a0[0], a0[2]);
+                    ka_bytes(w[W / 2 + 2 * k], magic, a0[1], a0[3]);
+                    ka_bytes(w[2 * k + 1], magic, a1[0], a1[2]);
+                    ka_bytes(w[W / 2 + 2 * k + 1], magic, a1[1], a1[3]);
+                }
+                const float s0 = ka_scale<NG>(s, 0, k), s1 = ka_scale<NG>(s, 1, k);
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                ka_lds4(q_at + k * 512, q);
+                ka_mma(c, a0, q[0], q[1]);
+                ka_mma(c, a1, q[2], q[3]);
+                x[0].x = fmaf(c[0], s0, x[0].x);
+                x[0].y = fmaf(c[1], s0, x[0].y);
+                x[1].x = fmaf(c[2], s1, x[1].x);
+                x[1].y = fmaf(c[3], s1, x[1].y);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {  // the high half's part and the low half's
+            x[e].x += __shfl_xor_sync(0xFFFFFFFFu, x[e].x, 2);
+            x[e].y += __shfl_xor_sync(0xFFFFFFFFu, x[e].y, 2);
+        }
+        uint32_t vs[NG];
+        ka_scales<NG>(vb + CODES, g, vs);
+        bool raise = ka_scale_above<HD>(vb + CODES, lane, top_all);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (!seen(lim.x, e)) x[e].x = -INFINITY;
+            if (!seen(lim.y, e)) x[e].y = -INFINITY;
+            raise |= x[e].x > r0.thr || x[e].y > r1.thr;
+        }
+        if (__any_sync(0xFFFFFFFFu, raise)) {
+            float m0 = fmaxf(r0.m, fmaxf(x[0].x, x[1].x)), m1 = fmaxf(r1.m, fmaxf(x[0].y, x[1].y));
+            uint32_t t0 = r0.top, t1 = r1.top;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                uint32_t big = 0;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                    const int i = e * NG + k;
+                    big = ka_scale_bits(i & 1 ? vs[i >> 1] >> 16 : vs[i >> 1], big);
+                }
+                if (seen(lim.x, e)) t0 = max(t0, big);
+                if (seen(lim.y, e)) t1 = max(t1, big);
+            }
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) {
+                m0 = fmaxf(m0, __shfl_xor_sync(0xFFFFFFFFu, m0, s));
+                m1 = fmaxf(m1, __shfl_xor_sync(0xFFFFFFFFu, m1, s));
+                t0 = max(t0, __shfl_xor_sync(0xFFFFFFFFu, t0, s));
+                t1 = max(t1, __shfl_xor_sync(0xFFFFFFFFu, t1, s));
+            }
+            const float f0 = r0.move(m0, t0, fr.x), f1 = r1.move(m1, t1, fr.y);
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+                o[d][0] *= f0;
+                o[d][1] *= f1;
+                o[d][2] *= f0;
+                o[d][3] *= f1;
+            }
+            top_all = __reduce_min_sync(0xFFFFFFFFu, min(r0.top, r1.top));
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float2 y = ka_fma2(x[e], fr, make_float2(r0.nref, r1.nref));
+            x[e] = make_float2(ka_exp2(y.x), ka_exp2(y.y));
+            r0.l += x[e].x;
+            r1.l += x[e].y;
+        }
+        uint32_t w[W];
+        ka_words<W>(vb, lane, w);
+        const float low = tq < 2 ? 0.f : -1.f;  // columns from 4 on take what the high half leaves
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            uint32_t pf[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float sc = ka_scale<NG>(vs, e, k);
+                float2 y = make_float2(x[e].x * sc, x[e].y * sc);
+                if (MASKED) {  // an unseen position's scale may be NaN
+                    if (!seen(lim.x, e)) y.x = 0.f;
+                    if (!seen(lim.y, e)) y.y = 0.f;
+                }
+                const float2 z = ka_fma2(ka_unpack(ka_pack(y.x, y.y)), make_float2(low, low), y);
+                pf[e] = ka_trans(ka_pack(z.x, z.y));
+            }
+#pragma unroll
+            for (int d = 2 * k; d < 2 * k + 2; ++d) {
+                uint32_t v[4];
+                if (BITS == 4) {
+                    ka_nibbles(w[d], magic, v);
+                } else {
+                    ka_bytes(w[2 * d], magic, v[0], v[2]);
+                    ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
+                }
+                ka_mma(o[d], v, pf[0], pf[1]);
+            }
+        }
+    }
+
+    // The warp's rows to slot [RT][HD], exponents and sums to stat; a warp that saw nothing says so by its exponent.
+    __device__ __forceinline__ void store(float* slot, float* exps, float* sums) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int row = 2 * tq + j;
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+                float2 y = make_float2(o[d][j], o[d][2 + j] * (BITS == 4 ? 0.0625f : 1.0f));
+                y.x += __shfl_xor_sync(0xFFFFFFFFu, y.x, 2);
+                y.y += __shfl_xor_sync(0xFFFFFFFFu, y.y, 2);
+                if (row < RT) *reinterpret_cast<float2*>(slot + row * HD + 16 * d + 2 * g) = y;
+            }
+            KvqRow& r = j ? r1 : r0;
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) r.l += __shfl_xor_sync(0xFFFFFFFFu, r.l, s);
+            if (g == 0 && row < RT) {
+                exps[row] = r.none() ? -INFINITY : -r.nref;
+                sums[row] = r.l;
+            }
+        }
+    }
+};
+
+// Up to 8 rows (NR 1: row g of M is q's high half, row g + 8 its low half) or 16 (NR 2: rows g and g + 8, the halves one
+// after the other).  A thread holds row g (and g + 8), positions 2 tq, 2 tq + 1 and 8 on of a block; of the output
+// columns 2 tq and 2 tq + 1, dims 16 d + 2 g and one on.
+template <int BITS, int HD, int NR>
+struct ManyRows {
+    static constexpr int RT = 8 * NR, NG = HD / 32, W = HD * BITS / 64, CODES = kvq_code_bytes(BITS, HD), BLOCK = kvq_block_bytes(BITS, HD);
+    static constexpr int NQ = (NG + KA_WARPS - 1) / KA_WARPS;
+    const uint8_t* q_at;
+    int lane, g, tq;
+    uint32_t magic;
+    float fr[NR];
+    int lim[NR];
+    KvqRow r[NR];
+    float o[NR][HD / 16][4];
+    uint32_t top_all;
+
+    // q to [NR][NG][2][lane] four registers
+    __device__ __forceinline__ void load_q(const KvqAttnArgs& a, const KvqSeg& sg, uint8_t* qs, float* q_max, int warp, float log2e_d) {
+        lane = threadIdx.x & 31;
+        g = lane >> 2;
+        tq = lane & 3;
+        magic = ka_magic();
+        q_at = qs + lane * 16;
+        float x[NR][NQ][8];
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            const int row = nr * 8 + g;
+            const bool valid = row < sg.rows;
+            const float* qp = kvq_query(a, sg, valid ? row : 0, HD) + tq * 8;
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int k = i * KA_WARPS + warp;
+                const bool in = valid && k < NG;
+                const float4 u = in ? *reinterpret_cast<const float4*>(qp + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
+                const float4 v = in ? *reinterpret_cast<const float4*>(qp + k * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+                float* y = x[nr][i];
+                y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w;
+                y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(y[j]));
+            }
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
+            if (tq == 0) q_max[warp * RT + row] = mx;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+            const int row = nr * 8 + g, sh = kvq_shift(kvq_row_max<RT>(q_max, row));
+            const float sc = __int_as_float((sh + 127) << 23);
+            fr[nr] = __int_as_float((127 - sh) << 23) * log2e_d;
+            lim[nr] = sg.n_ctx + (sg.r0 + row) / sg.rep;
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                const int k = i * KA_WARPS + warp;
+                if (k >= NG) continue;
+                uint32_t hi[4], lo[4];
+                kvq_split_q<BITS>(x[nr][i], sc, hi, lo);
+                uint32_t* dst = reinterpret_cast<uint32_t*>(qs + k * 1024 + lane * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t* d = dst + (j >> 1) * 128 + (j & 1) * 2;
+                    if (NR == 2) {
+                        d[nr] = hi[j];
+                        d[NG * 256 + nr] = lo[j];
+                    } else {
+                        d[0] = hi[j];
+                        d[1] = lo[j];
+                    }
+                }
+            }
+            r[nr].clear();
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) o[nr][d][0] = o[nr][d][1] = o[nr][d][2] = o[nr][d][3] = 0.f;
+        }
+        top_all = 0;
+        __syncthreads();
+    }
+
+    // The scales of positions 2 tq, 2 tq + 8, 2 tq + 1, 2 tq + 9, NG each, two to a word.
+    __device__ __forceinline__ void scales(const uint8_t* p, uint32_t (&s)[2 * NG]) const {
+#pragma unroll
+        for (int i = 0; i < 2 * NG; i += NG % 2 ? 2 : 4) {
+            if (NG % 2) ka_lds2(p + tq * (8 * NG) + 4 * i, &s[i]);
+            else ka_lds4(p + tq * (8 * NG) + 4 * i, &s[i]);
+        }
+    }
+    // Scale of group k of position 2 tq + e (e = 0, 1) or 2 tq + 6 + e (e = 2, 3).
+    static __device__ __forceinline__ float scale(const uint32_t (&s)[2 * NG], int e, int k) {
+        const int i = ((e & 1) * 2 + (e >> 1)) * NG + k;
+        const __half2 h = *reinterpret_cast<const __half2*>(&s[i >> 1]);
+        return i & 1 ? __high2float(h) : __low2float(h);
+    }
+
+    template <bool MASKED>
+    __device__ __forceinline__ void block(const uint8_t* kb, int p0) {
+        const uint8_t* vb = kb + BLOCK;
+        auto seen = [&](int nr, int e) { return !MASKED || p0 + 2 * tq + (e & 1) + (e >> 1) * 8 <= lim[nr]; };
+        float2 x[NR][2];
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) x[nr][0] = x[nr][1] = make_float2(0.f, 0.f);
+        {
+            uint32_t w[W], s[2 * NG];
+            ka_words<W>(kb, lane, w);
+            scales(kb + CODES, s);
+#pragma unroll
+            for (int k = 0; k < NG; ++k) {
+                uint32_t qf[NR][2][4];
+#pragma unroll
+                for (int part = 0; part < NR; ++part) {
+                    ka_lds4(q_at + (part * NG + k) * 1024, qf[part][0]);
+                    ka_lds4(q_at + (part * NG + k) * 1024 + 512, qf[part][1]);
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t f[4];
+                    if (BITS == 4) {
+                        ka_nibbles(w[half * (W / 2) + k], magic, f);
+                    } else {
+                        ka_bytes(w[half * (W / 2) + 2 * k], magic, f[0], f[1]);
+                        ka_bytes(w[half * (W / 2) + 2 * k + 1], magic, f[2], f[3]);
+                    }
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int part = NR - 1; part >= 0; --part) {  // the low halves first
+                        ka_mma(c, qf[part][0], f[0], f[1]);
+                        ka_mma(c, qf[part][1], f[2], f[3]);
+                    }
+                    const float2 sc = make_float2(scale(s, half * 2, k), scale(s, half * 2 + 1, k));
+                    x[NR - 1][half] = ka_fma2(make_float2(c[2], c[3]), sc, x[NR - 1][half]);
+                    x[0][half] = ka_fma2(make_float2(c[0], c[1]), sc, x[0][half]);
+                }
+            }
+        }
+        uint32_t vs[2 * NG];
+        scales(vb + CODES, vs);
+        bool raise = ka_scale_above<HD>(vb + CODES, lane, top_all);
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                if (!seen(nr, 2 * e)) x[nr][e].x = -INFINITY;
+                if (!seen(nr, 2 * e + 1)) x[nr][e].y = -INFINITY;
+                raise |= x[nr][e].x > r[nr].thr || x[nr][e].y > r[nr].thr;
+            }
+        if (__any_sync(0xFFFFFFFFu, raise)) {
+            uint32_t least = 0xFFFFu;
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) {
+                float mx = r[nr].m;
+                uint32_t tp = r[nr].top;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    mx = fmaxf(mx, e & 1 ? x[nr][e >> 1].y : x[nr][e >> 1].x);
+                    if (seen(nr, e)) {
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const int i = ((e & 1) * 2 + (e >> 1)) * NG + k;
+                            tp = ka_scale_bits(i & 1 ? vs[i >> 1] >> 16 : vs[i >> 1], tp);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int s = 1; s < 4; s <<= 1) {
+                    mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, s));
+                    tp = max(tp, __shfl_xor_sync(0xFFFFFFFFu, tp, s));
+                }
+                const float f = r[nr].move(mx, tp, fr[nr]);
+                least = min(least, r[nr].top);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float fc = __shfl_sync(0xFFFFFFFFu, f, (2 * tq + j) * 4);
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d) {
+                        o[nr][d][j] *= fc;
+                        o[nr][d][2 + j] *= fc;
+                    }
+                }
+            }
+            top_all = __reduce_min_sync(0xFFFFFFFFu, least);
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float2 y = ka_fma2(x[nr][e], make_float2(fr[nr], fr[nr]), make_float2(r[nr].nref, r[nr].nref));
+                x[nr][e] = make_float2(ka_exp2(y.x), ka_exp2(y.y));
+                r[nr].l += x[nr][e].x + x[nr][e].y;
+            }
+        uint32_t w[W];
+        ka_words<W>(vb, lane, w);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            uint32_t hi[NR][2], lo[NR][2];
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float2 y = ka_mul2(x[nr][e], make_float2(scale(vs, 2 * e, k), scale(vs, 2 * e + 1, k)));
+                    if (MASKED) {  // an unseen position's scale may be NaN
+                        if (!seen(nr, 2 * e)) y.x = 0.f;
+                        if (!seen(nr, 2 * e + 1)) y.y = 0.f;
+                    }
+                    // cut after 11 bits, and what is left
+                    const float2 h = make_float2(__uint_as_float(__float_as_uint(y.x) & 0xFFFFE000u), __uint_as_float(__float_as_uint(y.y) & 0xFFFFE000u));
+                    const float2 z = ka_fma2(h, make_float2(-1.f, -1.f), y);
+                    hi[nr][e] = ka_pack_rz(y.x, y.y);
+                    lo[nr][e] = ka_pack_rz(z.x, z.y);
+                }
+#pragma unroll
+            for (int d = 2 * k; d < 2 * k + 2; ++d) {
+                uint32_t v[4];
+                if (BITS == 4) {
+                    ka_nibbles(w[d], magic, v);
+                } else {
+                    ka_bytes(w[2 * d], magic, v[0], v[2]);
+                    ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
+                }
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) {
+                    ka_mma(o[nr][d], v, lo[nr][0], lo[nr][1]);
+                    ka_mma(o[nr][d], v, hi[nr][0], hi[nr][1]);
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(float* slot, float* exps, float* sums) {
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d)
+                    *reinterpret_cast<float2*>(slot + (nr * 8 + 2 * tq + j) * HD + 16 * d + 2 * g) =
+                        make_float2(o[nr][d][j], o[nr][d][2 + j] * (BITS == 4 ? 0.0625f : 1.0f));
+            r[nr].l += __shfl_xor_sync(0xFFFFFFFFu, r[nr].l, 1);
+            r[nr].l += __shfl_xor_sync(0xFFFFFFFFu, r[nr].l, 2);
+            if (tq == 0) {
+                exps[nr * 8 + g] = r[nr].none() ? -INFINITY : -r[nr].nref;
+                sums[nr * 8 + g] = r[nr].l;
+            }
+        }
+    }
+};
+template <int BITS, int HD, int MODE>
+struct KvqCore {
+    using type = ManyRows<BITS, HD, MODE>;
+};
+template <int BITS, int HD>
+struct KvqCore<BITS, HD, 0> {
+    using type = FewRows<BITS, HD>;
+};
+
 // CLUSTER: a cluster of pl.split CTAs per unit (all of them, from the sequences' T rows), which join over distributed
 // shared memory; else ranges, and a second launch.
 template <int BITS, int HD, int MODE, bool CLUSTER>
 __global__ void __launch_bounds__(KA_THREADS, KvqCfg<BITS, HD, MODE>::CTAS)
 tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     using F = KvqCfg<BITS, HD, MODE>;
-    constexpr int RT = F::RT, NG = HD / 32, W = HD * BITS / 64, CODES = kvq_code_bytes(BITS, HD);
-    constexpr int NR = MODE == 2 ? 2 : 1;  // rows of a thread: g, and g + 8
-    constexpr int QP = MODE == 2 ? 2 : 1;  // products of q's halves: side by side in M, or one after the other
-    constexpr int PP = MODE == 0 ? 1 : 2;  // products of p's halves: side by side in N, or one after the other
+    constexpr int RT = F::RT;
     extern __shared__ __align__(128) uint8_t smem[];
     if (!CLUSTER) pdl_trigger();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring_at = warp * (F::ST * F::STAGE), ring = smem_u32(smem) + ring_at;
-    uint8_t* qs = smem + KA_WARPS * F::RING;  // [QP][NG][2][lane] four registers
-    const uint8_t* q_at = qs + lane * 16;
+    uint8_t* qs = smem + KA_WARPS * F::RING;
     float* slot_all = reinterpret_cast<float*>(smem);  // where the rings are, once a segment's blocks are done
-    float* stat = reinterpret_cast<float*>(qs + F::QF);  // [warp][RT] exponents, then sums, then q's maxima
+    float* stat = reinterpret_cast<float*>(qs + F::QS);  // [warp][RT] exponents, then sums, then q's maxima
     float* q_max = stat + 2 * KA_WARPS * RT;
     KvqDesc* desc = static_cast<KvqDesc*>(a.ws);
     float* parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a.ws) + KA_DESC_BYTES);
@@ -298,8 +850,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
     }
     KvqDesc open = {-1, 0, 0, 0, 0, 0};  // the unit that begins here and ends in a later CTA
     const float log2e_d = 1.4426950408889634f * rsqrtf((float)HD);
-    uint32_t magic;
-    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+    typename KvqCore<BITS, HD, MODE>::type core;
 
 #pragma unroll 1
     for (int gpos = range.g0; gpos < range.g1;) {
@@ -345,337 +896,48 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             rows = min(RT, sq.n_new * pl.rep - r0);
         }
 
-        // this warp's turns of PB blocks: warp, and every KA_WARPS-th from there
-        const int turns = (blk1 - blk0 + F::PB - 1) / F::PB, n_mine = turns > warp ? (turns - warp + KA_WARPS - 1) / KA_WARPS : 0;
-        const long long where = sq.slot * a.slot_bytes + kvh * a.head_bytes + (long long)(blk0 + warp * F::PB) * F::BLOCK + lane * 16;
+        // this warp's blocks: blk0 + warp, and every KA_WARPS-th from there
+        const int n_mine = blk1 - blk0 > warp ? (blk1 - blk0 - warp + KA_WARPS - 1) / KA_WARPS : 0;
+        const long long where = sq.slot * a.slot_bytes + kvh * a.head_bytes + (long long)(blk0 + warp) * F::BLOCK + lane * 16;
         const uint8_t *kc = a.kc + where, *vc = a.vc + where;
-        int left = blk1 - blk0 - warp * F::PB;  // blocks from the next turn on
+        int left = n_mine;
         uint32_t fill = ring;
-        auto fetch = [&]() {  // the next turn into the next stage
+        auto fetch = [&]() {  // the next block into the next stage
             if (left > 0) {
                 const uint32_t dst = fill + lane * 16;
-                const int bytes = left >= F::PB ? F::PB * F::BLOCK : F::BLOCK;  // (a segment's last turn may lack a block)
-                if (F::PB == 1 || left >= F::PB) {
 #pragma unroll
-                    for (int c = 0; c < F::PB * F::BLOCK; c += 512)
-                        if (c + 512 <= F::PB * F::BLOCK || lane * 16 < F::PB * F::BLOCK - c) {
-                            ka_copy16(dst + c, kc + c);
-                            ka_copy16(dst + F::PB * F::BLOCK + c, vc + c);
-                        }
-                } else {
-                    for (int c = 0; c + lane * 16 < bytes; c += 512) {
+                for (int c = 0; c < F::BLOCK; c += 512)
+                    if (c + 512 <= F::BLOCK || lane * 16 < F::BLOCK - c) {
                         ka_copy16(dst + c, kc + c);
-                        ka_copy16(dst + F::PB * F::BLOCK + c, vc + c);
+                        ka_copy16(dst + F::BLOCK + c, vc + c);
                     }
-                }
-                left -= KA_WARPS * F::PB;
-                kc += KA_WARPS * F::PB * F::BLOCK;
-                vc += KA_WARPS * F::PB * F::BLOCK;
+                --left;
+                kc += KA_WARPS * F::BLOCK;
+                vc += KA_WARPS * F::BLOCK;
                 fill = fill == ring + (F::ST - 1) * F::STAGE ? ring : fill + F::STAGE;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
         for (int i = 0; i < F::ST - 1; ++i) fetch();
-
-        // q as A fragments in shared memory.  Rows g and g + 8 of M: the tile's rows (MODE 2), or the high and the low
-        // half of one.  Each warp lays out every KA_WARPS-th group.
-        constexpr int NQ = (NG + KA_WARPS - 1) / KA_WARPS;
-        float fr[NR];  // out of q's scale, to powers of two
-        int lim[NR];   // last position that the row sees
-        {
-            float x[NR][NQ][8];
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-                const int row = MODE == 0 ? g & 3 : nr * 8 + g, rr = r0 + row;
-                const bool valid = row < rows;
-                const int t = valid ? rr / pl.rep : 0, h = valid ? kvh * pl.rep + rr - t * pl.rep : 0;
-                const float* qp = a.q + ((long long)b * a.T + t) * a.ld_q + h * HD + tq * 8;
-                float mx = 0.f;
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    const int k = i * KA_WARPS + warp;
-                    const bool in = valid && k < NG;
-                    const float4 u = in ? *reinterpret_cast<const float4*>(qp + k * 32) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    const float4 v = in ? *reinterpret_cast<const float4*>(qp + k * 32 + 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    float* y = x[nr][i];
-                    y[0] = u.x; y[1] = u.y; y[2] = u.z; y[3] = u.w;
-                    y[4] = v.x; y[5] = v.y; y[6] = v.z; y[7] = v.w;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(y[j]));
-                }
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, 2));
-                if (tq == 0 && row < RT) q_max[warp * RT + row] = mx;
-                lim[nr] = sq.n_ctx + (r0 + row) / pl.rep;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-                const int row = MODE == 0 ? g & 3 : nr * 8 + g;
-                float mx = q_max[row];
-#pragma unroll
-                for (int i = 1; i < KA_WARPS; ++i) mx = fmaxf(mx, q_max[i * RT + row]);
-                // the row's largest value goes to [2^13, 2^14); rows of zeros, subnormals and infinities as they are
-                const int ex = (int)(__float_as_uint(mx) >> 23) - 127;
-                const int sh = ex <= -127 || ex == 128 ? 0 : max(-120, min(120, 13 - ex));
-                const float sc = __int_as_float((sh + 127) << 23);
-                fr[nr] = __int_as_float((127 - sh) << 23) * log2e_d;
-#pragma unroll
-                for (int i = 0; i < NQ; ++i) {
-                    const int k = i * KA_WARPS + warp;
-                    if (k >= NG) continue;
-                    uint32_t* dst = reinterpret_cast<uint32_t*>(qs + k * 1024 + lane * 16);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        // codes 4 apart share a register in 4 bits (odd ones times 16), codes 2 apart in 8
-                        const int e0 = BITS == 4 ? j : (j >> 1) * 4 + (j & 1), e1 = BITS == 4 ? j + 4 : e0 + 2;
-                        const float down = BITS == 4 && (j & 1) ? sc * 0.0625f : sc;
-                        const float u = x[nr][i][e0] * down, v = x[nr][i][e1] * down;
-                        const uint32_t hi = ka_pack(u, v);
-                        const float2 f = ka_unpack(hi);
-                        const uint32_t lo = ka_pack(u - f.x, v - f.y);
-                        uint32_t* d = dst + (j >> 1) * 128 + (j & 1) * 2;
-                        if (MODE == 2) {
-                            d[nr] = hi;
-                            d[NG * 256 + nr] = lo;
-                        } else {
-                            d[0] = hi;
-                            d[1] = lo;
-                        }
-                    }
-                }
-            }
-            __syncthreads();
-        }
-        const int open_to = sq.n_ctx + r0 / pl.rep;  // every row sees the positions up to here
-
-        // Columns 2 tq and 2 tq + 1 of the output; dims 16 d + 2 g and one on.
-        float o[NR][HD / 16][4];
-        // Row g (and g + 8): largest score and the one that moves it (both in q's scale), exponent that p is
-        // relative to, sum
-        float m[NR], ref[NR], thr[NR], l[NR];
-        uint32_t top[NR];          // largest V scale that the row saw, rounded up within its binary order
-        uint32_t top_all = 0;      // the least of all rows' tops, twice
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-#pragma unroll
-            for (int j = 0; j < HD / 16; ++j) o[nr][j][0] = o[nr][j][1] = o[nr][j][2] = o[nr][j][3] = 0.f;
-            m[nr] = thr[nr] = -INFINITY;
-            ref[nr] = l[nr] = 0.f;
-            top[nr] = 0;
-        }
-
-        // One turn at `at` (its K, then its V), from position p0 on.
-        constexpr int PB = F::PB;
-        auto turn = [&](auto masked_c, const uint8_t* at, const int p0) {
-            constexpr bool MASKED = decltype(masked_c)::value;
-            const int end = MASKED ? min(p0 + 16 * PB, blk1 * 16) : 0;
-            // scores of row g (and g + 8) against positions 2 tq, 2 tq + 1 (x, y), and 8 on, of each block
-            float2 x[PB][NR][2];
-#pragma unroll
-            for (int pb = 0; pb < PB; ++pb) {
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr) x[pb][nr][0] = x[pb][nr][1] = make_float2(0.f, 0.f);
-                const uint8_t* kb = at + pb * F::BLOCK;
-                uint32_t w[W], s[2 * NG];
-                ka_words<W>(kb, lane, w);
-                ka_scales<NG>(kb + CODES, tq, s);
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    uint32_t qf[QP][2][4];
-#pragma unroll
-                    for (int part = 0; part < QP; ++part) {
-                        ka_lds4(q_at + (part * NG + k) * 1024, qf[part][0]);
-                        ka_lds4(q_at + (part * NG + k) * 1024 + 512, qf[part][1]);
-                    }
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t f[4];
-                        if (BITS == 4) {
-                            ka_nibbles(w[half * (W / 2) + k], magic, f);
-                        } else {
-                            ka_bytes(w[half * (W / 2) + 2 * k], magic, f[0], f[1]);
-                            ka_bytes(w[half * (W / 2) + 2 * k + 1], magic, f[2], f[3]);
-                        }
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int part = QP - 1; part >= 0; --part) {  // the low halves first
-                            ka_mma(c, qf[part][0], f[0], f[1]);
-                            ka_mma(c, qf[part][1], f[2], f[3]);
-                        }
-                        const float2 sc = make_float2(ka_scale(s, half * 2, k), ka_scale(s, half * 2 + 1, k));
-                        x[pb][NR - 1][half] = ka_fma2(make_float2(c[2], c[3]), sc, x[pb][NR - 1][half]);
-                        x[pb][0][half] = ka_fma2(make_float2(c[0], c[1]), sc, x[pb][0][half]);
-                    }
-                }
-            }
-            const uint8_t* vb = at + PB * F::BLOCK;
-            auto seen = [&](int pb, int nr, int e) {
-                const int pos = p0 + 16 * pb + 2 * tq + (e & 1) + (e >> 1) * 8;
-                return !MASKED || (pos <= lim[nr] && pos < end);
-            };
-            bool raise = false;
-#pragma unroll
-            for (int pb = 0; pb < PB; ++pb) {
-                // a lane looks at one word of V's scales
-                const uint32_t word = *reinterpret_cast<const uint32_t*>(vb + pb * F::BLOCK + CODES + min(lane, HD / 4 - 1) * 4) & 0x7FFF7FFFu;
-                raise |= (word & 0xFFFFu) > top_all || word >> 16 > top_all;
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        if (!seen(pb, nr, 2 * e)) x[pb][nr][e].x = -INFINITY;
-                        if (!seen(pb, nr, 2 * e + 1)) x[pb][nr][e].y = -INFINITY;
-                        raise |= x[pb][nr][e].x > thr[nr] || x[pb][nr][e].y > thr[nr];
-                    }
-            }
-            if (__any_sync(0xFFFFFFFFu, raise)) {
-                uint32_t least = 0xFFFFu;
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr) {
-                    float mx = m[nr];
-                    uint32_t tp = top[nr];
-#pragma unroll
-                    for (int pb = 0; pb < PB; ++pb) {
-                        uint32_t vs[2 * NG];
-                        ka_scales<NG>(vb + pb * F::BLOCK + CODES, tq, vs);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            mx = fmaxf(mx, e & 1 ? x[pb][nr][e >> 1].y : x[pb][nr][e >> 1].x);
-                            if (seen(pb, nr, e)) {
-#pragma unroll
-                                for (int k = 0; k < NG; ++k) {  // NaN and infinity have no say
-                                    const uint32_t v = __half_as_ushort(__float2half_rn(fabsf(ka_scale(vs, e, k))));
-                                    if (v < 0x7C00u) tp = max(tp, v);
-                                }
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int s = 1; s < 4; s <<= 1) {
-                        mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, s));
-                        tp = max(tp, __shfl_xor_sync(0xFFFFFFFFu, tp, s));
-                    }
-                    // a row moves by what it sees alone, whichever row asked
-                    float f = 1.0f;
-                    if (mx > thr[nr] || tp > top[nr]) {
-                        tp |= 0x3FFu;  // scales are below 2^(tp / 1024 - 14)
-                        const float nref = mx == -INFINITY ? 0.f : mx * fr[nr] - (float)(15 - KA_SLACK + 14 - (int)(tp >> 10));
-                        // (a row that saw nothing yet has sums of zero, or NaN, which stays)
-                        f = m[nr] == -INFINITY ? 0.f : ka_exp2(ref[nr] - nref);
-                        m[nr] = mx;
-                        thr[nr] = mx + (float)KA_SLACK / fr[nr];
-                        ref[nr] = nref;
-                        top[nr] = tp;
-                        l[nr] *= f;
-                    }
-                    least = min(least, top[nr]);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float fc = __shfl_sync(0xFFFFFFFFu, f, (2 * tq + j) * 4);
-#pragma unroll
-                        for (int d = 0; d < HD / 16; ++d) {
-                            o[nr][d][j] *= fc;
-                            o[nr][d][2 + j] *= fc;
-                        }
-                    }
-                }
-                top_all = __reduce_min_sync(0xFFFFFFFFu, least);
-            }
-#pragma unroll
-            for (int pb = 0; pb < PB; ++pb) {
-#pragma unroll
-                for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float2 y = ka_fma2(x[pb][nr][e], make_float2(fr[nr], fr[nr]), make_float2(-ref[nr], -ref[nr]));
-                        x[pb][nr][e] = make_float2(ka_exp2(y.x), ka_exp2(y.y));
-                        l[nr] += x[pb][nr][e].x + x[pb][nr][e].y;
-                    }
-                uint32_t w[W], vs[2 * NG];
-                ka_scales<NG>(vb + pb * F::BLOCK + CODES, tq, vs);
-                ka_words<W>(vb + pb * F::BLOCK, lane, w);
-                // p is cut after 11 bits, and what is left again; MODE 0: columns 0 .. 3 take the first part, 4 .. 7 the
-                // second (the cut of the others is to nothing)
-                const uint32_t cut = MODE == 0 && g < 4 ? 0u : 0xFFFFE000u;
-#pragma unroll
-                for (int k = 0; k < NG; ++k) {
-                    uint32_t pf[NR][PP][2];
-#pragma unroll
-                    for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float2 y = ka_mul2(x[pb][nr][half], make_float2(ka_scale(vs, 2 * half, k), ka_scale(vs, 2 * half + 1, k)));
-                            if (MASKED) {  // an unseen position's scale may be NaN
-                                if (!seen(pb, nr, 2 * half)) y.x = 0.f;
-                                if (!seen(pb, nr, 2 * half + 1)) y.y = 0.f;
-                            }
-                            const float2 h = make_float2(__uint_as_float(__float_as_uint(y.x) & cut), __uint_as_float(__float_as_uint(y.y) & cut));
-                            const float2 z = ka_fma2(h, make_float2(-1.f, -1.f), y);
-                            if (MODE != 0) pf[nr][0][half] = ka_pack_rz(y.x, y.y);
-                            pf[nr][PP - 1][half] = ka_pack_rz(z.x, z.y);
-                        }
-#pragma unroll
-                    for (int d = 2 * k; d < 2 * k + 2; ++d) {
-                        uint32_t v[4];
-                        if (BITS == 4) {
-                            ka_nibbles(w[d], magic, v);
-                        } else {
-                            ka_bytes(w[2 * d], magic, v[0], v[2]);
-                            ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
-                        }
-#pragma unroll
-                        for (int nr = 0; nr < NR; ++nr)
-#pragma unroll
-                            for (int part = PP - 1; part >= 0; --part) ka_mma(o[nr][d], v, pf[nr][part][0], pf[nr][part][1]);
-                    }
-                }
-            }
-        };
+        const KvqSeg sg = {b, kvh, r0, rows, pl.rep, a.T, sq.n_ctx, sq.n_ctx + r0 / pl.rep};
+        core.load_q(a, sg, qs, q_max, warp, log2e_d);
 
         uint32_t at = ring_at;
-        int p0 = (blk0 + warp * PB) * 16;
-        const int last = min(open_to, blk1 * 16 - 1);  // up to here every position of a turn is seen
+        int p0 = (blk0 + warp) * 16;
 #pragma unroll 1
         for (int i = 0; i < n_mine; ++i) {
             asm volatile("cp.async.wait_group %0;" ::"n"(F::ST - 2) : "memory");
             __syncwarp();  // everyone's copies of this stage are visible, and the stage before is read
             fetch();
-            if (p0 + 16 * PB - 1 <= last) turn(std::false_type(), smem + at, p0);
-            else turn(std::true_type(), smem + at, p0);
-            p0 += KA_WARPS * PB * 16;
+            if (p0 + 15 <= sg.open_to) core.template block<false>(smem + at, p0);
+            else core.template block<true>(smem + at, p0);
+            p0 += KA_WARPS * 16;
             at = at == ring_at + (F::ST - 1) * F::STAGE ? ring_at : at + F::STAGE;
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-
-        __syncthreads();
-        // the warp's rows into its slot: dims 16 d + 2 g and one on, rows 2 tq and one on
-#pragma unroll
-        for (int nr = 0; nr < NR; ++nr) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int row = nr * 8 + 2 * tq + j;
-#pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                    float2 y = make_float2(o[nr][d][j], o[nr][d][2 + j] * (BITS == 4 ? 0.0625f : 1.0f));
-                    if (MODE == 0) {
-                        y.x += __shfl_xor_sync(0xFFFFFFFFu, y.x, 2);
-                        y.y += __shfl_xor_sync(0xFFFFFFFFu, y.y, 2);
-                    }
-                    if (row < RT) *reinterpret_cast<float2*>(slot_all + (warp * RT + row) * HD + 16 * d + 2 * g) = y;
-                }
-            }
-            l[nr] += __shfl_xor_sync(0xFFFFFFFFu, l[nr], 1);
-            l[nr] += __shfl_xor_sync(0xFFFFFFFFu, l[nr], 2);
-            const int row = nr * 8 + g;
-            if (tq == 0 && row < RT) {
-                // a warp without blocks, or whose rows saw nothing: its exponent says so
-                const bool none = n_mine == 0 || (m[nr] == -INFINITY && l[nr] == 0.f);
-                stat[warp * RT + row] = none ? -INFINITY : ref[nr];
-                stat[(KA_WARPS + warp) * RT + row] = l[nr];
-            }
-        }
+        __syncthreads();  // the rings are read: the warps' rows take their place
+        core.store(slot_all + warp * RT * HD, stat + warp * RT, stat + (KA_WARPS + warp) * RT);
         __syncthreads();
         const bool begins = blk0 == 0, ends = blk1 == sq.blocks, whole = CLUSTER ? pl.split == 1 : begins && ends;
         // what this CTA hands on: rows, then their exponents and sums (CLUSTER: in shared memory, where q was)
