@@ -23,7 +23,9 @@
 // dims, so p is split once for each group): p = 2^(x - m + k), two f16 halves of p scale.  m is the row's
 // running maximum, up to 2^8 behind; k comes from the largest V scale that the row has seen, so that p scale
 // stays below 2^15 and its low half keeps 2^-24 / 2^7 of the largest; it is a row's own, since a row's bits must
-// not hang on what only another row sees.
+// not hang on what only another row sees.  A block's P V is summed from zero and joins the output by an fp32
+// addition (3 % of the time): the matrix accumulator truncates, and a sum of one sign carried in it through 166
+// blocks is off by 2.5e-5.
 //
 // Work is cut into units (sequence, kv head, row tile) and each unit into blocks of 16 positions.  A CTA's warps take
 // its blocks in turn, each with its own ring of cp.async copies (no barrier in the loop), and join at the end.
@@ -41,8 +43,8 @@ namespace tfb {
 
 constexpr int KA_THREADS = 128;
 constexpr int KA_WARPS = KA_THREADS / 32;
-constexpr int KA_UNIT_COST = 8;    // blocks that a unit's start and end take the time of
-constexpr int KA_MIN_RANGE = 16;   // blocks of a CTA's range at least
+constexpr int KA_UNIT_COST = 24;    // blocks that a unit's start and end take the time of
+constexpr int KA_MIN_RANGE = 24;   // blocks of a CTA's range at least
 constexpr int KA_MAX_SPLIT = 8;    // CTAs of a cluster
 constexpr int KA_SNAP = 6;         // a cut this near to a unit's first or last block moves there
 constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
@@ -63,7 +65,8 @@ struct alignas(32) KvqDesc {  // a unit split over CTAs c0 .. c1
 
 __host__ __device__ inline size_t kvq_part_floats(int rt, int hd) { return (size_t)rt * (hd + 2); }
 
-// 0: up to 4 rows (both halves of q and p side by side in the 8 columns), 1: up to 8, 2: up to 16
+// Row tiles: 0: 4 rows, 1: 8, 2: 16.  (32 share a block's codes over more rows, but need 255 registers at 128 dims: 32
+// sequences of 5 x 6 rows over 1144 positions 16.2 -> 19.3 us, 16 of 16 x 4 over 4000, 64 dims, 55.9 -> 57.4.)
 __host__ __device__ constexpr int kvq_rt(int mode) { return mode == 0 ? 4 : mode == 1 ? 8 : 16; }
 
 __host__ __device__ constexpr int kvq_ctas(int mode) { return mode == 2 ? 3 : 4; }  // 168 or 128 registers a thread
@@ -149,6 +152,14 @@ __device__ __forceinline__ float2 ka_fma2(float2 a, float2 b, float2 c) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
+}
+__device__ __forceinline__ void ka_add4(float (&a)[4], const float (&b)[4]) {
+    asm("{\n\t.reg .b64 a0, a1, b0, b1;\n\t"
+        "mov.b64 a0, {%0, %1};\n\tmov.b64 a1, {%2, %3};\n\tmov.b64 b0, {%4, %5};\n\tmov.b64 b1, {%6, %7};\n\t"
+        "add.rn.f32x2 a0, a0, b0;\n\tadd.rn.f32x2 a1, a1, b1;\n\t"
+        "mov.b64 {%0, %1}, a0;\n\tmov.b64 {%2, %3}, a1;\n\t}"
+        : "+f"(a[0]), "+f"(a[1]), "+f"(a[2]), "+f"(a[3])
+        : "f"(b[0]), "f"(b[1]), "f"(b[2]), "f"(b[3]));
 }
 __device__ __forceinline__ float2 ka_mul2(float2 a, float2 b) {
     float2 d;
@@ -537,7 +548,9 @@ struct FewRows {
                     ka_bytes(w[2 * d], magic, v[0], v[2]);
                     ka_bytes(w[2 * d + 1], magic, v[1], v[3]);
                 }
-                ka_mma(o[d], v, pf[0], pf[1]);
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                ka_mma(c, v, pf[0], pf[1]);
+                ka_add4(o[d], c);
             }
         }
     }
@@ -786,8 +799,10 @@ struct ManyRows {
                 }
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
-                    ka_mma(o[nr][d], v, lo[nr][0], lo[nr][1]);
-                    ka_mma(o[nr][d], v, hi[nr][0], hi[nr][1]);
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    ka_mma(c, v, lo[nr][0], lo[nr][1]);
+                    ka_mma(c, v, hi[nr][0], hi[nr][1]);
+                    ka_add4(o[nr][d], c);
                 }
             }
         }
@@ -1129,9 +1144,9 @@ static int kvq_sms() {
 // KA_TURNS blocks at the cache's capacity (lengths are on the device; longer ones are balanced better by ranges).
 constexpr int KA_TURNS = 10;
 static int kvq_split_of(long long units, int cap, int slots) {
-    for (int s = KA_MAX_SPLIT; s >= 1; s >>= 1)
-        if (units * s <= slots) return cap / 16 <= s * KA_WARPS * KA_TURNS ? s : 0;
-    return 0;
+    if (units > slots) return 0;
+    const int s = (int)(slots / units) < KA_MAX_SPLIT ? (int)(slots / units) : KA_MAX_SPLIT;
+    return cap / 16 <= s * KA_WARPS * KA_TURNS ? s : 0;
 }
 static int kvq_mode(int rows) { return rows <= 4 ? 0 : rows <= 8 ? 1 : 2; }
 

@@ -212,7 +212,7 @@ int tf_op_attn_quant(float* out, int ld_out, const float* q, int ld_q, const voi
     if (!aligned(ws, 256)) return set_error("the workspace must be 256-byte aligned");
     if (ws_bytes < kvq_attn_ws_bytes(T, n_heads, n_kv_heads, head_dim)) return set_error("workspace too small");
     if (!kvq_attn_fits(B, T, n_heads, n_kv_heads, cap))
-        return set_error("B * n_kv_heads * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 8) must be below 2^31");
+        return set_error("B * n_kv_heads * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 24) must be below 2^31");
     if (B == 0) return 0;
     KvqAttnArgs a = {};
     if (op_err_word(&a.err)) return -1;

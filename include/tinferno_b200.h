@@ -418,7 +418,7 @@ TF_API int tf_op_qkv_store(float* q_out, int ld_qo, void* k_cache, void* v_cache
  * whatever they hold.  Scores, softmax and sums are fp32-equivalent: errors are relative to the
  * largest key and value that a row sees.  T <= 64, any number of query heads per kv head, up to 1024
  * heads.  Workspace: as for tf_op_attn_tree.  Work is counted in 32 bits: B * n_kv_heads *
- * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 8) must be below 2^31. */
+ * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 24) must be below 2^31. */
 TF_API int tf_op_attn_quant_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
 TF_API int tf_op_attn_quant(float* out, int ld_out, const float* q, int ld_q, const void* k_cache, const void* v_cache,
                             int kv_type, long long slot_stride, int cap, int n_slots, const int* slots,

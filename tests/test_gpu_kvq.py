@@ -562,6 +562,35 @@ def test_offsets_beyond_32_bits():
     assert (out.double().reshape(HK, hd) - want).norm() <= 5e-6 * want.norm()
 
 
+@pytest.mark.parametrize("kv", TYPES)
+def test_long_sums_do_not_drift(kv):
+    """Values of one sign over a cache that a warp walks for hundreds of blocks: an accumulator that truncates loses
+    2^-24 of the sum at every step (2.5e-5 in all), which the norm's bound does not allow."""
+    B, HK, rep, hd, n = 80, 8, 6, 32, 16384
+    L = native.lib()
+    nb = lay.block_bytes(kv, hd)
+    codes = 16 * hd * lay.BITS[kv] // 8
+    g = torch.Generator(device="cuda").manual_seed(1)
+    c = torch.randint(0, 256, (2, B, HK, n // 16, nb), generator=g, device="cuda", dtype=torch.uint8)
+    c[1, ..., :codes] |= 0x88 if kv == native.TF_KV_Q4_0 else 0x80     # values are not negative
+    scale = (0.02 + 0.1 * torch.rand((2, B, HK, n // 16, hd // 2), generator=g, device="cuda")).half()
+    c[..., codes:] = scale.view(torch.uint8)
+    q = torch.randn((B, HK * rep * hd), generator=g, device="cuda")
+    out = torch.zeros_like(q)
+    ctx = i32([n - 1] * B)
+    size = C.c_size_t(0)
+    native.check(L.tf_op_attn_quant_workspace(B, 1, HK * rep, HK, hd, C.byref(size)))
+    ws = torch.empty(size.value, dtype=torch.uint8, device="cuda")
+    native.check(L.tf_op_attn_quant(ptr(out), HK * rep * hd, ptr(q), HK * rep * hd, ptr(c[0]), ptr(c[1]), kv, HK * n * hd, n, B, None, ptr(ctx), None,
+                                    B, 1, HK * rep, HK, hd, ptr(ws), size.value, None))
+    assert device_error() == 0
+    for b, h in ((0, 0), (37, 5), (79, 7)):
+        k, v = (torch.from_numpy(lay.values(c[i, b, h].cpu().numpy(), kind, kv, hd).reshape(n, hd)).cuda() for i, kind in ((0, "k"), (1, "v")))
+        w = torch.softmax(q[b].double().reshape(HK, rep, hd)[h] @ k.T / hd ** 0.5, -1) @ v
+        got = out[b].double().reshape(HK, rep, hd)[h]
+        assert (got - w).norm() <= 5e-6 * w.norm(), float((got - w).norm() / w.norm())
+
+
 # ---- together --------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("kv", TYPES)
