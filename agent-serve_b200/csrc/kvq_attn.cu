@@ -13,8 +13,8 @@
 //                       side; probabilities go to the second product's operand by movmatrix;
 //   more (ManyRows)     rows as M, positions as N: the scores' registers are the second product's operand as they
 //                       stand; up to 8 rows, the 16 rows of M hold q's two halves.
-// 64 sequences over 16384 positions, 8 kv heads of 128, 4 rows each: 267 us as FewRows, 309 as ManyRows; 16 sequences of 16
-// new rows over 4000 positions, 64 dims: 61 and 56.
+// 64 sequences over 8192 positions, 8 kv heads of 128, 4 rows each, 4 bits: 141 us as FewRows, 153 as ManyRows; 16 sequences
+// of 16 new rows over 4000 positions, 64 dims: 61 and 56.
 //
 // Arithmetic (fp32-equivalent).  Codes less their zero are exact in f16: (code | 0x6400) is 1024 + code, and
 // the high nibble in place 1024 + 16 code; the 16 is taken out of q (K) or of the output row (V).  q is split
@@ -34,6 +34,11 @@
 //   the device, so ragged batches stay balanced); a unit that a range cuts leaves partial results for
 //   tf_kvq_combine_kernel.
 // All joins are in a fixed order: results repeat bit for bit.
+//
+// Measured: 64 sequences over 1161 to 8128 positions, 8 kv heads of 128, 4 rows each: 4 bits 91 us (3.8 TB/s: 360
+// instructions per block and warp, issue slots 65 %, ALU and FMA pipes 44 %, DRAM 41 %; the copies alone take 62 us);
+// 32 such sequences in 8 bits 64 us (5.0 TB/s).  1 sequence over 96 positions, 64 dims: 4.3 us, a launch and four
+// dependent reads.
 #include <atomic>
 #include <type_traits>
 
@@ -43,8 +48,13 @@ namespace tfb {
 
 constexpr int KA_THREADS = 128;
 constexpr int KA_WARPS = KA_THREADS / 32;
-constexpr int KA_UNIT_COST = 24;    // blocks that a unit's start and end take the time of
-constexpr int KA_MIN_RANGE = 24;   // blocks of a CTA's range at least
+// Blocks that a unit's start and end take the time of in a range: 8 / 16 / 24 / 32, 64 sequences over up to 8128 positions
+// 89.6 / 87.8 / 87.9 / 88.6 us, 128 over up to 4000 (8 bits, 64 dims) 68.9 / 66.3 / 64.5 / 64.0, 16 of 16 new rows 55.7 /
+// 53.7 / 52.0 / 52.0.
+constexpr int KA_UNIT_COST = 24;
+// Blocks of a CTA's range at least: 8 / 16 / 24 / 32, 1 sequence over 32001 positions 14.3 / 10.8 / 10.8 / 11.2 us, 1 of 4
+// new rows over 8000 14.1 / 14.4 / 14.2 / 17.7.
+constexpr int KA_MIN_RANGE = 24;
 constexpr int KA_MAX_SPLIT = 8;    // CTAs of a cluster
 constexpr int KA_SNAP = 6;         // a cut this near to a unit's first or last block moves there
 constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
@@ -1142,6 +1152,9 @@ static int kvq_sms() {
 }
 // CTAs per unit where a cluster takes each unit: as many as leave all units resident, while a warp has no more than
 // KA_TURNS blocks at the cache's capacity (lengths are on the device; longer ones are balanced better by ranges).
+// Clusters / ranges: 32 sequences of 5 new rows over 1144 positions (9 blocks a warp) 15.8 / 20.4 us, 4 of 8 over 2000 (8)
+// 16.9 / 25.4, 1 of 4 over 8000 (16) 18.9 / 14.7, 3 of 1 over 9000 (18) 17.9 / 11.9.  Clusters of 16 gain 0 to 5 % from 3000
+// positions on and lose 20 % on the shortest calls.
 constexpr int KA_TURNS = 10;
 static int kvq_split_of(long long units, int cap, int slots) {
     if (units > slots) return 0;

@@ -18,6 +18,11 @@
 // 2 t + 9), so values are taken four rows at a time: neighbouring rows of the call that lie in one block at
 // rising positions (a run) share their quads out over the run's warps.  Row by row, the bytes of a head's V
 // touch 16 lines an instruction.
+//
+// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 66 us, 5.6 TB/s (106
+// instructions a vector, issue slots 60 %, DRAM 62 % of its peak).  The same with values and 8-bit writing, 5003 rows: 58 us
+// (issue 59 %; a key's vector takes twice a query's instructions).  8192 rows of 8 heads of 64 in 4 bits: 22 us to write
+// (a warp has four vectors, and its dependent reads dominate), 10 us to read.
 #include <type_traits>
 
 #include "kvq.cuh"
@@ -197,7 +202,8 @@ __device__ __forceinline__ Run find_run(int row, int slot, int pos) {
 
 // LH lanes per head.  A row has `split` warps for its queries and keys (vectors of 32 / LH heads: first, first +
 // split, ...) and `vsplit` for its share of the run's values.
-// TURN: with a rotation.
+// TURN: with a rotation.  (CTAs per SM with the first vectors loaded ahead, 3 / 4: 9001 rows 66 / 73 us, 5003 rows written and
+// read 71 / 80; without loading ahead 65 and 83 at 4.)
 template <int LH, int BITS, bool TURN>
 __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(const KvqRowsArgs a, int split, int vsplit) {
     constexpr int HPW = 32 / LH;

@@ -373,9 +373,9 @@ TF_API int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_laye
  *
  * Rows: row r of an operand is ld floats from the next, heads * head_dim of them are used; rows are
  * 16-byte aligned and strides multiples of 4.  Row r belongs to position pos[r] of slot slots[r]
- * (slots nullptr: slot r).  A row whose slot is negative (a padded batch) is left out: nothing of
- * it is read or written.  A slot or a position outside the cache leaves the row out too and goes to
- * tf_op_device_error.  Rows written by one call name distinct places.  head_dim: 32, 64, 96 or 128.
+ * (slots nullptr: slot r).  A row whose slot is negative (a padded batch) is left out: nothing is
+ * written for it, in the cache or in an output.  A slot or a position outside the cache leaves the
+ * row out too and goes to tf_op_device_error.  Rows written by one call name distinct places.  head_dim: 32, 64, 96 or 128.
  * The calls allocate nothing and do not synchronise. */
 
 /* Per-head RMS norm of queries and keys and the rotation of both, in one pass:
