@@ -74,9 +74,9 @@ __device__ __forceinline__ float kr_max_nan(float a, float b) {  // NaN if eithe
 // Codes and scale of a group of 32 over eight neighbouring lanes, four values each.  A code is the low 16 bits of
 // code[i]; above them lies what packing drops.
 //
-// rint(x / scale) without a quotient: rint of the product with the reciprocal is right unless the product is
-// next to a half; there (one vector in 500 of random values) the remainder x - q scale, which is exact, says which
-// integer is nearest.  Adding 1.5 2^23 rounds to an integer, ties to even, in the low bits.
+// rint(x / scale) without a quotient: rint of the product with the reciprocal (two roundings: off by 1.5e-5 at 127) is
+// right unless the product is next to a half; there (one vector in 200 of random values) the remainder x - q scale,
+// which is exact, says which integer is nearest.  Adding 1.5 2^23 rounds to an integer, ties to even, in the low bits.
 template <int BITS>
 __device__ __forceinline__ void quantise(const float4& x, int lane, uint32_t (&code)[4], __half& scale) {
     constexpr float LO = BITS == 4 ? -8.0f : -127.0f, HI = BITS == 4 ? 7.0f : 127.0f, Z = BITS == 4 ? 8.0f : 128.0f;
@@ -106,7 +106,7 @@ __device__ __forceinline__ void quantise(const float4& x, int lane, uint32_t (&c
     for (int i = 0; i < 4; ++i) {
         const float r = fminf(fmaxf(__fmul_rn(v[i], inv), LO), HI);
         const float t = __fadd_rn(r, M);
-        doubt |= fabsf(__fadd_rn(r, -__fadd_rn(t, -M))) > 0.49999f;
+        doubt |= fabsf(__fadd_rn(r, -__fadd_rn(t, -M))) > 0.49998f;
         code[i] = __float_as_uint(t);
     }
     if (__any_sync(0xFFFFFFFFu, doubt)) {

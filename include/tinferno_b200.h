@@ -372,7 +372,7 @@ TF_API int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_laye
  * then the scales: position p, group k at index (2 (p % 8) + p / 8) head_dim / 32 + k.
  *
  * Rows: row r of an operand is ld floats from the next, heads * head_dim of them are used; rows are
- * 16-byte aligned and strides multiples of 4.  Row r belongs to position pos[r] of slot slots[r]
+ * 16-byte aligned (norm weights too) and strides multiples of 4.  Row r belongs to position pos[r] of slot slots[r]
  * (slots nullptr: slot r).  A row whose slot is negative (a padded batch) is left out: nothing is
  * written for it, in the cache or in an output.  A slot or a position outside the cache leaves the
  * row out too and goes to tf_op_device_error.  Rows written by one call name distinct places.  head_dim: 32, 64, 96 or 128.

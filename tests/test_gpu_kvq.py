@@ -135,6 +135,37 @@ def test_write_and_read(kv, hd, HK, rows, cap):
 
 
 @pytest.mark.parametrize("kv", TYPES)
+def test_values_next_to_the_border_of_two_codes(kv):
+    """Every half between two codes, and its neighbours in fp32 on both sides, at scales of all mantissas: the code is the
+    nearest, ties to even."""
+    top = 8 if kv == native.TF_KV_Q4_0 else 127
+    rng = np.random.default_rng(11)
+    scale = rng.uniform(2.0 ** -12, 2.0 ** 6, 8192).astype(np.float16).astype(np.float32)
+    x = np.zeros((len(scale), 32), np.float32)
+    half = rng.integers(-top, top, (len(scale), 31)) + 0.5
+    half[:, 0], half[:, 1] = top - 1.5, -top + 1.5
+    mid = (scale[:, None] * half).astype(np.float32)          # exact: 11 + 8 bits
+    x[:, 1:] = np.where(np.arange(31) % 3 == 0, mid, np.nextafter(mid, np.float32(np.inf) * np.where(np.arange(31) % 3 == 1, 1, -1), dtype=np.float32))
+    x[:, 0] = -top * scale
+    rows, HK, hd = 64, 32, 128
+    x = x.reshape(rows, HK, hd)
+    c = Cache(kv, hd, HK, 64, 1, 5)
+    codes, scales = lay.quantise(kv, x)
+    assert (scales.astype(np.float32).reshape(-1) == scale).all()
+    k, v = np.zeros_like(c.k), np.zeros_like(c.v)
+    c.k, c.v = k, v
+    c.upload()
+    for r in range(rows):
+        for h in range(HK):
+            lay.write(c.k, "k", kv, hd, 0, h, r, codes[r, h], scales[r, h])
+            lay.write(c.v, "v", kv, hd, 0, h, r, codes[r, h], scales[r, h])
+    d, s, p = cuda(x), i32([0] * rows), i32(range(rows))
+    native.check(native.lib().tf_op_kv_quant(*c.args(), ptr(s), ptr(p), ptr(d), HK * hd, ptr(d), HK * hd, rows, HK, hd, None))
+    assert device_error() == 0
+    assert c.same()
+
+
+@pytest.mark.parametrize("kv", TYPES)
 def test_rows_outside_the_cache(kv):
     c = Cache(kv, 64, 2, 32, 3, 1).upload()
     x = torch.randn((5, 2, 128), device="cuda")
