@@ -71,42 +71,63 @@ __device__ __forceinline__ float kr_max_nan(float a, float b) {  // NaN if eithe
     return d;
 }
 
+__device__ __forceinline__ float kr_rcp(float x) {  // to 2^-23
+    float d;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d) : "f"(x));
+    return d;
+}
+
 // Codes and scale of a group of 32 over eight neighbouring lanes, four values each.  A code is the low 16 bits of
 // code[i]; above them lies what packing drops.
 //
-// rint(x / scale) without a quotient: rint of the product with the reciprocal (two roundings: off by 1.5e-5 at 127) is
-// right unless the product is next to a half; there (one vector in 200 of random values) the remainder x - q scale,
+// rint(x / scale) without a quotient: rint of the product with the reciprocal (off by 2.3e-5 at 127) is
+// right unless the product is next to a half; there (one vector in 130 of random values) the remainder x - q scale,
 // which is exact, says which integer is nearest.  Adding 1.5 2^23 rounds to an integer, ties to even, in the low bits.
 template <int BITS>
 __device__ __forceinline__ void quantise(const float4& x, int lane, uint32_t (&code)[4], __half& scale) {
     constexpr float LO = BITS == 4 ? -8.0f : -127.0f, HI = BITS == 4 ? 7.0f : 127.0f, Z = BITS == 4 ? 8.0f : 128.0f;
     constexpr float M = 12582912.0f + Z;
     const float v[4] = {x.x, x.y, x.z, x.w};
-    const float mine = kr_max_nan(kr_max_nan(fabsf(v[0]), fabsf(v[1])), kr_max_nan(fabsf(v[2]), fabsf(v[3])));
-    float top = mine;
-#pragma unroll
-    for (int o = 1; o < 8; o <<= 1) top = kr_max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-    float d;
+    float top, d;
     if (BITS == 4) {
-        float m = v[3];
+        // the larger of the group's largest and least; where they tie, whichever comes first
+        float hi = kr_max_nan(kr_max_nan(v[0], v[1]), kr_max_nan(v[2], v[3])), lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
 #pragma unroll
-        for (int i = 2; i >= 0; --i)
-            if (fabsf(v[i]) == top) m = v[i];
-        const unsigned has = __ballot_sync(0xFFFFFFFFu, mine == top) >> (lane & 24) & 0xFFu;
-        m = __shfl_sync(0xFFFFFFFFu, m, (lane & 24) + __ffs(has) - 1);  // (NaN: no lane has it, any will do)
+        for (int o = 1; o < 8; o <<= 1) {
+            hi = kr_max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+            lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+        }
+        float m = hi >= -lo ? hi : lo;
+        if (__any_sync(0xFFFFFFFFu, hi == -lo)) {
+            float f = v[3];
+            bool here = fabsf(f) == hi;
+#pragma unroll
+            for (int i = 2; i >= 0; --i)
+                if (fabsf(v[i]) == hi) {
+                    f = v[i];
+                    here = true;
+                }
+            const unsigned has = __ballot_sync(0xFFFFFFFFu, here) >> (lane & 24) & 0xFFu;
+            f = __shfl_sync(0xFFFFFFFFu, f, (lane & 24) + (has ? __ffs(has) - 1 : 0));
+            if (hi == -lo) m = f;
+        }
+        top = kr_max_nan(hi, -lo);
         d = __fmul_rn(m, -0.125f);
     } else {
+        top = kr_max_nan(kr_max_nan(fabsf(v[0]), fabsf(v[1])), kr_max_nan(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = kr_max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
         d = __fmul_rn(top, 1.0f / 127.0f);
     }
     const bool bad = !(top < INFINITY);
     scale = bad ? __ushort_as_half(0x7FFF) : __float2half_rn(fminf(fmaxf(d, -65504.0f), 65504.0f));
-    const float s = __half2float(scale), inv = s == 0.0f ? 0.0f : __frcp_rn(s);
+    const float s = __half2float(scale), inv = s == 0.0f ? 0.0f : kr_rcp(s);
     bool doubt = bad;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float r = fminf(fmaxf(__fmul_rn(v[i], inv), LO), HI);
         const float t = __fadd_rn(r, M);
-        doubt |= fabsf(__fadd_rn(r, -__fadd_rn(t, -M))) > 0.49998f;
+        doubt |= fabsf(__fadd_rn(r, -__fadd_rn(t, -M))) > 0.49997f;
         code[i] = __float_as_uint(t);
     }
     if (__any_sync(0xFFFFFFFFu, doubt)) {
@@ -150,6 +171,7 @@ struct Run {
     int first, len, index;
     unsigned mask;
     __device__ __forceinline__ int row(int p) const {  // the row of position p of the block, or -1
+        if (mask == 0xFFFFu) return first + p;
         return mask >> p & 1 ? first + __popc(mask & ((1u << p) - 1)) : -1;
     }
     __device__ __forceinline__ int quads() const {  // bit t: quad t holds a row
@@ -299,7 +321,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                 float4 x[KR_VEC];
 #pragma unroll
                 for (int u = 0; u < KR_VEC; ++u) x[u] = ahead[u];
-                load(h + step * KR_VEC);
+                if (TURN || left > split * KR_VEC) load(h + step * KR_VEC);
                 // The squares of the four vectors are summed together: at each of the first two steps a lane hands on
                 // the half of its sums that its partner keeps, so that a lane ends with the sum of one of them.
                 float inv = 1.0f;
