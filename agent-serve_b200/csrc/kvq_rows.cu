@@ -459,18 +459,19 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
 }
 
 // ---- reading back -------------------------------------------------------------------------------------
+// Values of four codes; a code as the low bits of 2^23 + code is exact, without a conversion.
 template <int BITS>
 __device__ __forceinline__ float4 kr_values(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, float s) {
-    constexpr float Z = BITS == 4 ? 8.0f : 128.0f;
-    // a code as the low bits of 2^23 + code: exact, without a conversion
-    auto f = [](uint32_t c) { return __uint_as_float(0x4B000000u | c) - (8388608.0f + Z); };
-    return make_float4(f(c0) * s, f(c1) * s, f(c2) * s, f(c3) * s);
+    constexpr float Z = 8388608.0f + (BITS == 4 ? 8.0f : 128.0f);
+    return make_float4((__uint_as_float(c0) - Z) * s, (__uint_as_float(c1) - Z) * s, (__uint_as_float(c2) - Z) * s, (__uint_as_float(c3) - Z) * s);
 }
+// 2^23 + byte j of x, or its low or high half
+__device__ __forceinline__ uint32_t kr_byte(uint32_t x, int j) { return __byte_perm(x, 0x4B000000u, 0x7650 + j); }
+__device__ __forceinline__ uint32_t kr_nibble(uint32_t x, int j) { return (x >> 4 * j & 15u) | 0x4B000000u; }
 
 template <int LH, int BITS>
 __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadArgs a, int split, int vsplit) {
     constexpr int HPW = 32 / LH;
-    constexpr uint32_t M = (1u << BITS) - 1;
     const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
     const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
@@ -512,7 +513,8 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
                 if (h >= a.n_kv || !live) continue;
                 const uint32_t c = code[u];
                 *reinterpret_cast<float4*>(a.k + (long long)row * a.ld_k + h * a.hd + d0) =
-                    kr_values<BITS>(c & M, c >> BITS & M, c >> 2 * BITS & M, c >> 3 * BITS & M, s[u]);
+                    BITS == 4 ? kr_values<4>(kr_nibble(c, 0), kr_nibble(c, 1), kr_nibble(c, 2), kr_nibble(c, 3), s[u])
+                              : kr_values<8>(kr_byte(c, 0), kr_byte(c, 1), kr_byte(c, 2), kr_byte(c, 3), s[u]);
             }
         }
         return;
@@ -540,10 +542,9 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
         for (int j = 0; j < 4; ++j) {
             const int r = run.row(quad_pos(t, j));
             if (r < 0) continue;
-            const int b = 8 * j;
             *reinterpret_cast<float4*>(a.v + (long long)r * a.ld_v + h * a.hd + d0) =
-                BITS == 4 ? kr_values<4>(w[0] >> b & 15, w[0] >> (b + 4) & 15, w[1] >> b & 15, w[1] >> (b + 4) & 15, s[j])
-                          : kr_values<8>(w[0] >> b & 255, w[1] >> b & 255, w[2] >> b & 255, w[3] >> b & 255, s[j]);
+                BITS == 4 ? kr_values<4>(kr_nibble(w[0], 2 * j), kr_nibble(w[0], 2 * j + 1), kr_nibble(w[1], 2 * j), kr_nibble(w[1], 2 * j + 1), s[j])
+                          : kr_values<8>(kr_byte(w[0], j), kr_byte(w[1], j), kr_byte(w[2], j), kr_byte(w[3], j), s[j]);
         }
     }
 }
