@@ -427,6 +427,53 @@ def test_attention_split_over_ctas(kv, hd, H, HK, T, lens):
     Case(kv, hd, H, HK, lens, [T] * len(lens), T, T).run().check()
 
 
+@pytest.mark.parametrize("kv", TYPES)
+@pytest.mark.parametrize("hd,H,HK,T", [(64, 8, 2, 1), (128, 6, 1, 1), (32, 10, 2, 3), (96, 6, 3, 20)])
+def test_short_contexts_in_a_long_cache(kv, hd, H, HK, T):
+    """The split is chosen by the capacity: short and empty contexts where long ones could be."""
+    lens = [0, 1, 95, 96, 97, 370, 13, 0, 1800]
+    news = [T, T, T, T, T, T, 0, 1, max(1, T - 1)]
+    Case(kv, hd, H, HK, lens, news, T, 3 * T, cap=8192).run().check()
+
+
+@pytest.mark.parametrize("n", [385, 480, 481, 800, 1137])
+def test_every_cut(n):
+    """Ranges that end next to a unit's first and last blocks."""
+    Case(native.TF_KV_Q4_0, 32, 4, 4, [n, n + 30, 5, n - 16], [1, 1, 1, 1], 1, n, cap=8192).run().check()
+
+
+@pytest.mark.parametrize("cap", [0, 8192])
+def test_two_streams_at_once(cap):
+    """Calls in flight together, each with its workspace; then both through one workspace, one after the other."""
+    a = Case(native.TF_KV_Q4_0, 64, 8, 2, [900, 40], [1, 1], 1, 1, cap=cap or None).run()
+    b = Case(native.TF_KV_Q8_0, 64, 14, 2, [700, 1111], [2, 2], 2, 2, cap=cap or None).run()
+    one, two = a.got(), b.got()
+    a.check(one), b.check(two)
+    s, t = torch.cuda.Stream(), torch.cuda.Stream()
+    a.out.zero_(), b.out.zero_()
+    a.out[..., a.H * a.hd:] = b.out[..., b.H * b.hd:] = 7.0
+    torch.cuda.synchronize()
+    for _ in range(20):
+        a.run(stream=s.cuda_stream, ws=a.ws, upload=False)
+        b.run(stream=t.cuda_stream, ws=b.ws, upload=False)
+    assert (a.got() == one).all() and (b.got() == two).all()
+    big = a.ws if a.ws.numel() > b.ws.numel() else b.ws
+    graphs = []
+    for c in (a, b):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            c.run(stream=s.cuda_stream, ws=big, upload=False)
+        graphs.append(g)
+    for c in (a, b):
+        c.out[..., :c.H * c.hd] = 0
+    with torch.cuda.stream(s):
+        for _ in range(5):
+            for g in graphs:
+                g.replay()
+    torch.cuda.synchronize()
+    assert (a.got() == one).all() and (b.got() == two).all()
+
+
 def test_many_sequences():
     """More sequences than lanes and CTAs, most of them short."""
     rng = np.random.default_rng(3)
@@ -451,11 +498,12 @@ def test_without_slots_and_counts(kv):
     c.run(slots=None, n_new=None).check()
 
 
-def test_sequences_that_do_not_fit():
+@pytest.mark.parametrize("cap", [96, 8192])
+def test_sequences_that_do_not_fit(cap):
     """Refused on the device: their rows are zero, the others' are right."""
-    c = Case(native.TF_KV_Q4_0, 64, 8, 2, [40, 90, 33, 20], [2, 2, 2, 2], 2, 1, cap=96).run()
+    c = Case(native.TF_KV_Q4_0, 64, 8, 2, [40, 90, 33, 20], [2, 2, 2, 2], 2, 1, cap=cap).run()
     good = c.got()
-    for bad, code in [(dict(slots=[9, 1, 2, 3]), 0), (dict(slots=[-1, 1, 2, 3]), 0), (dict(n_ctx=[40, 95, 33, 20]), 1), (dict(n_ctx=[-1, 90, 33, 20]), 0),
+    for bad, code in [(dict(slots=[9, 1, 2, 3]), 0), (dict(slots=[-1, 1, 2, 3]), 0), (dict(n_ctx=[40, cap - 1, 33, 20]), 1), (dict(n_ctx=[-1, 90, 33, 20]), 0),
                       (dict(n_new=[2, 2, -1, 2]), 2)]:
         kw = {k: i32(v if k != "slots" else [s if not 0 <= s < 4 or i == code else c.slots[i] for i, s in enumerate(v)]) for k, v in bad.items()}
         c.out.fill_(7.0)
