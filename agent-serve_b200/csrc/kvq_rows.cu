@@ -21,8 +21,8 @@
 //
 // Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 66 us, 5.6 TB/s (106
 // instructions a vector, issue slots 60 %, DRAM 62 % of its peak).  The same with values and 8-bit writing, 5003 rows: 58 us
-// (issue 59 %; a key's vector takes twice a query's instructions).  8192 rows of 8 heads of 64 in 4 bits: 22 us to write
-// (a warp has four vectors, and its dependent reads dominate), 10 us to read.
+// (issue 59 %; a key's vector takes twice a query's instructions).  8192 rows of 8 heads of 64 in 4 bits: 20 us to write
+// (185 instructions a vector, issue 70 %; a warp has only four), 10 us to read.
 #include <type_traits>
 
 #include "kvq.cuh"
