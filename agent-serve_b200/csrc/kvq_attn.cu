@@ -228,7 +228,7 @@ struct KvqSeq {
     int slot, n_ctx, n_new, blocks, units;
     bool bad;
 };
-__device__ __forceinline__ KvqSeq kvq_seq(const KvqAttnArgs& a, const KvqPlan& pl, int b) {
+__device__ __forceinline__ KvqSeq kvq_seq(const KvqAttnArgs& a, int rep, int rt, int b) {
     KvqSeq s;
     s.slot = a.slots ? a.slots[b] : b;
     s.n_ctx = a.n_ctx[b];
@@ -236,7 +236,7 @@ __device__ __forceinline__ KvqSeq kvq_seq(const KvqAttnArgs& a, const KvqPlan& p
     s.bad = s.slot < 0 || s.slot >= a.n_slots || s.n_ctx < 0 || s.n_new < 0 || s.n_ctx > a.cap - s.n_new;
     if (s.bad) s.n_new = 0;
     s.blocks = s.n_new ? (s.n_ctx + s.n_new + 15) >> 4 : 0;
-    s.units = a.n_kv * ((s.n_new * pl.rep + pl.rt - 1) / pl.rt);
+    s.units = a.n_kv * ((s.n_new * rep + rt - 1) / rt);
     return s;
 }
 __device__ __forceinline__ int kvq_len(const KvqSeq& s) { return s.n_new ? s.units * (s.blocks + KA_UNIT_COST) : 0; }
@@ -250,13 +250,14 @@ __device__ __forceinline__ int kvq_cut(int t, int n) { return t < KA_SNAP ? 0 : 
 struct KvqRange {
     int g0, g1, per, b, base;
 };
+template <int RT>
 __device__ __forceinline__ KvqRange kvq_range(const KvqAttnArgs& a, const KvqPlan& pl) {
     const int lane = threadIdx.x & 31;
     const int chunk = (a.B + 31) >> 5, lo = min(a.B, lane * chunk), hi = min(a.B, lo + chunk);
     int mine = 0;
-#pragma unroll 1
+#pragma unroll 4
     for (int b = lo; b < hi; ++b) {
-        const KvqSeq s = kvq_seq(a, pl, b);
+        const KvqSeq s = kvq_seq(a, pl.rep, RT, b);
         mine += kvq_len(s);
         if (s.bad && blockIdx.x == 0 && threadIdx.x < 32) atomicCAS(a.err, 0, ERR_POS);
     }
@@ -869,7 +870,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
         rank = blockIdx.x % pl.split;
         b = blockIdx.x / (pl.split * pl.tiles * a.n_kv);
     } else {
-        range = kvq_range(a, pl);
+        range = kvq_range<RT>(a, pl);
         b = range.b;
         base = range.base;
     }
@@ -879,7 +880,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
 
 #pragma unroll 1
     for (int gpos = range.g0; gpos < range.g1;) {
-        KvqSeq sq = kvq_seq(a, pl, b);
+        KvqSeq sq = kvq_seq(a, pl.rep, RT, b);
         int blk0, blk1, kvh, tile, rows, r0, ub = 0;
         if (CLUSTER) {
             gpos = range.g1;
@@ -904,7 +905,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             int len = kvq_len(sq);
             while (gpos >= base + len && b + 1 < a.B) {  // gpos is below the total: a sequence with work follows
                 base += len;
-                sq = kvq_seq(a, pl, ++b);
+                sq = kvq_seq(a, pl.rep, RT, ++b);
                 len = kvq_len(sq);
             }
             if (gpos >= base + len) break;
@@ -1047,7 +1048,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
 
     // rows behind a sequence's new ones, and rows of a sequence that was refused, are zero
     for (int s = blockIdx.x; s < a.B; s += pl.grid) {
-        const KvqSeq sq = kvq_seq(a, pl, s);
+        const KvqSeq sq = kvq_seq(a, pl.rep, RT, s);
         const int n = a.n_head * HD / 4;
         for (int t = sq.n_new; t < a.T; ++t)
             for (int i = threadIdx.x; i < n; i += KA_THREADS)
@@ -1066,7 +1067,7 @@ __global__ void __launch_bounds__(ROWS * WAYS * 32) tf_kvq_combine_kernel(const 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lr = warp / WAYS, way = warp % WAYS, r = blockIdx.y * ROWS + lr;
     if (pl.by_unit) {  // a unit that does not exist has no descriptor
-        const KvqSeq sq = kvq_seq(a, pl, blockIdx.x / (a.n_kv * pl.tiles));
+        const KvqSeq sq = kvq_seq(a, pl.rep, pl.rt, blockIdx.x / (a.n_kv * pl.tiles));
         if ((int)(blockIdx.x % pl.tiles) * a.n_kv >= sq.units) return;
     }
     const KvqDesc de = static_cast<const KvqDesc*>(a.ws)[blockIdx.x];
