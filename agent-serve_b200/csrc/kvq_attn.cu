@@ -1146,11 +1146,16 @@ __global__ void __launch_bounds__(ROWS * WAYS * 32) tf_kvq_combine_kernel(const 
 
 // ---- host ------------------------------------------------------------------------------------------
 static int kvq_sms() {
+    static std::atomic<int> known[64] = {};  // per device: a quarter of a microsecond a call
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && known[dev].load() > 0) return known[dev].load();
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms < 1 ? 1 : (4 * sms > KA_MAX_GRID ? KA_MAX_GRID / 4 : sms);
+    sms = sms < 1 ? 1 : (4 * sms > KA_MAX_GRID ? KA_MAX_GRID / 4 : sms);
+    if (dev >= 0 && dev < 64) known[dev].store(sms);
+    return sms;
 }
+
 // CTAs per unit where a cluster takes each unit: as many as leave all units resident, while a warp has no more than
 // KA_TURNS blocks at the cache's capacity (lengths are on the device; longer ones are balanced better by ranges).
 // Clusters / ranges: 32 sequences of 5 new rows over 1144 positions (9 blocks a warp) 15.8 / 20.4 us, 4 of 8 over 2000 (8)
