@@ -65,10 +65,15 @@ struct KvqPlan {
     int grid;
     int rt;        // rows per row tile
     int rep;       // query heads per kv head
+    unsigned inv;  // 2^32 / rep, rounded up
     int tiles;     // row tiles of T rows
     int split;     // CTAs of a unit, one cluster; 0: ranges of all units' blocks
     int by_unit;   // descriptors are found by unit (there are at most `grid`), else by the CTA that begins it
 };
+// x / rep for x < 2^16 and rep <= 1024 (the error x 2^-32 stays below 1 / rep)
+__host__ __device__ __forceinline__ int kvq_div(int x, int rep, unsigned inv) {
+    return rep == 1 ? x : (int)((unsigned long long)(unsigned)x * inv >> 32);
+}
 struct alignas(32) KvqDesc {  // a unit split over CTAs c0 .. c1
     int b, kvh, tile, rows, c0, c1;  // b < 0: no unit, or one that was not split
 };
@@ -305,11 +310,13 @@ __device__ __forceinline__ float4 ka_remote4(const float* p, int rank) {
 // ---- a warp's work on a unit's blocks --------------------------------------------------------------------
 // What a segment of a unit is to its warps.
 struct KvqSeg {
-    int b, kvh, r0, rows, rep, T, n_ctx;  // rows r0 .. r0 + rows - 1 of the unit's (new row, head) pairs
-    int open_to;                          // every row sees the positions up to here
+    int b, kvh, r0, rows;  // rows r0 .. r0 + rows - 1 of the unit's (new row, head) pairs
+    int rep, T, n_ctx;
+    unsigned inv;
+    int open_to;           // every row sees the positions up to here
 };
 __device__ __forceinline__ const float* kvq_query(const KvqAttnArgs& a, const KvqSeg& sg, int row, int hd) {
-    const int rr = sg.r0 + row, t = rr / sg.rep, h = sg.kvh * sg.rep + rr - t * sg.rep;
+    const int rr = sg.r0 + row, t = kvq_div(rr, sg.rep, sg.inv), h = sg.kvh * sg.rep + rr - t * sg.rep;
     return a.q + ((long long)sg.b * sg.T + t) * a.ld_q + h * hd;
 }
 // A row's largest value goes to [2^13, 2^14); rows of zeros, subnormals and infinities stay as they are.
@@ -434,8 +441,8 @@ struct FewRows {
         const int c = (2 * tq) & 3;
         fr.x = __int_as_float((127 - kvq_shift(kvq_row_max<RT>(q_max, c))) << 23) * log2e_d;
         fr.y = __int_as_float((127 - kvq_shift(kvq_row_max<RT>(q_max, c + 1))) << 23) * log2e_d;
-        lim.x = sg.n_ctx + (sg.r0 + c) / sg.rep;
-        lim.y = sg.n_ctx + (sg.r0 + c + 1) / sg.rep;
+        lim.x = sg.n_ctx + kvq_div(sg.r0 + c, sg.rep, sg.inv);
+        lim.y = sg.n_ctx + kvq_div(sg.r0 + c + 1, sg.rep, sg.inv);
         __syncthreads();
         r0.clear();
         r1.clear();
@@ -641,7 +648,7 @@ struct ManyRows {
             const int row = nr * 8 + g, sh = kvq_shift(kvq_row_max<RT>(q_max, row));
             const float sc = __int_as_float((sh + 127) << 23);
             fr[nr] = __int_as_float((127 - sh) << 23) * log2e_d;
-            lim[nr] = sg.n_ctx + (sg.r0 + row) / sg.rep;
+            lim[nr] = sg.n_ctx + kvq_div(sg.r0 + row, sg.rep, sg.inv);
 #pragma unroll
             for (int i = 0; i < NQ; ++i) {
                 const int k = i * KA_WARPS + warp;
@@ -895,7 +902,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             // the tile's rows behind the new ones are zero
             const int all = min(RT, a.T * pl.rep - r0), first = max(0, sq.n_new * pl.rep - r0);
             for (int i = first * (HD / 4) + rank * KA_THREADS + threadIdx.x; i < all * (HD / 4); i += pl.split * KA_THREADS) {
-                const int row = i / (HD / 4), rr = r0 + row, t = rr / pl.rep, h = kvh * pl.rep + rr - t * pl.rep;
+                const int row = i / (HD / 4), rr = r0 + row, t = kvq_div(rr, pl.rep, pl.inv), h = kvh * pl.rep + rr - t * pl.rep;
                 *reinterpret_cast<float4*>(a.out + ((long long)b * a.T + t) * a.ld_out + h * HD + (i - row * (HD / 4)) * 4) =
                     make_float4(0.f, 0.f, 0.f, 0.f);
             }
@@ -946,7 +953,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
         };
 #pragma unroll
         for (int i = 0; i < F::ST - 1; ++i) fetch();
-        const KvqSeg sg = {b, kvh, r0, rows, pl.rep, a.T, sq.n_ctx, sq.n_ctx + r0 / pl.rep};
+        const KvqSeg sg = {b, kvh, r0, rows, pl.rep, a.T, sq.n_ctx, pl.inv, sq.n_ctx + kvq_div(r0, pl.rep, pl.inv)};
         core.load_q(a, sg, qs, q_max, warp, log2e_d);
 
         uint32_t at = ring_at;
@@ -988,7 +995,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                 y.w = fmaf(u.w, f, y.w);
             }
             if (whole) {
-                const int rr = r0 + row, t = rr / pl.rep, h = kvh * pl.rep + rr - t * pl.rep;
+                const int rr = r0 + row, t = kvq_div(rr, pl.rep, pl.inv), h = kvh * pl.rep + rr - t * pl.rep;
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 *reinterpret_cast<float4*>(a.out + ((long long)b * a.T + t) * a.ld_out + h * HD + d) =
                     make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
@@ -1027,7 +1034,7 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
                         y.z = fmaf(u[c].z, f, y.z);
                         y.w = fmaf(u[c].w, f, y.w);
                     }
-                const int rr = r0 + row, t = rr / pl.rep, h = kvh * pl.rep + rr - t * pl.rep;
+                const int rr = r0 + row, t = kvq_div(rr, pl.rep, pl.inv), h = kvh * pl.rep + rr - t * pl.rep;
                 const float inv = L == 0.f ? 0.f : 1.0f / L;
                 *reinterpret_cast<float4*>(a.out + ((long long)b * a.T + t) * a.ld_out + h * HD + d) =
                     make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
@@ -1066,11 +1073,11 @@ __global__ void __launch_bounds__(ROWS * WAYS * 32) tf_kvq_combine_kernel(const 
     pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int lr = warp / WAYS, way = warp % WAYS, r = blockIdx.y * ROWS + lr;
+    const KvqDesc de = static_cast<const KvqDesc*>(a.ws)[blockIdx.x];
     if (pl.by_unit) {  // a unit that does not exist has no descriptor
         const KvqSeq sq = kvq_seq(a, pl.rep, pl.rt, blockIdx.x / (a.n_kv * pl.tiles));
         if ((int)(blockIdx.x % pl.tiles) * a.n_kv >= sq.units) return;
     }
-    const KvqDesc de = static_cast<const KvqDesc*>(a.ws)[blockIdx.x];
     if (de.b < 0 || (int)blockIdx.y * ROWS >= de.rows) return;
     const float* parts = reinterpret_cast<const float*>(static_cast<const uint8_t*>(a.ws) + KA_DESC_BYTES);
     const int hd = a.hd, rt = pl.rt, n = de.c1 - de.c0 + 1, d = lane * 4;
@@ -1138,7 +1145,7 @@ __global__ void __launch_bounds__(ROWS * WAYS * 32) tf_kvq_combine_kernel(const 
         }
     }
     if (r >= de.rows || d >= hd) return;
-    const int rep = pl.rep, rr = de.tile * rt + r, t = rr / rep, h = de.kvh * rep + rr - t * rep;
+    const int rep = pl.rep, rr = de.tile * rt + r, t = kvq_div(rr, rep, pl.inv), h = de.kvh * rep + rr - t * rep;
     const float inv = L == 0.f ? 0.f : 1.0f / L;
     *reinterpret_cast<float4*>(a.out + ((long long)de.b * a.T + t) * a.ld_out + h * hd + d) =
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
@@ -1220,6 +1227,7 @@ static cudaError_t mode_launch(const KvqAttnArgs& a, cudaStream_t st) {
     const int slots = kvq_sms() * F::CTAS;
     pl.rt = F::RT;
     pl.rep = a.n_head / a.n_kv;
+    pl.inv = (unsigned)(((1ull << 32) + pl.rep - 1) / pl.rep);  // (1: not used)
     pl.tiles = (a.T * pl.rep + F::RT - 1) / F::RT;
     const long long units = (long long)a.B * a.n_kv * pl.tiles;
     pl.by_unit = units <= slots;
@@ -1238,8 +1246,8 @@ static cudaError_t mode_launch(const KvqAttnArgs& a, cudaStream_t st) {
     e = kvq_launch((const void*)tf_kvq_attn_kernel<BITS, HD, MODE, false>, dim3(pl.grid), KA_THREADS, F::SMEM, 1, args, st, false);
     if (e != cudaSuccess) return e;
     const int found = pl.by_unit ? (int)units : pl.grid;
-    // few units have many parts each: eight warps to a row
-    if (found * F::RT <= 1024) return kvq_launch((const void*)tf_kvq_combine_kernel<1, 8>, dim3(found, F::RT), 256, 0, 1, args, st, true);
+    // few units have many parts each: eight warps to a row, else one, which has eight parts in flight
+    if (units * 8 <= slots) return kvq_launch((const void*)tf_kvq_combine_kernel<1, 8>, dim3(found, F::RT), 256, 0, 1, args, st, true);
     return kvq_launch((const void*)tf_kvq_combine_kernel<4, 1>, dim3(found, F::RT / 4), 128, 0, 1, args, st, true);
 }
 template <int BITS, int HD>
