@@ -37,7 +37,7 @@
 //
 // Measured: 64 sequences over 1161 to 8128 positions, 8 kv heads of 128, 4 rows each: 4 bits 91 us (3.8 TB/s: 360
 // instructions per block and warp, issue slots 65 %, ALU and FMA pipes 44 %, DRAM 41 %; the copies alone take 62 us);
-// 32 such sequences in 8 bits 64 us (5.0 TB/s).  1 sequence over 96 positions, 64 dims: 4.3 us, a launch and four
+// 32 such sequences in 8 bits 60 us (5.4 TB/s).  1 sequence over 96 positions, 64 dims: 4.0 us, a launch and four
 // dependent reads.
 #include <atomic>
 #include <type_traits>
