@@ -267,6 +267,24 @@ def test_norm_rope(hd, rot, H, HK, normed, rows):
     assert torch.equal(q2, q) and torch.equal(k2, k)
 
 
+def test_rotation_of_values_that_are_not_finite():
+    """An infinity or NaN reaches its own pair alone, as the formula has it, in queries and in keys."""
+    rng = np.random.default_rng(4)
+    x = rng.standard_normal((6, 4, 64)).astype(np.float32)
+    x[0, 0, 3], x[1, 1, 40], x[2, 2, 5], x[3, 3, 63], x[4, 3, 0] = np.inf, -np.inf, np.inf, np.nan, -np.inf
+    pos, freq = np.array([5, 0, 9, 1, 0, 77]), (10000.0 ** (-np.arange(0, 64, 2) / 64)).astype(np.float32)
+    d, df, dp, out = cuda(x), cuda(freq), i32(pos.tolist()), torch.zeros((6, 4, 64), device="cuda")
+    native.check(native.lib().tf_op_qk_norm_rope(ptr(out), 256, ptr(out) + 512, 256, ptr(d), 256, ptr(d) + 512, 256, None, None, 0.0, ptr(df), 64,
+                                                 ptr(dp), 6, 2, 2, 64, None))
+    with np.errstate(invalid="ignore"):
+        want, tol = norm_rope_64(x, None, 0.0, freq, pos)
+        got = out.cpu().numpy()
+        fin = np.isfinite(want)
+        assert (np.isfinite(got) == fin).all() and (np.isnan(got) == np.isnan(want)).all()
+        assert (got[np.isinf(want)] == want[np.isinf(want)]).all()
+        assert (np.abs(got - want) <= tol)[fin].all()
+
+
 def test_norm_alone_and_copy():
     """Without a rotation no positions are needed; without weights either, rows are copied."""
     x = torch.randn((9, 6, 64), device="cuda")
@@ -311,6 +329,12 @@ def test_store_is_norm_rope_then_quant(kv, H, HK, hd, rot, rows, normed):
     assert torch.equal(a.dk, b.dk) and torch.equal(a.dv, b.dv)
     keep = torch.from_numpy(slots >= 0).cuda()
     assert torch.equal(q1[keep], q2[keep]) and (q1[~keep] == 7.0).all()
+    # queries in place, in a fused row
+    y = x.clone()
+    native.check(L.tf_op_qkv_store(ptr(y), ld, *b.args(), ptr(s), ptr(p), ptr(y), ld, ptr(y) + 4 * H * hd, ld, ptr(y) + 4 * (H + HK) * hd, ld, wq, wk,
+                                   1e-6, ptr(freq), rot, rows, H, HK, hd, None))
+    assert torch.equal(y[keep, :H * hd], q1[keep]) and torch.equal(y[~keep], x[~keep]) and torch.equal(y[:, H * hd:], x[:, H * hd:])
+    assert torch.equal(a.dk, b.dk) and torch.equal(a.dv, b.dv)
     assert not torch.equal(a.dk.cpu(), torch.from_numpy(a.k)) or not keep.any()
 
 
