@@ -552,8 +552,8 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
 // ---- host ---------------------------------------------------------------------------------------------
 // Warps per row: one when rows alone fill the device (`fill` warps on each of its SMs), else a row's vectors are
 // shared out so that few rows finish in one round of loads.  16 warps, and twice what an SM holds where they carry
-// a whole row of queries and keys, whose last round would else be long: 5003 rows of 32 + 8 + 8 heads of 128, 71 us
-// with 16, FILL48 with 48.
+// a whole row of queries and keys, whose last round would else be long: 5003 rows of 32 + 8 + 8 heads of 128 written
+// in 8 bits and read back, 69.6 us with 16, 68.4 with 48; 9001 rows of 32 + 8 have one warp each either way, 66.6.
 constexpr int KR_FILL = 16, KR_FILL_TURN = 48;
 static int kvq_split(int rows, int vectors, int fill = KR_FILL) {
     const int want = (int)((148ll * fill + rows - 1) / rows);
