@@ -30,7 +30,7 @@
 namespace tfb {
 
 constexpr int KR_THREADS = 256;
-constexpr int KR_VEC = 4;  // vectors of a warp in flight
+constexpr int KR_VEC = 4;  // vectors of a warp in flight (a lane owns a group of one of four)
 
 __device__ __forceinline__ float2 kr_mul2(float2 a, float2 b) {
     float2 d;
@@ -77,51 +77,73 @@ __device__ __forceinline__ float kr_rcp(float x) {  // to 2^-23
     return d;
 }
 
-// Codes and scale of a group of 32 over eight neighbouring lanes, four values each.  A code is the low 16 bits of
-// code[i]; above them lies what packing drops.
+// Scales of the groups of 32, eight neighbouring lanes each, of four vectors.  The vectors are reduced together: at
+// each of the first two steps a lane hands on the half of them that its partner keeps, so that a lane ends with one
+// vector's group (vector `own_vector`) and works its scale out once, not four times.  inv is the scale's reciprocal; the
+// result says that a group holds an infinity or NaN.
+__device__ __forceinline__ int own_vector(int lane) { return lane >> 1 & 3; }
+__device__ __forceinline__ int vector_owner(int lane, int u) { return (lane & 24) + 2 * u; }
+template <class F>
+__device__ __forceinline__ float reduce_groups(const float (&v)[4], int lane, F f) {
+    const bool up = lane & 4, odd = lane & 2;
+    const float k0 = f(up ? v[2] : v[0], __shfl_xor_sync(0xFFFFFFFFu, up ? v[0] : v[2], 4));
+    const float k1 = f(up ? v[3] : v[1], __shfl_xor_sync(0xFFFFFFFFu, up ? v[1] : v[3], 4));
+    const float k = f(odd ? k1 : k0, __shfl_xor_sync(0xFFFFFFFFu, odd ? k0 : k1, 2));
+    return f(k, __shfl_xor_sync(0xFFFFFFFFu, k, 1));
+}
+template <int BITS>
+__device__ __forceinline__ bool group_scales(const float4 (&x)[4], int lane, __half& scale, float& inv) {
+    auto up = [](float a, float b) { return kr_max_nan(a, b); };
+    auto down = [](float a, float b) { return fminf(a, b); };
+    float top, d, v[4];
+    if (BITS == 4) {
+        // the larger of the group's largest and least; where they tie, whichever comes first
+        float w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            v[u] = up(up(x[u].x, x[u].y), up(x[u].z, x[u].w));
+            w[u] = down(down(x[u].x, x[u].y), down(x[u].z, x[u].w));
+        }
+        const float hi = reduce_groups(v, lane, up), lo = reduce_groups(w, lane, down);
+        float m = hi >= -lo ? hi : lo;
+        top = up(hi, -lo);
+        const bool tie = hi == -lo && hi > 0.0f;
+        if (__any_sync(0xFFFFFFFFu, tie)) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float a = __shfl_sync(0xFFFFFFFFu, hi, vector_owner(lane, u));
+                float f = x[u].w;
+                f = fabsf(x[u].z) == a ? x[u].z : f;
+                f = fabsf(x[u].y) == a ? x[u].y : f;
+                f = fabsf(x[u].x) == a ? x[u].x : f;
+                const unsigned has = __ballot_sync(0xFFFFFFFFu, fabsf(f) == a) >> (lane & 24) & 0xFFu;
+                f = __shfl_sync(0xFFFFFFFFu, f, (lane & 24) + (has ? __ffs(has) - 1 : 0));
+                if (tie && own_vector(lane) == u) m = f;
+            }
+        }
+        d = __fmul_rn(m, -0.125f);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v[u] = up(up(fabsf(x[u].x), fabsf(x[u].y)), up(fabsf(x[u].z), fabsf(x[u].w)));
+        top = reduce_groups(v, lane, up);
+        d = __fmul_rn(top, 1.0f / 127.0f);
+    }
+    const bool bad = !(top < INFINITY);
+    scale = bad ? __ushort_as_half(0x7FFF) : __float2half_rn(fminf(fmaxf(d, -65504.0f), 65504.0f));
+    const float s = __half2float(scale);
+    inv = s == 0.0f ? 0.0f : kr_rcp(s);
+    return __any_sync(0xFFFFFFFFu, bad);
+}
+// Codes of vector u.  A code is the low 16 bits of code[i]; above them lies what packing drops.
 //
 // rint(x / scale) without a quotient: rint of the product with the reciprocal (off by 2.3e-5 at 127) is
 // right unless the product is next to a half; there (one vector in 130 of random values) the remainder x - q scale,
 // which is exact, says which integer is nearest.  Adding 1.5 2^23 rounds to an integer, ties to even, in the low bits.
 template <int BITS>
-__device__ __forceinline__ void quantise(const float4& x, int lane, uint32_t (&code)[4], __half& scale) {
+__device__ __forceinline__ void vector_codes(const float4& x, int lane, int u, __half scale, float own_inv, bool bad, uint32_t (&code)[4]) {
     constexpr float LO = BITS == 4 ? -8.0f : -127.0f, HI = BITS == 4 ? 7.0f : 127.0f, Z = BITS == 4 ? 8.0f : 128.0f;
     constexpr float M = 12582912.0f + Z;
-    const float v[4] = {x.x, x.y, x.z, x.w};
-    float top, d;
-    if (BITS == 4) {
-        // the larger of the group's largest and least; where they tie, whichever comes first
-        float hi = kr_max_nan(kr_max_nan(v[0], v[1]), kr_max_nan(v[2], v[3])), lo = fminf(fminf(v[0], v[1]), fminf(v[2], v[3]));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) {
-            hi = kr_max_nan(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
-            lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-        }
-        float m = hi >= -lo ? hi : lo;
-        if (__any_sync(0xFFFFFFFFu, hi == -lo)) {
-            float f = v[3];
-            bool here = fabsf(f) == hi;
-#pragma unroll
-            for (int i = 2; i >= 0; --i)
-                if (fabsf(v[i]) == hi) {
-                    f = v[i];
-                    here = true;
-                }
-            const unsigned has = __ballot_sync(0xFFFFFFFFu, here) >> (lane & 24) & 0xFFu;
-            f = __shfl_sync(0xFFFFFFFFu, f, (lane & 24) + (has ? __ffs(has) - 1 : 0));
-            if (hi == -lo) m = f;
-        }
-        top = kr_max_nan(hi, -lo);
-        d = __fmul_rn(m, -0.125f);
-    } else {
-        top = kr_max_nan(kr_max_nan(fabsf(v[0]), fabsf(v[1])), kr_max_nan(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = kr_max_nan(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-        d = __fmul_rn(top, 1.0f / 127.0f);
-    }
-    const bool bad = !(top < INFINITY);
-    scale = bad ? __ushort_as_half(0x7FFF) : __float2half_rn(fminf(fmaxf(d, -65504.0f), 65504.0f));
-    const float s = __half2float(scale), inv = s == 0.0f ? 0.0f : kr_rcp(s);
+    const float v[4] = {x.x, x.y, x.z, x.w}, inv = __shfl_sync(0xFFFFFFFFu, own_inv, vector_owner(lane, u));
     bool doubt = bad;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -131,13 +153,15 @@ __device__ __forceinline__ void quantise(const float4& x, int lane, uint32_t (&c
         code[i] = __float_as_uint(t);
     }
     if (__any_sync(0xFFFFFFFFu, doubt)) {
+        const float s = __half2float(__shfl_sync(0xFFFFFFFFu, scale, vector_owner(lane, u)));
+        const bool none = !(fabsf(s) > 0.0f);  // zero, or NaN
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float r = fminf(fmaxf(__fmul_rn(v[i], inv), LO), HI);
             const float q = __fadd_rn(__fadd_rn(r, M), -M), e = __fmaf_rn(-q, s, v[i]), e2 = fabsf(e + e);
             const bool next = e2 > fabsf(s) || (e2 == fabsf(s) && ((int)q & 1));
             const float to = next ? (__float_as_int(e) ^ __float_as_int(s)) < 0 ? q - 1.0f : q + 1.0f : q;
-            code[i] = __float_as_uint((bad || s == 0.0f ? 0.0f : fminf(fmaxf(to, LO), HI)) + M);
+            code[i] = __float_as_uint((none ? 0.0f : fminf(fmaxf(to, LO), HI)) + M);
         }
     }
 }
@@ -346,7 +370,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                 for (int u = 0; u < KR_VEC; ++u) {
                     if (left - u * split <= 0) continue;
                     const bool mine = h + u * step < heads && live;
-                    float4 y = x[u];
+                    float4& y = x[u];
                     if (weight) {
                         const float f = __shfl_sync(0xFFFFFFFFu, inv, (lane & ~(LH / 2 + LH / 4)) + (u >> 1) * (LH / 2) + (u & 1) * (LH / 4));
                         y.x = __fmul_rn(__fmul_rn(y.x, f), w.x);
@@ -375,15 +399,22 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                         }
                     }
                     if (out && mine) *reinterpret_cast<float4*>(out + (h + u * step) * a.hd) = y;
-                    if (IS_K && blk) {
+                }
+                if (IS_K && blk) {
+                    __half scale;
+                    float back;
+                    const bool bad = group_scales<BITS>(x, lane, scale, back);
+                    const int own = h + own_vector(lane) * step;
+                    if (own < heads && live && (hl & 1) == 0) *reinterpret_cast<__half*>(blk + own * a.head_bytes + sat) = scale;
+#pragma unroll
+                    for (int u = 0; u < KR_VEC; ++u) {
+                        if (left - u * split <= 0) continue;
                         uint32_t code[4];
-                        __half scale;
-                        quantise<BITS>(y, lane, code, scale);
-                        if (mine) {
+                        vector_codes<BITS>(x[u], lane, u, scale, back, bad, code);
+                        if (h + u * step < heads && live) {
                             uint8_t* to = blk + (h + u * step) * a.head_bytes;
                             if (BITS == 4) *reinterpret_cast<uint16_t*>(to + kat) = (uint16_t)(code[0] + 16 * code[1] + 256 * code[2] + 4096 * code[3]);
                             else *reinterpret_cast<uint32_t*>(to + kat) = kr_bytes(code[0], code[1], code[2], code[3]);
-                            if ((hl & 7) == 0) *reinterpret_cast<__half*>(to + sat) = scale;
                         }
                     }
                 }
@@ -416,18 +447,20 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
             if (r >= 0 && h < a.n_kv && live) x[j] = *reinterpret_cast<const float4*>(a.v + (long long)r * a.ld_v + h * a.hd + d0);
         }
         uint8_t* blk = a.vc + off + h * a.head_bytes;
+        __half scale;
+        float back;
+        const bool bad = group_scales<BITS>(x, lane, scale, back);
+        const int own = quad_pos(t, own_vector(lane));
+        if ((run.mask >> own & 1) && h < a.n_kv && live && (hl & 1) == 0)
+            *reinterpret_cast<__half*>(blk + scale_place(BITS, a.hd, own, hl >> 3)) = scale;
         uint32_t w[4] = {0, 0, 0, 0};  // bytes of dims 0 and 1, and 2 and 3 (Q8_0: a word each)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             uint32_t code[4];
-            __half scale;
-            quantise<BITS>(x[j], lane, code, scale);
+            vector_codes<BITS>(x[j], lane, j, scale, back, bad, code);
 #pragma unroll
             for (int e = 0; e < (BITS == 4 ? 2 : 4); ++e)  // byte j of word e
                 w[e] = __byte_perm(w[e], BITS == 4 ? code[2 * e & 3] + 16 * code[(2 * e + 1) & 3] : code[e & 3], j == 0 ? 0x3214 : j == 1 ? 0x3240 : j == 2 ? 0x3410 : 0x4210);
-            const int p = quad_pos(t, j);
-            if ((run.mask >> p & 1) && h < a.n_kv && live && (hl & 7) == 0)
-                *reinterpret_cast<__half*>(blk + scale_place(BITS, a.hd, p, hl >> 3)) = scale;
         }
         if (h >= a.n_kv || !live) continue;
         int next;
