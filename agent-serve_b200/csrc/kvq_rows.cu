@@ -210,6 +210,8 @@ __device__ __forceinline__ int nth_quad(unsigned quads, int n) {
         if (i < n) quads &= quads - 1;
     return __ffs(quads) - 1;
 }
+// i / n for n = 1 .. 4 and i below 2^13
+__device__ __forceinline__ int small_div(int i, int n) { return i * (n == 4 ? 16384 : n == 3 ? 21846 : n == 2 ? 32768 : 65536) >> 16; }
 // Position of byte i of a quad's words.
 __device__ __forceinline__ int quad_pos(int t, int i) { return 2 * t + (i >> 1) + (i & 1) * 8; }
 
@@ -246,16 +248,31 @@ __device__ __forceinline__ Run find_run(int row, int slot, int pos) {
     return r;
 }
 
+// How a row is dealt out to warps.
+struct RowSplit {
+    int split, vsplit;         // warps for queries and keys, and for values
+    int turn;                  // warp i's keys begin at vector i + turn, modulo split
+    unsigned long long inv;    // 2^64 / (split + vsplit), rounded up (2 or more)
+};
+__device__ __forceinline__ unsigned task_row(unsigned task, const RowSplit& sp) {  // task / (split + vsplit)
+    return sp.split + sp.vsplit == 1 ? task : (unsigned)__umul64hi(task, sp.inv);
+}
+static RowSplit row_split(int split, int vsplit, int q_vectors) {
+    const unsigned n = (unsigned)(split + vsplit);
+    return {split, vsplit, split ? (split - q_vectors % split) % split : 0, n > 1 ? ~0ull / n + 1 : 0};
+}
+
 // LH lanes per head.  A row has `split` warps for its queries and keys (vectors of 32 / LH heads: first, first +
 // split, ...) and `vsplit` for its share of the run's values.
 // TURN: with a rotation.  (CTAs per SM with the first vectors loaded ahead, 3 / 4: 9001 rows 66 / 73 us, 5003 rows written and
 // read 71 / 80; without loading ahead 65 and 83 at 4.)
 template <int LH, int BITS, bool TURN>
-__global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(const KvqRowsArgs a, int split, int vsplit) {
+__global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(const KvqRowsArgs a, const RowSplit sp) {
     constexpr int HPW = 32 / LH;
     const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
-    const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
+    const int row = (int)task_row(task, sp), split = sp.split, vsplit = sp.vsplit;
+    const int first = (int)(task - (unsigned)row * (split + vsplit));
     if ((unsigned)row >= (unsigned)a.rows) return;
     Window win = {0, 0};
     int pos = 0, slot = 0;
@@ -425,7 +442,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                        nullptr, first, true);
         // keys go on where the queries' share ended, so that a row's warps have equal shares
         if (a.k) {
-            const int q_vectors = a.q ? (a.n_head + HPW - 1) / HPW : 0, begin = (first + split - q_vectors % split) % split;
+            const int begin = first + sp.turn - (first + sp.turn >= split ? split : 0);
             vectors_of(std::true_type(), a.k + (long long)row * a.ld_k + d0, a.k_out ? a.k_out + (long long)row * a.ld_ko + d0 : nullptr, a.n_kv,
                        a.k_weight, a.kc ? a.kc + off : nullptr, begin, !a.q);
         }
@@ -436,7 +453,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
     const Run run = find_run(row, win.slot, win.pos);
     const int quads = run.quads(), nquad = __popc(quads), vv = (a.n_kv + HPW - 1) / HPW;
     for (int i = run.index * vsplit + first - split; i < nquad * vv; i += run.len * vsplit) {
-        const int vec = i / nquad, t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
+        const int vec = small_div(i, nquad), t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
         float4 x[4];
         bool all = true;
 #pragma unroll
@@ -503,11 +520,12 @@ __device__ __forceinline__ uint32_t kr_byte(uint32_t x, int j) { return __byte_p
 __device__ __forceinline__ uint32_t kr_nibble(uint32_t x, int j) { return (x >> 4 * j & 15u) | 0x4B000000u; }
 
 template <int LH, int BITS>
-__global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadArgs a, int split, int vsplit) {
+__global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadArgs a, const RowSplit sp) {
     constexpr int HPW = 32 / LH;
     const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
-    const int row = (int)(task / (unsigned)(split + vsplit)), first = (int)(task - (unsigned)row * (split + vsplit));
+    const int row = (int)task_row(task, sp), split = sp.split, vsplit = sp.vsplit;
+    const int first = (int)(task - (unsigned)row * (split + vsplit));
     if ((unsigned)row >= (unsigned)a.rows) return;
     Window win = {0, 0};
     int pos, slot;
@@ -555,7 +573,7 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
     const Run run = find_run(row, win.slot, win.pos);
     const int quads = run.quads(), nquad = __popc(quads);
     for (int i = run.index * vsplit + first - split; i < nquad * vectors; i += run.len * vsplit) {
-        const int vec = i / nquad, t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
+        const int vec = small_div(i, nquad), t = nth_quad(quads, i - vec * nquad), h = vec * HPW + sub;
         if (h >= a.n_kv || !live) continue;
         const uint8_t* blk = a.vc + off + h * a.head_bytes;
         int next;
@@ -595,19 +613,20 @@ static int kvq_split(int rows, int vectors, int fill = KR_FILL) {
 
 template <int LH, int BITS>
 static cudaError_t rows_launch(const KvqRowsArgs& a, cudaStream_t st) {
-    const int hpw = 32 / LH, vectors = (a.q ? (a.n_head + hpw - 1) / hpw : 0) + (a.k ? (a.n_kv + hpw - 1) / hpw : 0);
+    const int hpw = 32 / LH, q_vectors = a.q ? (a.n_head + hpw - 1) / hpw : 0, vectors = q_vectors + (a.k ? (a.n_kv + hpw - 1) / hpw : 0);
     const int split = vectors ? kvq_split(a.rows, vectors, a.freq ? KR_FILL_TURN : KR_FILL) : 0, vsplit = a.v ? kvq_split(a.rows, (a.n_kv * LH + 31) / 32) : 0;
+    const RowSplit sp = row_split(split, vsplit, q_vectors);
     const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;  // below 2^32: kvq_split
     const unsigned grid = (unsigned)((warps + per - 1) / per);
-    if (a.freq) tf_kvq_rows_kernel<LH, BITS, true><<<grid, KR_THREADS, 0, st>>>(a, split, vsplit);
-    else tf_kvq_rows_kernel<LH, BITS, false><<<grid, KR_THREADS, 0, st>>>(a, split, vsplit);
+    if (a.freq) tf_kvq_rows_kernel<LH, BITS, true><<<grid, KR_THREADS, 0, st>>>(a, sp);
+    else tf_kvq_rows_kernel<LH, BITS, false><<<grid, KR_THREADS, 0, st>>>(a, sp);
     return cudaGetLastError();
 }
 template <int LH, int BITS>
 static cudaError_t read_launch(const KvqReadArgs& a, cudaStream_t st) {
     const int each = kvq_split(a.rows, (a.n_kv * LH + 31) / 32), split = a.k ? each : 0, vsplit = a.v ? each : 0;
     const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;
-    tf_kvq_read_kernel<LH, BITS><<<(unsigned)((warps + per - 1) / per), KR_THREADS, 0, st>>>(a, split, vsplit);
+    tf_kvq_read_kernel<LH, BITS><<<(unsigned)((warps + per - 1) / per), KR_THREADS, 0, st>>>(a, row_split(split, vsplit, 0));
     return cudaGetLastError();
 }
 
