@@ -264,11 +264,13 @@ static RowSplit row_split(int split, int vsplit, int q_vectors) {
 
 // LH lanes per head.  A row has `split` warps for its queries and keys (vectors of 32 / LH heads: first, first +
 // split, ...) and `vsplit` for its share of the run's values.
-// TURN: with a rotation.  (CTAs per SM with the first vectors loaded ahead, 3 / 4: 9001 rows 66 / 73 us, 5003 rows written and
-// read 71 / 80; without loading ahead 65 and 83 at 4.)
-template <int LH, int BITS, bool TURN>
-__global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(const KvqRowsArgs a, const RowSplit sp) {
+// KIND 0: rows are only written, 1: normed or copied too, 2: rotated too.  (A kernel of its own for writing is shorter and has
+// fewer registers: 8192 rows of 8 heads of 64 in 4 bits written and read, 4 CTAs an SM 27.2 -> 26.2 us, 5 25.7.  Rotated,
+// with the first vectors loaded ahead, 3 / 4: 9001 rows 66 / 73 us, 5003 rows written and read 71 / 80.)
+template <int LH, int BITS, int KIND>
+__global__ void __launch_bounds__(KR_THREADS, KIND == 2 ? 3 : KIND == 1 ? 4 : 5) tf_kvq_rows_kernel(const KvqRowsArgs a, const RowSplit sp) {
     constexpr int HPW = 32 / LH;
+    constexpr bool TURN = KIND == 2, WRITE = KIND == 0;
     const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
     const int row = (int)task_row(task, sp), split = sp.split, vsplit = sp.vsplit;
@@ -278,8 +280,8 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
     int pos = 0, slot = 0;
     float4 ahead[KR_VEC];  // the first vectors of the warp's share, on their way while the position is
     if (first < split) {
-        const float* in = a.q ? a.q + (long long)row * a.ld_q : a.k + (long long)row * a.ld_k;
-        const int heads = a.q ? a.n_head : a.n_kv;
+        const float* in = !WRITE && a.q ? a.q + (long long)row * a.ld_q : a.k + (long long)row * a.ld_k;
+        const int heads = !WRITE && a.q ? a.n_head : a.n_kv;
 #pragma unroll
         for (int u = 0; u < KR_VEC; ++u) {
             const int h = (first + u * split) * HPW + sub;
@@ -294,7 +296,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
         slot = __shfl_sync(0xFFFFFFFFu, win.slot, 15);
     }
     long long off = 0;
-    if (a.kc) {
+    if (WRITE || a.kc) {
         if (slot < 0) return;
         if (slot >= a.n_slots || pos < 0 || pos >= a.cap) {
             if (first == 0 && lane == 0) atomicCAS(a.err, 0, slot >= a.n_slots ? ERR_BAD_TOKEN : ERR_POS);
@@ -346,7 +348,8 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
         auto vectors_of = [&](auto is_k, const float* in, float* out, int heads, const float* weight, uint8_t* blk, int begin, bool loaded) {
             constexpr bool IS_K = decltype(is_k)::value;
             float4 w = make_float4(1.f, 1.f, 1.f, 1.f);
-            if (weight && live) w = *reinterpret_cast<const float4*>(weight + d0);
+            const bool norm = !WRITE && weight;
+            if (norm && live) w = *reinterpret_cast<const float4*>(weight + d0);
             const int step = split * HPW;
             int h = begin * HPW + sub;
             const int kat = k_place<BITS>(a.hd, pos & 15, hl), sat = scale_place(BITS, a.hd, pos & 15, hl >> 3);
@@ -366,7 +369,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                 // The squares of the four vectors are summed together: at each of the first two steps a lane hands on
                 // the half of its sums that its partner keeps, so that a lane ends with the sum of one of them.
                 float inv = 1.0f;
-                if (weight) {
+                if (norm) {
                     double ss[KR_VEC];
 #pragma unroll
                     for (int u = 0; u < KR_VEC; ++u) {
@@ -388,7 +391,7 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                     if (left - u * split <= 0) continue;
                     const bool mine = h + u * step < heads && live;
                     float4& y = x[u];
-                    if (weight) {
+                    if (norm) {
                         const float f = __shfl_sync(0xFFFFFFFFu, inv, (lane & ~(LH / 2 + LH / 4)) + (u >> 1) * (LH / 2) + (u & 1) * (LH / 4));
                         y.x = __fmul_rn(__fmul_rn(y.x, f), w.x);
                         y.y = __fmul_rn(__fmul_rn(y.y, f), w.y);
@@ -415,9 +418,9 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                             }
                         }
                     }
-                    if (out && mine) *reinterpret_cast<float4*>(out + (h + u * step) * a.hd) = y;
+                    if (!WRITE && out && mine) *reinterpret_cast<float4*>(out + (h + u * step) * a.hd) = y;
                 }
-                if (IS_K && blk) {
+                if (WRITE || (IS_K && blk)) {
                     __half scale;
                     float back;
                     const bool bad = group_scales<BITS>(x, lane, scale, back);
@@ -437,14 +440,14 @@ __global__ void __launch_bounds__(KR_THREADS, TURN ? 3 : 4) tf_kvq_rows_kernel(c
                 }
             }
         };
-        if (a.q)
+        if (!WRITE && a.q)
             vectors_of(std::false_type(), a.q + (long long)row * a.ld_q + d0, a.q_out + (long long)row * a.ld_qo + d0, a.n_head, a.q_weight,
                        nullptr, first, true);
         // keys go on where the queries' share ended, so that a row's warps have equal shares
-        if (a.k) {
+        if (WRITE || a.k) {
             const int begin = first + sp.turn - (first + sp.turn >= split ? split : 0);
             vectors_of(std::true_type(), a.k + (long long)row * a.ld_k + d0, a.k_out ? a.k_out + (long long)row * a.ld_ko + d0 : nullptr, a.n_kv,
-                       a.k_weight, a.kc ? a.kc + off : nullptr, begin, !a.q);
+                       a.k_weight, a.kc ? a.kc + off : nullptr, begin, WRITE || !a.q);
         }
         return;
     }
@@ -618,8 +621,10 @@ static cudaError_t rows_launch(const KvqRowsArgs& a, cudaStream_t st) {
     const RowSplit sp = row_split(split, vsplit, q_vectors);
     const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;  // below 2^32: kvq_split
     const unsigned grid = (unsigned)((warps + per - 1) / per);
-    if (a.freq) tf_kvq_rows_kernel<LH, BITS, true><<<grid, KR_THREADS, 0, st>>>(a, sp);
-    else tf_kvq_rows_kernel<LH, BITS, false><<<grid, KR_THREADS, 0, st>>>(a, sp);
+    const bool write = !a.q && !a.k_out && !a.k_weight;
+    if (a.freq) tf_kvq_rows_kernel<LH, BITS, 2><<<grid, KR_THREADS, 0, st>>>(a, sp);
+    else if (!write) tf_kvq_rows_kernel<LH, BITS, 1><<<grid, KR_THREADS, 0, st>>>(a, sp);
+    else tf_kvq_rows_kernel<LH, BITS, 0><<<grid, KR_THREADS, 0, st>>>(a, sp);
     return cudaGetLastError();
 }
 template <int LH, int BITS>
