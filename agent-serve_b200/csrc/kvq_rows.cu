@@ -264,13 +264,13 @@ static RowSplit row_split(int split, int vsplit, int q_vectors) {
 
 // LH lanes per head.  A row has `split` warps for its queries and keys (vectors of 32 / LH heads: first, first +
 // split, ...) and `vsplit` for its share of the run's values.
-// KIND 0: rows are only written, 1: normed or copied too, 2: rotated too.  (A kernel of its own for writing is shorter and has
-// fewer registers: 8192 rows of 8 heads of 64 in 4 bits written and read, 4 CTAs an SM 27.2 -> 26.2 us, 5 25.7.  Rotated,
-// with the first vectors loaded ahead, 3 / 4: 9001 rows 66 / 73 us, 5003 rows written and read 71 / 80.)
+// KIND 0: rows are only written, 1: normed or copied, and written if there is a cache, 2: rotated too, without a cache, 3: with
+// one.  (Kernels of their own are shorter and have fewer registers: 8192 rows of 8 heads of 64 in 4 bits written and read, as
+// KIND 1 27.2 us, at 4 CTAs an SM 26.2, at 5 25.7; 9001 rows rotated, as KIND 3 65.4, alone 63.3, at 4 CTAs an SM 69.)
 template <int LH, int BITS, int KIND>
-__global__ void __launch_bounds__(KR_THREADS, KIND == 2 ? 3 : KIND == 1 ? 4 : 5) tf_kvq_rows_kernel(const KvqRowsArgs a, const RowSplit sp) {
+__global__ void __launch_bounds__(KR_THREADS, KIND >= 2 ? 3 : KIND == 1 ? 4 : 5) tf_kvq_rows_kernel(const KvqRowsArgs a, const RowSplit sp) {
     constexpr int HPW = 32 / LH;
-    constexpr bool TURN = KIND == 2, WRITE = KIND == 0;
+    constexpr bool TURN = KIND >= 2, WRITE = KIND == 0, CACHE = KIND == 0 || KIND == 3;
     const int lane = threadIdx.x & 31, hl = lane & (LH - 1), sub = lane / LH;
     const unsigned task = blockIdx.x * (KR_THREADS / 32) + (threadIdx.x >> 5);
     const int row = (int)task_row(task, sp), split = sp.split, vsplit = sp.vsplit;
@@ -289,14 +289,14 @@ __global__ void __launch_bounds__(KR_THREADS, KIND == 2 ? 3 : KIND == 1 ? 4 : 5)
             if (h < heads && hl * 4 < a.hd) ahead[u] = *reinterpret_cast<const float4*>(in + h * a.hd + hl * 4);
         }
         if (a.pos) pos = a.pos[row];
-        if (a.kc) slot = row_slot(a, row);
+        if (CACHE || (KIND == 1 && a.kc)) slot = row_slot(a, row);
     } else {
         win = load_window(a, row);
         pos = __shfl_sync(0xFFFFFFFFu, win.pos, 15);
         slot = __shfl_sync(0xFFFFFFFFu, win.slot, 15);
     }
     long long off = 0;
-    if (WRITE || a.kc) {
+    if (CACHE || (KIND == 1 && a.kc)) {
         if (slot < 0) return;
         if (slot >= a.n_slots || pos < 0 || pos >= a.cap) {
             if (first == 0 && lane == 0) atomicCAS(a.err, 0, slot >= a.n_slots ? ERR_BAD_TOKEN : ERR_POS);
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(KR_THREADS, KIND == 2 ? 3 : KIND == 1 ? 4 : 5)
                     }
                     if (!WRITE && out && mine) *reinterpret_cast<float4*>(out + (h + u * step) * a.hd) = y;
                 }
-                if (WRITE || (IS_K && blk)) {
+                if (WRITE || (IS_K && (CACHE || (KIND == 1 && blk)))) {
                     __half scale;
                     float back;
                     const bool bad = group_scales<BITS>(x, lane, scale, back);
@@ -452,6 +452,7 @@ __global__ void __launch_bounds__(KR_THREADS, KIND == 2 ? 3 : KIND == 1 ? 4 : 5)
         return;
     }
 
+    if (KIND == 2) return;  // (no values)
     // values: (quad, vector) pairs of the run, dealt out to its warps
     const Run run = find_run(row, win.slot, win.pos);
     const int quads = run.quads(), nquad = __popc(quads), vv = (a.n_kv + HPW - 1) / HPW;
@@ -622,7 +623,8 @@ static cudaError_t rows_launch(const KvqRowsArgs& a, cudaStream_t st) {
     const long long warps = (long long)a.rows * (split + vsplit), per = KR_THREADS / 32;  // below 2^32: kvq_split
     const unsigned grid = (unsigned)((warps + per - 1) / per);
     const bool write = !a.q && !a.k_out && !a.k_weight;
-    if (a.freq) tf_kvq_rows_kernel<LH, BITS, 2><<<grid, KR_THREADS, 0, st>>>(a, sp);
+    if (a.freq && a.kc) tf_kvq_rows_kernel<LH, BITS, 3><<<grid, KR_THREADS, 0, st>>>(a, sp);
+    else if (a.freq) tf_kvq_rows_kernel<LH, 4, 2><<<grid, KR_THREADS, 0, st>>>(a, sp);
     else if (!write) tf_kvq_rows_kernel<LH, BITS, 1><<<grid, KR_THREADS, 0, st>>>(a, sp);
     else tf_kvq_rows_kernel<LH, BITS, 0><<<grid, KR_THREADS, 0, st>>>(a, sp);
     return cudaGetLastError();
