@@ -19,10 +19,10 @@
 // rising positions (a run) share their quads out over the run's warps.  Row by row, the bytes of a head's V
 // touch 16 lines an instruction.
 //
-// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 66 us, 5.6 TB/s (106
-// instructions a vector, issue slots 60 %, DRAM 62 % of its peak).  The same with values and 8-bit writing, 5003 rows: 58 us
-// (issue 59 %; a key's vector takes twice a query's instructions).  8192 rows of 8 heads of 64 in 4 bits: 20 us to write
-// (185 instructions a vector, issue 70 %; a warp has only four), 10 us to read.
+// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 63.5 us, 5.8 TB/s (101
+// instructions a vector, issue slots 59 %).  The same with values and 8-bit writing, 5003 rows: 55 us (131 a vector, issue
+// 58 %; a key's vector takes twice a query's instructions).  8192 rows of 8 heads of 64 in 4 bits: 16.7 us to write (142 a
+// vector, issue 70 %, ALU 57 %; a warp has only four), 9 us to read.
 #include <type_traits>
 
 #include "kvq.cuh"
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
 // Warps per row: one when rows alone fill the device (`fill` warps on each of its SMs), else a row's vectors are
 // shared out so that few rows finish in one round of loads.  16 warps, and twice what an SM holds where they carry
 // a whole row of queries and keys, whose last round would else be long: 5003 rows of 32 + 8 + 8 heads of 128 written
-// in 8 bits and read back, 69.6 us with 16, 68.4 with 48; 9001 rows of 32 + 8 have one warp each either way, 66.6.
+// in 8 bits and read back, 69.6 us with 16, 68.4 with 48.
 constexpr int KR_FILL = 16, KR_FILL_TURN = 48;
 static int kvq_split(int rows, int vectors, int fill = KR_FILL) {
     const int want = (int)((148ll * fill + rows - 1) / rows);

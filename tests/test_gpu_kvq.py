@@ -135,6 +135,23 @@ def test_write_and_read(kv, hd, HK, rows, cap):
 
 
 @pytest.mark.parametrize("kv", TYPES)
+@pytest.mark.parametrize("hd,HK,first,rows", [(32, 7, 0, 64), (64, 9, 3, 61), (96, 5, 16, 48), (128, 8, 1, 30), (128, 1, 0, 16)])
+def test_every_group_its_own_corner(kv, hd, HK, first, rows):
+    """Rows of neighbouring positions: groups that the kernel reduces together are of different kinds."""
+    rng = np.random.default_rng(hd + rows)
+    c = Cache(kv, hd, HK, 64, 1, 5).upload()
+    corners = awkward_rows(rng, 40, 1, 32).reshape(40, 32)
+    x = corners[rng.integers(0, 40, rows * 2 * HK * hd // 32)].reshape(rows, 2 * HK, hd)
+    for r in range(rows):
+        c.put(0, first + r, x[r, :HK], x[r, HK:])
+    s, p, d = i32([0] * rows), i32(range(first, first + rows)), cuda(x.reshape(rows, -1))
+    ld = 2 * HK * hd
+    native.check(native.lib().tf_op_kv_quant(*c.args(), ptr(s), ptr(p), ptr(d), ld, ptr(d) + 4 * HK * hd, ld, rows, HK, hd, None))
+    assert device_error() == 0
+    assert c.same()
+
+
+@pytest.mark.parametrize("kv", TYPES)
 def test_values_next_to_the_border_of_two_codes(kv):
     """Every half between two codes, and its neighbours in fp32 on both sides, at scales of all mantissas: the code is the
     nearest, ties to even."""
