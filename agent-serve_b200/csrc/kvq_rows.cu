@@ -4,10 +4,12 @@
 //   norm    y = (x inv) w, inv = 1 / sqrt(mean x^2 + eps), the mean in 64 bits (the row norm's own order)
 //   rotate  pairs (j, j + rot / 2): (a, b) -> (a c - b s, a s + b c), c and s the cosine and sine of
 //           pos freq[j].  The angle is a product in 64 bits: in fp32 a far position's angle is off by
-//           2^-24 of itself, 0.004 at 65536.  Queries: a product and an fma.  Keys: the two products and their
-//           sum are carried with their rounding errors (Dekker's product by fma, Knuth's sum) and rounded once, so
-//           that a key next to the border of two codes takes the same code wherever it is computed.  (In 64 bits:
-//           12 conversions a vector through a pipe of 4 lanes a cycle; 9001 rows of 32 + 8 heads of 128, 135 us.)
+//           2^-24 of itself, 0.004 at 65536.  The two products and their sum are carried with their rounding
+//           errors (Dekker's product by fma, Knuth's sum) and rounded once, in queries and in keys: pairs whose
+//           products cancel keep their last bits, and a key next to the border of two codes takes the same code
+//           wherever it is computed.  (A product and an fma, for queries alone: 9001 rows of 32 + 8 heads of 128 63.5
+//           us instead of 69.0, and off by 2^-25 of the larger product.  In 64 bits it
+//           would take 12 conversions a vector through a pipe of 4 lanes a cycle.)
 //   Q4_0    scale = f16(m / -8), m the group's first value of largest magnitude; code = rint(x / scale) in [-8, 7]
 //   Q8_0    scale = f16(max|x| r), r = 1 / 127 in fp32; code = rint(x / scale) in [-127, 127]
 // A group with an infinity or NaN gets a NaN for its scale and reads back as NaN; a scale beyond f16 is held at
@@ -19,9 +21,8 @@
 // rising positions (a run) share their quads out over the run's warps.  Row by row, the bytes of a head's V
 // touch 16 lines an instruction.
 //
-// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 63.5 us, 5.8 TB/s (101
-// instructions a vector, issue slots 59 %).  The same with values and 8-bit writing, 5003 rows: 55 us (131 a vector, issue
-// 58 %; a key's vector takes twice a query's instructions).  8192 rows of 8 heads of 64 in 4 bits: 16.7 us to write (142 a
+// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 69.0 us, 5.3 TB/s.  The same
+// with values and 8-bit writing, and read back, 5003 rows: 76.3 us.  8192 rows of 8 heads of 64 in 4 bits: 16.7 us to write (142 a
 // vector, issue 70 %, ALU 57 %; a warp has only four), 9 us to read.
 #include <type_traits>
 
@@ -405,17 +406,17 @@ __global__ void __launch_bounds__(KR_THREADS, KIND >= 2 ? 3 : KIND == 1 ? 4 : 5)
                         m.z = __shfl_sync(0xFFFFFFFFu, y.z, mate);
                         m.w = __shfl_sync(0xFFFFFFFFu, y.w, mate);
                         if (turn) {
-                            const float4 z = make_float4(__fmaf_rn(y.x, c.x, __fmul_rn(m.x, s.x)), __fmaf_rn(y.y, c.y, __fmul_rn(m.y, s.y)),
-                                                         __fmaf_rn(y.z, c.z, __fmul_rn(m.z, s.z)), __fmaf_rn(y.w, c.w, __fmul_rn(m.w, s.w)));
-                            if (IS_K) {
-                                const float2 r0 = kr_turn(make_float2(y.x, y.y), make_float2(c.x, c.y), make_float2(m.x, m.y), make_float2(s.x, s.y));
-                                const float2 r1 = kr_turn(make_float2(y.z, y.w), make_float2(c.z, c.w), make_float2(m.z, m.w), make_float2(s.z, s.w));
+                            const float2 r0 = kr_turn(make_float2(y.x, y.y), make_float2(c.x, c.y), make_float2(m.x, m.y), make_float2(s.x, s.y));
+                            const float2 r1 = kr_turn(make_float2(y.z, y.w), make_float2(c.z, c.w), make_float2(m.z, m.w), make_float2(s.z, s.w));
+                            float4 z = make_float4(r0.x, r0.y, r1.x, r1.y);
+                            if (!(kr_max_nan(kr_max_nan(fabsf(z.x), fabsf(z.y)), kr_max_nan(fabsf(z.z), fabsf(z.w))) < INFINITY)) {
                                 // an infinity's rounding error is NaN
-                                y = make_float4(fabsf(r0.x) < INFINITY ? r0.x : z.x, fabsf(r0.y) < INFINITY ? r0.y : z.y,
-                                                fabsf(r1.x) < INFINITY ? r1.x : z.z, fabsf(r1.y) < INFINITY ? r1.y : z.w);
-                            } else {
-                                y = z;
+                                if (!(fabsf(z.x) < INFINITY)) z.x = __fmaf_rn(y.x, c.x, __fmul_rn(m.x, s.x));
+                                if (!(fabsf(z.y) < INFINITY)) z.y = __fmaf_rn(y.y, c.y, __fmul_rn(m.y, s.y));
+                                if (!(fabsf(z.z) < INFINITY)) z.z = __fmaf_rn(y.z, c.z, __fmul_rn(m.z, s.z));
+                                if (!(fabsf(z.w) < INFINITY)) z.w = __fmaf_rn(y.w, c.w, __fmul_rn(m.w, s.w));
                             }
+                            y = z;
                         }
                     }
                     if (!WRITE && out && mine) *reinterpret_cast<float4*>(out + (h + u * step) * a.hd) = y;

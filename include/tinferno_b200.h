@@ -384,7 +384,8 @@ TF_API int tf_op_kv_commit(void* k_cache, void* v_cache, int kv_type, int n_laye
  *   pairs (j, j + rope_dim / 2) of the first rope_dim dims turned by the angle pos[r] freq[j]
  *                                             (apply_rope, src/attention.hpp:25; freq nullptr: none)
  * The angle is a product in 64 bits (tf_op_rope keeps the reference's fp32 product, off by 2^-24 of
- * itself); cosine and sine are fp32, their two products are summed in 64 bits and rounded once.
+ * itself); cosine and sine are fp32, their two products and the sum are rounded once, in queries and in
+ * keys alike (as in 64 bits, but for sums within 2^-46 of the products of a tie).
  * q (or k) may be nullptr together with its output; outputs may be the inputs themselves (same
  * pointer and stride), else in memory of their own.  pos [rows]: a negative one leaves its row as it
  * is; nullptr where nothing is rotated.  head_dim and rope_dim: multiples of 8, head_dim up to 128. */
