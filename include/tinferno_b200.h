@@ -417,7 +417,9 @@ TF_API int tf_op_qkv_store(float* q_out, int ld_qo, void* k_cache, void* v_cache
  * n_new[b] on are zero, and so are all rows of a sequence whose slot, n_ctx or n_new does not fit
  * the cache (which goes to tf_op_device_error).  Cache rows that a row does not see do not reach it,
  * whatever they hold.  Scores, softmax and sums are fp32-equivalent: errors are relative to the
- * largest key and value that a row sees.  T <= 64, any number of query heads per kv head, up to 1024
+ * largest key that a row sees, and to each group of 32 dims' own values (of weights times values, what is
+ * below 2^-18 of the row's largest weight times its largest value is held to less).  T <= 64, any number
+ * of query heads per kv head, up to 1024
  * heads.  Workspace: as for tf_op_attn_tree.  Work is counted in 32 bits: B * n_kv_heads *
  * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 24) must be below 2^31. */
 TF_API int tf_op_attn_quant_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);
