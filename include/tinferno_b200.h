@@ -414,8 +414,9 @@ TF_API int tf_op_qkv_store(float* q_out, int ld_qo, void* k_cache, void* v_cache
 /* Attention of up to T new rows of B sequences over the cache, their own keys and values written
  * before: row t < n_new[b] (nullptr: T) of sequence b, in slot slots[b] (nullptr: b), sees cache
  * rows 0 .. n_ctx[b] + t.  B = 1, T = 1 is decode attention.  q and out: row b * T + t.  Rows from
- * n_new[b] on are zero, and so are all rows of a sequence whose slot, n_ctx or n_new does not fit
- * the cache (which goes to tf_op_device_error).  Cache rows that a row does not see do not reach it,
+ * n_new[b] on are zero.  A sequence with n_new[b] = 0 (a padded batch) is empty, whatever its slot and
+ * n_ctx say.  All rows of a sequence whose slot, n_ctx or n_new does not fit the cache are zero too, and
+ * tf_op_device_error has TF_DEV_ERR_POS.  Cache rows that a row does not see do not reach it,
  * whatever they hold.  Scores, softmax and sums are fp32-equivalent: errors are relative to the
  * largest key that a row sees, and to each group of 32 dims' own values (of weights times values, what is
  * below 2^-18 of the row's largest weight times its largest value is held to less).  T <= 64, any number
