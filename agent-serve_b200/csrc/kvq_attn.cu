@@ -235,9 +235,9 @@ __device__ __forceinline__ KvqSeq kvq_seq(const KvqAttnArgs& a, int rep, int rt,
     KvqSeq s;
     s.slot = a.slots ? a.slots[b] : b;
     s.n_ctx = a.n_ctx[b];
-    s.n_new = a.n_new ? min(a.n_new[b], a.T) : a.T;
+    s.n_new = a.n_new ? a.n_new[b] : a.T;
     // without new rows a sequence is empty (a padded batch), whatever its slot and length say
-    s.bad = s.n_new < 0 || (s.n_new > 0 && (s.slot < 0 || s.slot >= a.n_slots || s.n_ctx < 0 || s.n_ctx > a.cap - s.n_new));
+    s.bad = s.n_new < 0 || s.n_new > a.T || (s.n_new > 0 && (s.slot < 0 || s.slot >= a.n_slots || s.n_ctx < 0 || s.n_ctx > a.cap - s.n_new));
     if (s.bad) s.n_new = 0;
     s.blocks = s.n_new ? (s.n_ctx + s.n_new + 15) >> 4 : 0;
     s.units = a.n_kv * ((s.n_new * rep + rt - 1) / rt);

@@ -415,12 +415,12 @@ TF_API int tf_op_qkv_store(float* q_out, int ld_qo, void* k_cache, void* v_cache
  * before: row t < n_new[b] (nullptr: T) of sequence b, in slot slots[b] (nullptr: b), sees cache
  * rows 0 .. n_ctx[b] + t.  B = 1, T = 1 is decode attention.  q and out: row b * T + t.  Rows from
  * n_new[b] on are zero.  A sequence with n_new[b] = 0 (a padded batch) is empty, whatever its slot and
- * n_ctx say.  All rows of a sequence whose slot, n_ctx or n_new does not fit the cache are zero too, and
- * tf_op_device_error has TF_DEV_ERR_POS.  Cache rows that a row does not see do not reach it,
- * whatever they hold.  Scores, softmax and sums are fp32-equivalent: errors are relative to the
- * largest key that a row sees, and to each group of 32 dims' own values (of weights times values, what is
- * below 2^-18 of the row's largest weight times its largest value is held to less).  T <= 64, any number
- * of query heads per kv head, up to 1024
+ * n_ctx say.  All rows of a sequence whose slot, n_ctx or n_new does not fit the cache, or whose n_new is
+ * above T, are zero too, and tf_op_device_error has TF_DEV_ERR_POS.  Cache rows that a row does not see do
+ * not reach it, whatever they hold.  Scores, softmax and sums are fp32-equivalent: errors are relative to
+ * the largest key that a row sees, and to each group of 32 dims' own values (of weights times values, what
+ * is below 2^-18 of the row's largest weight times its largest value is held to less).  T <= 64, any
+ * number of query heads per kv head, up to 1024
  * heads.  Workspace: as for tf_op_attn_tree.  Work is counted in 32 bits: B * n_kv_heads *
  * ceil(T * (n_heads / n_kv_heads) / 4) * (cap / 16 + 24) must be below 2^31. */
 TF_API int tf_op_attn_quant_workspace(int B, int T, int n_heads, int n_kv_heads, int head_dim, size_t* bytes);

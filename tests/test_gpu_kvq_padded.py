@@ -41,6 +41,19 @@ def test_nothing_but_padding(cap):
     assert (c.got() == 0).all() and device_error() == 0
 
 
+@pytest.mark.parametrize("cap", [96, 8192])
+def test_more_new_rows_than_the_call_holds(cap):
+    """n_new above T is refused like a length that does not fit, not cut."""
+    c = Case(native.TF_KV_Q8_0, 64, 8, 2, [40, 70, 33], [2, 2, 2], 2, 1, cap=cap).run()
+    for n in (3, 2 ** 31 - 1):
+        c.out.fill_(7.0)
+        c.run(upload=False, n_new=i32([2, n, 2]))
+        got = c.got()
+        assert device_error() == native.TF_DEV_ERR_POS
+        assert (got[1] == 0).all()
+        others_hold(c, got, (0, 2))
+
+
 @pytest.mark.parametrize("kv", TYPES)
 @pytest.mark.parametrize("captured", [False, True])
 def test_padded_step(kv, captured):
