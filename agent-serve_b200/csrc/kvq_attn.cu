@@ -59,6 +59,7 @@ constexpr int KA_UNIT_COST = 24;
 // new rows over 8000 14.1 / 14.4 / 14.2 / 17.7.
 constexpr int KA_MIN_RANGE = 24;
 constexpr int KA_MAX_SPLIT = 8;    // CTAs of a cluster
+constexpr int KA_SNAP = 6;         // a cut this near to a unit's first or last block moves there
 constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
 constexpr int KA_MAX_GRID = 1024;  // descriptors of 32 bytes in the workspace's first 32 KB
 constexpr size_t KA_DESC_BYTES = 32768;
@@ -244,7 +245,12 @@ __device__ __forceinline__ KvqSeq kvq_seq(const KvqAttnArgs& a, int rep, int rt,
 }
 __device__ __forceinline__ int kvq_len(const KvqSeq& s) { return s.n_new ? s.units * (s.blocks + KA_UNIT_COST) : 0; }
 
-// A CTA's range [g0, g1) of the flattened blocks: `b` is the sequence it begins in, `base` that one's start.
+// Where the cut at offset t of a unit of n blocks falls: near a unit's ends it would cost a partial result for
+// next to nothing.
+__device__ __forceinline__ int kvq_cut(int t, int n) { return t < KA_SNAP ? 0 : n - t < KA_SNAP ? max(t, n) : t; }
+
+// A CTA's range [g0, g1) of the flattened blocks, before its ends are moved (kvq_cut): `b` is the sequence it
+// begins in, `base` that one's start.
 struct KvqRange {
     int g0, g1, per, b, base;
 };
@@ -918,8 +924,8 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
             if (gpos >= base + len) break;
             const int per_unit = sq.blocks + KA_UNIT_COST, unit = (gpos - base) / per_unit;
             ub = base + unit * per_unit;
-            blk0 = gpos - ub;
-            blk1 = min(sq.blocks, range.g1 - ub);
+            blk0 = kvq_cut(gpos - ub, sq.blocks);
+            blk1 = min(sq.blocks, range.g1 - ub < per_unit ? kvq_cut(range.g1 - ub, sq.blocks) : per_unit);
             gpos = min(range.g1, ub + per_unit);
             if (blk0 >= blk1) continue;
             const int tiles = sq.units / a.n_kv;
@@ -1044,7 +1050,8 @@ tf_kvq_attn_kernel(const KvqAttnArgs a, const KvqPlan pl) {
         }
         __syncthreads();
         if (begins) {
-            const int c1 = (ub + sq.blocks - 1) / range.per;  // the CTA with the last block
+            const int last = (ub + sq.blocks - 1) / range.per;  // the CTA with the last block, if its cut stays
+            const int c1 = kvq_cut(last * range.per - ub, sq.blocks) >= sq.blocks ? last - 1 : last;
             const KvqDesc de = {ends ? -1 : b, kvh, tile, rows, (int)blockIdx.x, c1};
             if (!ends) open = de;
             if (pl.by_unit && threadIdx.x == 0) desc[(b * a.n_kv + kvh) * pl.tiles + tile] = de;
