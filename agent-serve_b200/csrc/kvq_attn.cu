@@ -13,8 +13,8 @@
 //                       side; probabilities go to the second product's operand by movmatrix;
 //   more (ManyRows)     rows as M, positions as N: the scores' registers are the second product's operand as they
 //                       stand; up to 8 rows, the 16 rows of M hold q's two halves.
-// 64 sequences over 8192 positions, 8 kv heads of 128, 4 rows each, 4 bits: 141 us as FewRows, 153 as ManyRows; 16 sequences
-// of 16 new rows over 4000 positions, 64 dims: 61 and 56.
+// 64 sequences over 8192 positions, 8 kv heads of 128, 4 rows each, 4 bits: 148 us as FewRows, 191 as ManyRows; 16 sequences
+// of 16 new rows over up to 4000 positions, 64 dims: 104 and 56.
 //
 // Arithmetic (fp32-equivalent).  Codes less their zero are exact in f16: (code | 0x6400) is 1024 + code, and
 // the high nibble in place 1024 + 16 code; the 16 is taken out of q (K) or of the output row (V).  q is split
@@ -26,9 +26,9 @@
 // A group of dims whose values are 2^-18 of the row's largest, or a position whose weight is, so has 24 bits.  (Without
 // the 2^11, cut towards zero, 64 sequences over up to 8128 positions take 90.5 us instead of 91.6 and calls with 5 rows or
 // more a kv head 1 to 8 % less, but a group at 2^-14 is off by 2e-5 to 4e-5, and 20000 weights of e^-18 by 7e-5.)  k is a
-// row's own: its bits must not hang on what only another row sees.  A block's P V is summed from zero and joins the output by an fp32
-// addition (3 % of the time): the matrix accumulator truncates, and a sum of one sign carried in it through 166
-// blocks is off by 2.5e-5.
+// row's own: its bits must not hang on what only another row sees.  A block's P V is summed from zero and joins the output
+// by an fp32 addition (3 % of the time): the matrix accumulator truncates, and a sum of one sign carried in it through
+// 166 blocks is off by 2.5e-5.
 //
 // Work is cut into units (sequence, kv head, row tile) and each unit into blocks of 16 positions.  A CTA's warps take
 // its blocks in turn, each with its own ring of cp.async copies (no barrier in the loop), and join at the end.
@@ -38,10 +38,10 @@
 //   tf_kvq_combine_kernel.
 // All joins are in a fixed order: results repeat bit for bit.
 //
-// Measured: 64 sequences over 1161 to 8128 positions, 8 kv heads of 128, 4 rows each: 4 bits 91 us (3.8 TB/s: 360
-// instructions per block and warp, issue slots 65 %, ALU and FMA pipes 44 %, DRAM 41 %; the copies alone take 62 us);
-// 32 such sequences in 8 bits 60 us (5.4 TB/s).  1 sequence over 96 positions, 64 dims: 4.0 us, a launch and four
-// dependent reads.
+// Measured: 64 sequences over 1161 to 8128 positions, 8 kv heads of 128, 4 rows each: 4 bits 92 us (3.7 TB/s: 384
+// instructions per block and warp, issue slots 64 to 67 %, FMA pipe 45 %, ALU 42 %, DRAM 40 %, 24 bytes a thread spilled; the
+// copies alone take 62 us); 32 such sequences in 8 bits 61 us (5.3 TB/s).  1 sequence over 96 positions, 64 dims: 4.0 us in a cache
+// of 112 positions, a launch and four dependent reads; 6.1 in one of 8192, where the capacity asks for ranges.
 #include <atomic>
 #include <type_traits>
 
@@ -52,15 +52,19 @@ namespace tfb {
 constexpr int KA_THREADS = 128;
 constexpr int KA_WARPS = KA_THREADS / 32;
 // Blocks that a unit's start and end take the time of in a range: 8 / 16 / 24 / 32, 64 sequences over up to 8128 positions
-// 89.6 / 87.8 / 87.9 / 88.6 us, 128 over up to 4000 (8 bits, 64 dims) 68.9 / 66.3 / 64.5 / 64.0, 16 of 16 new rows 55.7 /
-// 53.7 / 52.0 / 52.0.
+// 93.2 / 91.7 / 92.0 / 92.9 us, 128 over up to 4000 (8 bits, 64 dims) 68.4 / 65.4 / 63.8 / 63.9, 16 of 16 new rows 58.2 /
+// 56.6 / 56.5 / 56.8.
 constexpr int KA_UNIT_COST = 24;
-// Blocks of a CTA's range at least: 8 / 16 / 24 / 32, 1 sequence over 32001 positions 14.3 / 10.8 / 10.8 / 11.2 us, 1 of 4
-// new rows over 8000 14.1 / 14.4 / 14.2 / 17.7.
+// Blocks of a CTA's range at least: 8 / 16 / 24 / 32, 1 sequence over 32001 positions 14.3 / 10.7 / 11.0 / 11.4 us, 1 over
+// 16000 (64 dims) 11.8 / 11.3 / 10.6 / 11.7, 1 of 4 new rows over 8000 14.8 / 15.7 / 16.0 / 17.9.
 constexpr int KA_MIN_RANGE = 24;
 constexpr int KA_MAX_SPLIT = 8;    // CTAs of a cluster
-constexpr int KA_SNAP = 6;         // a cut this near to a unit's first or last block moves there
-constexpr int KA_SLACK = 8;        // binary orders that a running maximum may lag behind
+// A cut this near to a unit's first or last block moves there: 0 / 6, 1 sequence over 96 positions in a cache of 8192 7.0 / 6.1
+// us, 64 over up to 100 8.4 / 7.5, 64 over up to 8128 91.9 / 92.3, 33 of 4 rows over up to 2000 24.7 / 26.1.
+constexpr int KA_SNAP = 6;
+// Binary orders that a running maximum may lag behind: 4 / 6 / 8, 64 sequences over up to 8128 positions 92.6 / 91.8 / 91.6 us,
+// 32 of 5 new rows over 1144 17.0 / 16.4 / 16.3.
+constexpr int KA_SLACK = 8;
 constexpr int KA_MAX_GRID = 1024;  // descriptors of 32 bytes in the workspace's first 32 KB
 constexpr size_t KA_DESC_BYTES = 32768;
 
@@ -83,11 +87,13 @@ struct alignas(32) KvqDesc {  // a unit split over CTAs c0 .. c1
 
 __host__ __device__ inline size_t kvq_part_floats(int rt, int hd) { return (size_t)rt * (hd + 2); }
 
-// Row tiles: 0: 4 rows, 1: 8, 2: 16.  (32 share a block's codes over more rows, but need 255 registers at 128 dims: 32
-// sequences of 5 x 6 rows over 1144 positions 16.2 -> 19.3 us, 16 of 16 x 4 over 4000, 64 dims, 55.9 -> 57.4.)
+// Row tiles: 0: 4 rows, 1: 8, 2: 16.  (32 share a block's codes over more rows, but need 255 registers at 128 dims.  Before the
+// second half of p carried 2^11: 32 sequences of 5 x 6 rows over 1144 positions 16.2 -> 19.3 us, 16 of 16 x 4 over 4000, 64
+// dims, 55.9 -> 57.4.)
 __host__ __device__ constexpr int kvq_rt(int mode) { return mode == 0 ? 4 : mode == 1 ? 8 : 16; }
 
-__host__ __device__ constexpr int kvq_ctas(int mode) { return mode == 2 ? 3 : 4; }  // 168 or 128 registers a thread
+// 168 or 128 registers a thread (at 128 dims 48 to 84 and up to 28 bytes spilled)
+__host__ __device__ constexpr int kvq_ctas(int mode) { return mode == 2 ? 3 : 4; }
 
 template <int BITS, int HD, int MODE>
 struct KvqCfg {
@@ -1171,9 +1177,10 @@ static int kvq_sms() {
 
 // CTAs per unit where a cluster takes each unit: as many as leave all units resident, while a warp has no more than
 // KA_TURNS blocks at the cache's capacity (lengths are on the device; longer ones are balanced better by ranges).
-// Clusters / ranges: 32 sequences of 5 new rows over 1144 positions (9 blocks a warp) 15.8 / 20.4 us, 4 of 8 over 2000 (8)
-// 16.9 / 25.4, 1 of 4 over 8000 (16) 18.9 / 14.7, 3 of 1 over 9000 (18) 17.9 / 11.9.  Clusters of 16 gain 0 to 5 % from 3000
-// positions on and lose 20 % on the shortest calls.
+// Clusters / ranges: 32 sequences of 5 new rows over 1144 positions (9 blocks a warp) 16.5 / 23.0 us, 4 of 8 over 2000 (8)
+// 19.2 / 23.0, 1 of 4 over 8000 (16) 22.1 / 16.0, 3 of 1 over 9000 (18) 14.4 / 12.5.  Capacity stands for lengths that the host
+// does not know: short contexts in a long cache take ranges (32 of 5 rows over 1144 in a cache of 8192: 22.9).  Clusters of 16
+// gain 0 to 5 % from 3000 positions on and lose 20 % on the shortest calls.
 constexpr int KA_TURNS = 10;
 static int kvq_split_of(long long units, int cap, int slots) {
     if (units > slots) return 0;

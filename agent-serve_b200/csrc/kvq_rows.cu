@@ -8,7 +8,7 @@
 //           errors (Dekker's product by fma, Knuth's sum) and rounded once, in queries and in keys: pairs whose
 //           products cancel keep their last bits, and a key next to the border of two codes takes the same code
 //           wherever it is computed.  (A product and an fma, for queries alone: 9001 rows of 32 + 8 heads of 128 63.5
-//           us instead of 69.0, and off by 2^-25 of the larger product.  In 64 bits it
+//           us instead of 69.1, and off by 2^-25 of the larger product.  In 64 bits it
 //           would take 12 conversions a vector through a pipe of 4 lanes a cycle.)
 //   Q4_0    scale = f16(m / -8), m the group's first value of largest magnitude; code = rint(x / scale) in [-8, 7]
 //   Q8_0    scale = f16(max|x| r), r = 1 / 127 in fp32; code = rint(x / scale) in [-127, 127]
@@ -21,9 +21,12 @@
 // rising positions (a run) share their quads out over the run's warps.  Row by row, the bytes of a head's V
 // touch 16 lines an instruction.
 //
-// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 69.0 us, 5.3 TB/s.  The same
-// with values and 8-bit writing, and read back, 5003 rows: 76.3 us.  8192 rows of 8 heads of 64 in 4 bits: 16.7 us to write (142 a
-// vector, issue 70 %, ALU 57 %; a warp has only four), 9 us to read.
+// Bound by memory and by instructions.  Norm and rotation of 9001 rows of 32 + 8 heads of 128: 69.1 us, 5.3 TB/s (132
+// instructions a vector, issue slots 64 %, DRAM 54 %).  The same with values and 8-bit writing, 5003 rows: 65.3 us (158 a
+// vector, issue 55 %, 0.7 of a stall per issue for want of instructions: the kernel is long).  8192 rows of 8 heads of 64
+// in 4 bits: 15.0 us to write (142 a vector, issue 70 %, ALU 57 %; a warp has only four, and spills 52 bytes a thread to have five
+// CTAs an SM), 11.8 us to read, where a plain write of the same rows takes 6.5.  Reading 16384 rows of 8 heads of 128 in 8
+// bits: 35.7 us, a plain write 20.9; the loads' latency (10 of 16 stalls per issue; a warp of values has one quad on its way).
 #include <type_traits>
 
 #include "kvq.cuh"
@@ -266,8 +269,8 @@ static RowSplit row_split(int split, int vsplit, int q_vectors) {
 // LH lanes per head.  A row has `split` warps for its queries and keys (vectors of 32 / LH heads: first, first +
 // split, ...) and `vsplit` for its share of the run's values.
 // KIND 0: rows are only written, 1: normed or copied, and written if there is a cache, 2: rotated too, without a cache, 3: with
-// one.  (Kernels of their own are shorter and have fewer registers: 8192 rows of 8 heads of 64 in 4 bits written and read, as
-// KIND 1 27.2 us, at 4 CTAs an SM 26.2, at 5 25.7; 9001 rows rotated, as KIND 3 65.4, alone 63.3, at 4 CTAs an SM 69.)
+// one.  (Kernels of their own are shorter and have fewer registers.  CTAs an SM, 9001 rows rotated 2 / 3 / 4: 73.8 / 69.1 / 82.3 us,
+// 5003 stored and read 82.4 / 76.5 / 83.7, 8192 rows of 8 heads of 64 in 4 bits written and read 3 / 4 / 5: 28.1 / 26.1 / 25.6.)
 template <int LH, int BITS, int KIND>
 __global__ void __launch_bounds__(KR_THREADS, KIND >= 2 ? 3 : KIND == 1 ? 4 : 5) tf_kvq_rows_kernel(const KvqRowsArgs a, const RowSplit sp) {
     constexpr int HPW = 32 / LH;
@@ -609,7 +612,7 @@ __global__ void __launch_bounds__(KR_THREADS) tf_kvq_read_kernel(const KvqReadAr
 // Warps per row: one when rows alone fill the device (`fill` warps on each of its SMs), else a row's vectors are
 // shared out so that few rows finish in one round of loads.  16 warps, and twice what an SM holds where they carry
 // a whole row of queries and keys, whose last round would else be long: 5003 rows of 32 + 8 + 8 heads of 128 written
-// in 8 bits and read back, 69.6 us with 16, 68.4 with 48.
+// in 8 bits and read back, 79.5 us with 16, 76.5 with 48.
 constexpr int KR_FILL = 16, KR_FILL_TURN = 48;
 static int kvq_split(int rows, int vectors, int fill = KR_FILL) {
     const int want = (int)((148ll * fill + rows - 1) / rows);
